@@ -184,6 +184,127 @@ bool tcg_mha_images(float *out, float *out_hi, float *out_lo, const float *qkv,
 bool tcg_add(float *out, const float *a, const float *b, size_t n);
 bool tcg_scale(float *out, const float *x, float s, size_t n);
 
+/* ------------------------------- language-model operators (new)
+ * What a decode or prefill step of a GGUF language model needs between the
+ * projections (tcg_matvec_q, tcg_linear_q, tcg_linear): rotary positions,
+ * head norms, an 8-bit key/value cache and the attention that reads it.
+ * Rows are tokens; a row's heads lie side by side (head h at h * head_dim)
+ * and successive rows are ld elements apart, so the parts of a fused QKV row
+ * are passed as pointers into it. Types: GGML_TYPE_F32, F16 and BF16, the
+ * arithmetic is fp32 and each result is rounded once. No call allocates or
+ * keeps anything between calls: all of them can be captured into CUDA graphs
+ * and run on several streams at once, as long as they do not write the same
+ * rows or pages.
+ *
+ * Lengths and page numbers are read on the device. What is out of range
+ * there is skipped, without any access, and raises the device error word
+ * (tcg_device_error): */
+#define TCG_ERR_KV8_LENGTHS 64  /* a sequence's rows or lengths: the whole sequence is skipped */
+#define TCG_ERR_KV8_PAGE    65  /* a page number: its tokens are not written, read as 0, and masked in attention */
+
+/* ---- rotary positions. A plain host struct, filled by tcg_rope_init and
+ * the tcg_rope_scale_* calls (all host only, no GPU), passed by pointer and
+ * copied into each launch. Pair i of a token at position p turns by
+ * p * turns[i] revolutions, reduced in 64 bits (exact to 2^-50 of a
+ * revolution up to position 2^20); the rotated values are multiplied by
+ * mscale. Dims from n_rot on are not rotated. */
+#define TCG_ROPE_INTERLEAVED 0          /* pair i: dims 2i and 2i + 1             */
+#define TCG_ROPE_HALF        1          /* pair i: dims i and i + n_rot / 2       */
+#define TCG_ROPE_MAX_DIM     256
+typedef struct {
+    int head_dim, n_rot, layout;
+    float mscale;
+    double base;
+    double turns[TCG_ROPE_MAX_DIM / 2];
+} tcg_rope_t;
+
+/* turns[i] = base^(-2i / n_rot) / (2 pi), mscale 1. head_dim even and at most
+ * TCG_ROPE_MAX_DIM, n_rot even, 2 .. head_dim; base > 0. */
+bool tcg_rope_init(tcg_rope_t *r, int head_dim, int n_rot, int layout, double base);
+/* Contexts longer than the trained one. linear: every pair `factor` times
+ * slower. yarn (Peng et al. 2023): pairs that turn more than beta_fast times
+ * over orig_ctx tokens keep their speed, those that turn less than beta_slow
+ * times are slowed by factor, with a ramp over the pair index between; mscale
+ * is multiplied by attn_factor, or by 0.1 ln(factor) + 1 when that is 0.
+ * bands: pairs that turn at most `low` times over orig_ctx are slowed by
+ * factor, those that turn at least `high` times keep their speed, between
+ * them linearly in the number of turns. factors: pair i's speed divided by
+ * f[i] (HOST array of n_rot / 2; GGUF's rope_freqs.weight). */
+bool tcg_rope_scale_linear(tcg_rope_t *r, double factor);
+bool tcg_rope_scale_yarn(tcg_rope_t *r, double factor, int orig_ctx, double beta_fast, double beta_slow,
+                         double attn_factor);
+bool tcg_rope_scale_bands(tcg_rope_t *r, double factor, int orig_ctx, double low, double high);
+bool tcg_rope_scale_factors(tcg_rope_t *r, const float *f, int n);
+/* The same from a GGUF language model's metadata: <arch>.rope.freq_base
+ * (10000 when absent), .rope.dimension_count, .attention.key_length (or
+ * embedding_length / attention.head_count), .rope.scaling.type (none,
+ * linear, yarn) with .factor, .original_context_length and .attn_factor, and
+ * the F32 tensor rope_freqs.weight. The pair layout is the architecture's;
+ * the file does not record it. */
+bool tcg_rope_from_gguf(tcg_rope_t *r, const gguf_t *g, int layout);
+
+/* out = x rotated: n_tok rows of n_head heads, token i at position pos[i]
+ * (DEVICE, any 32-bit value). In place (out == x, the same ld) or out of
+ * place without overlap. */
+bool tcg_rope(void *out, const void *x, const int32_t *pos, const tcg_rope_t *r, int n_tok, int n_head,
+              int64_t ld_out, int64_t ld_x, ggml_type_t t);
+/* Root-mean-square norm of every query and key head, then the rotation, in
+ * one pass over both: y = x / sqrt(mean(x^2) + eps) * w (w fp32 [head_dim],
+ * DEVICE). Either side may be absent (n_head or n_kv_head 0). In place or out
+ * of place as tcg_rope. */
+bool tcg_qk_norm_rope(void *q_out, void *k_out, const void *q, const void *k, const float *q_w, const float *k_w,
+                      float eps, const int32_t *pos, const tcg_rope_t *r, int n_tok, int n_head, int n_kv_head,
+                      int64_t ld_q_out, int64_t ld_k_out, int64_t ld_q, int64_t ld_k, ggml_type_t t);
+
+/* ---- the 8-bit key/value cache: pages of TCG_KV8_PAGE tokens, each (page,
+ * head) with one fp32 scale for K and one for V; value = code * scale, codes
+ * -127 .. 127. The caller owns the memory (DEVICE, 16-byte aligned codes):
+ *   k  [n_pages, n_kv_head, 64, head_dim]   token-major
+ *   v  [n_pages, n_kv_head, head_dim, 64]   dim-major: the second product of
+ *      attention then reads 16 tokens of a dim as one 128-bit word
+ *   k_scale, v_scale [n_pages, n_kv_head]
+ * head_dim a multiple of 16, 16 .. 128. Fresh pages need no initialisation. */
+#define TCG_KV8_PAGE 64
+typedef struct {
+    int8_t *k, *v;
+    float *k_scale, *v_scale;
+    int n_pages, n_kv_head, head_dim;
+} tcg_kv8_t;
+
+/* One step's rows. Sequence b has rows tok_start[b] .. tok_start[b+1] - 1 of
+ * the n_tok rows of the call, which are its LAST tokens: with n of them and
+ * kv_len[b] tokens in all (these included), row i stands for position
+ * kv_len[b] - n + i. Position p lies in page table[b * table_ld + p / 64].
+ * tok_start [n_seq + 1], kv_len [n_seq] and table are DEVICE arrays. max_new
+ * bounds every sequence's rows (a sequence with more is refused on the
+ * device); max_kv is the expected longest kv_len and only sizes the launch.
+ * Table entries behind a sequence's last page are never read. */
+typedef struct {
+    const int32_t *tok_start, *kv_len, *table;
+    int table_ld, n_seq, n_tok, max_new, max_kv;
+} tcg_kv8_step_t;
+
+/* Write the step's K and V rows (n_kv_head heads each) into the cache. A
+ * page's scale grows to max(scale, |largest new value| / 127); when it grows
+ * the page's older codes become round(code * (old / new)). Codes are
+ * round(x / scale), ties to even, all in fp32; a NaN is stored as 0, an
+ * infinity as the largest finite value. A page that a call writes must belong
+ * to one sequence of it only (pages that are only read may be shared). */
+bool tcg_kv8_append(const tcg_kv8_t *c, const tcg_kv8_step_t *s, const void *k, const void *v,
+                    int64_t ld_k, int64_t ld_v, ggml_type_t t);
+/* Read the step's rows back as values (code * scale, rounded to t). */
+bool tcg_kv8_read(void *k, void *v, const tcg_kv8_t *c, const tcg_kv8_step_t *s, int64_t ld_k, int64_t ld_v,
+                  ggml_type_t t);
+/* Attention of the step's queries (n_head heads, a multiple of n_kv_head;
+ * query head h reads key head h / (n_head / n_kv_head)) over the cache, which
+ * already holds the step's own tokens: out = sum_j softmax_j(scale q.k_j) v_j.
+ * causal: a query sees the positions up to its own, and with window > 0 only
+ * the last `window` of them; not causal: all kv_len positions (window 0). A
+ * query that sees nothing gets zeros. Rows from tok_start[n_seq] on are left
+ * as they were. scale > 0. out must not overlap q. */
+bool tcg_kv8_attention(void *out, const void *q, const tcg_kv8_t *c, const tcg_kv8_step_t *s, int n_head,
+                       int64_t ld_out, int64_t ld_q, float scale, bool causal, int window, ggml_type_t t);
+
 /* ------------------------------------------------- batched ViT (new)
  * The forward of tc_vit_encode (src/vit.c:305-391) over a batch of images.
  * Weights are uploaded once (fp32 plus the tf32 hi/lo split the 3xTF32

@@ -1,0 +1,733 @@
+// kv8_attn.cu -- attention over the 8-bit key/value cache (tcg_kv8_attention).
+//
+// For the query rows of one key head (row = token * G + query head of the
+// group, G = n_head / n_kv_head) and pages of 64 keys with scales sk, sv:
+//   S = Q K^T, P = exp2(c S - m), O = O 2^(m_old - m) + P V, out = O / sum P
+// with c = scale log2(e), m the running maximum. Both products run on the
+// 8-bit integer tensor path (mma.sync m16n8k32, s32 accumulators), on the
+// cache's bytes as they lie there: nothing is converted to a wider type.
+//   Q is quantised per row, once, to a whole number of 15 bits (fp16, bf16
+//     inputs) or 23 bits (fp32): q = q_scale * (d1 256 + d0), or with d2 65536
+//     too, digits of 8 bits in -128 .. 127. The sum over dims is exact.
+//   P in [0, 1] becomes a whole number of 16 or 23 bits the same way, by one
+//     fused multiply-add whose result's mantissa is that number, and byte
+//     permutes; P V is exact per tile and folded into fp32 with sv.
+// NP = 2 digits leave 2^-16 of a row's largest |q| and 2^-17 of the largest
+// weight (below the half step of fp16, 2^-11, by 2^5); NP = 3 2^-24 of both.
+//
+// Why no shuffles: the mma's k order is free as long as A and B agree. A
+// thread (row g = lane / 4, t = lane % 4) takes 16 consecutive bytes of a K
+// row or of a V row (V is stored dim-major) as one 128-bit shared-memory word
+// for four k-quads; key 16 t + 2 j + c is column 2 t + c of score tile j, so
+// the scores a thread holds are exactly the P bytes its own A fragments need.
+//
+// A tile is one page's K block (64 keys x D, a TMA box per 64 dims, zeros past
+// D) and V block (D x 64, one bulk copy); K and V tiles alternate through a
+// ring of slots, each with an mbarrier. The last warp to release a slot issues
+// the copy that refills it, so there is no producer warp.
+//
+// Work split: WM warps take 16 rows each of the same tiles, WN groups of warps
+// take alternate tiles, and a cluster of S CTAs takes S consecutive shares of
+// the keys; partial results (m, l, O) meet in shared memory, then over
+// distributed shared memory, in a fixed order. No workspace, one launch.
+#include "lm.cuh"
+#include "tc05.cuh"
+
+#include <math.h>
+
+namespace tcg {
+namespace {
+
+constexpr int PAGE = TCG_KV8_PAGE;
+constexpr int ERR_WAIT = 66;             // device error word: a tile's copy did not land in time
+
+struct AttnArgs {
+    const void *q;
+    void *out;
+    long long ld_q, ld_out;
+    int type, q_vec, out_vec;            // ggml type; 16-byte loads / 4-element stores possible
+    const int8_t *v;
+    const float *k_scale, *v_scale;
+    KvStep step;
+    int n_pages, n_kv, D, G;
+    float scale_log2;
+    int causal, window, S;
+    int *err;
+};
+
+__device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_u8s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ uint32_t mapa(uint32_t a, int rank)
+{
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t a)
+{
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t a)
+{
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// 16 consecutive values of a query row.
+__device__ __forceinline__ void load_q16(const AttnArgs &p, long long off, float (&x)[16])
+{
+    if (p.type == GGML_TYPE_F32) {
+        const float *s = (const float *)p.q + off;
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            if (p.q_vec) {
+                const float4 v = *(const float4 *)(s + i);
+                x[i] = v.x, x[i + 1] = v.y, x[i + 2] = v.z, x[i + 3] = v.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[i + e] = s[i + e];
+            }
+        }
+        return;
+    }
+    const unsigned short *s = (const unsigned short *)p.q + off;
+    uint32_t w[8];
+    if (p.q_vec) {
+        const uint4 a = *(const uint4 *)s, b = *(const uint4 *)(s + 8);
+        w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[i] = (uint32_t)s[2 * i] | (uint32_t)s[2 * i + 1] << 16;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        if (p.type == GGML_TYPE_BF16) {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        } else {
+            x[2 * i] = __half2float(__ushort_as_half((unsigned short)w[i]));
+            x[2 * i + 1] = __half2float(__ushort_as_half((unsigned short)(w[i] >> 16)));
+        }
+    }
+}
+
+template <int V>
+__device__ __forceinline__ void store_out(const AttnArgs &p, long long off, const float (&x)[V])
+{
+    if (p.type == GGML_TYPE_F32) {
+        float *o = (float *)p.out + off;
+        if (p.out_vec) store_pack<float, V>(o, x);
+        else
+#pragma unroll
+            for (int i = 0; i < V; i++) o[i] = x[i];
+    } else if (p.type == GGML_TYPE_F16) {
+        __half *o = (__half *)p.out + off;
+        if (p.out_vec) store_pack<__half, V>(o, x);
+        else
+#pragma unroll
+            for (int i = 0; i < V; i++) o[i] = __float2half_rn(x[i]);
+    } else {
+        __nv_bfloat16 *o = (__nv_bfloat16 *)p.out + off;
+        if (p.out_vec) store_pack<__nv_bfloat16, V>(o, x);
+        else
+#pragma unroll
+            for (int i = 0; i < V; i++) o[i] = __float2bfloat16_rn(x[i]);
+    }
+}
+
+// Sum of weights -> factor on O. A row that saw nothing has the sum 0 and
+// gets zeros; a NaN sum (a query with a NaN or an infinity) stays NaN.
+__device__ __forceinline__ float inverse(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
+
+template <int KS, int WM, int WN, int NSLOT>
+struct Shape {
+    static constexpr int DP = KS * 32;                       // dims, padded
+    static constexpr int SLOT = PAGE * DP;                   // bytes of a K or V tile
+    static constexpr int RING = WN * NSLOT * SLOT;
+    static constexpr int ROWS = 16 * WM;
+    static constexpr int PITCH = DP + 8;                     // floats of a partial O row
+    static constexpr int EXCH = (WN * ROWS * (PITCH + 2) + 18 * ROWS) * 4;   // partial O, m, l; weights of <= 16 CTAs, sum
+    static constexpr int BODY = RING > EXCH ? RING : EXCH;
+    static_assert(BODY % 16 == 0, "the barriers follow");
+    static constexpr size_t SMEM = 128 + BODY + WN * NSLOT * 12 + 16;
+};
+
+template <int KS, int NP, int WM, int WN, int NSLOT, int MINB>
+__global__ void __launch_bounds__(32 * WM * WN, MINB)
+kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUtensorMap kmap)
+{
+    using Sh = Shape<KS, WM, WN, NSLOT>;
+    constexpr int NT = KS * 4;                               // 8-dim output tiles
+    extern __shared__ uint8_t raw[];
+    uint8_t *const base = (uint8_t *)(((uintptr_t)raw + 127) & ~(uintptr_t)127);
+    const uint32_t ring = su32(base), bars = ring + Sh::BODY;
+    int *const count = (int *)(base + Sh::BODY + WN * NSLOT * 8);
+    volatile int *const abort = (volatile int *)(count + WN * NSLOT);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int wm = warp % WM, wn = warp / WM;
+    const int rank = blockIdx.x % p.S, ntile = gridDim.x / p.S;
+    const int head = blockIdx.y, b = blockIdx.z;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < WN * NSLOT; i++) {
+            bar_init(bars + 8 * i, 1);
+            count[i] = 0;
+        }
+        *abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncthreads();
+    pdl_wait();
+
+    kv8_seq_t seq;
+    const bool report = threadIdx.x == 0;
+    if (!kv_seq(p.step, b, seq, p.err, report)) return;      // the same for the whole cluster
+    const int R = seq.n * p.G, r0 = (p.causal ? ntile - 1 - (int)blockIdx.x / p.S : (int)blockIdx.x / p.S) * Sh::ROWS;
+    if (r0 >= R) return;
+    auto hi_of = [&](int tok) { return kv8_hi(&seq, tok, p.causal); };
+    auto lo_of = [&](int tok) { return kv8_lo(&seq, tok, p.window); };
+    int t0;                                                  // this warp group's tiles: t0, t0 + WN, ...
+    const int mine = kv8_tiles(&seq, r0 / p.G, (min(r0 + Sh::ROWS, R) - 1) / p.G, p.causal, p.window, rank, p.S, wn, WN, &t0);
+
+    // This thread's two rows.
+    int hi[2], lo[2];
+    long long row_off[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int r = min(r0 + 16 * wm + g + 8 * i, R - 1), tok = r / p.G;
+        hi[i] = hi_of(tok);
+        lo[i] = lo_of(tok);
+        row_off[i] = (long long)(head * p.G + r % p.G) * p.D;
+    }
+    const int row_a = min(r0 + 16 * wm, R - 1) / p.G, row_z = min(r0 + 16 * wm + 15, R - 1) / p.G;
+    const int all_hi = hi_of(row_a), all_lo = lo_of(row_z);  // keys that every row of the warp sees
+    const int any_hi = hi_of(row_z), any_lo = lo_of(row_a);  // keys that some row of the warp sees
+
+    // Pages and scales of 32 tiles at a time, one per lane; the next 32 pages too.
+    auto page_at = [&](int i) {
+        return i < mine ? kv_page(p.step, b, t0 + i * WN, p.n_pages, p.err, true) : 0;
+    };
+    int page = page_at(lane), page_next = page_at(32 + lane);
+    float sk = 0.0f, sv = 0.0f;
+    auto scales = [&]() {
+        const long long at = (long long)max(page, 0) * p.n_kv + head;
+        sk = p.k_scale[at];
+        sv = p.v_scale[at];
+    };
+
+    const uint32_t my_ring = ring + wn * NSLOT * Sh::SLOT, my_bars = bars + wn * NSLOT * 8;
+    int *const my_count = count + wn * NSLOT;
+    // Item n = K (even) or V (odd) of tile n / 2, into slot n % NSLOT. A page that does not exist is masked; its copy
+    // takes page 0 instead.
+    auto issue = [&](int n, int slot, int pg) {
+        const uint32_t dst = my_ring + slot * Sh::SLOT, bar = my_bars + 8 * slot;
+        const long long at = (long long)max(pg, 0) * p.n_kv + head;
+        if (n & 1) {
+            const uint32_t bytes = (uint32_t)p.D * PAGE;
+            bar_expect_tx(bar, bytes);
+            bulk_load(dst, p.v + at * p.D * PAGE, bytes, bar);
+        } else {
+            bar_expect_tx(bar, Sh::SLOT);
+#pragma unroll
+            for (int c = 0; c < KS / 2; c++) tma_load(dst + c * 4096, &kmap, bar, 64 * c, (int)(at * PAGE));
+        }
+    };
+    auto page_of = [&](int i, int now) {                     // whole warp
+        return __shfl_sync(0xFFFFFFFFu, (i >> 5) == (now >> 5) ? page : page_next, i & 31);
+    };
+    if (wm == 0) {
+#pragma unroll
+        for (int n = 0; n < NSLOT; n++) {
+            const int pg = page_of(n >> 1, 0);
+            if (lane == 0 && n < 2 * mine) issue(n, n, pg);
+        }
+    }
+    scales();
+
+    // Q digits, in the k order of the tiles: k-step 2 c + s of chunk c takes bytes 64 c + 16 t + 8 s + 0..7.
+    uint32_t qd[NP][KS][4];
+    float qs[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        float x[KS / 2][16], m = 0.0f;
+        bool odd = false;                                    // a NaN or an infinity
+        const int r = min(r0 + 16 * wm + g + 8 * i, R - 1);
+        const long long off = (seq.row0 + r / p.G) * p.ld_q + row_off[i];
+#pragma unroll
+        for (int c = 0; c < KS / 2; c++) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) x[c][e] = 0.0f;
+            if (64 * c + 16 * t < p.D) load_q16(p, off + 64 * c + 16 * t, x[c]);
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                odd |= !(fabsf(x[c][e]) <= 3.402823466e38f);
+                m = fmaxf(m, fabsf(x[c][e]));
+            }
+        }
+        m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+        odd = odd | __shfl_xor_sync(0xFFFFFFFFu, (int)odd, 1);
+        odd = odd | __shfl_xor_sync(0xFFFFFFFFu, (int)odd, 2);
+        constexpr float Q = NP == 3 ? 8300000.0f : 32512.0f; // the digits' largest sums
+        const float up = Q / fmaxf(m, 1e-30f);
+        qs[i] = odd ? __int_as_float(0x7FC00000) : fmaxf(m, 1e-30f) * (p.scale_log2 / Q);
+#pragma unroll
+        for (int c = 0; c < KS / 2; c++)
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                uint32_t d[NP] = {};
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    int v = __float2int_rn(x[c][4 * w + e] * up);
+#pragma unroll
+                    for (int n = 0; n < NP; n++) {
+                        const int dig = (int)(int8_t)v;
+                        d[n] |= (uint32_t)(dig & 0xFF) << (8 * e);
+                        v = (v - dig) >> 8;
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NP; n++) qd[n][2 * c + (w >> 1)][2 * (w & 1) + i] = d[n];
+            }
+    }
+
+    float o[NT][4], m[2], l[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        m[i] = -INFINITY;
+        l[i] = 0.0f;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[n][e] = 0.0f;
+
+    int slot = 0, parity = 0;
+    bool ok = true;
+    // Whole warp: this warp is done with item n in `slot`; whoever is last refills it.
+    auto release = [&](int n) {
+        const int next = n + NSLOT, pg = page_of(next >> 1, n >> 1);
+        __syncwarp();
+        if (lane == 0) {
+            bool last = true;
+            if (WM > 1) {
+                __threadfence_block();
+                last = atomicAdd(my_count + slot, 1) == WM - 1;
+                if (last) {
+                    my_count[slot] = 0;
+                    __threadfence_block();
+                }
+            }
+            if (last && next < 2 * mine) {
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                issue(next, slot, pg);
+            }
+        }
+        if (++slot == NSLOT) {
+            slot = 0;
+            parity ^= 1;
+        }
+    };
+    auto landed = [&]() {
+        return __all_sync(0xFFFFFFFFu, bar_wait(my_bars + 8 * slot, parity, abort, p.err, ERR_WAIT));
+    };
+
+    for (int i = 0; i < mine; i++) {
+        if (i && (i & 31) == 0) {
+            page = page_next;
+            page_next = page_at(i + 32 + lane);
+            scales();
+        }
+        const int key0 = (t0 + i * WN) * PAGE;
+        const bool real = __shfl_sync(0xFFFFFFFFu, page, i & 31) >= 0 && key0 <= any_hi && key0 + PAGE > any_lo;
+        const float tk = __shfl_sync(0xFFFFFFFFu, sk, i & 31), tv = __shfl_sync(0xFFFFFFFFu, sv, i & 31);
+
+        ok = landed();
+        if (!ok) break;
+        float f[8][4];
+        if (real) {
+            const uint32_t kt = my_ring + slot * Sh::SLOT + (16 * (g >> 1) + (g & 1)) * 64 + 16 * t;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                uint4 w[KS / 2];
+#pragma unroll
+                for (int c = 0; c < KS / 2; c++) w[c] = lds128(kt + c * 4096 + j * 128);
+                int a[4] = {}, top[4] = {};
+                if (NP == 3) {
+#pragma unroll
+                    for (int c = 0; c < KS / 2; c++) {
+                        mma_s8(top, qd[NP - 1][2 * c], w[c].x, w[c].y);
+                        mma_s8(top, qd[NP - 1][2 * c + 1], w[c].z, w[c].w);
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < KS / 2; c++) {
+                    mma_s8(a, qd[1][2 * c], w[c].x, w[c].y);
+                    mma_s8(a, qd[1][2 * c + 1], w[c].z, w[c].w);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) a[e] <<= 8;      // |a| < 2^21 (128 dims), so below 2^30 with the next digit
+#pragma unroll
+                for (int c = 0; c < KS / 2; c++) {
+                    mma_s8(a, qd[0][2 * c], w[c].x, w[c].y);
+                    mma_s8(a, qd[0][2 * c + 1], w[c].z, w[c].w);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    f[j][e] = NP == 3 ? fmaf((float)top[e], 65536.0f, (float)a[e]) : (float)a[e];
+            }
+        }
+        release(2 * i);
+
+        uint32_t pd[NP][2][4];
+        if (real) {
+            if (key0 < all_lo || key0 + PAGE - 1 > all_hi) {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int key = key0 + 16 * t + 2 * j + (e & 1);
+                        if (key > hi[e >> 1] || key < lo[e >> 1]) f[j][e] = -INFINITY;
+                    }
+            }
+            bool grew = false;
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < 8; j++) top = fmaxf(top, fmaxf(f[j][2 * r], f[j][2 * r + 1]));
+                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+                // a zero factor would turn a masked -inf into NaN; a NaN factor (a NaN query) has to stay
+                float cs = qs[r] * tk;
+                cs = cs < 1e-37f ? 1e-37f : cs;
+                // raised by 2^-22 of itself, so that rounding never puts a weight above 1 (its digits would overflow)
+                float mt = top * cs;
+                mt = fmaf(fabsf(mt), 0x1p-22f, mt);
+                const float mn = fmaxf(m[r], top == -INFINITY ? -INFINITY : mt);
+                const float use = mn == -INFINITY ? 0.0f : mn, alpha = ex2(m[r] - use);
+                grew |= mn != m[r];
+                m[r] = mn;
+                float sum = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        float &v = f[j][2 * r + c];
+                        v = ex2(fmaf(v, cs, -use));
+                        sum += v;
+                        v = NP == 3 ? fmaf(v, 8388607.0f, 8388608.0f) : fmaf(v, 65535.0f / 65536.0f, 128.0f);
+                    }
+                l[r] = fmaf(l[r], alpha, sum);
+                if (__any_sync(0xFFFFFFFFu, grew)) {
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        o[n][2 * r] *= alpha;
+                        o[n][2 * r + 1] *= alpha;
+                    }
+                }
+                // bytes of the four weights of keys 16 t + 4 w + 0..3
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    const uint32_t y0 = __float_as_uint(f[2 * w][2 * r]), y1 = __float_as_uint(f[2 * w][2 * r + 1]);
+                    const uint32_t y2 = __float_as_uint(f[2 * w + 1][2 * r]), y3 = __float_as_uint(f[2 * w + 1][2 * r + 1]);
+                    const uint32_t u = __byte_perm(y0, y1, 0x5140), v = __byte_perm(y2, y3, 0x5140);
+                    pd[0][w >> 1][2 * (w & 1) + r] = __byte_perm(u, v, 0x5410);
+                    pd[1][w >> 1][2 * (w & 1) + r] = __byte_perm(u, v, 0x7632);
+                    if (NP == 3)
+                        pd[NP - 1][w >> 1][2 * (w & 1) + r] =
+                            __byte_perm(__byte_perm(y0, y1, 0x0062), __byte_perm(y2, y3, 0x0062), 0x5410);
+                }
+            }
+        }
+
+        ok = landed();
+        if (!ok) break;
+        if (real) {
+            const uint32_t vt = my_ring + slot * Sh::SLOT + g * 64 + 16 * t;
+            const float fs = tv * (NP == 3 ? 1.0f / 8388607.0f : 1.0f / 65535.0f);
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                const uint4 w = lds128(vt + n * 512);
+                int a[4] = {}, top[4] = {};
+                if (NP == 3) {
+                    mma_u8s8(top, pd[NP - 1][0], w.x, w.y);
+                    mma_u8s8(top, pd[NP - 1][1], w.z, w.w);
+                }
+                mma_u8s8(a, pd[1][0], w.x, w.y);
+                mma_u8s8(a, pd[1][1], w.z, w.w);
+#pragma unroll
+                for (int e = 0; e < 4; e++) a[e] <<= 8;      // |a| <= 255 * 128 * 64 < 2^21
+                mma_u8s8(a, pd[0][0], w.x, w.y);
+                mma_u8s8(a, pd[0][1], w.z, w.w);
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    o[n][e] = fmaf(NP == 3 ? fmaf((float)top[e], 65536.0f, (float)a[e]) : (float)a[e], fs, o[n][e]);
+            }
+        }
+        release(2 * i + 1);
+    }
+
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+        l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 1);
+        l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 2);
+    }
+
+    if (!ok) {
+        // A copy did not land in time: the error word is set. Nothing is reused; each group waits, bounded, for the
+        // copies it has in flight before the CTA may end (or its ring be overwritten).
+        for (int s = 0; s < NSLOT; s++) bar_wait(my_bars + 8 * s, parity ^ (s < slot), abort, p.err, ERR_WAIT, false);
+    }
+    if (WN == 1 && p.S == 1) {
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            const int row = r0 + 16 * wm + g + 8 * r;
+            if (row >= R) continue;
+            const float inv = inverse(l[r]);
+            const long long off = (seq.row0 + row / p.G) * p.ld_out + row_off[r];
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                if (8 * n >= p.D) break;
+                const float v[2] = { o[n][2 * r] * inv, o[n][2 * r + 1] * inv };
+                store_out<2>(p, off + 8 * n + 2 * t, v);
+            }
+        }
+        return;
+    }
+
+    // Partial results meet: the WN groups of this CTA, then the S CTAs of the cluster.
+    __syncthreads();                                         // every tile is consumed: the ring is free
+    float *const po = (float *)base;                         // [WN][ROWS][PITCH]
+    float *const pm = po + WN * Sh::ROWS * Sh::PITCH;        // [WN][ROWS]
+    float *const pl = pm + WN * Sh::ROWS;
+    float *const pw = pl + WN * Sh::ROWS;                    // [16][ROWS] weights of the cluster's CTAs
+    float *const ps = pw + 16 * Sh::ROWS;                    // [ROWS] 1 / sum
+    const int rows = min(Sh::ROWS, R - r0), d4 = p.D / 4;
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+        const int at = wn * Sh::ROWS + 16 * wm + g + 8 * r;
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+            *(float2 *)(po + at * Sh::PITCH + 8 * n + 2 * t) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
+        if (t == 0) {
+            pm[at] = m[r];
+            pl[at] = l[r];
+        }
+    }
+    __syncthreads();
+    if (WN > 1) {
+        for (int i = threadIdx.x; i < rows * d4; i += blockDim.x) {
+            const int r = i / d4, d = 4 * (i % d4);
+            float top = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < WN; w++) top = fmaxf(top, pm[w * Sh::ROWS + r]);
+            top = top == -INFINITY ? 0.0f : top;
+            float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < WN; w++) {
+                const float a = ex2(pm[w * Sh::ROWS + r] - top);
+                const float4 v = *(const float4 *)(po + (w * Sh::ROWS + r) * Sh::PITCH + d);
+                s.x = fmaf(a, v.x, s.x), s.y = fmaf(a, v.y, s.y), s.z = fmaf(a, v.z, s.z), s.w = fmaf(a, v.w, s.w);
+            }
+            *(float4 *)(po + r * Sh::PITCH + d) = s;         // group 0's place: read by this thread only
+        }
+        __syncthreads();
+        if ((int)threadIdx.x < rows) {
+            const int r = threadIdx.x;
+            float top = -INFINITY, sum = 0.0f;
+            for (int w = 0; w < WN; w++) top = fmaxf(top, pm[w * Sh::ROWS + r]);
+            for (int w = 0; w < WN; w++) sum += pl[w * Sh::ROWS + r] * ex2(pm[w * Sh::ROWS + r] - (top == -INFINITY ? 0.0f : top));
+            pm[r] = top;
+            pl[r] = sum;
+        }
+        __syncthreads();
+    }
+    const uint32_t a_po = su32(po), a_pm = su32(pm), a_pl = su32(pl);
+    if (p.S > 1) cluster_sync();
+    for (int r = threadIdx.x; r < rows; r += blockDim.x) {
+        float top = -INFINITY, sum = 0.0f;
+        for (int s = 0; s < p.S; s++) top = fmaxf(top, p.S > 1 ? ld_cluster(mapa(a_pm + 4 * r, s)) : pm[r]);
+        top = top == -INFINITY ? 0.0f : top;
+        for (int s = 0; s < p.S; s++) {
+            const float a = ex2((p.S > 1 ? ld_cluster(mapa(a_pm + 4 * r, s)) : pm[r]) - top);
+            pw[s * Sh::ROWS + r] = a;
+            sum = fmaf(a, p.S > 1 ? ld_cluster(mapa(a_pl + 4 * r, s)) : pl[r], sum);
+        }
+        ps[r] = inverse(sum);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x + rank * blockDim.x; i < rows * d4; i += blockDim.x * p.S) {
+        const int r = i / d4, d = 4 * (i % d4);
+        float v[4] = {};
+        for (int s = 0; s < p.S; s++) {
+            const uint32_t at = a_po + 4 * (r * Sh::PITCH + d);
+            const float4 x = p.S > 1 ? ld_cluster4(mapa(at, s)) : *(const float4 *)(po + r * Sh::PITCH + d);
+            const float a = pw[s * Sh::ROWS + r];
+            v[0] = fmaf(a, x.x, v[0]), v[1] = fmaf(a, x.y, v[1]), v[2] = fmaf(a, x.z, v[2]), v[3] = fmaf(a, x.w, v[3]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] *= ps[r];
+        const int row = r0 + r;
+        store_out<4>(p, (seq.row0 + row / p.G) * p.ld_out + (long long)(head * p.G + row % p.G) * p.D + d, v);
+    }
+    if (p.S > 1) cluster_sync();                             // no CTA leaves while another reads its shared memory
+}
+
+typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                             const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                             CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn attn_encode_fn()
+{
+    static EncodeFn fn = nullptr;
+    if (!fn) {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = (EncodeFn)p;
+        else
+            cudaGetLastError();
+    }
+    return fn;
+}
+
+template <int KS, int NP, int WM, int WN, int NSLOT, int MINB>
+bool attn_launch(AttnArgs &p, const CUtensorMap &map, int ntile, int n_seq)
+{
+    using Sh = Shape<KS, WM, WN, NSLOT>;
+    auto fn = kv8_attn_kernel<KS, NP, WM, WN, NSLOT, MINB>;
+    static bool ready[64];
+    const int dev = ctx().device & 63;
+    if (!ready[dev]) {
+        TCG_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::SMEM));
+        ready[dev] = true;
+    }
+    cudaLaunchAttribute attrs[2];
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3((unsigned)(ntile * p.S), (unsigned)p.n_kv, (unsigned)n_seq);
+    lc.blockDim = dim3(32 * WM * WN);
+    lc.dynamicSmemBytes = Sh::SMEM;
+    lc.stream = ctx().cur;
+    lc.attrs = attrs;
+    lc.numAttrs = pdl_attr(attrs);
+    if (p.S > 1) {
+        attrs[lc.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attrs[lc.numAttrs].val.clusterDim.x = (unsigned)p.S;
+        attrs[lc.numAttrs].val.clusterDim.y = 1;
+        attrs[lc.numAttrs].val.clusterDim.z = 1;
+        lc.numAttrs++;
+    }
+    TCG_CUDA(cudaLaunchKernelEx(&lc, fn, p, map));
+    return true;
+}
+
+}  // namespace
+}  // namespace tcg
+
+using namespace tcg;
+
+extern "C" bool tcg_kv8_attention(void *out, const void *q, const tcg_kv8_t *c, const tcg_kv8_step_t *s, int n_head,
+                                  int64_t ld_out, int64_t ld_q, float scale, bool causal, int window, ggml_type_t t)
+{
+    const char *who = "tcg_kv8_attention";
+    if (!kv8_check(who, c, s, t)) return false;
+    if (n_head < 1 || n_head % c->n_kv_head || n_head / c->n_kv_head > 4096)
+        return fail("%s: %d query heads over %d key heads", who, n_head, c->n_kv_head);
+    if (!(scale > 0.0f) || scale > 1e30f) return fail("%s: scale %g is not positive", who, (double)scale);
+    if (window < 0 || (window && !causal)) return fail("%s: window %d%s", who, window, causal ? "" : " without causal");
+    const size_t size = lm_type_size(t);
+    if (s->n_tok && (!out || !q)) return fail("%s: no queries or no output", who);
+    if (((uintptr_t)out | (uintptr_t)q) % size) return fail("%s: misaligned queries or output", who);
+    const int64_t wide = (int64_t)n_head * c->head_dim;
+    if ((ld_q < wide || ld_out < wide) && s->n_tok > 1)
+        return fail("%s: rows of %lld values do not fit strides of %lld and %lld", who, (long long)wide, (long long)ld_q,
+                    (long long)ld_out);
+
+    const int longest = s->max_new < s->n_tok ? s->max_new : s->n_tok, G = n_head / c->n_kv_head;
+    const long long R = (long long)(longest > 0 ? longest : 1) * G;
+    if (R > 0x3fffffffll) return fail("%s: %d rows of %d heads are too many for one call", who, longest, n_head);
+    if (!lm_ready(who)) return false;
+    if (s->n_seq == 0 || s->n_tok == 0) return true;
+    AttnArgs p = {};
+    p.q = q, p.out = out, p.ld_q = ld_q, p.ld_out = ld_out, p.type = (int)t;
+    p.q_vec = (uintptr_t)q % 16 == 0 && ld_q * (int64_t)size % 16 == 0;
+    p.out_vec = (uintptr_t)out % (4 * size) == 0 && ld_out % 4 == 0;
+    p.v = c->v, p.k_scale = c->k_scale, p.v_scale = c->v_scale;
+    p.step = kv_step(*s);
+    p.n_pages = c->n_pages, p.n_kv = c->n_kv_head, p.D = c->head_dim, p.G = G;
+    p.scale_log2 = scale * 1.44269504088896340736f;
+    p.causal = causal, p.window = window, p.err = ctx().d_err;
+
+    // K as [pages x heads x 64, D] bytes; a box is 64 keys of 64 dims, zeros past D
+    EncodeFn fn = attn_encode_fn();
+    if (!fn) return fail("cuTensorMapEncodeTiled is not available from the driver");
+    CUtensorMap map;
+    const cuuint64_t dims[2] = { (cuuint64_t)p.D, (cuuint64_t)c->n_pages * c->n_kv_head * PAGE };
+    const cuuint64_t strides[1] = { (cuuint64_t)p.D };
+    const cuuint32_t box[2] = { 64, PAGE }, estr[2] = { 1, 1 };
+    const CUresult r = fn(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void *)c->k, dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail("cuTensorMapEncodeTiled failed (%d) for the K cache", (int)r);
+
+    long long keys = s->max_kv;
+    if (window && keys > (long long)window + longest) keys = (long long)window + longest;
+    const long long tiles = (keys + PAGE - 1) / PAGE;
+    // Up to 16 rows (a decode step) one warp's rows hold them all and the 8 warps of a CTA take alternate tiles;
+    // more rows share their tiles between 4 warps of 16 rows. Keys are split over a cluster while that
+    // fills more SMs and leaves every warp group a tile.
+    const bool few = R <= 16;
+    const int rows = few ? 16 : 64, groups = few ? 8 : 1;
+    const long long ntile = (R + rows - 1) / rows, ctas = ntile * p.n_kv * s->n_seq;
+    p.S = 1;
+    while (p.S < 8 && ctas * p.S * 2 <= 2 * ctx().sms && tiles >= 2 * p.S * groups) p.S *= 2;
+    const bool wide_q = t == GGML_TYPE_F32, big = p.D > 64;
+    if (few) {
+        if (big) return wide_q ? attn_launch<4, 3, 1, 8, 3, 1>(p, map, (int)ntile, s->n_seq)
+                               : attn_launch<4, 2, 1, 8, 3, 1>(p, map, (int)ntile, s->n_seq);
+        return wide_q ? attn_launch<2, 3, 1, 8, 6, 1>(p, map, (int)ntile, s->n_seq)
+                      : attn_launch<2, 2, 1, 8, 6, 1>(p, map, (int)ntile, s->n_seq);
+    }
+    if (big) return wide_q ? attn_launch<4, 3, 4, 1, 6, 2>(p, map, (int)ntile, s->n_seq)
+                           : attn_launch<4, 2, 4, 1, 6, 2>(p, map, (int)ntile, s->n_seq);
+    return wide_q ? attn_launch<2, 3, 4, 1, 8, 2>(p, map, (int)ntile, s->n_seq)
+                  : attn_launch<2, 2, 4, 1, 8, 2>(p, map, (int)ntile, s->n_seq);
+}

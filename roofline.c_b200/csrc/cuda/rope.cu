@@ -1,0 +1,286 @@
+// rope.cu -- rotary positions (tcg_rope), and the root-mean-square norm of
+// every query and key head with the rotation in the same pass
+// (tcg_qk_norm_rope).
+//
+// Pair i of a head at position p turns by the angle 2 pi p turns[i]:
+//   (a, b) -> m (a cos - b sin, a sin + b cos).
+// p * turns[i] is taken in 64 bits, its nearest whole number subtracted (the
+// fraction of a revolution is then good to 2^-53 p turns, where a 32-bit
+// angle at p = 2^20 would be off by 2^-4 radians), and only the fraction goes
+// to fp32: sincospi(2 f). The norm is y = x / sqrt(mean(x^2) + eps) * w, its
+// sum of squares in fp32 over the lanes of a head.
+//
+// Bound by memory: 2 * 4 bytes an element (fp32) for ~10 operations. A lane
+// owns one "unit" of 2 V dims of a head, two vectors of V: V pairs of the
+// rotated part, or 2 V dims of the rest. It computes its V sines and cosines
+// once per token and applies them to the heads of the token one after the
+// other, up to four heads' loads in flight. 32 / L heads side by side in a
+// warp, L = the lanes a head needs.
+#include "lm.cuh"
+
+namespace tcg {
+namespace {
+
+constexpr int ROPE_WARPS = 4;
+constexpr int ROPE_AHEAD = 4;    // heads whose loads are in flight
+
+struct RopeArgs {
+    const void *x[2];            // q (or the only tensor), k
+    void *y[2];
+    const float *w[2];           // norm weights
+    long long ldx[2], ldy[2];
+    const int32_t *pos;
+    int heads[2];
+    int n_tok, splits;           // a token's heads are dealt out to `splits` warps
+    int D, n_rot, lanes;         // lanes of a head: a power of two, 1 .. 32
+    float mscale, eps;
+    double turns[TCG_ROPE_MAX_DIM / 2];
+};
+
+// The two vectors of unit u start at dims a and b.
+template <int V, bool HALF>
+__device__ __forceinline__ void unit_dims(int u, int n_rot, int &a, int &b)
+{
+    const int half = n_rot / 2;
+    if (HALF && u * V < half) {
+        a = u * V;
+        b = a + half;
+    } else {
+        a = 2 * V * u;
+        b = a + V;
+    }
+}
+
+template <typename T, int V, int U, bool HALF, bool NORM>
+__global__ void __launch_bounds__(32 * ROPE_WARPS) rope_kernel(const __grid_constant__ RopeArgs p)
+{
+    const int lane = threadIdx.x & 31, L = p.lanes;
+    const int sub = lane / L, l = lane % L, side = 32 / L;
+    const long long task = (long long)blockIdx.x * ROPE_WARPS + (threadIdx.x >> 5);
+    const int tok = (int)(task / p.splits), part = (int)(task % p.splits);
+    pdl_wait();
+    if (tok >= p.n_tok) return;
+    const int units = p.D / (2 * V);
+    const double at = (double)p.pos[tok];
+
+    float cs[U][V], sn[U][V], w0[U][2 * V], w1[U][2 * V];
+    int da[U], db[U];
+    bool live[U], turn[U];
+#pragma unroll
+    for (int k = 0; k < U; k++) {
+        const int u = l + 32 * k;
+        live[k] = u < units;
+        unit_dims<V, HALF>(live[k] ? u : 0, p.n_rot, da[k], db[k]);
+        turn[k] = live[k] && u * V < p.n_rot / 2;
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            cs[k][i] = 1.0f;
+            sn[k][i] = 0.0f;
+            if (turn[k]) {
+                const double t = at * p.turns[u * V + i];
+                const float f = (float)(2.0 * (t - rint(t)));
+                sincospif(f, &sn[k][i], &cs[k][i]);
+                sn[k][i] *= p.mscale;
+                cs[k][i] *= p.mscale;
+            }
+        }
+        if (NORM && live[k]) {
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                w0[k][i] = p.heads[0] ? p.w[0][da[k] + i] : 0.0f;
+                w0[k][V + i] = p.heads[0] ? p.w[0][db[k] + i] : 0.0f;
+                w1[k][i] = p.heads[1] ? p.w[1][da[k] + i] : 0.0f;
+                w1[k][V + i] = p.heads[1] ? p.w[1][db[k] + i] : 0.0f;
+            }
+        }
+    }
+
+    const int all = p.heads[0] + p.heads[1], step = side * p.splits;
+    for (int h0 = part * side + sub; h0 - sub < all; h0 += step * ROPE_AHEAD) {   // the warp's lanes leave together
+        float x[ROPE_AHEAD][U][2 * V];
+#pragma unroll
+        for (int j = 0; j < ROPE_AHEAD; j++) {
+            const int h = h0 + j * step;
+            const int s = h >= p.heads[0];
+            const T *row = (const T *)p.x[s] + tok * p.ldx[s] + (long long)(h - (s ? p.heads[0] : 0)) * p.D;
+#pragma unroll
+            for (int k = 0; k < U; k++) {
+                float a[V] = {}, b[V] = {};
+                if (h < all && live[k]) {
+                    load_pack<T, V>(row + da[k], a);
+                    load_pack<T, V>(row + db[k], b);
+                }
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    x[j][k][i] = a[i];
+                    x[j][k][V + i] = b[i];
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < ROPE_AHEAD; j++) {
+            const int h = h0 + j * step;
+            if (h0 - sub + j * step >= all) break;               // no lane of the warp has a head
+            const int s = h >= p.heads[0];
+            float inv = 1.0f;
+            if (NORM) {
+                float ss = 0.0f;
+#pragma unroll
+                for (int k = 0; k < U; k++)
+#pragma unroll
+                    for (int i = 0; i < 2 * V; i++) ss = fmaf(x[j][k][i], x[j][k][i], ss);
+                for (int o = L >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+                inv = rsqrtf(ss / (float)p.D + p.eps);
+            }
+            if (h >= all) continue;
+            T *row = (T *)p.y[s] + tok * p.ldy[s] + (long long)(h - (s ? p.heads[0] : 0)) * p.D;
+#pragma unroll
+            for (int k = 0; k < U; k++) {
+                if (!live[k]) continue;
+                float v[2 * V], a[V], b[V];
+#pragma unroll
+                for (int i = 0; i < 2 * V; i++) v[i] = NORM ? x[j][k][i] * inv * (s ? w1[k][i] : w0[k][i]) : x[j][k][i];
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    // the two values of pair i: one of each vector, or neighbours
+                    float &lo = HALF ? v[i] : v[2 * i], &hi = HALF ? v[V + i] : v[2 * i + 1];
+                    const float c = cs[k][i], d = sn[k][i], e = lo;
+                    if (turn[k]) {
+                        lo = fmaf(e, c, -(hi * d));
+                        hi = fmaf(e, d, hi * c);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    a[i] = v[i];
+                    b[i] = v[V + i];
+                }
+                store_pack<T, V>(row + da[k], a);
+                store_pack<T, V>(row + db[k], b);
+            }
+        }
+    }
+}
+
+template <typename T, int V, int U>
+bool rope_launch_v(const RopeArgs &p, bool half, bool norm, unsigned grid)
+{
+    void (*fn)(const RopeArgs) = half ? (norm ? rope_kernel<T, V, U, true, true> : rope_kernel<T, V, U, true, false>)
+                                      : (norm ? rope_kernel<T, V, U, false, true> : rope_kernel<T, V, U, false, false>);
+    TCG_CUDA(launch_pdl(fn, dim3(grid), dim3(32 * ROPE_WARPS), 0, ctx().cur, p));
+    return true;
+}
+
+// Whether every vector of V elements of T starts at a multiple of its size:
+// the units split both the rotated part and the rest, and rows and pointers
+// are aligned.
+template <typename T>
+bool fits(const RopeArgs &p, bool half, int V)
+{
+    if (p.D % (2 * V) || (half ? p.n_rot / 2 % V || (p.D - p.n_rot) % (2 * V) : p.n_rot % (2 * V))) return false;
+    for (int s = 0; s < 2; s++) {
+        if (!p.heads[s]) continue;
+        if (((uintptr_t)p.x[s] | (uintptr_t)p.y[s]) % (V * sizeof(T)) || p.ldx[s] % V || p.ldy[s] % V) return false;
+    }
+    return true;
+}
+
+template <typename T>
+bool rope_launch(RopeArgs &p, bool half, bool norm)
+{
+    const int V = sizeof(T) == 2 && fits<T>(p, half, 8) ? 8 : fits<T>(p, half, 4) ? 4 : 1;
+    const int units = p.D / (2 * V);
+    p.lanes = 1;
+    while (p.lanes < units && p.lanes < 32) p.lanes <<= 1;
+    // A warp that takes all heads of its token computes the angles once; one
+    // token or a few are dealt out to more warps, down to one head a lane
+    // group, until there are 16 warps an SM.
+    const int side = 32 / p.lanes, all = p.heads[0] + p.heads[1], most = (all + side - 1) / side;
+    long long want = ((long long)ctx().sms * 16 + p.n_tok - 1) / p.n_tok;
+    p.splits = (int)(want < 1 ? 1 : want > most ? most : want);
+    const long long warps = (long long)p.n_tok * p.splits;
+    const long long grid = (warps + ROPE_WARPS - 1) / ROPE_WARPS;
+    if (grid > 0x7fffffffll) return fail("rope: %d tokens of %d heads are too many for one call", p.n_tok, all);
+    if constexpr (sizeof(T) == 2)
+        if (V == 8) return rope_launch_v<T, 8, 1>(p, half, norm, (unsigned)grid);
+    if (V == 4) return rope_launch_v<T, 4, 1>(p, half, norm, (unsigned)grid);
+    if (units <= 32) return rope_launch_v<T, 1, 1>(p, half, norm, (unsigned)grid);
+    return rope_launch_v<T, 1, TCG_ROPE_MAX_DIM / 64>(p, half, norm, (unsigned)grid);
+}
+
+bool rope_checks(const char *who, const tcg_rope_t *r, const int32_t *pos, int n_tok, ggml_type_t t)
+{
+    if (!lm_type_size(t)) return fail("%s: type %d is not F32, F16 or BF16", who, (int)t);
+    if (!r || r->head_dim < 2 || r->head_dim > TCG_ROPE_MAX_DIM || (r->head_dim & 1) || r->n_rot < 2 ||
+        r->n_rot > r->head_dim || (r->n_rot & 1) || (r->layout != TCG_ROPE_INTERLEAVED && r->layout != TCG_ROPE_HALF))
+        return fail("%s: the plan is not initialised (tcg_rope_init)", who);
+    if (n_tok < 0) return fail("%s: %d tokens", who, n_tok);
+    if (n_tok && !pos) return fail("%s: no positions", who);
+    return true;
+}
+
+bool rope_side(const char *who, const char *name, RopeArgs &p, int s, void *y, const void *x, const float *w, bool norm,
+               int heads, int D, int64_t ldy, int64_t ldx, ggml_type_t t)
+{
+    p.heads[s] = heads;
+    if (!heads) return true;
+    if (!y || !x || (norm && !w)) return fail("%s: no %s, its output or its weights", who, name);
+    if (((uintptr_t)y | (uintptr_t)x) % lm_type_size(t) || (uintptr_t)w % 4) return fail("%s: misaligned %s", who, name);
+    if ((ldy < (int64_t)heads * D || ldx < (int64_t)heads * D) && p.n_tok > 1)
+        return fail("%s: %s rows of %d heads of %d do not fit strides of %lld and %lld elements", who, name, heads, D,
+                    (long long)ldx, (long long)ldy);
+    p.x[s] = x;
+    p.y[s] = y;
+    p.w[s] = w;
+    p.ldx[s] = ldx;
+    p.ldy[s] = ldy;
+    return true;
+}
+
+bool rope_go(const char *who, RopeArgs &p, const tcg_rope_t *r, const int32_t *pos, ggml_type_t t, bool norm)
+{
+    if (!lm_ready(who)) return false;
+    if (p.n_tok == 0 || p.heads[0] + p.heads[1] == 0) return true;
+    p.pos = pos;
+    p.D = r->head_dim;
+    p.n_rot = r->n_rot;
+    p.mscale = r->mscale;
+    for (int i = 0; i < r->n_rot / 2; i++) p.turns[i] = r->turns[i];
+    return lm_by_type(t, [&](auto v) { return rope_launch<decltype(v)>(p, r->layout == TCG_ROPE_HALF, norm); });
+}
+
+}  // namespace
+}  // namespace tcg
+
+using namespace tcg;
+
+extern "C" bool tcg_rope(void *out, const void *x, const int32_t *pos, const tcg_rope_t *r, int n_tok, int n_head,
+                         int64_t ld_out, int64_t ld_x, ggml_type_t t)
+{
+    const char *who = "tcg_rope";
+    if (!rope_checks(who, r, pos, n_tok, t)) return false;
+    if (n_head < 0 || n_head > (1 << 20)) return fail("%s: %d heads", who, n_head);
+    RopeArgs p = {};
+    p.n_tok = n_tok;
+    if (n_tok && !rope_side(who, "x", p, 0, out, x, nullptr, false, n_head, r->head_dim, ld_out, ld_x, t)) return false;
+    return rope_go(who, p, r, pos, t, false);
+}
+
+extern "C" bool tcg_qk_norm_rope(void *q_out, void *k_out, const void *q, const void *k, const float *q_w,
+                                 const float *k_w, float eps, const int32_t *pos, const tcg_rope_t *r, int n_tok,
+                                 int n_head, int n_kv_head, int64_t ld_q_out, int64_t ld_k_out, int64_t ld_q,
+                                 int64_t ld_k, ggml_type_t t)
+{
+    const char *who = "tcg_qk_norm_rope";
+    if (!rope_checks(who, r, pos, n_tok, t)) return false;
+    if (n_head < 0 || n_kv_head < 0 || n_head > (1 << 20) || n_kv_head > (1 << 20))
+        return fail("%s: %d and %d heads", who, n_head, n_kv_head);
+    if (!(eps >= 0.0f) || eps > 1e30f) return fail("%s: eps %g", who, (double)eps);
+    RopeArgs p = {};
+    p.n_tok = n_tok;
+    p.eps = eps;
+    if (n_tok && (!rope_side(who, "q", p, 0, q_out, q, q_w, true, n_head, r->head_dim, ld_q_out, ld_q, t) ||
+                  !rope_side(who, "k", p, 1, k_out, k, k_w, true, n_kv_head, r->head_dim, ld_k_out, ld_k, t)))
+        return false;
+    return rope_go(who, p, r, pos, t, true);
+}

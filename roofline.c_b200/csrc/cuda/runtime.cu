@@ -3,6 +3,7 @@
 // over one cudaMalloc allocation).
 #include "tcg_common.cuh"
 #include "gemm.cuh"
+#include "tcg_internal.h"
 
 #include <stdarg.h>
 #include <stdio.h>
@@ -84,6 +85,15 @@ using tcg::ctx;
 extern "C" {
 
 const char *tcg_last_error(void) { return tcg::g_err; }
+
+bool host_fail(const char *fmt, ...)
+{
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(tcg::g_err, sizeof tcg::g_err, fmt, ap);
+    va_end(ap);
+    return false;
+}
 const char *tcg_version(void) { return "libtcg 0.1 (sm_100a)"; }
 
 bool tcg_init(int device)

@@ -9,6 +9,9 @@
 extern "C" {
 #endif
 
+/* Sets tcg_last_error() from the C host layer; returns false. */
+bool host_fail(const char *fmt, ...) __attribute__((format(printf, 1, 2)));
+
 /* tc_dequant's device path: host src -> device, convert, -> host dst. */
 bool tcg_dequant_host(float *dst, const void *src, size_t n, ggml_type_t t);
 

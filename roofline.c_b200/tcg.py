@@ -16,12 +16,12 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libtcg.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
-F32, F16, Q4_K, Q6_K = 0, 1, 12, 14
+F32, F16, Q4_K, Q6_K, BF16 = 0, 1, 12, 14, 30
 QK_K = 256
 BLOCK_BYTES = {F32: 4, F16: 2, Q4_K: 144, Q6_K: 210}
 BLOCK_ELEMS = {F32: 1, F16: 1, Q4_K: 256, Q6_K: 256}
 
-vp, sz, i32, f32, boolean = C.c_void_p, C.c_size_t, C.c_int, C.c_float, C.c_bool
+vp, sz, i32, i64, f32, boolean = C.c_void_p, C.c_size_t, C.c_int, C.c_int64, C.c_float, C.c_bool
 TAP_FN = C.CFUNCTYPE(None, C.c_void_p, C.c_char_p, C.POINTER(C.c_float), C.c_int, C.c_int)
 
 
@@ -89,6 +89,26 @@ class Roofline(C.Structure):          # include/tcg.h tc_roofline_t
     _fields_ = [(n, C.c_double) for n in ("weight_bytes", "hbm_gbs", "tensor_tflops", "flops_per_unit",
                                           "mem_units_per_s", "compute_units_per_s", "ridge_batch")] + \
                [("encoder", C.c_bool)]
+
+
+ROPE_INTERLEAVED, ROPE_HALF, ROPE_MAX_DIM = 0, 1, 256
+KV8_PAGE = 64
+ERR_KV8_LENGTHS, ERR_KV8_PAGE = 64, 65
+
+
+class Rope(C.Structure):              # include/tcg.h tcg_rope_t
+    _fields_ = [(n, C.c_int) for n in ("head_dim", "n_rot", "layout")] + \
+               [("mscale", C.c_float), ("base", C.c_double), ("turns", C.c_double * (ROPE_MAX_DIM // 2))]
+
+
+class Kv8(C.Structure):               # include/tcg.h tcg_kv8_t
+    _fields_ = [(n, vp) for n in ("k", "v", "k_scale", "v_scale")] + \
+               [(n, C.c_int) for n in ("n_pages", "n_kv_head", "head_dim")]
+
+
+class Kv8Step(C.Structure):           # include/tcg.h tcg_kv8_step_t
+    _fields_ = [(n, vp) for n in ("tok_start", "kv_len", "table")] + \
+               [(n, C.c_int) for n in ("table_ld", "n_seq", "n_tok", "max_new", "max_kv")]
 
 
 # (name, restype, argtypes) of every entry point the binding uses
@@ -187,6 +207,20 @@ _SIGS = [
     ("tcg_preprocess_rgb8", boolean, [vp, vp, i32, i32, i32, i32, C.POINTER(C.c_float), C.POINTER(C.c_float), i32]),
     ("tcg_vit_preprocess", boolean, [C.POINTER(Vit), vp, vp, i32, i32, i32]),
     ("tc_roofline_b200", boolean, [C.POINTER(Gguf), C.c_double, C.c_double, C.POINTER(Roofline)]),
+    # language-model operators
+    ("tcg_rope_init", boolean, [C.POINTER(Rope), i32, i32, i32, C.c_double]),
+    ("tcg_rope_scale_linear", boolean, [C.POINTER(Rope), C.c_double]),
+    ("tcg_rope_scale_yarn", boolean, [C.POINTER(Rope), C.c_double, i32, C.c_double, C.c_double, C.c_double]),
+    ("tcg_rope_scale_bands", boolean, [C.POINTER(Rope), C.c_double, i32, C.c_double, C.c_double]),
+    ("tcg_rope_scale_factors", boolean, [C.POINTER(Rope), vp, i32]),
+    ("tcg_rope_from_gguf", boolean, [C.POINTER(Rope), C.POINTER(Gguf), i32]),
+    ("tcg_rope", boolean, [vp, vp, vp, C.POINTER(Rope), i32, i32, i64, i64, C.c_int]),
+    ("tcg_qk_norm_rope", boolean, [vp, vp, vp, vp, vp, vp, f32, vp, C.POINTER(Rope), i32, i32, i32,
+                                   i64, i64, i64, i64, C.c_int]),
+    ("tcg_kv8_append", boolean, [C.POINTER(Kv8), C.POINTER(Kv8Step), vp, vp, i64, i64, C.c_int]),
+    ("tcg_kv8_read", boolean, [vp, vp, C.POINTER(Kv8), C.POINTER(Kv8Step), i64, i64, C.c_int]),
+    ("tcg_kv8_attention", boolean, [vp, vp, C.POINTER(Kv8), C.POINTER(Kv8Step), i32, i64, i64, f32, boolean, i32,
+                                    C.c_int]),
     ("tcg_nccl_unique_id", boolean, [C.c_char_p]),
     ("tcg_vit_upload_bcast", vp, [C.POINTER(Vit), i32, i32, i32, C.c_char_p]),
 ]
