@@ -34,6 +34,8 @@
 #include "tc05.cuh"
 
 #include <math.h>
+#include <stdio.h>
+#include <stdlib.h>
 
 namespace tcg {
 namespace {
@@ -57,13 +59,13 @@ struct AttnArgs {
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_u8s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -173,12 +175,12 @@ __device__ __forceinline__ void store_out(const AttnArgs &p, long long off, cons
 // gets zeros; a NaN sum (a query with a NaN or an infinity) stays NaN.
 __device__ __forceinline__ float inverse(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
 
-template <int KS, int WM, int WN, int NSLOT>
+template <int KS, int RW, int WM, int WN, int NSLOT>
 struct Shape {
     static constexpr int DP = KS * 32;                       // dims, padded
     static constexpr int SLOT = PAGE * DP;                   // bytes of a K or V tile
     static constexpr int RING = WN * NSLOT * SLOT;
-    static constexpr int ROWS = 16 * WM;
+    static constexpr int ROWS = 8 * RW * WM;
     static constexpr int PITCH = DP + 8;                     // floats of a partial O row
     static constexpr int EXCH = (WN * ROWS * (PITCH + 2) + 18 * ROWS) * 4;   // partial O, m, l; weights of <= 16 CTAs, sum
     static constexpr int BODY = RING > EXCH ? RING : EXCH;
@@ -186,11 +188,11 @@ struct Shape {
     static constexpr size_t SMEM = 128 + BODY + WN * NSLOT * 12 + 16;
 };
 
-template <int KS, int NP, int WM, int WN, int NSLOT, int MINB>
+template <int KS, int NP, int RW, int WM, int WN, int NSLOT, int MINB>
 __global__ void __launch_bounds__(32 * WM * WN, MINB)
 kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUtensorMap kmap)
 {
-    using Sh = Shape<KS, WM, WN, NSLOT>;
+    using Sh = Shape<KS, RW, WM, WN, NSLOT>;
     constexpr int NT = KS * 4;                               // 8-dim output tiles
     extern __shared__ uint8_t raw[];
     uint8_t *const base = (uint8_t *)(((uintptr_t)raw + 127) & ~(uintptr_t)127);
@@ -225,17 +227,18 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
     int t0;                                                  // this warp group's tiles: t0, t0 + WN, ...
     const int mine = kv8_tiles(&seq, r0 / p.G, (min(r0 + Sh::ROWS, R) - 1) / p.G, p.causal, p.window, rank, p.S, wn, WN, &t0);
 
-    // This thread's two rows.
-    int hi[2], lo[2];
-    long long row_off[2];
+    // This thread's rows.
+    constexpr int RPW = 8 * RW;                              // rows of a warp
+    int hi[RW], lo[RW];
+    long long row_off[RW];
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int r = min(r0 + 16 * wm + g + 8 * i, R - 1), tok = r / p.G;
+    for (int i = 0; i < RW; i++) {
+        const int r = min(r0 + RPW * wm + g + 8 * i, R - 1), tok = r / p.G;
         hi[i] = hi_of(tok);
         lo[i] = lo_of(tok);
         row_off[i] = (long long)(head * p.G + r % p.G) * p.D;
     }
-    const int row_a = min(r0 + 16 * wm, R - 1) / p.G, row_z = min(r0 + 16 * wm + 15, R - 1) / p.G;
+    const int row_a = min(r0 + RPW * wm, R - 1) / p.G, row_z = min(r0 + RPW * wm + RPW - 1, R - 1) / p.G;
     const int all_hi = hi_of(row_a), all_lo = lo_of(row_z);  // keys that every row of the warp sees
     const int any_hi = hi_of(row_z), any_lo = lo_of(row_a);  // keys that some row of the warp sees
 
@@ -281,13 +284,16 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
     scales();
 
     // Q digits, in the k order of the tiles: k-step 2 c + s of chunk c takes bytes 64 c + 16 t + 8 s + 0..7.
-    uint32_t qd[NP][KS][4];
-    float qs[2];
+    // RW = 2: qd[n] is digit n's A fragment. RW = 1: the first fragment holds the two upper digits, as rows g and g + 8;
+    // with three digits a second one holds the lowest as row g + 8.
+    constexpr int NA = RW == 2 ? NP : NP - 1;                // A fragments, mma's per product
+    uint32_t qd[NA][KS][4] = {};
+    float qs[RW];
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
+    for (int i = 0; i < RW; i++) {
         float x[KS / 2][16], m = 0.0f;
         bool odd = false;                                    // a NaN or an infinity
-        const int r = min(r0 + 16 * wm + g + 8 * i, R - 1);
+        const int r = min(r0 + RPW * wm + g + 8 * i, R - 1);
         const long long off = (seq.row0 + r / p.G) * p.ld_q + row_off[i];
 #pragma unroll
         for (int c = 0; c < KS / 2; c++) {
@@ -322,21 +328,27 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
                         v = (v - dig) >> 8;
                     }
                 }
+                if (RW == 2) {
 #pragma unroll
-                for (int n = 0; n < NP; n++) qd[n][2 * c + (w >> 1)][2 * (w & 1) + i] = d[n];
+                    for (int n = 0; n < NP; n++) qd[n % NA][2 * c + (w >> 1)][2 * (w & 1) + i] = d[n];
+                } else {
+                    qd[0][2 * c + (w >> 1)][2 * (w & 1)] = d[NP - 1];
+                    qd[0][2 * c + (w >> 1)][2 * (w & 1) + 1] = d[NP - 2];
+                    if (NP == 3) qd[NA - 1][2 * c + (w >> 1)][2 * (w & 1) + 1] = d[0];
+                }
             }
     }
 
-    float o[NT][4], m[2], l[2];
+    float o[NT][2 * RW], m[RW], l[RW];
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
+    for (int i = 0; i < RW; i++) {
         m[i] = -INFINITY;
         l[i] = 0.0f;
     }
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) o[n][e] = 0.0f;
+        for (int e = 0; e < 2 * RW; e++) o[n][e] = 0.0f;
 
     int slot = 0, parity = 0;
     bool ok = true;
@@ -380,55 +392,72 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
 
         ok = landed();
         if (!ok) break;
-        float f[8][4];
+        float f[8][2 * RW];
         if (real) {
             const uint32_t kt = my_ring + slot * Sh::SLOT + (16 * (g >> 1) + (g & 1)) * 64 + 16 * t;
+            constexpr int B = 4;                             // score tiles side by side: independent mma chains
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                uint4 w[KS / 2];
+            for (int j0 = 0; j0 < 8; j0 += B) {
+                uint4 w[KS / 2][B];
+                int a[B][4] = {}, top[B][4] = {};
 #pragma unroll
-                for (int c = 0; c < KS / 2; c++) w[c] = lds128(kt + c * 4096 + j * 128);
-                int a[4] = {}, top[4] = {};
-                if (NP == 3) {
+                for (int c = 0; c < KS / 2; c++)
+#pragma unroll
+                    for (int j = 0; j < B; j++) w[c][j] = lds128(kt + c * 4096 + (j0 + j) * 128);
+                auto dims = [&](int (&d)[B][4], const uint32_t (&q)[KS][4]) {
 #pragma unroll
                     for (int c = 0; c < KS / 2; c++) {
-                        mma_s8(top, qd[NP - 1][2 * c], w[c].x, w[c].y);
-                        mma_s8(top, qd[NP - 1][2 * c + 1], w[c].z, w[c].w);
+#pragma unroll
+                        for (int j = 0; j < B; j++) mma_s8(d[j], q[2 * c], w[c][j].x, w[c][j].y);
+#pragma unroll
+                        for (int j = 0; j < B; j++) mma_s8(d[j], q[2 * c + 1], w[c][j].z, w[c][j].w);
                     }
+                };
+                if constexpr (RW == 2) {
+                    dims(a, qd[1]);
+                    if (NP == 3) dims(top, qd[NA - 1]);
+#pragma unroll
+                    for (int j = 0; j < B; j++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) a[j][e] <<= 8;   // |a| < 2^21 (128 dims): below 2^30 with the next digit
+                    dims(a, qd[0]);
+#pragma unroll
+                    for (int j = 0; j < B; j++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            f[j0 + j][e] = NP == 3 ? fmaf((float)top[j][e], 65536.0f, (float)a[j][e]) : (float)a[j][e];
+                } else {
+                    dims(a, qd[0]);
+                    if (NP == 3) {
+#pragma unroll
+                        for (int j = 0; j < B; j++) a[j][2] <<= 8, a[j][3] <<= 8;
+                        dims(a, qd[NA - 1]);                 // its rows 0..7 are zero
+                    }
+#pragma unroll
+                    for (int j = 0; j < B; j++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++)
+                            f[j0 + j][e] = NP == 3 ? fmaf((float)a[j][e], 65536.0f, (float)a[j][2 + e])
+                                                   : (float)(a[j][e] * 256 + a[j][2 + e]);
                 }
-#pragma unroll
-                for (int c = 0; c < KS / 2; c++) {
-                    mma_s8(a, qd[1][2 * c], w[c].x, w[c].y);
-                    mma_s8(a, qd[1][2 * c + 1], w[c].z, w[c].w);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; e++) a[e] <<= 8;      // |a| < 2^21 (128 dims), so below 2^30 with the next digit
-#pragma unroll
-                for (int c = 0; c < KS / 2; c++) {
-                    mma_s8(a, qd[0][2 * c], w[c].x, w[c].y);
-                    mma_s8(a, qd[0][2 * c + 1], w[c].z, w[c].w);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    f[j][e] = NP == 3 ? fmaf((float)top[e], 65536.0f, (float)a[e]) : (float)a[e];
             }
         }
         release(2 * i);
 
-        uint32_t pd[NP][2][4];
+        uint32_t pd[NA][2][4] = {};
         if (real) {
             if (key0 < all_lo || key0 + PAGE - 1 > all_hi) {
 #pragma unroll
                 for (int j = 0; j < 8; j++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
+                    for (int e = 0; e < 2 * RW; e++) {
                         const int key = key0 + 16 * t + 2 * j + (e & 1);
                         if (key > hi[e >> 1] || key < lo[e >> 1]) f[j][e] = -INFINITY;
                     }
             }
             bool grew = false;
 #pragma unroll
-            for (int r = 0; r < 2; r++) {
+            for (int r = 0; r < RW; r++) {
                 float top = -INFINITY;
 #pragma unroll
                 for (int j = 0; j < 8; j++) top = fmaxf(top, fmaxf(f[j][2 * r], f[j][2 * r + 1]));
@@ -468,11 +497,18 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
                     const uint32_t y0 = __float_as_uint(f[2 * w][2 * r]), y1 = __float_as_uint(f[2 * w][2 * r + 1]);
                     const uint32_t y2 = __float_as_uint(f[2 * w + 1][2 * r]), y3 = __float_as_uint(f[2 * w + 1][2 * r + 1]);
                     const uint32_t u = __byte_perm(y0, y1, 0x5140), v = __byte_perm(y2, y3, 0x5140);
-                    pd[0][w >> 1][2 * (w & 1) + r] = __byte_perm(u, v, 0x5410);
-                    pd[1][w >> 1][2 * (w & 1) + r] = __byte_perm(u, v, 0x7632);
-                    if (NP == 3)
-                        pd[NP - 1][w >> 1][2 * (w & 1) + r] =
-                            __byte_perm(__byte_perm(y0, y1, 0x0062), __byte_perm(y2, y3, 0x0062), 0x5410);
+                    const uint32_t d0 = __byte_perm(u, v, 0x5410), d1 = __byte_perm(u, v, 0x7632);
+                    const uint32_t d2 = __byte_perm(__byte_perm(y0, y1, 0x0062), __byte_perm(y2, y3, 0x0062), 0x5410);
+                    uint32_t (&first)[4] = pd[0][w >> 1], (&last)[4] = pd[NA - 1][w >> 1];
+                    if constexpr (RW == 2) {
+                        pd[1][w >> 1][2 * (w & 1) + r] = d1;
+                        if (NP == 3) last[2 * (w & 1) + r] = d2;
+                        first[2 * (w & 1) + r] = d0;
+                    } else {
+                        first[2 * (w & 1)] = NP == 3 ? d2 : d1;
+                        first[2 * (w & 1) + 1] = NP == 3 ? d1 : d0;
+                        if (NP == 3) last[2 * (w & 1) + 1] = d0;
+                    }
                 }
             }
         }
@@ -482,30 +518,54 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
         if (real) {
             const uint32_t vt = my_ring + slot * Sh::SLOT + g * 64 + 16 * t;
             const float fs = tv * (NP == 3 ? 1.0f / 8388607.0f : 1.0f / 65535.0f);
+            constexpr int B = 4;                             // output tiles side by side
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-                const uint4 w = lds128(vt + n * 512);
-                int a[4] = {}, top[4] = {};
-                if (NP == 3) {
-                    mma_u8s8(top, pd[NP - 1][0], w.x, w.y);
-                    mma_u8s8(top, pd[NP - 1][1], w.z, w.w);
+            for (int n0 = 0; n0 < NT; n0 += B) {
+                uint4 w[B];
+                int a[B][4] = {}, top[B][4] = {};
+#pragma unroll
+                for (int n = 0; n < B; n++) w[n] = lds128(vt + (n0 + n) * 512);
+                auto keys = [&](int (&d)[B][4], const uint32_t (&q)[2][4]) {
+#pragma unroll
+                    for (int n = 0; n < B; n++) mma_u8s8(d[n], q[0], w[n].x, w[n].y);
+#pragma unroll
+                    for (int n = 0; n < B; n++) mma_u8s8(d[n], q[1], w[n].z, w[n].w);
+                };
+                if constexpr (RW == 2) {
+                    keys(a, pd[1]);
+                    if (NP == 3) keys(top, pd[NA - 1]);
+#pragma unroll
+                    for (int n = 0; n < B; n++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) a[n][e] <<= 8;   // |a| <= 255 * 128 * 64 < 2^21
+                    keys(a, pd[0]);
+#pragma unroll
+                    for (int n = 0; n < B; n++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            o[n0 + n][e] = fmaf(NP == 3 ? fmaf((float)top[n][e], 65536.0f, (float)a[n][e]) : (float)a[n][e],
+                                                fs, o[n0 + n][e]);
+                } else {
+                    keys(a, pd[0]);
+                    if (NP == 3) {
+#pragma unroll
+                        for (int n = 0; n < B; n++) a[n][2] <<= 8, a[n][3] <<= 8;
+                        keys(a, pd[NA - 1]);
+                    }
+#pragma unroll
+                    for (int n = 0; n < B; n++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++)
+                            o[n0 + n][e] = fmaf(NP == 3 ? fmaf((float)a[n][e], 65536.0f, (float)a[n][2 + e])
+                                                        : (float)(a[n][e] * 256 + a[n][2 + e]), fs, o[n0 + n][e]);
                 }
-                mma_u8s8(a, pd[1][0], w.x, w.y);
-                mma_u8s8(a, pd[1][1], w.z, w.w);
-#pragma unroll
-                for (int e = 0; e < 4; e++) a[e] <<= 8;      // |a| <= 255 * 128 * 64 < 2^21
-                mma_u8s8(a, pd[0][0], w.x, w.y);
-                mma_u8s8(a, pd[0][1], w.z, w.w);
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    o[n][e] = fmaf(NP == 3 ? fmaf((float)top[e], 65536.0f, (float)a[e]) : (float)a[e], fs, o[n][e]);
             }
         }
         release(2 * i + 1);
     }
 
 #pragma unroll
-    for (int r = 0; r < 2; r++) {
+    for (int r = 0; r < RW; r++) {
         l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 1);
         l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 2);
     }
@@ -517,8 +577,8 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
     }
     if (WN == 1 && p.S == 1) {
 #pragma unroll
-        for (int r = 0; r < 2; r++) {
-            const int row = r0 + 16 * wm + g + 8 * r;
+        for (int r = 0; r < RW; r++) {
+            const int row = r0 + RPW * wm + g + 8 * r;
             if (row >= R) continue;
             const float inv = inverse(l[r]);
             const long long off = (seq.row0 + row / p.G) * p.ld_out + row_off[r];
@@ -541,8 +601,8 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
     float *const ps = pw + 16 * Sh::ROWS;                    // [ROWS] 1 / sum
     const int rows = min(Sh::ROWS, R - r0), d4 = p.D / 4;
 #pragma unroll
-    for (int r = 0; r < 2; r++) {
-        const int at = wn * Sh::ROWS + 16 * wm + g + 8 * r;
+    for (int r = 0; r < RW; r++) {
+        const int at = wn * Sh::ROWS + RPW * wm + g + 8 * r;
 #pragma unroll
         for (int n = 0; n < NT; n++)
             *(float2 *)(po + at * Sh::PITCH + 8 * n + 2 * t) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
@@ -629,15 +689,16 @@ EncodeFn attn_encode_fn()
     return fn;
 }
 
-template <int KS, int NP, int WM, int WN, int NSLOT, int MINB>
+template <int KS, int NP, int RW, int WM, int WN, int NSLOT, int MINB>
 bool attn_launch(AttnArgs &p, const CUtensorMap &map, int ntile, int n_seq)
 {
-    using Sh = Shape<KS, WM, WN, NSLOT>;
-    auto fn = kv8_attn_kernel<KS, NP, WM, WN, NSLOT, MINB>;
+    using Sh = Shape<KS, RW, WM, WN, NSLOT>;
+    auto fn = kv8_attn_kernel<KS, NP, RW, WM, WN, NSLOT, MINB>;
     static bool ready[64];
     const int dev = ctx().device & 63;
     if (!ready[dev]) {
         TCG_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::SMEM));
+        TCG_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         ready[dev] = true;
     }
     cudaLaunchAttribute attrs[2];
@@ -655,6 +716,7 @@ bool attn_launch(AttnArgs &p, const CUtensorMap &map, int ntile, int n_seq)
         attrs[lc.numAttrs].val.clusterDim.z = 1;
         lc.numAttrs++;
     }
+    if (getenv("OCC")) { int nc = -1; cudaOccupancyMaxActiveClusters(&nc, fn, &lc); printf("S %d clusters %d\n", p.S, nc); }
     TCG_CUDA(cudaLaunchKernelEx(&lc, fn, p, map));
     return true;
 }
@@ -715,19 +777,25 @@ extern "C" bool tcg_kv8_attention(void *out, const void *q, const tcg_kv8_t *c, 
     // more rows share their tiles between 4 warps of 16 rows. Keys are split over a cluster while that
     // fills more SMs and leaves every warp group a tile.
     const bool few = R <= 16;
-    const int rows = few ? 16 : 64, groups = few ? 8 : 1;
+    const int rows = R <= 8 ? 8 : few ? 16 : 64, groups = few ? 8 : 1;
     const long long ntile = (R + rows - 1) / rows, ctas = ntile * p.n_kv * s->n_seq;
     p.S = 1;
     while (p.S < 8 && ctas * p.S * 2 <= 2 * ctx().sms && tiles >= 2 * p.S * groups) p.S *= 2;
     const bool wide_q = t == GGML_TYPE_F32, big = p.D > 64;
-    if (few) {
-        if (big) return wide_q ? attn_launch<4, 3, 1, 8, 3, 1>(p, map, (int)ntile, s->n_seq)
-                               : attn_launch<4, 2, 1, 8, 3, 1>(p, map, (int)ntile, s->n_seq);
-        return wide_q ? attn_launch<2, 3, 1, 8, 6, 1>(p, map, (int)ntile, s->n_seq)
-                      : attn_launch<2, 2, 1, 8, 6, 1>(p, map, (int)ntile, s->n_seq);
+    if (rows == 8) {
+        if (big) return wide_q ? attn_launch<4, 3, 1, 1, 8, 3, 1>(p, map, (int)ntile, s->n_seq)
+                               : attn_launch<4, 2, 1, 1, 8, 3, 1>(p, map, (int)ntile, s->n_seq);
+        return wide_q ? attn_launch<2, 3, 1, 1, 8, 6, 1>(p, map, (int)ntile, s->n_seq)
+                      : attn_launch<2, 2, 1, 1, 8, 6, 1>(p, map, (int)ntile, s->n_seq);
     }
-    if (big) return wide_q ? attn_launch<4, 3, 4, 1, 6, 2>(p, map, (int)ntile, s->n_seq)
-                           : attn_launch<4, 2, 4, 1, 6, 2>(p, map, (int)ntile, s->n_seq);
-    return wide_q ? attn_launch<2, 3, 4, 1, 8, 2>(p, map, (int)ntile, s->n_seq)
-                  : attn_launch<2, 2, 4, 1, 8, 2>(p, map, (int)ntile, s->n_seq);
+    if (few) {
+        if (big) return wide_q ? attn_launch<4, 3, 2, 1, 8, 3, 1>(p, map, (int)ntile, s->n_seq)
+                               : attn_launch<4, 2, 2, 1, 8, 3, 1>(p, map, (int)ntile, s->n_seq);
+        return wide_q ? attn_launch<2, 3, 2, 1, 8, 6, 1>(p, map, (int)ntile, s->n_seq)
+                      : attn_launch<2, 2, 2, 1, 8, 6, 1>(p, map, (int)ntile, s->n_seq);
+    }
+    if (big) return wide_q ? attn_launch<4, 3, 2, 4, 1, 6, 2>(p, map, (int)ntile, s->n_seq)
+                           : attn_launch<4, 2, 2, 4, 1, 6, 2>(p, map, (int)ntile, s->n_seq);
+    return wide_q ? attn_launch<2, 3, 2, 4, 1, 8, 2>(p, map, (int)ntile, s->n_seq)
+                  : attn_launch<2, 2, 2, 4, 1, 8, 2>(p, map, (int)ntile, s->n_seq);
 }
