@@ -34,8 +34,8 @@
 #include "tc05.cuh"
 
 #include <math.h>
-#include <stdio.h>
-#include <stdlib.h>
+
+#include <type_traits>
 
 namespace tcg {
 namespace {
@@ -689,25 +689,61 @@ EncodeFn attn_encode_fn()
     return fn;
 }
 
+constexpr int MAX_SPLIT = 10;            // CTAs of a cluster; of 11 or more a B200 holds 7 clusters at a time
+
+// The grid of one call: `ctas` blocks of rows, at most `tiles` tiles of keys each.
+struct Work {
+    long long ntile, ctas, tiles;
+    int n_seq;
+};
+
 template <int KS, int NP, int RW, int WM, int WN, int NSLOT, int MINB>
-bool attn_launch(AttnArgs &p, const CUtensorMap &map, int ntile, int n_seq)
+bool attn_launch(AttnArgs &p, const CUtensorMap &map, long long R, Work w)
 {
     using Sh = Shape<KS, RW, WM, WN, NSLOT>;
     auto fn = kv8_attn_kernel<KS, NP, RW, WM, WN, NSLOT, MINB>;
-    static bool ready[64];
-    const int dev = ctx().device & 63;
-    if (!ready[dev]) {
-        TCG_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::SMEM));
-        TCG_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-        ready[dev] = true;
-    }
+    w.ntile = (R + Sh::ROWS - 1) / Sh::ROWS;
+    w.ctas = w.ntile * p.n_kv * w.n_seq;
     cudaLaunchAttribute attrs[2];
     cudaLaunchConfig_t lc = {};
-    lc.gridDim = dim3((unsigned)(ntile * p.S), (unsigned)p.n_kv, (unsigned)n_seq);
+    lc.gridDim = dim3((unsigned)w.ntile, (unsigned)p.n_kv, (unsigned)w.n_seq);
     lc.blockDim = dim3(32 * WM * WN);
     lc.dynamicSmemBytes = Sh::SMEM;
     lc.stream = ctx().cur;
     lc.attrs = attrs;
+
+    // CTAs the device holds at once, by cluster size (a property of the kernel and the device).
+    static int held[64][MAX_SPLIT + 1];
+    int *const cap = held[ctx().device & 63];
+    if (!cap[1]) {
+        TCG_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::SMEM));
+        TCG_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        attrs[0].id = cudaLaunchAttributeClusterDimension;
+        attrs[0].val.clusterDim.y = attrs[0].val.clusterDim.z = 1;
+        cudaLaunchConfig_t one = lc;
+        one.numAttrs = 1;
+        for (int S = MAX_SPLIT; S > 1; S--) {
+            int n = 0;
+            one.gridDim = dim3((unsigned)S);
+            attrs[0].val.clusterDim.x = (unsigned)S;
+            if (cudaOccupancyMaxActiveClusters(&n, fn, &one) != cudaSuccess) {
+                cudaGetLastError();
+                n = 0;
+            }
+            cap[S] = n * S;
+        }
+        cap[1] = MINB * ctx().sms;
+    }
+    // Keys split over a cluster of S CTAs: the S with the least rounds in a row, where a wave of CTAs lasts its rounds of
+    // tiles and about two more (start, merge).
+    p.S = 1;
+    long long best = 0;
+    for (int S = 1; S <= MAX_SPLIT; S++) {
+        if (!cap[S] || (S > 1 && w.tiles < (long long)S * WN)) continue;
+        const long long rounds = ((w.tiles + S - 1) / S + WN - 1) / WN, t = (w.ctas * S + cap[S] - 1) / cap[S] * (rounds + 2);
+        if (S == 1 || t < best) best = t, p.S = S;
+    }
+    lc.gridDim.x = (unsigned)(w.ntile * p.S);
     lc.numAttrs = pdl_attr(attrs);
     if (p.S > 1) {
         attrs[lc.numAttrs].id = cudaLaunchAttributeClusterDimension;
@@ -716,7 +752,6 @@ bool attn_launch(AttnArgs &p, const CUtensorMap &map, int ntile, int n_seq)
         attrs[lc.numAttrs].val.clusterDim.z = 1;
         lc.numAttrs++;
     }
-    if (getenv("OCC")) { int nc = -1; cudaOccupancyMaxActiveClusters(&nc, fn, &lc); printf("S %d clusters %d\n", p.S, nc); }
     TCG_CUDA(cudaLaunchKernelEx(&lc, fn, p, map));
     return true;
 }
@@ -772,30 +807,15 @@ extern "C" bool tcg_kv8_attention(void *out, const void *q, const tcg_kv8_t *c, 
 
     long long keys = s->max_kv;
     if (window && keys > (long long)window + longest) keys = (long long)window + longest;
-    const long long tiles = (keys + PAGE - 1) / PAGE;
-    // Up to 16 rows (a decode step) one warp's rows hold them all and the 8 warps of a CTA take alternate tiles;
-    // more rows share their tiles between 4 warps of 16 rows. Keys are split over a cluster while that
-    // fills more SMs and leaves every warp group a tile.
-    const bool few = R <= 16;
-    const int rows = R <= 8 ? 8 : few ? 16 : 64, groups = few ? 8 : 1;
-    const long long ntile = (R + rows - 1) / rows, ctas = ntile * p.n_kv * s->n_seq;
-    p.S = 1;
-    while (p.S < 8 && ctas * p.S * 2 <= 2 * ctx().sms && tiles >= 2 * p.S * groups) p.S *= 2;
-    const bool wide_q = t == GGML_TYPE_F32, big = p.D > 64;
-    if (rows == 8) {
-        if (big) return wide_q ? attn_launch<4, 3, 1, 1, 8, 3, 1>(p, map, (int)ntile, s->n_seq)
-                               : attn_launch<4, 2, 1, 1, 8, 3, 1>(p, map, (int)ntile, s->n_seq);
-        return wide_q ? attn_launch<2, 3, 1, 1, 8, 6, 1>(p, map, (int)ntile, s->n_seq)
-                      : attn_launch<2, 2, 1, 1, 8, 6, 1>(p, map, (int)ntile, s->n_seq);
-    }
-    if (few) {
-        if (big) return wide_q ? attn_launch<4, 3, 2, 1, 8, 3, 1>(p, map, (int)ntile, s->n_seq)
-                               : attn_launch<4, 2, 2, 1, 8, 3, 1>(p, map, (int)ntile, s->n_seq);
-        return wide_q ? attn_launch<2, 3, 2, 1, 8, 6, 1>(p, map, (int)ntile, s->n_seq)
-                      : attn_launch<2, 2, 2, 1, 8, 6, 1>(p, map, (int)ntile, s->n_seq);
-    }
-    if (big) return wide_q ? attn_launch<4, 3, 2, 4, 1, 6, 2>(p, map, (int)ntile, s->n_seq)
-                           : attn_launch<4, 2, 2, 4, 1, 6, 2>(p, map, (int)ntile, s->n_seq);
-    return wide_q ? attn_launch<2, 3, 2, 4, 1, 8, 2>(p, map, (int)ntile, s->n_seq)
-                  : attn_launch<2, 2, 2, 4, 1, 8, 2>(p, map, (int)ntile, s->n_seq);
+    const Work w = { 0, 0, (keys + PAGE - 1) / PAGE, s->n_seq };
+    // Up to 8 or 16 rows (a decode step): one or two warps of 8 rows, and the CTA's other warps take other tiles. More
+    // rows share their tiles between 4 warps of 16.
+    const bool big = p.D > 64;
+    auto go = [&](auto digits) {
+        constexpr int NP = decltype(digits)::value;
+        if (R <= 8) return big ? attn_launch<4, NP, 1, 1, 12, 2, 1>(p, map, R, w) : attn_launch<2, NP, 1, 1, 12, 4, 1>(p, map, R, w);
+        if (R <= 16) return big ? attn_launch<4, NP, 1, 2, 6, 4, 1>(p, map, R, w) : attn_launch<2, NP, 1, 2, 6, 8, 1>(p, map, R, w);
+        return big ? attn_launch<4, NP, 2, 4, 1, 6, 2>(p, map, R, w) : attn_launch<2, NP, 2, 4, 1, 8, 2>(p, map, R, w);
+    };
+    return t == GGML_TYPE_F32 ? go(std::integral_constant<int, 3>()) : go(std::integral_constant<int, 2>());
 }
