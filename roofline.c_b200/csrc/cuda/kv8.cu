@@ -8,10 +8,9 @@
 //   older codes <- rint(fl(code * fl(s / s')))    when s' > s,
 // each fl one rounding to fp32, so that the stored bytes are defined exactly.
 // One CTA owns a (page, head, K or V) and everything in it, so no two CTAs
-// write the same bytes; it reads its new rows twice, once for the largest
-// magnitude and once (from L1/L2) for the codes. Bound by memory for prompts
-// (4 or 2 bytes in, 1 out per element) and by the latency of four dependent
-// loads (lengths, page, scale, row) for a decode step.
+// write the same bytes; its new rows are read once, into registers. Bound by
+// memory for prompts (4 or 2 bytes in, 1 out per element) and by the latency
+// of dependent loads (lengths, page, scale) for a decode step.
 #include "lm.cuh"
 
 namespace tcg {
@@ -37,6 +36,7 @@ bool kv8_check(const char *who, const tcg_kv8_t *c, const tcg_kv8_step_t *s, ggm
 
 namespace {
 
+// Grid: (sequence x page that its rows touch, head, K or V).
 struct RowsArgs {
     const void *x[2];             // new K rows, new V rows (append)
     void *y[2];                   // rows to fill (read)
@@ -48,29 +48,41 @@ struct RowsArgs {
     int *err;
 };
 
-// This CTA's page: grid (sequence x page, head, K or V). False when there is
-// nothing to do; page -1 when the table names none.
-__device__ __forceinline__ bool place_of(const RowsArgs &p, kv8_place_t &at, int &page)
-{
-    const int b = blockIdx.x / p.reach, j = blockIdx.x % p.reach;
-    const bool report = threadIdx.x == 0;
-    kv8_seq_t q;
-    if (!kv_seq(p.step, b, q, p.err, report) || !kv8_place(&q, j, &at)) return false;
-    page = kv_page(p.step, b, at.index, p.n_pages, p.err, report);
-    return true;
-}
-
-__device__ __forceinline__ int8_t code_of(float x, float s)
-{
-    // x finite; the clamp is for the quotients of a subnormal scale
-    return s > 0.0f ? (int8_t)(int)fminf(fmaxf(rintf(__fdiv_rn(x, s)), -127.0f), 127.0f) : (int8_t)0;
-}
-
 // What is stored for a value: 0 for a NaN, the largest finite magnitude for an infinity.
 __device__ __forceinline__ float finite(float x)
 {
     return x == x ? fminf(fmaxf(x, -3.402823466e38f), 3.402823466e38f) : 0.0f;
 }
+
+// The format's code for x at scale s, as it is defined. The clamp is for the quotients of a subnormal scale.
+__device__ __forceinline__ int code_of(float x, float s)
+{
+    return s > 0.0f ? (int)fminf(fmaxf(rintf(__fdiv_rn(finite(x), s)), -127.0f), 127.0f) : 0;
+}
+
+// The same for N values of magnitude at most 127 s, as bytes in the low bits, with one product instead of a division:
+// x * fl(1 / s) is within 127 * 2^-22 < 4e-5 of fl(x / s), so both round to the same whole number unless the product
+// lies that near to a half (one value in 10,000); then the thread takes its values again by the definition. `plain`:
+// every new value of the page is finite and s is at least 2^-100.
+template <int N>
+__device__ __forceinline__ void codes_of(const float (&x)[N], float s, float inv, bool plain, uint32_t (&c)[N])
+{
+    float off = plain ? 0.0f : 1.0f;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const float r = x[i] * inv, y = r + 12582912.0f;     // 1.5 * 2^23: the sum's low bits are rint(r)
+        off = fmaxf(off, fabsf(r - (y - 12582912.0f)));
+        c[i] = __float_as_uint(y);
+    }
+    if (off > 0.4999f) {
+#pragma unroll 1
+        for (int i = 0; i < N; i++) c[i] = (uint32_t)code_of(x[i], s);
+    }
+}
+
+// Whether codes_of may take products: m is the largest magnitude of the page's new values, odd NaN if one of them is a
+// NaN or an infinity, else 0.
+__device__ __forceinline__ bool plain_page(float odd, float s) { return odd == 0.0f && s >= 0x1p-100f; }
 
 // A code after its page's scale grew by 1 / ratio.
 __device__ __forceinline__ int moved(int code, float ratio) { return (int)rintf(__fmul_rn((float)code, ratio)); }
@@ -83,131 +95,301 @@ __device__ __forceinline__ uint32_t moved4(uint32_t w, float ratio)
     return r;
 }
 
+constexpr int ROWS_THREADS = 256;
+constexpr int QUADS = TCG_KV8_PAGE / 4;      // groups of 4 slots
+constexpr int S_PITCH = TCG_KV8_PAGE + 4;    // bytes of a dim's 64 codes in shared memory
+
+// A thread owns V dims of 4 consecutive slots, up to 8 / V times (32 values):
+// dims (thread % per) * V, quads thread / per, + `stride`, ..., per = D / V.
+// Lanes run along a row, so rows are read and written whole; the 4 slots of a
+// dim are one word of the dim-major V block.
+template <int V>
+struct Mine {
+    static constexpr int N = 8 / V;
+    int d, quad, stride;
+    bool in;
+    __device__ explicit Mine(int D)
+    {
+        const int per = D / V;
+        stride = ROWS_THREADS / per;
+        quad = threadIdx.x / per;
+        d = threadIdx.x % per * V;
+        in = quad < stride;
+    }
+};
+
 template <typename T, int V>
-__global__ void __launch_bounds__(256) append_kernel(const RowsArgs p)
+__global__ void __launch_bounds__(ROWS_THREADS) append_kernel(const RowsArgs p)
 {
-    __shared__ float s_max[8];
-    __shared__ __align__(16) uint8_t s_code[128 * 68];   // V: [dim][slot], rows of 68 bytes
+    __shared__ float s_max[ROWS_THREADS / 32], s_odd[ROWS_THREADS / 32];
+    __shared__ __align__(16) uint8_t s_code[128 * S_PITCH];
     pdl_wait();
     kv8_place_t at;
-    int page;
-    if (!place_of(p, at, page) || page < 0) return;
-    const int side = blockIdx.z, head = blockIdx.y, D = p.D, n = at.hi - at.lo, per = D / V;
-    const T *x = (const T *)p.x[side] + at.row * p.ld[side] + (long long)head * D;
-    const long long ld = p.ld[side], ph = (long long)page * p.n_kv + head;
+    kv8_seq_t q;
+    const int b = blockIdx.x / p.reach, side = blockIdx.z, head = blockIdx.y, D = p.D;
+    if (!kv_seq(p.step, b, q, p.err, threadIdx.x == 0) || !kv8_place(&q, blockIdx.x % p.reach, &at)) return;
+
+    const Mine<V> my(D);
+    const T *x = (const T *)p.x[side] + (at.row - at.lo) * p.ld[side] + (long long)head * D + my.d;
+    const long long ld = p.ld[side];
+    Pack<T, V> raw[Mine<V>::N][4];
+#pragma unroll
+    for (int k = 0; k < Mine<V>::N; k++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int slot = 4 * (my.quad + k * my.stride) + j;
+            raw[k][j] = Pack<T, V>{};
+            if (my.in && slot >= at.lo && slot < at.hi) raw[k][j] = *(const Pack<T, V> *)(x + slot * ld);
+        }
+    const int page = kv_page(p.step, b, at.index, p.n_pages, p.err, threadIdx.x == 0);
+    if (page < 0) return;
+    const long long ph = (long long)page * p.n_kv + head;
     float *const scale = p.scale[side] + ph;
     const float was = at.lo ? *scale : 0.0f;
 
-    float m = 0.0f;
-    for (int i = threadIdx.x; i < n * per; i += blockDim.x) {
-        float v[V];
-        load_pack<T, V>(x + (i / per) * ld + (i % per) * V, v);
+    float m = 0.0f, odd = 0.0f;
 #pragma unroll
-        for (int e = 0; e < V; e++) m = fmaxf(m, fabsf(finite(v[e])));
+    for (int k = 0; k < Mine<V>::N; k++)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                const float v = to_f32(raw[k][j].v[e]);
+                m = fmaxf(m, fabsf(v));                  // drops a NaN
+                odd = fmaf(v, 0.0f, odd);
+            }
+    for (int o = 16; o > 0; o >>= 1) {
+        m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+        odd += __shfl_xor_sync(0xFFFFFFFFu, odd, o);
     }
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
+    if ((threadIdx.x & 31) == 0) {
+        s_max[threadIdx.x >> 5] = m;
+        s_odd[threadIdx.x >> 5] = odd;
+    }
     __syncthreads();                                     // also: `was` is read by all before it is replaced
-    m = s_max[0];
-    for (int i = 1; i < (int)blockDim.x / 32; i++) m = fmaxf(m, s_max[i]);
+#pragma unroll
+    for (int i = 0; i < ROWS_THREADS / 32; i++) {
+        m = fmaxf(m, s_max[i]);
+        odd += s_odd[i];
+    }
+    m = finite(m);
     const float now = fmaxf(was, __fdiv_rn(m, 127.0f));
     const float ratio = now > was && now > 0.0f ? __fdiv_rn(was, now) : 1.0f;
     if (threadIdx.x == 0) *scale = now;
+    const bool plain = plain_page(odd, now);
+    const float inv = plain ? __fdiv_rn(1.0f, now) : 0.0f;
 
     int8_t *const code = p.code[side] + ph * TCG_KV8_PAGE * D;
     const bool move = ratio != 1.0f && at.lo;
     if (side == 0) {                                     // K: token-major
         if (move) {
             uint32_t *w = (uint32_t *)code;
-            for (int i = threadIdx.x; i < at.lo * D / 4; i += blockDim.x) w[i] = moved4(w[i], ratio);
+            for (int i = threadIdx.x; i < at.lo * D / 4; i += ROWS_THREADS) w[i] = moved4(w[i], ratio);
         }
-        for (int i = threadIdx.x; i < n * per; i += blockDim.x) {
-            float v[V];
-            load_pack<T, V>(x + (i / per) * ld + (i % per) * V, v);
-            Pack<int8_t, V> c;
 #pragma unroll
-            for (int e = 0; e < V; e++) c.v[e] = code_of(finite(v[e]), now);
-            *(Pack<int8_t, V> *)(code + (at.lo + i / per) * D + (i % per) * V) = c;
-        }
+        for (int k = 0; k < Mine<V>::N; k++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int slot = 4 * (my.quad + k * my.stride) + j;
+                if (!my.in || slot < at.lo || slot >= at.hi) continue;
+                float v[V];
+                uint32_t q[V];
+                Pack<int8_t, V> c;
+#pragma unroll
+                for (int e = 0; e < V; e++) v[e] = to_f32(raw[k][j].v[e]);
+                codes_of(v, now, inv, plain, q);
+#pragma unroll
+                for (int e = 0; e < V; e++) c.v[e] = (int8_t)q[e];
+                *(Pack<int8_t, V> *)(code + slot * D + my.d) = c;
+            }
         return;
     }
-    // V: dim-major. The codes go to shared memory as [dim][slot]; then the words (4 slots) that hold a new token, or
-    // an older one to move, are put together and written.
-    for (int i = threadIdx.x; i < n * per; i += blockDim.x) {
-        float v[V];
-        load_pack<T, V>(x + (i / per) * ld + (i % per) * V, v);
+    // V: dim-major. The new codes go to shared memory as [dim][slot], a word of 4 slots at a time; then the 16-byte
+    // pieces of a dim that are all new are written whole, and of the others the words that hold a new token, or an
+    // older one to move.
 #pragma unroll
-        for (int e = 0; e < V; e++)
-            s_code[((i % per) * V + e) * 68 + at.lo + i / per] =
-                (uint8_t)code_of(finite(v[e]), now);
+    for (int k = 0; k < Mine<V>::N; k++) {
+        const int quad = my.quad + k * my.stride;
+        if (!my.in || quad >= QUADS || 4 * quad + 3 < at.lo || 4 * quad >= at.hi) continue;
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+            float v[4];
+            uint32_t q[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = to_f32(raw[k][j].v[e]);
+            codes_of(v, now, inv, plain, q);
+            *(uint32_t *)(s_code + (my.d + e) * S_PITCH + 4 * quad) =
+                __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+        }
     }
     __syncthreads();
-    const int w0 = move ? 0 : at.lo / 4, w1 = (at.hi + 3) / 4, nw = w1 - w0;
-    uint32_t *const row = (uint32_t *)code;
-    for (int i = threadIdx.x; i < D * nw; i += blockDim.x) {
-        const int d = i / nw, w = w0 + i % nw;
-        uint32_t *const dst = row + d * (TCG_KV8_PAGE / 4) + w;
-        uint32_t fresh = 0;                              // bytes of the word that are new tokens
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-            if (4 * w + e >= at.lo && 4 * w + e < at.hi) fresh |= 0xFFu << (8 * e);
-        uint32_t v = 0;
-        if (fresh) v = *(const uint32_t *)(s_code + d * 68 + 4 * w) & fresh;
-        if (fresh != 0xFFFFFFFFu) {
-            const uint32_t old = *dst;
-            uint32_t keep = old;
-            if (move) {
-                const uint32_t mv = moved4(old, ratio);
-                uint32_t older = 0;
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (4 * w + e < at.lo) older |= 0xFFu << (8 * e);
-                keep = (mv & older) | (old & ~older);
-            }
-            v |= keep & ~fresh;
+    for (int i = threadIdx.x; i < D * 4; i += ROWS_THREADS) {
+        const int d = i / 4, s0 = i % 4 * 16;
+        const uint32_t *const src = (const uint32_t *)(s_code + d * S_PITCH + s0);
+        uint32_t *const dst = (uint32_t *)(code + d * TCG_KV8_PAGE + s0);
+        if (s0 >= at.lo && s0 + 16 <= at.hi) {
+            *(uint4 *)dst = make_uint4(src[0], src[1], src[2], src[3]);
+            continue;
         }
-        *dst = v;
+        for (int w = 0; w < 4; w++) {
+            const int slot = s0 + 4 * w;
+            uint32_t fresh = 0, older = 0;               // bytes that are new tokens, and older ones
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (slot + e >= at.lo && slot + e < at.hi) fresh |= 0xFFu << (8 * e);
+                if (slot + e < at.lo) older |= 0xFFu << (8 * e);
+            }
+            if (!fresh && !(move && older)) continue;
+            uint32_t v = fresh ? src[w] & fresh : 0;
+            if (fresh != 0xFFFFFFFFu) {
+                const uint32_t old = dst[w];
+                v |= (move ? (moved4(old, ratio) & older) | (old & ~older) : old) & ~fresh;
+            }
+            dst[w] = v;
+        }
+    }
+}
+
+// The same for up to FEW new tokens a sequence (a decode step): one warp per (page, head, side), a lane for 4 dims, no
+// shared memory and no barrier.
+constexpr int FEW = 4, FEW_WARPS = 4;
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(32 * FEW_WARPS) append_few_kernel(const RowsArgs p, unsigned tasks)
+{
+    const unsigned task = blockIdx.x * FEW_WARPS + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, D = p.D, d = 4 * lane;
+    pdl_wait();
+    if (task >= tasks) return;
+    const int side = task & 1, head = (task >> 1) % p.n_kv, bj = (task >> 1) / p.n_kv, b = bj / p.reach;
+    kv8_place_t at;
+    kv8_seq_t q;
+    if (!kv_seq(p.step, b, q, p.err, lane == 0) || !kv8_place(&q, bj % p.reach, &at)) return;
+    const int n = at.hi - at.lo;                         // at most FEW: a sequence has no more rows
+    const T *x = (const T *)p.x[side] + at.row * p.ld[side] + (long long)head * D + d;
+    float v[FEW][4] = {};
+#pragma unroll
+    for (int i = 0; i < FEW; i++)
+        if (i < n && d < D) {
+            if (VEC) {
+                load_pack<T, 4>(x + i * p.ld[side], v[i]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[i][e] = to_f32(x[i * p.ld[side] + e]);
+            }
+        }
+    const int page = kv_page(p.step, b, at.index, p.n_pages, p.err, lane == 0);
+    if (page < 0) return;
+    const long long ph = (long long)page * p.n_kv + head;
+    float *const scale = p.scale[side] + ph;
+    const float was = at.lo ? *scale : 0.0f;
+    float m = 0.0f, odd = 0.0f;
+#pragma unroll
+    for (int i = 0; i < FEW; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            m = fmaxf(m, fabsf(v[i][e]));
+            odd = fmaf(v[i][e], 0.0f, odd);
+        }
+    for (int o = 16; o > 0; o >>= 1) {
+        m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+        odd += __shfl_xor_sync(0xFFFFFFFFu, odd, o);
+    }
+    const float now = fmaxf(was, __fdiv_rn(finite(m), 127.0f));
+    const float ratio = now > was && now > 0.0f ? __fdiv_rn(was, now) : 1.0f;
+    if (lane == 0) *scale = now;                         // read by the whole warp before the shuffles
+    const bool plain = plain_page(odd, now);
+    const float inv = plain ? __fdiv_rn(1.0f, now) : 0.0f;
+    int8_t *const code = p.code[side] + ph * TCG_KV8_PAGE * D;
+    if (ratio != 1.0f && at.lo) {
+        // older codes; in V's words those of the slots from lo on are kept
+        uint32_t *const w = (uint32_t *)code;
+        const int words = side == 0 ? at.lo * D / 4 : D * QUADS;
+#pragma unroll 4
+        for (int i = lane; i < words; i += 32) {
+            const int over = side == 0 ? 0 : 4 * (i % QUADS) + 4 - at.lo;    // slots of the word that are not older
+            if (over >= 4) continue;
+            const uint32_t keep = over <= 0 ? 0 : 0xFFFFFFFFu << (8 * (4 - over));
+            w[i] = (moved4(w[i], ratio) & ~keep) | (w[i] & keep);
+        }
+        __syncwarp();
+    }
+    if (d >= D) return;
+#pragma unroll
+    for (int i = 0; i < FEW; i++) {
+        if (i >= n) break;
+        uint32_t c[4];
+        codes_of(v[i], now, inv, plain, c);
+        if (side == 0) {
+            *(uint32_t *)(code + (at.lo + i) * D + d) =
+                __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) code[(d + e) * TCG_KV8_PAGE + at.lo + i] = (int8_t)c[e];
+        }
     }
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(256) read_kernel(const RowsArgs p)
+__global__ void __launch_bounds__(ROWS_THREADS) read_kernel(const RowsArgs p)
 {
-    __shared__ __align__(16) uint8_t s_code[128 * 68];
+    __shared__ __align__(16) uint8_t s_code[128 * S_PITCH];
     pdl_wait();
     kv8_place_t at;
-    int page;
-    if (!place_of(p, at, page)) return;
-    const int side = blockIdx.z, head = blockIdx.y, D = p.D, n = at.hi - at.lo, per = D / V;
-    T *y = (T *)p.y[side] + at.row * p.ld[side] + (long long)head * D;
+    kv8_seq_t q;
+    const int b = blockIdx.x / p.reach, side = blockIdx.z, head = blockIdx.y, D = p.D;
+    if (!kv_seq(p.step, b, q, p.err, threadIdx.x == 0) || !kv8_place(&q, blockIdx.x % p.reach, &at)) return;
+    const int page = kv_page(p.step, b, at.index, p.n_pages, p.err, threadIdx.x == 0);
+
+    const Mine<V> my(D);
     const bool bad = page < 0;
+    T *y = (T *)p.y[side] + (at.row - at.lo) * p.ld[side] + (long long)head * D + my.d;
     const long long ld = p.ld[side], ph = (long long)(bad ? 0 : page) * p.n_kv + head;
-    const float scale = bad ? 0.0f : p.scale[side][ph];
+    const float scale = p.scale[side][ph];
     const int8_t *const code = p.code[side] + ph * TCG_KV8_PAGE * D;
+    uint32_t w[Mine<V>::N][V];                           // side V: 4 slots of a dim; side K: the bytes of 4 slots below
+    Pack<int8_t, V> c[Mine<V>::N][4];
     if (side == 1) {
-        const int w0 = at.lo / 4, nw = (at.hi + 3) / 4 - w0;
-        const uint32_t *const row = (const uint32_t *)code;
-        for (int i = threadIdx.x; i < D * nw; i += blockDim.x) {
-            const int d = i / nw, w = w0 + i % nw;
-            *(uint32_t *)(s_code + d * 68 + 4 * w) = row[d * (TCG_KV8_PAGE / 4) + w];
+        for (int i = threadIdx.x; i < D * 4; i += ROWS_THREADS) {
+            const int d = i / 4, s0 = i % 4 * 16;
+            if (s0 + 16 <= at.lo || s0 >= at.hi) continue;
+            const uint4 v = *(const uint4 *)(code + d * TCG_KV8_PAGE + s0);
+            uint32_t *const dst = (uint32_t *)(s_code + d * S_PITCH + s0);
+            dst[0] = v.x, dst[1] = v.y, dst[2] = v.z, dst[3] = v.w;
         }
         __syncthreads();
     }
-    for (int i = threadIdx.x; i < n * per; i += blockDim.x) {
-        const int r = i / per, d = (i % per) * V;
-        float v[V];
-        if (side == 0) {
-            const Pack<int8_t, V> c = *(const Pack<int8_t, V> *)(code + (at.lo + r) * D + d);
 #pragma unroll
-            for (int e = 0; e < V; e++) v[e] = (float)c.v[e];
+    for (int k = 0; k < Mine<V>::N; k++) {
+        const int quad = my.quad + k * my.stride;
+        const bool any = my.in && quad < QUADS && 4 * quad + 3 >= at.lo && 4 * quad < at.hi;
+        if (side == 1) {
+#pragma unroll
+            for (int e = 0; e < V; e++) w[k][e] = any ? *(const uint32_t *)(s_code + (my.d + e) * S_PITCH + 4 * quad) : 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int e = 0; e < V; e++) c[k][j].v[e] = (int8_t)(w[k][e] >> (8 * j));
         } else {
 #pragma unroll
-            for (int e = 0; e < V; e++) v[e] = (float)(int8_t)s_code[(d + e) * 68 + at.lo + r];
+            for (int j = 0; j < 4; j++) {
+                const int slot = 4 * quad + j;
+                c[k][j] = Pack<int8_t, V>{};
+                if (any && slot >= at.lo && slot < at.hi) c[k][j] = *(const Pack<int8_t, V> *)(code + slot * D + my.d);
+            }
         }
-#pragma unroll
-        for (int e = 0; e < V; e++) v[e] = bad ? 0.0f : v[e] * scale;
-        store_pack<T, V>(y + r * ld + d, v);
     }
+#pragma unroll
+    for (int k = 0; k < Mine<V>::N; k++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int slot = 4 * (my.quad + k * my.stride) + j;
+            if (!my.in || slot < at.lo || slot >= at.hi) continue;
+            float v[V];
+#pragma unroll
+            for (int e = 0; e < V; e++) v[e] = bad ? 0.0f : (float)c[k][j].v[e] * scale;
+            store_pack<T, V>(y + slot * ld, v);
+        }
 }
 
 bool rows_go(const char *who, const tcg_kv8_t *c, const tcg_kv8_step_t *s, const void *k, const void *v, bool append,
@@ -236,12 +418,20 @@ bool rows_go(const char *who, const tcg_kv8_t *c, const tcg_kv8_step_t *s, const
     p.err = ctx().d_err;
     const long long gx = (long long)s->n_seq * p.reach;
     if (gx > 0x7fffffffll) return fail("%s: %d sequences of up to %d tokens are too many for one call", who, s->n_seq, longest);
-    const bool vec = ((uintptr_t)k | (uintptr_t)v) % (4 * size) == 0 && ld_k % 4 == 0 && ld_v % 4 == 0;
-    const dim3 grid((unsigned)gx, (unsigned)c->n_kv_head, 2), block(longest >= 8 ? 256 : 64);
+    const dim3 grid((unsigned)gx, (unsigned)c->n_kv_head, 2), block(ROWS_THREADS);
     return lm_by_type(t, [&](auto e) {
         using T = decltype(e);
-        void (*fn)(const RowsArgs) = append ? (vec ? append_kernel<T, 4> : append_kernel<T, 1>)
-                                            : (vec ? read_kernel<T, 4> : read_kernel<T, 1>);
+        if (append && longest <= FEW && gx * c->n_kv_head * 2 <= 0x7fffffffll) {
+            const unsigned tasks = (unsigned)(gx * c->n_kv_head * 2);
+            const bool four = ((uintptr_t)k | (uintptr_t)v) % (4 * sizeof(T)) == 0 && ld_k % 4 == 0 && ld_v % 4 == 0;
+            TCG_CUDA(launch_pdl(four ? append_few_kernel<T, true> : append_few_kernel<T, false>, dim3((tasks + FEW_WARPS - 1) / FEW_WARPS),
+                                dim3(32 * FEW_WARPS), 0, ctx().cur, p, tasks));
+            return true;
+        }
+        constexpr int W = 16 / sizeof(T);                // 16-byte packs where rows and pointers allow, else single values
+        const bool vec = ((uintptr_t)k | (uintptr_t)v) % 16 == 0 && ld_k % W == 0 && ld_v % W == 0;
+        void (*fn)(const RowsArgs) = append ? (vec ? append_kernel<T, W> : append_kernel<T, 1>)
+                                            : (vec ? read_kernel<T, W> : read_kernel<T, 1>);
         TCG_CUDA(launch_pdl(fn, grid, block, 0, ctx().cur, p));
         return true;
     });

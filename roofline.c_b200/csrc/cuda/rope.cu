@@ -14,7 +14,7 @@
 // owns one "unit" of 2 V dims of a head, two vectors of V: V pairs of the
 // rotated part, or 2 V dims of the rest. It computes its V sines and cosines
 // once per token and applies them to the heads of the token one after the
-// other, up to four heads' loads in flight. 32 / L heads side by side in a
+// other, ROPE_AHEAD heads' loads in flight. 32 / L heads side by side in a
 // warp, L = the lanes a head needs.
 #include "lm.cuh"
 
@@ -52,18 +52,14 @@ __device__ __forceinline__ void unit_dims(int u, int n_rot, int &a, int &b)
 }
 
 template <typename T, int V, int U, bool HALF, bool NORM>
-__global__ void __launch_bounds__(32 * ROPE_WARPS) rope_kernel(const __grid_constant__ RopeArgs p)
+__global__ void __launch_bounds__(32 * ROPE_WARPS, 4) rope_kernel(const __grid_constant__ RopeArgs p)
 {
     const int lane = threadIdx.x & 31, L = p.lanes;
     const int sub = lane / L, l = lane % L, side = 32 / L;
-    const long long task = (long long)blockIdx.x * ROPE_WARPS + (threadIdx.x >> 5);
+    const unsigned task = blockIdx.x * ROPE_WARPS + (threadIdx.x >> 5);
     const int tok = (int)(task / p.splits), part = (int)(task % p.splits);
-    pdl_wait();
-    if (tok >= p.n_tok) return;
-    const int units = p.D / (2 * V);
-    const double at = (double)p.pos[tok];
+    const int units = p.D / (2 * V), all = p.heads[0] + p.heads[1], step = side * p.splits;
 
-    float cs[U][V], sn[U][V], w0[U][2 * V], w1[U][2 * V];
     int da[U], db[U];
     bool live[U], turn[U];
 #pragma unroll
@@ -72,63 +68,69 @@ __global__ void __launch_bounds__(32 * ROPE_WARPS) rope_kernel(const __grid_cons
         live[k] = u < units;
         unit_dims<V, HALF>(live[k] ? u : 0, p.n_rot, da[k], db[k]);
         turn[k] = live[k] && u * V < p.n_rot / 2;
+    }
+    pdl_wait();
+    if (tok >= p.n_tok) return;
+
+    // Batches of ROPE_AHEAD heads: the loads of a batch go out together, those of the first before the angles are computed.
+    Pack<T, V> xa[ROPE_AHEAD][U], xb[ROPE_AHEAD][U];
+    auto load = [&](int h0) {
+#pragma unroll
+        for (int j = 0; j < ROPE_AHEAD; j++) {
+            const int h = h0 + j * step, s = h >= p.heads[0];
+            const T *row = (const T *)p.x[s] + tok * p.ldx[s] + (long long)(h - (s ? p.heads[0] : 0)) * p.D;
+#pragma unroll
+            for (int k = 0; k < U; k++) {
+                xa[j][k] = Pack<T, V>{};
+                xb[j][k] = Pack<T, V>{};
+                if (h < all && live[k]) {
+                    xa[j][k] = *(const Pack<T, V> *)(row + da[k]);
+                    xb[j][k] = *(const Pack<T, V> *)(row + db[k]);
+                }
+            }
+        }
+    };
+    const int h_first = part * side + sub;
+    load(h_first);
+
+    const double at = (double)p.pos[tok];
+    float cs[U][V], sn[U][V];
+#pragma unroll
+    for (int k = 0; k < U; k++)
 #pragma unroll
         for (int i = 0; i < V; i++) {
             cs[k][i] = 1.0f;
             sn[k][i] = 0.0f;
             if (turn[k]) {
-                const double t = at * p.turns[u * V + i];
+                const double t = at * p.turns[(l + 32 * k) * V + i];
                 const float f = (float)(2.0 * (t - rint(t)));
                 sincospif(f, &sn[k][i], &cs[k][i]);
                 sn[k][i] *= p.mscale;
                 cs[k][i] *= p.mscale;
             }
         }
-        if (NORM && live[k]) {
-#pragma unroll
-            for (int i = 0; i < V; i++) {
-                w0[k][i] = p.heads[0] ? p.w[0][da[k] + i] : 0.0f;
-                w0[k][V + i] = p.heads[0] ? p.w[0][db[k] + i] : 0.0f;
-                w1[k][i] = p.heads[1] ? p.w[1][da[k] + i] : 0.0f;
-                w1[k][V + i] = p.heads[1] ? p.w[1][db[k] + i] : 0.0f;
-            }
-        }
-    }
 
-    const int all = p.heads[0] + p.heads[1], step = side * p.splits;
-    for (int h0 = part * side + sub; h0 - sub < all; h0 += step * ROPE_AHEAD) {   // the warp's lanes leave together
-        float x[ROPE_AHEAD][U][2 * V];
+    for (int h0 = h_first; h0 - sub < all; h0 += step * ROPE_AHEAD) {   // the warp's lanes leave together
+        if (h0 != h_first) load(h0);
 #pragma unroll
         for (int j = 0; j < ROPE_AHEAD; j++) {
             const int h = h0 + j * step;
+            if (h - sub >= all) break;                           // no lane of the warp has a head
             const int s = h >= p.heads[0];
-            const T *row = (const T *)p.x[s] + tok * p.ldx[s] + (long long)(h - (s ? p.heads[0] : 0)) * p.D;
+            float v[U][2 * V], inv = 1.0f;
 #pragma unroll
-            for (int k = 0; k < U; k++) {
-                float a[V] = {}, b[V] = {};
-                if (h < all && live[k]) {
-                    load_pack<T, V>(row + da[k], a);
-                    load_pack<T, V>(row + db[k], b);
-                }
+            for (int k = 0; k < U; k++)
 #pragma unroll
                 for (int i = 0; i < V; i++) {
-                    x[j][k][i] = a[i];
-                    x[j][k][V + i] = b[i];
+                    v[k][i] = to_f32(xa[j][k].v[i]);
+                    v[k][V + i] = to_f32(xb[j][k].v[i]);
                 }
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < ROPE_AHEAD; j++) {
-            const int h = h0 + j * step;
-            if (h0 - sub + j * step >= all) break;               // no lane of the warp has a head
-            const int s = h >= p.heads[0];
-            float inv = 1.0f;
             if (NORM) {
                 float ss = 0.0f;
 #pragma unroll
                 for (int k = 0; k < U; k++)
 #pragma unroll
-                    for (int i = 0; i < 2 * V; i++) ss = fmaf(x[j][k][i], x[j][k][i], ss);
+                    for (int i = 0; i < 2 * V; i++) ss = fmaf(v[k][i], v[k][i], ss);
                 for (int o = L >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
                 inv = rsqrtf(ss / (float)p.D + p.eps);
             }
@@ -137,13 +139,19 @@ __global__ void __launch_bounds__(32 * ROPE_WARPS) rope_kernel(const __grid_cons
 #pragma unroll
             for (int k = 0; k < U; k++) {
                 if (!live[k]) continue;
-                float v[2 * V], a[V], b[V];
+                float a[V], b[V];
+                if (NORM) {
+                    const float *w = p.w[s];
 #pragma unroll
-                for (int i = 0; i < 2 * V; i++) v[i] = NORM ? x[j][k][i] * inv * (s ? w1[k][i] : w0[k][i]) : x[j][k][i];
+                    for (int i = 0; i < V; i++) {
+                        v[k][i] = v[k][i] * inv * __ldg(w + da[k] + i);
+                        v[k][V + i] = v[k][V + i] * inv * __ldg(w + db[k] + i);
+                    }
+                }
 #pragma unroll
                 for (int i = 0; i < V; i++) {
                     // the two values of pair i: one of each vector, or neighbours
-                    float &lo = HALF ? v[i] : v[2 * i], &hi = HALF ? v[V + i] : v[2 * i + 1];
+                    float &lo = HALF ? v[k][i] : v[k][2 * i], &hi = HALF ? v[k][V + i] : v[k][2 * i + 1];
                     const float c = cs[k][i], d = sn[k][i], e = lo;
                     if (turn[k]) {
                         lo = fmaf(e, c, -(hi * d));
@@ -152,8 +160,8 @@ __global__ void __launch_bounds__(32 * ROPE_WARPS) rope_kernel(const __grid_cons
                 }
 #pragma unroll
                 for (int i = 0; i < V; i++) {
-                    a[i] = v[i];
-                    b[i] = v[V + i];
+                    a[i] = v[k][i];
+                    b[i] = v[k][V + i];
                 }
                 store_pack<T, V>(row + da[k], a);
                 store_pack<T, V>(row + db[k], b);
@@ -200,7 +208,7 @@ bool rope_launch(RopeArgs &p, bool half, bool norm)
     p.splits = (int)(want < 1 ? 1 : want > most ? most : want);
     const long long warps = (long long)p.n_tok * p.splits;
     const long long grid = (warps + ROPE_WARPS - 1) / ROPE_WARPS;
-    if (grid > 0x7fffffffll) return fail("rope: %d tokens of %d heads are too many for one call", p.n_tok, all);
+    if (warps > 0x7fffffffll) return fail("rope: %d tokens of %d heads are too many for one call", p.n_tok, all);
     if constexpr (sizeof(T) == 2)
         if (V == 8) return rope_launch_v<T, 8, 1>(p, half, norm, (unsigned)grid);
     if (V == 4) return rope_launch_v<T, 4, 1>(p, half, norm, (unsigned)grid);
