@@ -70,19 +70,22 @@ __device__ __forceinline__ void codes_of(const float (&x)[N], float s, float inv
     float off = plain ? 0.0f : 1.0f;
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        const float r = x[i] * inv, y = r + 12582912.0f;     // 1.5 * 2^23: the sum's low bits are rint(r)
-        off = fmaxf(off, fabsf(r - (y - 12582912.0f)));
+        const float y = fmaf(x[i], inv, 12582912.0f);        // 1.5 * 2^23: the sum's low bits are the whole number
+        off = fmaxf(off, fabsf(fmaf(x[i], inv, 12582912.0f - y)));
         c[i] = __float_as_uint(y);
     }
     if (off > 0.4999f) {
-#pragma unroll 1
+#pragma unroll
         for (int i = 0; i < N; i++) c[i] = (uint32_t)code_of(x[i], s);
     }
 }
 
-// Whether codes_of may take products: m is the largest magnitude of the page's new values, odd NaN if one of them is a
-// NaN or an infinity, else 0.
-__device__ __forceinline__ bool plain_page(float odd, float s) { return odd == 0.0f && s >= 0x1p-100f; }
+// The larger magnitude, NaN when either is.
+__device__ __forceinline__ float max_nan(float m, float x)
+{
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(m), "f"(fabsf(x)));
+    return m;
+}
 
 // A code after its page's scale grew by 1 / ratio.
 __device__ __forceinline__ int moved(int code, float ratio) { return (int)rintf(__fmul_rn((float)code, ratio)); }
@@ -121,7 +124,7 @@ struct Mine {
 template <typename T, int V>
 __global__ void __launch_bounds__(ROWS_THREADS) append_kernel(const RowsArgs p)
 {
-    __shared__ float s_max[ROWS_THREADS / 32], s_odd[ROWS_THREADS / 32];
+    __shared__ float s_max[ROWS_THREADS / 32];
     __shared__ __align__(16) uint8_t s_code[128 * S_PITCH];
     pdl_wait();
     kv8_place_t at;
@@ -147,36 +150,37 @@ __global__ void __launch_bounds__(ROWS_THREADS) append_kernel(const RowsArgs p)
     float *const scale = p.scale[side] + ph;
     const float was = at.lo ? *scale : 0.0f;
 
-    float m = 0.0f, odd = 0.0f;
+    float m = 0.0f;
 #pragma unroll
     for (int k = 0; k < Mine<V>::N; k++)
 #pragma unroll
         for (int j = 0; j < 4; j++)
 #pragma unroll
-            for (int e = 0; e < V; e++) {
-                const float v = to_f32(raw[k][j].v[e]);
-                m = fmaxf(m, fabsf(v));                  // drops a NaN
-                odd = fmaf(v, 0.0f, odd);
-            }
-    for (int o = 16; o > 0; o >>= 1) {
-        m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-        odd += __shfl_xor_sync(0xFFFFFFFFu, odd, o);
-    }
-    if ((threadIdx.x & 31) == 0) {
-        s_max[threadIdx.x >> 5] = m;
-        s_odd[threadIdx.x >> 5] = odd;
-    }
-    __syncthreads();                                     // also: `was` is read by all before it is replaced
+            for (int e = 0; e < V; e++) m = max_nan(m, to_f32(raw[k][j].v[e]));
+    auto reduce = [&]() {
+        for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+        if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
+        __syncthreads();                                 // also: `was` is read by all before it is replaced
 #pragma unroll
-    for (int i = 0; i < ROWS_THREADS / 32; i++) {
-        m = fmaxf(m, s_max[i]);
-        odd += s_odd[i];
+        for (int i = 0; i < ROWS_THREADS / 32; i++) m = max_nan(m, s_max[i]);
+    };
+    reduce();
+    bool plain = m <= 3.402823466e38f;                   // the same for the whole CTA
+    if (!plain) {
+        __syncthreads();
+        m = 0.0f;
+#pragma unroll
+        for (int k = 0; k < Mine<V>::N; k++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int e = 0; e < V; e++) m = max_nan(m, finite(to_f32(raw[k][j].v[e])));
+        reduce();
     }
-    m = finite(m);
     const float now = fmaxf(was, __fdiv_rn(m, 127.0f));
     const float ratio = now > was && now > 0.0f ? __fdiv_rn(was, now) : 1.0f;
     if (threadIdx.x == 0) *scale = now;
-    const bool plain = plain_page(odd, now);
+    plain = plain && now >= 0x1p-100f;
     const float inv = plain ? __fdiv_rn(1.0f, now) : 0.0f;
 
     int8_t *const code = p.code[side] + ph * TCG_KV8_PAGE * D;
@@ -283,22 +287,22 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) append_few_kernel(const RowsAr
     const long long ph = (long long)page * p.n_kv + head;
     float *const scale = p.scale[side] + ph;
     const float was = at.lo ? *scale : 0.0f;
-    float m = 0.0f, odd = 0.0f;
+    float m = 0.0f, top = 0.0f;
 #pragma unroll
     for (int i = 0; i < FEW; i++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            m = fmaxf(m, fabsf(v[i][e]));
-            odd = fmaf(v[i][e], 0.0f, odd);
+            m = max_nan(m, v[i][e]);
+            top = fmaxf(top, fabsf(finite(v[i][e])));
         }
     for (int o = 16; o > 0; o >>= 1) {
-        m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-        odd += __shfl_xor_sync(0xFFFFFFFFu, odd, o);
+        m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
     }
-    const float now = fmaxf(was, __fdiv_rn(finite(m), 127.0f));
+    const float now = fmaxf(was, __fdiv_rn(top, 127.0f));
     const float ratio = now > was && now > 0.0f ? __fdiv_rn(was, now) : 1.0f;
     if (lane == 0) *scale = now;                         // read by the whole warp before the shuffles
-    const bool plain = plain_page(odd, now);
+    const bool plain = m <= 3.402823466e38f && now >= 0x1p-100f;
     const float inv = plain ? __fdiv_rn(1.0f, now) : 0.0f;
     int8_t *const code = p.code[side] + ph * TCG_KV8_PAGE * D;
     if (ratio != 1.0f && at.lo) {

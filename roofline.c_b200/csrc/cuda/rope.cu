@@ -12,9 +12,9 @@
 //
 // Bound by memory: 2 * 4 bytes an element (fp32) for ~10 operations. A lane
 // owns one "unit" of 2 V dims of a head, two vectors of V: V pairs of the
-// rotated part, or 2 V dims of the rest. It computes its V sines and cosines
-// once per token and applies them to the heads of the token one after the
-// other, ROPE_AHEAD heads' loads in flight. 32 / L heads side by side in a
+// rotated part, or 2 V dims of the rest. The warp computes its token's sines
+// and cosines once, one pair a lane, and applies them to the heads of the
+// token one after the other, ROPE_AHEAD heads' loads in flight. 32 / L heads side by side in a
 // warp, L = the lanes a head needs.
 #include "lm.cuh"
 
@@ -22,7 +22,7 @@ namespace tcg {
 namespace {
 
 constexpr int ROPE_WARPS = 4;
-constexpr int ROPE_AHEAD = 4;    // heads whose loads are in flight
+constexpr int ROPE_AHEAD = 2;    // heads whose loads are in flight
 
 struct RopeArgs {
     const void *x[2];            // q (or the only tensor), k
@@ -37,12 +37,17 @@ struct RopeArgs {
     double turns[TCG_ROPE_MAX_DIM / 2];
 };
 
-// The two vectors of unit u start at dims a and b.
+// The two vectors of unit u start at dims a and b. Pairs of the half layout
+// and the dims that are not rotated come from two halves, each read by
+// consecutive lanes without gaps.
 template <int V, bool HALF>
-__device__ __forceinline__ void unit_dims(int u, int n_rot, int &a, int &b)
+__device__ __forceinline__ void unit_dims(int u, int n_rot, int D, int &a, int &b)
 {
     const int half = n_rot / 2;
-    if (HALF && u * V < half) {
+    if (u * V >= half) {
+        a = n_rot + u * V - half;
+        b = a + (D - n_rot) / 2;
+    } else if (HALF) {
         a = u * V;
         b = a + half;
     } else {
@@ -52,8 +57,9 @@ __device__ __forceinline__ void unit_dims(int u, int n_rot, int &a, int &b)
 }
 
 template <typename T, int V, int U, bool HALF, bool NORM>
-__global__ void __launch_bounds__(32 * ROPE_WARPS, 4) rope_kernel(const __grid_constant__ RopeArgs p)
+__global__ void __launch_bounds__(32 * ROPE_WARPS, 6) rope_kernel(const __grid_constant__ RopeArgs p)
 {
+    __shared__ __align__(16) float2 s_ang[ROPE_WARPS][TCG_ROPE_MAX_DIM / 2];
     const int lane = threadIdx.x & 31, L = p.lanes;
     const int sub = lane / L, l = lane % L, side = 32 / L;
     const unsigned task = blockIdx.x * ROPE_WARPS + (threadIdx.x >> 5);
@@ -66,7 +72,7 @@ __global__ void __launch_bounds__(32 * ROPE_WARPS, 4) rope_kernel(const __grid_c
     for (int k = 0; k < U; k++) {
         const int u = l + 32 * k;
         live[k] = u < units;
-        unit_dims<V, HALF>(live[k] ? u : 0, p.n_rot, da[k], db[k]);
+        unit_dims<V, HALF>(live[k] ? u : 0, p.n_rot, p.D, da[k], db[k]);
         turn[k] = live[k] && u * V < p.n_rot / 2;
     }
     pdl_wait();
@@ -93,21 +99,24 @@ __global__ void __launch_bounds__(32 * ROPE_WARPS, 4) rope_kernel(const __grid_c
     const int h_first = part * side + sub;
     load(h_first);
 
+    // The token's sines and cosines, a pair a lane, shared by the warp.
     const double at = (double)p.pos[tok];
+    float2 *const ang = s_ang[threadIdx.x >> 5];
+    for (int i = lane; i < p.n_rot / 2; i += 32) {
+        const double t = at * p.turns[i];
+        float2 a;
+        sincospif((float)(2.0 * (t - rint(t))), &a.y, &a.x);
+        ang[i] = make_float2(a.x * p.mscale, a.y * p.mscale);
+    }
+    __syncwarp();
     float cs[U][V], sn[U][V];
 #pragma unroll
     for (int k = 0; k < U; k++)
 #pragma unroll
         for (int i = 0; i < V; i++) {
-            cs[k][i] = 1.0f;
-            sn[k][i] = 0.0f;
-            if (turn[k]) {
-                const double t = at * p.turns[(l + 32 * k) * V + i];
-                const float f = (float)(2.0 * (t - rint(t)));
-                sincospif(f, &sn[k][i], &cs[k][i]);
-                sn[k][i] *= p.mscale;
-                cs[k][i] *= p.mscale;
-            }
+            const float2 a = turn[k] ? ang[(l + 32 * k) * V + i] : make_float2(1.0f, 0.0f);
+            cs[k][i] = a.x;
+            sn[k][i] = a.y;
         }
 
     for (int h0 = h_first; h0 - sub < all; h0 += step * ROPE_AHEAD) {   // the warp's lanes leave together
