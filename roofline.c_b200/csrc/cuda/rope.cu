@@ -14,7 +14,7 @@
 // owns one "unit" of 2 V dims of a head, two vectors of V: V pairs of the
 // rotated part, or 2 V dims of the rest. The warp computes its token's sines
 // and cosines once, one pair a lane, and applies them to the heads of the
-// token one after the other, ROPE_AHEAD heads' loads in flight. 32 / L heads side by side in a
+// token one after the other. 32 / L heads side by side in a
 // warp, L = the lanes a head needs.
 #include "lm.cuh"
 
@@ -22,7 +22,18 @@ namespace tcg {
 namespace {
 
 constexpr int ROPE_WARPS = 4;
-constexpr int ROPE_AHEAD = 2;    // heads whose loads are in flight
+
+// How a warp keeps loads in flight, by the element's size. 16-bit rows: one
+// head's loads while the head before it is computed, and a token's heads dealt
+// out until there are 64 warps an SM (6001 rows of 36 heads of 128 in bf16:
+// 23.5 us; two heads at a time without that overlap 28.5, 16 warps 25.2).
+// fp32 rows: two heads' loads at a time, 16 warps an SM (4096 rows of 40 heads
+// with norms: 30.0 us; overlapped 32.3 to 41, 64 warps 35.3).
+template <typename T>
+struct Flow {
+    static constexpr bool PIPE = sizeof(T) == 2;
+    static constexpr int AHEAD = PIPE ? 1 : 2, WARPS_PER_SM = PIPE ? 64 : 16, CTAS = PIPE ? 8 : 6;
+};
 
 struct RopeArgs {
     const void *x[2];            // q (or the only tensor), k
@@ -57,9 +68,11 @@ __device__ __forceinline__ void unit_dims(int u, int n_rot, int D, int &a, int &
 }
 
 template <typename T, int V, int U, bool HALF, bool NORM>
-__global__ void __launch_bounds__(32 * ROPE_WARPS, 6) rope_kernel(const __grid_constant__ RopeArgs p)
+__global__ void __launch_bounds__(32 * ROPE_WARPS, Flow<T>::CTAS) rope_kernel(const __grid_constant__ RopeArgs p)
 {
     __shared__ __align__(16) float2 s_ang[ROPE_WARPS][TCG_ROPE_MAX_DIM / 2];
+    constexpr int ROPE_AHEAD = Flow<T>::AHEAD;
+    constexpr bool PIPE = Flow<T>::PIPE;
     const int lane = threadIdx.x & 31, L = p.lanes;
     const int sub = lane / L, l = lane % L, side = 32 / L;
     const unsigned task = blockIdx.x * ROPE_WARPS + (threadIdx.x >> 5);
@@ -78,26 +91,29 @@ __global__ void __launch_bounds__(32 * ROPE_WARPS, 6) rope_kernel(const __grid_c
     pdl_wait();
     if (tok >= p.n_tok) return;
 
-    // Batches of ROPE_AHEAD heads: the loads of a batch go out together, those of the first before the angles are computed.
-    Pack<T, V> xa[ROPE_AHEAD][U], xb[ROPE_AHEAD][U];
-    auto load = [&](int h0) {
+    // Batches of ROPE_AHEAD heads, whose loads go out together: the first before the angles are computed, with PIPE each
+    // before the batch ahead of it is.
+    struct Batch {
+        Pack<T, V> a[ROPE_AHEAD][U], b[ROPE_AHEAD][U];
+    };
+    auto load = [&](Batch &x, int h0) {
 #pragma unroll
         for (int j = 0; j < ROPE_AHEAD; j++) {
             const int h = h0 + j * step, s = h >= p.heads[0];
-            const T *row = (const T *)p.x[s] + tok * p.ldx[s] + (long long)(h - (s ? p.heads[0] : 0)) * p.D;
+            const T *row = (const T *)p.x[s] + tok * p.ldx[s] + (h - (s ? p.heads[0] : 0)) * p.D;
 #pragma unroll
             for (int k = 0; k < U; k++) {
-                xa[j][k] = Pack<T, V>{};
-                xb[j][k] = Pack<T, V>{};
+                x.a[j][k] = x.b[j][k] = Pack<T, V>{};
                 if (h < all && live[k]) {
-                    xa[j][k] = *(const Pack<T, V> *)(row + da[k]);
-                    xb[j][k] = *(const Pack<T, V> *)(row + db[k]);
+                    x.a[j][k] = *(const Pack<T, V> *)(row + da[k]);
+                    x.b[j][k] = *(const Pack<T, V> *)(row + db[k]);
                 }
             }
         }
     };
     const int h_first = part * side + sub;
-    load(h_first);
+    Batch now, next;
+    load(now, h_first);
 
     // The token's sines and cosines, a pair a lane, shared by the warp.
     const double at = (double)p.pos[tok];
@@ -119,8 +135,11 @@ __global__ void __launch_bounds__(32 * ROPE_WARPS, 6) rope_kernel(const __grid_c
             sn[k][i] = a.y;
         }
 
+    float w[U][2 * V];
+    int have = -1;                                               // the side whose weights these are
     for (int h0 = h_first; h0 - sub < all; h0 += step * ROPE_AHEAD) {   // the warp's lanes leave together
-        if (h0 != h_first) load(h0);
+        if (PIPE) load(next, h0 + step * ROPE_AHEAD);
+        else if (h0 != h_first) load(now, h0);
 #pragma unroll
         for (int j = 0; j < ROPE_AHEAD; j++) {
             const int h = h0 + j * step;
@@ -131,8 +150,8 @@ __global__ void __launch_bounds__(32 * ROPE_WARPS, 6) rope_kernel(const __grid_c
             for (int k = 0; k < U; k++)
 #pragma unroll
                 for (int i = 0; i < V; i++) {
-                    v[k][i] = to_f32(xa[j][k].v[i]);
-                    v[k][V + i] = to_f32(xb[j][k].v[i]);
+                    v[k][i] = to_f32(now.a[j][k].v[i]);
+                    v[k][V + i] = to_f32(now.b[j][k].v[i]);
                 }
             if (NORM) {
                 float ss = 0.0f;
@@ -144,28 +163,32 @@ __global__ void __launch_bounds__(32 * ROPE_WARPS, 6) rope_kernel(const __grid_c
                 inv = rsqrtf(ss / (float)p.D + p.eps);
             }
             if (h >= all) continue;
-            T *row = (T *)p.y[s] + tok * p.ldy[s] + (long long)(h - (s ? p.heads[0] : 0)) * p.D;
+            if (NORM && s != have) {
+                have = s;
+#pragma unroll
+                for (int k = 0; k < U; k++)
+#pragma unroll
+                    for (int i = 0; i < V; i++) {
+                        w[k][i] = p.w[s][da[k] + i];
+                        w[k][V + i] = p.w[s][db[k] + i];
+                    }
+            }
+            T *row = (T *)p.y[s] + tok * p.ldy[s] + (h - (s ? p.heads[0] : 0)) * p.D;
 #pragma unroll
             for (int k = 0; k < U; k++) {
                 if (!live[k]) continue;
                 float a[V], b[V];
                 if (NORM) {
-                    const float *w = p.w[s];
 #pragma unroll
-                    for (int i = 0; i < V; i++) {
-                        v[k][i] = v[k][i] * inv * __ldg(w + da[k] + i);
-                        v[k][V + i] = v[k][V + i] * inv * __ldg(w + db[k] + i);
-                    }
+                    for (int i = 0; i < 2 * V; i++) v[k][i] = v[k][i] * inv * w[k][i];
                 }
 #pragma unroll
                 for (int i = 0; i < V; i++) {
                     // the two values of pair i: one of each vector, or neighbours
                     float &lo = HALF ? v[k][i] : v[k][2 * i], &hi = HALF ? v[k][V + i] : v[k][2 * i + 1];
-                    const float c = cs[k][i], d = sn[k][i], e = lo;
-                    if (turn[k]) {
-                        lo = fmaf(e, c, -(hi * d));
-                        hi = fmaf(e, d, hi * c);
-                    }
+                    const float c = cs[k][i], d = sn[k][i], x = fmaf(lo, c, -(hi * d)), y = fmaf(lo, d, hi * c);
+                    lo = turn[k] ? x : lo;
+                    hi = turn[k] ? y : hi;
                 }
 #pragma unroll
                 for (int i = 0; i < V; i++) {
@@ -176,6 +199,7 @@ __global__ void __launch_bounds__(32 * ROPE_WARPS, 6) rope_kernel(const __grid_c
                 store_pack<T, V>(row + db[k], b);
             }
         }
+        if (PIPE) now = next;
     }
 }
 
@@ -211,9 +235,9 @@ bool rope_launch(RopeArgs &p, bool half, bool norm)
     while (p.lanes < units && p.lanes < 32) p.lanes <<= 1;
     // A warp that takes all heads of its token computes the angles once; one
     // token or a few are dealt out to more warps, down to one head a lane
-    // group, until there are 16 warps an SM.
+    // group, until there are enough warps an SM.
     const int side = 32 / p.lanes, all = p.heads[0] + p.heads[1], most = (all + side - 1) / side;
-    long long want = ((long long)ctx().sms * 16 + p.n_tok - 1) / p.n_tok;
+    long long want = ((long long)ctx().sms * Flow<T>::WARPS_PER_SM + p.n_tok - 1) / p.n_tok;
     p.splits = (int)(want < 1 ? 1 : want > most ? most : want);
     const long long warps = (long long)p.n_tok * p.splits;
     const long long grid = (warps + ROPE_WARPS - 1) / ROPE_WARPS;
