@@ -30,32 +30,16 @@
 // take alternate tiles, and a cluster of S CTAs takes S consecutive shares of
 // the keys; partial results (m, l, O) meet in shared memory, then over
 // distributed shared memory, in a fixed order. No workspace, one launch.
-#include "lm.cuh"
+#include "kv8_attn.cuh"
 #include "tc05.cuh"
 
 #include <math.h>
+#include <stdlib.h>
 
 #include <type_traits>
 
 namespace tcg {
 namespace {
-
-constexpr int PAGE = TCG_KV8_PAGE;
-constexpr int ERR_WAIT = 66;             // device error word: a tile's copy did not land in time
-
-struct AttnArgs {
-    const void *q;
-    void *out;
-    long long ld_q, ld_out;
-    int type, q_vec, out_vec;            // ggml type; 16-byte loads / 4-element stores possible
-    const int8_t *v;
-    const float *k_scale, *v_scale;
-    KvStep step;
-    int n_pages, n_kv, D, G;
-    float scale_log2;
-    int causal, window, S;
-    int *err;
-};
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
@@ -74,12 +58,6 @@ __device__ __forceinline__ uint4 lds128(uint32_t a)
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
     return v;
-}
-__device__ __forceinline__ float ex2(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
 {
@@ -108,72 +86,6 @@ __device__ __forceinline__ void cluster_sync()
 {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-
-// 16 consecutive values of a query row.
-__device__ __forceinline__ void load_q16(const AttnArgs &p, long long off, float (&x)[16])
-{
-    if (p.type == GGML_TYPE_F32) {
-        const float *s = (const float *)p.q + off;
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            if (p.q_vec) {
-                const float4 v = *(const float4 *)(s + i);
-                x[i] = v.x, x[i + 1] = v.y, x[i + 2] = v.z, x[i + 3] = v.w;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; e++) x[i + e] = s[i + e];
-            }
-        }
-        return;
-    }
-    const unsigned short *s = (const unsigned short *)p.q + off;
-    uint32_t w[8];
-    if (p.q_vec) {
-        const uint4 a = *(const uint4 *)s, b = *(const uint4 *)(s + 8);
-        w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) w[i] = (uint32_t)s[2 * i] | (uint32_t)s[2 * i + 1] << 16;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        if (p.type == GGML_TYPE_BF16) {
-            x[2 * i] = __uint_as_float(w[i] << 16);
-            x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-        } else {
-            x[2 * i] = __half2float(__ushort_as_half((unsigned short)w[i]));
-            x[2 * i + 1] = __half2float(__ushort_as_half((unsigned short)(w[i] >> 16)));
-        }
-    }
-}
-
-template <int V>
-__device__ __forceinline__ void store_out(const AttnArgs &p, long long off, const float (&x)[V])
-{
-    if (p.type == GGML_TYPE_F32) {
-        float *o = (float *)p.out + off;
-        if (p.out_vec) store_pack<float, V>(o, x);
-        else
-#pragma unroll
-            for (int i = 0; i < V; i++) o[i] = x[i];
-    } else if (p.type == GGML_TYPE_F16) {
-        __half *o = (__half *)p.out + off;
-        if (p.out_vec) store_pack<__half, V>(o, x);
-        else
-#pragma unroll
-            for (int i = 0; i < V; i++) o[i] = __float2half_rn(x[i]);
-    } else {
-        __nv_bfloat16 *o = (__nv_bfloat16 *)p.out + off;
-        if (p.out_vec) store_pack<__nv_bfloat16, V>(o, x);
-        else
-#pragma unroll
-            for (int i = 0; i < V; i++) o[i] = __float2bfloat16_rn(x[i]);
-    }
-}
-
-// Sum of weights -> factor on O. A row that saw nothing has the sum 0 and
-// gets zeros; a NaN sum (a query with a NaN or an infinity) stays NaN.
-__device__ __forceinline__ float inverse(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
 
 template <int KS, int RW, int WM, int WN, int NSLOT>
 struct Shape {
@@ -793,6 +705,8 @@ extern "C" bool tcg_kv8_attention(void *out, const void *q, const tcg_kv8_t *c, 
     p.scale_log2 = scale * 1.44269504088896340736f;
     p.causal = causal, p.window = window, p.err = ctx().d_err;
 
+    const int rows_tc = getenv("TCROWS") ? atoi(getenv("TCROWS")) : 64;
+    if (R > rows_tc) return launch_kv8_attn_tc(p, c->k, R, s->n_seq);
     // K as [pages x heads x 64, D] bytes; a box is 64 keys of 64 dims, zeros past D
     EncodeFn fn = attn_encode_fn();
     if (!fn) return fail("cuTensorMapEncodeTiled is not available from the driver");

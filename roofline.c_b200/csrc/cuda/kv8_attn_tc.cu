@@ -1,0 +1,443 @@
+// kv8_attn_tc.cu -- tcg_kv8_attention for many rows (prompts and chunks of
+// prompts) on the 5th-generation tensor cores.
+//
+// One CTA of 256 threads takes 128 consecutive query rows (row = token * G +
+// query head of the group) of one key head; threads r and r + 128 share row r
+// = TMEM lane r. A tile is two pages, 128 keys: thread r takes the first
+// page's, r + 128 the second's, and half of the output dims each. A page's
+// int8 K [64, D] and V [D, 64] are loaded into registers ahead of use,
+// converted to fp16 (whole numbers up to 127: exact) and written to shared
+// memory in the K-major, 128-byte-swizzled layout the MMA reads; V is
+// dim-major in the cache, so neither is transposed. Then
+//   S = Q K^T    128 x 128 fp32 in TMEM, Q as fp16 in shared memory;
+//   softmax      x = S cs - m, cs = scale log2(e) 2^-e sk, P = exp2(x + 8);
+//   P V          128 x D fp32 in TMEM, P as fp16 in TMEM over S's columns,
+//                accumulated there over a group of tiles;
+//   O = O 2^(m_old - m) + sv0 P V at a group's end.
+// Within a group the reference m and the V scale sv0 stay: a page's sv enters
+// as log2(sv / sv0) in the exponent. A group ends where a row's maximum
+// outgrows its reference by 2^7, where sv and sv0 are 2^6 apart, or after 4
+// tiles with fp32 inputs (32 otherwise): the tensor core's accumulation
+// truncates, by about 2e-8 of the result per MMA, 64 (256) of them a group.
+// O is used at a group's end only and lives in local memory.
+// Q is scaled by a power of two per row into [2^14, 2^15). With fp16 or bf16
+// inputs it is exact as one fp16, and P's rounding to fp16 (2^-12 of itself)
+// is below the output's; with fp32 inputs Q and P are two fp16 pieces of 11
+// bits each (NP = 2), the small piece's products first.
+//
+// Why fp16 and not the 8-bit integers of the cache, as the kernel for few rows
+// does: with one thread a row the integer path is bound by the threads' work
+// on the accumulators (a conversion and a multiply-add for every digit of
+// every value), which fp32 accumulators do not need; the conversion of K and V
+// is shared by 128 rows.
+//
+// K and V of a tile take turns in one buffer (S is done with K before V is
+// needed), so two CTAs fit an SM (with 256 TMEM columns each): the one's
+// products run while the other's threads compute. Every wait is bounded as in
+// attn_tc.cu.
+#include "kv8_attn.cuh"
+#include "numerics.cuh"
+#include "tc05.cuh"
+
+#include <math.h>
+
+namespace tcg {
+namespace {
+
+constexpr int TC_THREADS = 256;
+constexpr int TC_ROWS = 128;
+constexpr uint32_t TC_COLS = 256;                // S, and P over it: 0 .. 127; P V: from 128
+constexpr uint32_t Q_TILE = 128 * 128;           // [128 rows or keys x 64 fp16]
+constexpr float P_BIAS = 8.0f, GROWTH = 7.0f;    // weights are up to 2^8, and 2^15 before a group ends (fp16: below 2^16)
+
+template <int DP, int NP>
+struct TcShape {
+    static constexpr uint32_t Q = 0, KV = NP * (DP / 64) * Q_TILE, END = KV + (DP / 64) * Q_TILE;   // K, or V of 2 pages
+    static constexpr uint32_t V_TILE = DP * 128;             // [DP dims x 64 keys]
+    static constexpr size_t SMEM = 1024 + END + 32 + TC_THREADS * 4 * 2;
+};
+
+// D fp32, A and B fp16, both K-major, M = 128.
+__device__ __forceinline__ constexpr uint32_t idesc_f16(int N)
+{
+    return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+// A from TMEM (row i in lane i, two fp16 of K per column), B from shared memory.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a_tmem, unsigned long long b, uint32_t id, uint32_t acc)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a_tmem), "l"(b), "r"(id), "r"(acc));
+}
+
+// 16 columns of this thread's TMEM lane from registers; waits for the store.
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0],"
+                 " {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n\t"
+                 "tcgen05.wait::st.sync.aligned;"
+                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]),
+                   "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+                   "r"(v[15])
+                 : "memory");
+}
+
+// Byte offset of 16-byte chunk c of row r of a swizzled tile with rows of 128 bytes.
+__device__ __forceinline__ uint32_t chunk_at(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
+
+// 16 codes as fp16, the two 16-byte chunks c and c + 1 of row r. A byte u =
+// code + 128 under the exponent byte 0x64 is the fp16 number 1024 + u.
+__device__ __forceinline__ void store_codes(uint8_t *tile, int r, int c, uint4 raw)
+{
+    const uint32_t w[4] = { raw.x, raw.y, raw.z, raw.w };
+    uint32_t h[8];
+    const __half2 off = __float2half2_rn(1152.0f);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t u = w[i] ^ 0x80808080u;
+        const uint32_t lo = __byte_perm(u, 0x64646464u, 0x4140), hi = __byte_perm(u, 0x64646464u, 0x4342);
+        const __half2 a = __hsub2(*(const __half2 *)&lo, off), b = __hsub2(*(const __half2 *)&hi, off);
+        h[2 * i] = *(const uint32_t *)&a;
+        h[2 * i + 1] = *(const uint32_t *)&b;
+    }
+    *(uint4 *)(tile + chunk_at(r, c)) = make_uint4(h[0], h[1], h[2], h[3]);
+    *(uint4 *)(tile + chunk_at(r, c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
+}
+
+template <int DP, int NP>
+__global__ void __launch_bounds__(TC_THREADS, 2)
+kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict__ kc)
+{
+    using Sh = TcShape<DP, NP>;
+    constexpr int DH = DP / 2;                               // dims of a thread
+    extern __shared__ uint8_t raw[];
+    uint8_t *const tiles = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    uint64_t *const bars = (uint64_t *)(tiles + Sh::END);
+    uint32_t *const tmem_slot = (uint32_t *)(bars + 2);
+    volatile int *const abort = (volatile int *)(tmem_slot + 1);
+    float *const xmax = (float *)(tiles + Sh::END + 32);     // [256] a tile's maxima, the two pages of each row
+    float *const xsum = xmax + TC_THREADS;
+    const int tid = threadIdx.x, warp = tid >> 5, r = tid & 127, h = tid >> 7;
+    const uint32_t bar_s = su32(bars), bar_o = su32(bars + 1);
+    const int head = blockIdx.y, b = blockIdx.z;
+
+    pdl_wait();
+    kv8_seq_t seq;
+    if (!kv_seq(p.step, b, seq, p.err, tid == 0)) return;
+    const int R = seq.n * p.G, r0 = (p.causal ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x) * TC_ROWS;
+    if (r0 >= R) return;
+    int t0;
+    const int np = kv8_tiles(&seq, r0 / p.G, (min(r0 + TC_ROWS, R) - 1) / p.G, p.causal, p.window, 0, 1, 0, 1, &t0);
+
+    if (tid == 0) {
+        bar_init(bar_s, 1);
+        bar_init(bar_o, 1);
+        *abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(su32(tmem_slot)), "r"(TC_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+
+    // This thread's row (the last one again where there are fewer) and its keys lo .. hi.
+    const int row = min(r0 + r, R - 1), tok = row / p.G;
+    const int hi = kv8_hi(&seq, tok, p.causal), lo = kv8_lo(&seq, tok, p.window);
+    const long long head_off = (long long)(head * p.G + row % p.G) * p.D;
+
+    // A page's K or V in registers: 16-byte pieces tid and tid + 256. K: piece i is key i / (D / 16), dims 16 (i % (D /
+    // 16))...; V: dim i / 4, keys 16 (i % 4)...
+    const int per = p.D / 16, pieces = 4 * p.D;
+    int krow[2], kcol[2];
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+        krow[u] = (tid + TC_THREADS * u) / per;
+        kcol[u] = (tid + TC_THREADS * u) % per;
+    }
+    const long long block = (long long)p.D * PAGE;           // bytes of a (page, head)
+    auto load_pages = [&](uint4 (&x)[2][2], const int8_t *codes, int a, int z) {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const uint4 *src = (const uint4 *)(codes + ((long long)max(j ? z : a, 0) * p.n_kv + head) * block);
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+                if (tid + TC_THREADS * u < pieces) x[j][u] = __ldg(src + tid + TC_THREADS * u);
+        }
+    };
+    // page i of this CTA; -1 for none, or one that does not exist
+    auto page_at = [&](int i) { return i < np ? kv_page(p.step, b, t0 + i, p.n_pages, p.err, tid == 0) : -1; };
+    auto store_k = [&](const uint4 (&x)[2][2]) {
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+                if (tid + TC_THREADS * u < pieces)
+                    store_codes(tiles + Sh::KV + (kcol[u] >> 2) * Q_TILE, 64 * j + krow[u], 2 * (kcol[u] & 3), x[j][u]);
+    };
+    auto store_v = [&](const uint4 (&x)[2][2]) {
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int i = tid + TC_THREADS * u;
+                if (i < pieces) store_codes(tiles + Sh::KV + j * Sh::V_TILE, i >> 2, 2 * (i & 3), x[j][u]);
+            }
+    };
+
+    uint4 raw4[2][2] = {};                                   // K of a tile, then its V, then K of the next ...
+    int pa = page_at(0), pb = page_at(1), na = page_at(2), nb = page_at(3);   // this tile's pages, and the next's
+    load_pages(raw4, kc, pa, pb);
+
+    // dims past D are zeros in Q (below); what K and V leave unwritten there only has to be finite
+    if (p.D < DP) {
+        for (int i = tid; i < (int)(Sh::END - Sh::KV) / 16; i += TC_THREADS)
+            *(uint4 *)(tiles + Sh::KV + 16 * i) = make_uint4(0, 0, 0, 0);
+    }
+    // Q: this thread's half row, scaled by 2^e, as fp16 pieces
+    float cs0;
+    {
+        float x[DH / 16][16], m = 0.0f;
+        bool odd = false;
+        const long long off = (seq.row0 + tok) * p.ld_q + head_off + DH * h;
+#pragma unroll
+        for (int c = 0; c < DH / 16; c++) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) x[c][e] = 0.0f;
+            if (DH * h + 16 * c < p.D) load_q16(p, off + 16 * c, x[c]);
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                odd |= !(fabsf(x[c][e]) <= 3.402823466e38f);
+                m = fmaxf(m, fabsf(x[c][e]));
+            }
+        }
+        xmax[tid] = odd ? __int_as_float(0x7F800000) : m;
+        __syncthreads();
+        m = fmaxf(xmax[r], xmax[r + 128]);
+        odd = !(m <= 3.402823466e38f);
+        const int e = f16_scale_exp(m);
+        const float f = odd ? 0.0f : __int_as_float((127 + e) << 23);
+        // a row with a NaN or an infinity: zeros here, and a NaN factor
+        cs0 = odd ? __int_as_float(0x7FC00000) : p.scale_log2 * __int_as_float((127 - e) << 23);
+#pragma unroll
+        for (int c = 0; c < DH / 8; c++) {
+            const int d = DH * h + 8 * c;
+            uint2 a[2], z[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                float y[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) y[k] = odd ? 0.0f : x[c / 2][8 * (c & 1) + 4 * i + k];
+                f16_pieces4(y, f, a[i], z[i]);
+            }
+            uint8_t *const q = tiles + Sh::Q + (d >> 6) * Q_TILE + chunk_at(r, (d & 63) >> 3);
+            *(uint4 *)q = make_uint4(a[0].x, a[0].y, a[1].x, a[1].y);
+            if (NP == 2) *(uint4 *)(q + (DP / 64) * Q_TILE) = make_uint4(z[0].x, z[0].y, z[1].x, z[1].y);
+        }
+    }
+    __syncthreads();                                         // the zeros and the maxima's readers are done
+    store_k(raw4);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *tmem_slot, tbase = su32(tiles);
+    const uint32_t lane_base = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+
+    auto issue_s = [&]() {
+#pragma unroll
+        for (int n = NP - 1; n >= 0; n--)
+#pragma unroll
+            for (int s = 0; s < DP / 16; s++)
+                mma_f16(tmem, sdesc<128>(tbase + Sh::Q + (n * (DP / 64) + (s >> 2)) * Q_TILE + (s & 3) * 32),
+                        sdesc<128>(tbase + Sh::KV + (s >> 2) * Q_TILE + (s & 3) * 32), idesc_f16(128),
+                        n < NP - 1 || s > 0 ? 1u : 0u);
+        mma_commit(bar_s);
+    };
+    // P of keys 64 j + 32 c + 16 s...: columns 64 j + 32 c + 16 piece + 8 s, the columns that held their scores
+    auto issue_o = [&](bool add) {
+#pragma unroll
+        for (int n = NP - 1; n >= 0; n--)
+#pragma unroll
+            for (int s = 0; s < 8; s++)
+                mma_f16_ts(tmem + 128, tmem + 32 * (s >> 1) + 16 * n + 8 * (s & 1),
+                           sdesc<128>(tbase + Sh::KV + (s >> 2) * Sh::V_TILE + (s & 3) * 32), idesc_f16(DP),
+                           n < NP - 1 || s > 0 || add ? 1u : 0u);
+        mma_commit(bar_o);
+    };
+    bool ok = true;
+    int last_s = -1, last_o = -1;                            // tiles of thread 0's latest commits
+    if (tid == 0) {
+        issue_s();
+        last_s = 0;
+    }
+    __syncwarp();
+
+    float o[DH], m = -INFINITY, l = 0.0f, sv0 = 0.0f;        // m, sv0: the group's references; l: this half's share
+#pragma unroll 1
+    for (int j = 0; j < DH; j++) o[j] = 0.0f;                // used at a group's end only: kept in local memory
+    int left = 0;                                            // tiles that the group may still take
+    // The group's P V, complete, joins O; then O and l move to the reference `now`.
+    auto fold = [&](float now, bool any) {
+        const float alpha = now == m ? 1.0f : ex2(m - now);
+#pragma unroll 1
+        for (int c = 0; c < DH; c += 32) {
+            uint32_t pv[32];
+            if (any) tmem_ld32(lane_base + 128 + DH * h + c, pv);
+#pragma unroll
+            for (int j = 0; j < 32; j++) o[c + j] = alpha * (any ? fmaf(__uint_as_float(pv[j]), sv0, o[c + j]) : o[c + j]);
+        }
+        l *= alpha;
+        m = now;
+    };
+
+    // Tile kb: S(kb) is under way. V(kb) replaces K(kb) when it is done; the maxima are posted and the CTA agrees whether
+    // the tile opens a group; the weights replace S(kb) and P V(kb) is issued; when that is done K(kb + 1) replaces V(kb).
+    const int tiles_n = (np + 1) / 2;
+    for (int kb = 0; kb < tiles_n; kb++) {
+        const int mine = h ? pb : pa, key0 = (t0 + 2 * kb + h) * PAGE;
+        const long long at_a = (long long)max(pa, 0) * p.n_kv + head, at_b = (long long)max(pb, 0) * p.n_kv + head;
+        const float sk = p.k_scale[h ? at_b : at_a];
+        const float va = pa < 0 ? 0.0f : p.v_scale[at_a], vb = pb < 0 ? 0.0f : p.v_scale[at_b], sv = h ? vb : va;
+        load_pages(raw4, p.v, pa, pb);
+        const float cs = cs0 * (mine < 0 ? 1.0f : sk), c = cs < 1e-37f ? 1e-37f : cs;   // not 0: a masked -inf stays -inf
+        float lr = sv == sv0 || mine < 0 ? 0.0f : __log2f(__fdividef(sv, sv0));
+        const bool whole = __all_sync(0xFFFFFFFFu, mine >= 0 && key0 >= lo && key0 + PAGE - 1 <= hi);
+        if (ok) ok = bar_wait(bar_s, (uint32_t)(kb & 1), abort, p.err, ERR_WAIT);
+        fence_after();
+        store_v(raw4);
+        // 32 scores of this thread's page, -inf where its row does not see the key
+        auto scores = [&](int q, float (&x)[32]) {
+            uint32_t s[32];
+            tmem_ld32(lane_base + 64 * h + 32 * q, s);
+            if (whole) {
+#pragma unroll
+                for (int j = 0; j < 32; j++) x[j] = __uint_as_float(s[j]);
+            } else {
+                const int k0 = key0 + 32 * q;
+#pragma unroll
+                for (int j = 0; j < 32; j++)
+                    x[j] = mine >= 0 && k0 + j >= lo && k0 + j <= hi ? __uint_as_float(s[j]) : -INFINITY;
+            }
+        };
+        float top = -INFINITY;
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+            float x[32];
+            scores(q, x);
+#pragma unroll
+            for (int j = 0; j < 32; j++) top = fmaxf(top, x[j]);
+        }
+        top = top == -INFINITY ? top : top * c;
+        xmax[tid] = top;
+        const bool group = __syncthreads_or(left == 0 || !(fabsf(lr) <= 6.0f) || top + lr > m + GROWTH);
+        if (group) {
+            fold(fmaxf(m, fmaxf(xmax[r], xmax[r + 128])), kb > 0);
+            sv0 = fmaxf(va, vb);
+            lr = sv == sv0 || mine < 0 ? 0.0f : fmaxf(__log2f(__fdividef(sv, sv0)), -60.0f);
+            left = NP == 2 ? 4 : 32;
+        }
+        left--;
+        const float use = P_BIAS + lr - (m == -INFINITY ? 0.0f : m);
+        float sum = 0.0f;
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+            float x[32];
+            uint32_t p1[16], p2[16];
+            scores(q, x);
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+                const float a = ex2(fmaf(x[j], c, use)), z = ex2(fmaf(x[j + 1], c, use));
+                sum += a + z;
+                const __half2 u = __floats2half2_rn(a, z);
+                p1[j / 2] = *(const uint32_t *)&u;
+                if (NP == 2) {
+                    const float2 w = __half22float2(u);
+                    const __half2 v = __floats2half2_rn(a - w.x, z - w.y);
+                    p2[j / 2] = *(const uint32_t *)&v;
+                }
+            }
+            tmem_st16(lane_base + 64 * h + 32 * q, p1);
+            if (NP == 2) tmem_st16(lane_base + 64 * h + 32 * q + 16, p2);
+        }
+        l = fmaf(sum, ex2(-lr), l);
+        if (kb + 1 < tiles_n) load_pages(raw4, kc, na, nb);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        fence_before();
+        __syncthreads();                                     // P(kb) and V(kb) in place; the maxima and a group's P V read
+        fence_after();
+        if (tid == 0 && ok) {
+            issue_o(!group);
+            last_o = kb;
+        }
+        __syncwarp();
+        pa = na, pb = nb;
+        na = page_at(2 * kb + 4), nb = page_at(2 * kb + 5);
+        if (ok) ok = bar_wait(bar_o, (uint32_t)(kb & 1), abort, p.err, ERR_WAIT);
+        fence_after();
+        if (kb + 1 < tiles_n) {
+            store_k(raw4);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            fence_before();
+            __syncthreads();                                 // K(kb + 1) in place
+            fence_after();
+            if (tid == 0 && ok) {
+                issue_s();
+                last_s = kb + 1;
+            }
+            __syncwarp();
+        }
+    }
+    fold(m, true);
+    xsum[tid] = l;
+    __syncthreads();
+    if (ok && r0 + r < R) {
+        const float inv = inverse(xsum[r] + xsum[r + 128]);
+        const long long off = (seq.row0 + tok) * p.ld_out + head_off + DH * h;
+#pragma unroll 1
+        for (int d = 0; d < DH && DH * h + d < p.D; d += 4) {
+            const float v[4] = { o[d] * inv, o[d + 1] * inv, o[d + 2] * inv, o[d + 3] * inv };
+            store_out<4>(p, off + d, v);
+        }
+    }
+    // MMAs that may still run (a wait gave up) must finish before TMEM is freed: thread 0 waits, bounded, for its last
+    // commits.
+    if (!ok && tid == 0) {
+        if (last_s >= 0) bar_wait(bar_s, (uint32_t)(last_s & 1), abort, p.err, ERR_WAIT, false);
+        if (last_o >= 0) bar_wait(bar_o, (uint32_t)(last_o & 1), abort, p.err, ERR_WAIT, false);
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TC_COLS) : "memory");
+    }
+}
+
+template <int DP, int NP>
+bool tc_launch(AttnArgs &p, const int8_t *k, long long R, int n_seq)
+{
+    using Sh = TcShape<DP, NP>;
+    auto fn = kv8_attn_tc_kernel<DP, NP>;
+    static bool ready[64];
+    const int dev = ctx().device & 63;
+    if (!ready[dev]) {
+        TCG_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::SMEM));
+        ready[dev] = true;
+    }
+    const dim3 grid((unsigned)((R + TC_ROWS - 1) / TC_ROWS), (unsigned)p.n_kv, (unsigned)n_seq);
+    TCG_CUDA(launch_pdl(fn, grid, dim3(TC_THREADS), Sh::SMEM, ctx().cur, p, k));
+    return true;
+}
+
+}  // namespace
+
+bool launch_kv8_attn_tc(AttnArgs &p, const int8_t *k, long long R, int n_seq)
+{
+    p.S = 1;
+    if (p.type == GGML_TYPE_F32) return p.D > 64 ? tc_launch<128, 2>(p, k, R, n_seq) : tc_launch<64, 2>(p, k, R, n_seq);
+    return p.D > 64 ? tc_launch<128, 1>(p, k, R, n_seq) : tc_launch<64, 1>(p, k, R, n_seq);
+}
+
+}  // namespace tcg
