@@ -34,7 +34,6 @@
 #include "tc05.cuh"
 
 #include <math.h>
-#include <stdlib.h>
 
 #include <type_traits>
 
@@ -64,29 +63,6 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
-__device__ __forceinline__ uint32_t mapa(uint32_t a, int rank)
-{
-    uint32_t r;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ float ld_cluster(uint32_t a)
-{
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a));
-    return v;
-}
-__device__ __forceinline__ float4 ld_cluster4(uint32_t a)
-{
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
-    return v;
-}
-__device__ __forceinline__ void cluster_sync()
-{
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
 template <int KS, int RW, int WM, int WN, int NSLOT>
 struct Shape {
     static constexpr int DP = KS * 32;                       // dims, padded
@@ -114,8 +90,9 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int wm = warp % WM, wn = warp / WM;
-    const int rank = blockIdx.x % p.S, ntile = gridDim.x / p.S;
-    const int head = blockIdx.y, b = blockIdx.z;
+    // grid: (rows from the last, sequence, head, rank), so that the blocks of rows with the most keys start first
+    const int rank = blockIdx.x % p.S, task = blockIdx.x / p.S, head = task % p.n_kv, b = task / p.n_kv % p.n_seq;
+    const int block_of = task / (p.n_kv * p.n_seq);
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < WN * NSLOT; i++) {
@@ -132,7 +109,7 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
     kv8_seq_t seq;
     const bool report = threadIdx.x == 0;
     if (!kv_seq(p.step, b, seq, p.err, report)) return;      // the same for the whole cluster
-    const int R = seq.n * p.G, r0 = (p.causal ? ntile - 1 - (int)blockIdx.x / p.S : (int)blockIdx.x / p.S) * Sh::ROWS;
+    const int R = seq.n * p.G, r0 = (p.ntile - 1 - block_of) * Sh::ROWS;
     if (r0 >= R) return;
     auto hi_of = [&](int tok) { return kv8_hi(&seq, tok, p.causal); };
     auto lo_of = [&](int tok) { return kv8_lo(&seq, tok, p.window); };
@@ -601,71 +578,12 @@ EncodeFn attn_encode_fn()
     return fn;
 }
 
-constexpr int MAX_SPLIT = 10;            // CTAs of a cluster; of 11 or more a B200 holds 7 clusters at a time
-
-// The grid of one call: `ctas` blocks of rows, at most `tiles` tiles of keys each.
-struct Work {
-    long long ntile, ctas, tiles;
-    int n_seq;
-};
-
 template <int KS, int NP, int RW, int WM, int WN, int NSLOT, int MINB>
-bool attn_launch(AttnArgs &p, const CUtensorMap &map, long long R, Work w)
+bool attn_launch(AttnArgs &p, const CUtensorMap &map, long long R, long long tiles)
 {
     using Sh = Shape<KS, RW, WM, WN, NSLOT>;
-    auto fn = kv8_attn_kernel<KS, NP, RW, WM, WN, NSLOT, MINB>;
-    w.ntile = (R + Sh::ROWS - 1) / Sh::ROWS;
-    w.ctas = w.ntile * p.n_kv * w.n_seq;
-    cudaLaunchAttribute attrs[2];
-    cudaLaunchConfig_t lc = {};
-    lc.gridDim = dim3((unsigned)w.ntile, (unsigned)p.n_kv, (unsigned)w.n_seq);
-    lc.blockDim = dim3(32 * WM * WN);
-    lc.dynamicSmemBytes = Sh::SMEM;
-    lc.stream = ctx().cur;
-    lc.attrs = attrs;
-
-    // CTAs the device holds at once, by cluster size (a property of the kernel and the device).
-    static int held[64][MAX_SPLIT + 1];
-    int *const cap = held[ctx().device & 63];
-    if (!cap[1]) {
-        TCG_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::SMEM));
-        TCG_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-        attrs[0].id = cudaLaunchAttributeClusterDimension;
-        attrs[0].val.clusterDim.y = attrs[0].val.clusterDim.z = 1;
-        cudaLaunchConfig_t one = lc;
-        one.numAttrs = 1;
-        for (int S = MAX_SPLIT; S > 1; S--) {
-            int n = 0;
-            one.gridDim = dim3((unsigned)S);
-            attrs[0].val.clusterDim.x = (unsigned)S;
-            if (cudaOccupancyMaxActiveClusters(&n, fn, &one) != cudaSuccess) {
-                cudaGetLastError();
-                n = 0;
-            }
-            cap[S] = n * S;
-        }
-        cap[1] = MINB * ctx().sms;
-    }
-    // Keys split over a cluster of S CTAs: the S with the least rounds in a row, where a wave of CTAs lasts its rounds of
-    // tiles and about two more (start, merge).
-    p.S = 1;
-    long long best = 0;
-    for (int S = 1; S <= MAX_SPLIT; S++) {
-        if (!cap[S] || (S > 1 && w.tiles < (long long)S * WN)) continue;
-        const long long rounds = ((w.tiles + S - 1) / S + WN - 1) / WN, t = (w.ctas * S + cap[S] - 1) / cap[S] * (rounds + 2);
-        if (S == 1 || t < best) best = t, p.S = S;
-    }
-    lc.gridDim.x = (unsigned)(w.ntile * p.S);
-    lc.numAttrs = pdl_attr(attrs);
-    if (p.S > 1) {
-        attrs[lc.numAttrs].id = cudaLaunchAttributeClusterDimension;
-        attrs[lc.numAttrs].val.clusterDim.x = (unsigned)p.S;
-        attrs[lc.numAttrs].val.clusterDim.y = 1;
-        attrs[lc.numAttrs].val.clusterDim.z = 1;
-        lc.numAttrs++;
-    }
-    TCG_CUDA(cudaLaunchKernelEx(&lc, fn, p, map));
-    return true;
+    p.ntile = (int)((R + Sh::ROWS - 1) / Sh::ROWS);
+    return attn_grid<kv8_attn_kernel<KS, NP, RW, WM, WN, NSLOT, MINB>>(p, dim3(32 * WM * WN), Sh::SMEM, Sh::ROWS, MINB, tiles, WN, map);
 }
 
 }  // namespace
@@ -701,12 +619,15 @@ extern "C" bool tcg_kv8_attention(void *out, const void *q, const tcg_kv8_t *c, 
     p.out_vec = (uintptr_t)out % (4 * size) == 0 && ld_out % 4 == 0;
     p.v = c->v, p.k_scale = c->k_scale, p.v_scale = c->v_scale;
     p.step = kv_step(*s);
-    p.n_pages = c->n_pages, p.n_kv = c->n_kv_head, p.D = c->head_dim, p.G = G;
+    p.n_pages = c->n_pages, p.n_kv = c->n_kv_head, p.n_seq = s->n_seq, p.D = c->head_dim, p.G = G;
     p.scale_log2 = scale * 1.44269504088896340736f;
     p.causal = causal, p.window = window, p.err = ctx().d_err;
 
-    const int rows_tc = getenv("TCROWS") ? atoi(getenv("TCROWS")) : 64;
-    if (R > rows_tc) return launch_kv8_attn_tc(p, c->k, R, s->n_seq);
+    long long keys = s->max_kv;
+    if (window && keys > (long long)window + longest) keys = (long long)window + longest;
+    const long long tiles = (keys + PAGE - 1) / PAGE;
+    if (R > 64) return launch_kv8_attn_tc(p, c->k, R, tiles);
+
     // K as [pages x heads x 64, D] bytes; a box is 64 keys of 64 dims, zeros past D
     EncodeFn fn = attn_encode_fn();
     if (!fn) return fail("cuTensorMapEncodeTiled is not available from the driver");
@@ -719,17 +640,14 @@ extern "C" bool tcg_kv8_attention(void *out, const void *q, const tcg_kv8_t *c, 
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail("cuTensorMapEncodeTiled failed (%d) for the K cache", (int)r);
 
-    long long keys = s->max_kv;
-    if (window && keys > (long long)window + longest) keys = (long long)window + longest;
-    const Work w = { 0, 0, (keys + PAGE - 1) / PAGE, s->n_seq };
-    // Up to 8 or 16 rows (a decode step): one or two warps of 8 rows, and the CTA's other warps take other tiles. More
+    // Up to 8 or 16 rows (a decode step): one or two warps of 8 rows, and the CTA's other warps take other tiles. Up to 64
     // rows share their tiles between 4 warps of 16.
     const bool big = p.D > 64;
     auto go = [&](auto digits) {
         constexpr int NP = decltype(digits)::value;
-        if (R <= 8) return big ? attn_launch<4, NP, 1, 1, 12, 2, 1>(p, map, R, w) : attn_launch<2, NP, 1, 1, 12, 4, 1>(p, map, R, w);
-        if (R <= 16) return big ? attn_launch<4, NP, 1, 2, 6, 4, 1>(p, map, R, w) : attn_launch<2, NP, 1, 2, 6, 8, 1>(p, map, R, w);
-        return big ? attn_launch<4, NP, 2, 4, 1, 6, 2>(p, map, R, w) : attn_launch<2, NP, 2, 4, 1, 8, 2>(p, map, R, w);
+        if (R <= 8) return big ? attn_launch<4, NP, 1, 1, 12, 2, 1>(p, map, R, tiles) : attn_launch<2, NP, 1, 1, 12, 4, 1>(p, map, R, tiles);
+        if (R <= 16) return big ? attn_launch<4, NP, 1, 2, 6, 4, 1>(p, map, R, tiles) : attn_launch<2, NP, 1, 2, 6, 8, 1>(p, map, R, tiles);
+        return big ? attn_launch<4, NP, 2, 4, 1, 6, 2>(p, map, R, tiles) : attn_launch<2, NP, 2, 4, 1, 8, 2>(p, map, R, tiles);
     };
     return t == GGML_TYPE_F32 ? go(std::integral_constant<int, 3>()) : go(std::integral_constant<int, 2>());
 }

@@ -17,9 +17,10 @@ struct AttnArgs {
     const int8_t *v;
     const float *k_scale, *v_scale;
     KvStep step;
-    int n_pages, n_kv, D, G;
+    int n_pages, n_kv, n_seq, D, G;
     float scale_log2;
-    int causal, window, S;
+    int causal, window;
+    int ntile, S;                        // blocks of rows a sequence; CTAs (a cluster) that share one's keys
     int *err;
 };
 
@@ -95,8 +96,96 @@ __device__ __forceinline__ void store_out(const AttnArgs &p, long long off, cons
 // gets zeros; a NaN sum (a query with a NaN or an infinity) stays NaN.
 __device__ __forceinline__ float inverse(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
 
+__device__ __forceinline__ uint32_t mapa(uint32_t a, int rank)
+{
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t a)
+{
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t a)
+{
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+constexpr int MAX_SPLIT = 10;            // CTAs of a cluster; of 11 or more a B200 holds 7 clusters at a time
+
+// Launches FN over ntile x n_seq x n_kv blocks of rows with `tiles` tiles of keys each at most, of which `groups` are
+// taken at a time, after choosing the split of the keys over a cluster of S CTAs. rows: of a block; per_sm: CTAs an SM.
+template <auto FN, typename X>
+bool attn_grid(AttnArgs &p, dim3 block, size_t smem, int rows, int per_sm, long long tiles, int groups, const X &arg)
+{
+    cudaLaunchAttribute attrs[2];
+    cudaLaunchConfig_t lc = {};
+    lc.blockDim = block;
+    lc.dynamicSmemBytes = smem;
+    lc.stream = ctx().cur;
+    lc.attrs = attrs;
+    // SMs that clusters of a size can use at once (a property of the device: its SMs come in groups that a cluster does not
+    // cross); the first call prepares the kernel, too.
+    static int usable[64][MAX_SPLIT + 1];
+    int *const sms = usable[ctx().device & 63];
+    if (!sms[1]) {
+        TCG_CUDA(cudaFuncSetAttribute(FN, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        TCG_CUDA(cudaFuncSetAttribute(FN, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        attrs[0].id = cudaLaunchAttributeClusterDimension;
+        attrs[0].val.clusterDim.y = attrs[0].val.clusterDim.z = 1;
+        cudaLaunchConfig_t one = lc;
+        one.numAttrs = 1;
+        for (int S = MAX_SPLIT; S > 1; S--) {
+            int n = 0;
+            one.gridDim = dim3((unsigned)S);
+            attrs[0].val.clusterDim.x = (unsigned)S;
+            if (cudaOccupancyMaxActiveClusters(&n, FN, &one) != cudaSuccess) {
+                cudaGetLastError();
+                n = 0;
+            }
+            sms[S] = n * S < ctx().sms ? n * S : ctx().sms;
+        }
+        sms[1] = ctx().sms;
+    }
+    // The split: the S with the least work for the busiest SM, in tiles: its CTAs' rounds of tiles and about two more each
+    // (start, merge). A second CTA on the SM fills the first one's waits: two take 1.5 times as long as one, measured.
+    const long long all = (long long)p.ntile * p.n_seq;
+    const long long full = ((long long)p.step.n_tok * p.G + rows - 1) / rows + p.n_seq;   // blocks with rows in them, at most
+    const long long ctas = all * p.n_kv, busy = (all < full ? all : full) * p.n_kv;
+    p.S = 1;
+    long long best = 0;
+    for (int S = 1; S <= MAX_SPLIT; S++) {
+        if (!sms[S] || (S > 1 && tiles < (long long)S * groups)) continue;
+        const long long n = (busy * S + sms[S] - 1) / sms[S];
+        const long long rounds = ((tiles + S - 1) / S + groups - 1) / groups, t = n * (rounds + 2) * (n > 1 && per_sm > 1 ? 3 : 4);
+        if (S == 1 || t < best) best = t, p.S = S;
+    }
+    if (ctas * p.S > 0x7fffffffll)
+        return fail("tcg_kv8_attention: %d sequences of %d row blocks and %d key heads are too many for one call", p.n_seq,
+                    p.ntile, p.n_kv);
+    lc.gridDim = dim3((unsigned)(ctas * p.S));
+    lc.numAttrs = pdl_attr(attrs);
+    if (p.S > 1) {
+        attrs[lc.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attrs[lc.numAttrs].val.clusterDim.x = (unsigned)p.S;
+        attrs[lc.numAttrs].val.clusterDim.y = 1;
+        attrs[lc.numAttrs].val.clusterDim.z = 1;
+        lc.numAttrs++;
+    }
+    TCG_CUDA(cudaLaunchKernelEx(&lc, FN, p, arg));
+    return true;
+}
+
 // The kernel for many rows (kv8_attn_tc.cu): 128 rows a CTA on the 5th-generation
-// tensor cores.
-bool launch_kv8_attn_tc(AttnArgs &p, const int8_t *k, long long R, int n_seq);
+// tensor cores. R: the most rows a sequence has, tiles: pages of keys.
+bool launch_kv8_attn_tc(AttnArgs &p, const int8_t *k, long long R, long long tiles);
 
 }  // namespace tcg

@@ -120,15 +120,17 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
     float *const xsum = xmax + TC_THREADS;
     const int tid = threadIdx.x, warp = tid >> 5, r = tid & 127, h = tid >> 7;
     const uint32_t bar_s = su32(bars), bar_o = su32(bars + 1);
-    const int head = blockIdx.y, b = blockIdx.z;
+    // grid: (rows from the last, sequence, head, rank), so that the blocks of rows with the most keys start first
+    const int rank = blockIdx.x % p.S, task = blockIdx.x / p.S, head = task % p.n_kv, b = task / p.n_kv % p.n_seq;
+    const int block_of = task / (p.n_kv * p.n_seq);
 
     pdl_wait();
     kv8_seq_t seq;
     if (!kv_seq(p.step, b, seq, p.err, tid == 0)) return;
-    const int R = seq.n * p.G, r0 = (p.causal ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x) * TC_ROWS;
+    const int R = seq.n * p.G, r0 = (p.ntile - 1 - block_of) * TC_ROWS;
     if (r0 >= R) return;
     int t0;
-    const int np = kv8_tiles(&seq, r0 / p.G, (min(r0 + TC_ROWS, R) - 1) / p.G, p.causal, p.window, 0, 1, 0, 1, &t0);
+    const int np = kv8_tiles(&seq, r0 / p.G, (min(r0 + TC_ROWS, R) - 1) / p.G, p.causal, p.window, rank, p.S, 0, 1, &t0);
 
     if (tid == 0) {
         bar_init(bar_s, 1);
@@ -147,23 +149,25 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
     const int hi = kv8_hi(&seq, tok, p.causal), lo = kv8_lo(&seq, tok, p.window);
     const long long head_off = (long long)(head * p.G + row % p.G) * p.D;
 
-    // A page's K or V in registers: 16-byte pieces tid and tid + 256. K: piece i is key i / (D / 16), dims 16 (i % (D /
-    // 16))...; V: dim i / 4, keys 16 (i % 4)...
+    // A page's K or V in registers: 16-byte pieces tid and tid + 256. K: a key's pieces side by side, but with 8 of them (D
+    // = 128) 8 lanes take the first or last 4 of two keys, which fall into 8 different bank groups when they are stored;
+    // V: dim i / 4, keys 16 (i % 4)...
     const int per = p.D / 16, pieces = 4 * p.D;
     int krow[2], kcol[2];
 #pragma unroll
     for (int u = 0; u < 2; u++) {
-        krow[u] = (tid + TC_THREADS * u) / per;
-        kcol[u] = (tid + TC_THREADS * u) % per;
+        const int i = tid + TC_THREADS * u;
+        krow[u] = per == 8 ? i >> 4 << 1 | (i >> 2 & 1) : i / per;
+        kcol[u] = per == 8 ? (i >> 3 & 1) << 2 | (i & 3) : i % per;
     }
     const long long block = (long long)p.D * PAGE;           // bytes of a (page, head)
-    auto load_pages = [&](uint4 (&x)[2][2], const int8_t *codes, int a, int z) {
+    auto load_pages = [&](uint4 (&x)[2][2], const int8_t *codes, int a, int z, bool k) {
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             const uint4 *src = (const uint4 *)(codes + ((long long)max(j ? z : a, 0) * p.n_kv + head) * block);
 #pragma unroll
             for (int u = 0; u < 2; u++)
-                if (tid + TC_THREADS * u < pieces) x[j][u] = __ldg(src + tid + TC_THREADS * u);
+                if (tid + TC_THREADS * u < pieces) x[j][u] = __ldg(src + (k ? krow[u] * per + kcol[u] : tid + TC_THREADS * u));
         }
     };
     // page i of this CTA; -1 for none, or one that does not exist
@@ -188,7 +192,7 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
 
     uint4 raw4[2][2] = {};                                   // K of a tile, then its V, then K of the next ...
     int pa = page_at(0), pb = page_at(1), na = page_at(2), nb = page_at(3);   // this tile's pages, and the next's
-    load_pages(raw4, kc, pa, pb);
+    load_pages(raw4, kc, pa, pb, true);
 
     // dims past D are zeros in Q (below); what K and V leave unwritten there only has to be finite
     if (p.D < DP) {
@@ -268,7 +272,7 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
     };
     bool ok = true;
     int last_s = -1, last_o = -1;                            // tiles of thread 0's latest commits
-    if (tid == 0) {
+    if (tid == 0 && np) {
         issue_s();
         last_s = 0;
     }
@@ -300,7 +304,7 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
         const long long at_a = (long long)max(pa, 0) * p.n_kv + head, at_b = (long long)max(pb, 0) * p.n_kv + head;
         const float sk = p.k_scale[h ? at_b : at_a];
         const float va = pa < 0 ? 0.0f : p.v_scale[at_a], vb = pb < 0 ? 0.0f : p.v_scale[at_b], sv = h ? vb : va;
-        load_pages(raw4, p.v, pa, pb);
+        load_pages(raw4, p.v, pa, pb, false);
         const float cs = cs0 * (mine < 0 ? 1.0f : sk), c = cs < 1e-37f ? 1e-37f : cs;   // not 0: a masked -inf stays -inf
         float lr = sv == sv0 || mine < 0 ? 0.0f : __log2f(__fdividef(sv, sv0));
         const bool whole = __all_sync(0xFFFFFFFFu, mine >= 0 && key0 >= lo && key0 + PAGE - 1 <= hi);
@@ -362,7 +366,7 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
             if (NP == 2) tmem_st16(lane_base + 64 * h + 32 * q + 16, p2);
         }
         l = fmaf(sum, ex2(-lr), l);
-        if (kb + 1 < tiles_n) load_pages(raw4, kc, na, nb);
+        if (kb + 1 < tiles_n) load_pages(raw4, kc, na, nb, true);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         fence_before();
         __syncthreads();                                     // P(kb) and V(kb) in place; the maxima and a group's P V read
@@ -389,17 +393,52 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
             __syncwarp();
         }
     }
-    fold(m, true);
+    fold(m, np > 0);
     xsum[tid] = l;
     __syncthreads();
-    if (ok && r0 + r < R) {
-        const float inv = inverse(xsum[r] + xsum[r + 128]);
-        const long long off = (seq.row0 + tok) * p.ld_out + head_off + DH * h;
+    if (p.S == 1) {
+        if (ok && r0 + r < R) {
+            const float inv = inverse(xsum[r] + xsum[r + 128]);
+            const long long off = (seq.row0 + tok) * p.ld_out + head_off + DH * h;
 #pragma unroll 1
-        for (int d = 0; d < DH && DH * h + d < p.D; d += 4) {
-            const float v[4] = { o[d] * inv, o[d + 1] * inv, o[d + 2] * inv, o[d + 3] * inv };
-            store_out<4>(p, off + d, v);
+            for (int d = 0; d < DH && DH * h + d < p.D; d += 4) {
+                const float v[4] = { o[d] * inv, o[d + 1] * inv, o[d + 2] * inv, o[d + 3] * inv };
+                store_out<4>(p, off + d, v);
+            }
         }
+    } else {
+        // The S CTAs of a cluster took consecutive shares of the keys: their O (over Q, K and V in shared memory, a row's
+        // 16-byte pieces permuted by the row against bank conflicts), m and l meet; each CTA joins every S-th row.
+        constexpr int P4 = DP / 4;                           // pieces of a row
+        float4 *const po = (float4 *)tiles;
+#pragma unroll 1
+        for (int d = 0; d < DH; d += 4)
+            po[r * P4 + ((DH * h + d) / 4 ^ (r & (P4 - 1)))] = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
+        if (h == 0) {
+            xmax[r] = m;
+            xmax[r + 128] = xsum[r] + xsum[r + 128];
+        }
+        const uint32_t a_po = su32(po), a_m = su32(xmax);
+        cluster_sync();
+        const int rows = min(TC_ROWS, R - r0), d4 = p.D / 4;
+        for (int i = tid; i < (rows + p.S - 1 - rank) / p.S * d4; i += TC_THREADS) {
+            const int q = rank + i / d4 * p.S, d = i % d4;
+            float top = -INFINITY, sum = 0.0f, v[4] = {};
+            for (int s = 0; s < p.S; s++) top = fmaxf(top, ld_cluster(mapa(a_m + 4 * q, s)));
+            top = top == -INFINITY ? 0.0f : top;
+            for (int s = 0; s < p.S; s++) {
+                const float w = ex2(ld_cluster(mapa(a_m + 4 * q, s)) - top);
+                const float4 x = ld_cluster4(mapa(a_po + 16 * (q * P4 + (d ^ (q & (P4 - 1)))), s));
+                sum = fmaf(w, ld_cluster(mapa(a_m + 4 * (q + 128), s)), sum);
+                v[0] = fmaf(w, x.x, v[0]), v[1] = fmaf(w, x.y, v[1]), v[2] = fmaf(w, x.z, v[2]), v[3] = fmaf(w, x.w, v[3]);
+            }
+            const float inv = inverse(sum);
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] *= inv;
+            const int row = r0 + q;
+            store_out<4>(p, (seq.row0 + row / p.G) * p.ld_out + (long long)(head * p.G + row % p.G) * p.D + 4 * d, v);
+        }
+        cluster_sync();                                      // no CTA leaves while another reads its shared memory
     }
     // MMAs that may still run (a wait gave up) must finish before TMEM is freed: thread 0 waits, bounded, for its last
     // commits.
@@ -416,28 +455,19 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
 }
 
 template <int DP, int NP>
-bool tc_launch(AttnArgs &p, const int8_t *k, long long R, int n_seq)
+bool tc_launch(AttnArgs &p, const int8_t *k, long long R, long long tiles)
 {
     using Sh = TcShape<DP, NP>;
-    auto fn = kv8_attn_tc_kernel<DP, NP>;
-    static bool ready[64];
-    const int dev = ctx().device & 63;
-    if (!ready[dev]) {
-        TCG_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::SMEM));
-        ready[dev] = true;
-    }
-    const dim3 grid((unsigned)((R + TC_ROWS - 1) / TC_ROWS), (unsigned)p.n_kv, (unsigned)n_seq);
-    TCG_CUDA(launch_pdl(fn, grid, dim3(TC_THREADS), Sh::SMEM, ctx().cur, p, k));
-    return true;
+    p.ntile = (int)((R + TC_ROWS - 1) / TC_ROWS);
+    return attn_grid<kv8_attn_tc_kernel<DP, NP>>(p, dim3(TC_THREADS), Sh::SMEM, TC_ROWS, 2, (tiles + 1) / 2, 1, k);
 }
 
 }  // namespace
 
-bool launch_kv8_attn_tc(AttnArgs &p, const int8_t *k, long long R, int n_seq)
+bool launch_kv8_attn_tc(AttnArgs &p, const int8_t *k, long long R, long long tiles)
 {
-    p.S = 1;
-    if (p.type == GGML_TYPE_F32) return p.D > 64 ? tc_launch<128, 2>(p, k, R, n_seq) : tc_launch<64, 2>(p, k, R, n_seq);
-    return p.D > 64 ? tc_launch<128, 1>(p, k, R, n_seq) : tc_launch<64, 1>(p, k, R, n_seq);
+    if (p.type == GGML_TYPE_F32) return p.D > 64 ? tc_launch<128, 2>(p, k, R, tiles) : tc_launch<64, 2>(p, k, R, tiles);
+    return p.D > 64 ? tc_launch<128, 1>(p, k, R, tiles) : tc_launch<64, 1>(p, k, R, tiles);
 }
 
 }  // namespace tcg
