@@ -275,10 +275,11 @@ typedef struct {
  * the n_tok rows of the call, which are its LAST tokens: with n of them and
  * kv_len[b] tokens in all (these included), row i stands for position
  * kv_len[b] - n + i. Position p lies in page table[b * table_ld + p / 64].
- * tok_start [n_seq + 1], kv_len [n_seq] and table are DEVICE arrays. max_new
+ * tok_start [n_seq + 1], kv_len [n_seq] and table [n_seq, table_ld] are
+ * DEVICE arrays. max_new
  * bounds every sequence's rows (a sequence with more is refused on the
  * device); max_kv is the expected longest kv_len and only sizes the launch.
- * Table entries behind a sequence's last page are never read. */
+ * Table entries behind a sequence's last page are not used. */
 typedef struct {
     const int32_t *tok_start, *kv_len, *table;
     int table_ld, n_seq, n_tok, max_new, max_kv;

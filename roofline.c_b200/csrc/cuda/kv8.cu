@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(ROWS_THREADS) append_kernel(const RowsArgs p)
 {
     __shared__ float s_max[ROWS_THREADS / 32];
     __shared__ __align__(16) uint8_t s_code[128 * S_PITCH];
-    pdl_wait();
+    lm_begin();
     kv8_place_t at;
     kv8_seq_t q;
     const int b = blockIdx.x / p.reach, side = blockIdx.z, head = blockIdx.y, D = p.D;
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) append_few_kernel(const RowsAr
 {
     const unsigned task = blockIdx.x * FEW_WARPS + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31, D = p.D, d = 4 * lane;
-    pdl_wait();
+    lm_begin();
     if (task >= tasks) return;
     const int side = task & 1, head = (task >> 1) % p.n_kv, bj = (task >> 1) / p.n_kv, b = bj / p.reach;
     kv8_place_t at;
@@ -338,7 +338,7 @@ template <typename T, int V>
 __global__ void __launch_bounds__(ROWS_THREADS) read_kernel(const RowsArgs p)
 {
     __shared__ __align__(16) uint8_t s_code[128 * S_PITCH];
-    pdl_wait();
+    lm_begin();
     kv8_place_t at;
     kv8_seq_t q;
     const int b = blockIdx.x / p.reach, side = blockIdx.z, head = blockIdx.y, D = p.D;

@@ -104,8 +104,12 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     __syncthreads();
-    pdl_wait();
+    lm_begin();
 
+    // Where the tiles start at key 0 and are this CTA's alone, the first pages are asked for along with the lengths; an
+    // entry behind the sequence's end is not used.
+    const bool from0 = p.S == 1 && !p.window;
+    const int ahead = wn + lane * WN, guess = from0 && ahead < p.step.table_ld ? p.step.table[(size_t)b * p.step.table_ld + ahead] : -1;
     kv8_seq_t seq;
     const bool report = threadIdx.x == 0;
     if (!kv_seq(p.step, b, seq, p.err, report)) return;      // the same for the whole cluster
@@ -135,7 +139,9 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
     auto page_at = [&](int i) {
         return i < mine ? kv_page(p.step, b, t0 + i * WN, p.n_pages, p.err, true) : 0;
     };
-    int page = page_at(lane), page_next = page_at(32 + lane);
+    int page = guess, page_next = page_at(32 + lane);
+    if (!from0 || (lane < mine && !kv8_page_ok(guess, p.n_pages))) page = page_at(lane);   // with its error, if it is one
+    if (lane >= mine) page = 0;
     float sk = 0.0f, sv = 0.0f;
     auto scales = [&]() {
         const long long at = (long long)max(page, 0) * p.n_kv + head;

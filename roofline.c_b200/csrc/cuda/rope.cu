@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(32 * ROPE_WARPS, Flow<T>::CTAS) rope_kernel(co
         unit_dims<V, HALF>(live[k] ? u : 0, p.n_rot, p.D, da[k], db[k]);
         turn[k] = live[k] && u * V < p.n_rot / 2;
     }
-    pdl_wait();
+    lm_begin();
     if (tok >= p.n_tok) return;
 
     // Batches of ROPE_AHEAD heads, whose loads go out together: the first before the angles are computed, with PIPE each
