@@ -104,7 +104,7 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     __syncthreads();
-    lm_begin();
+    lm_begin(p.brief);
 
     // Where the tiles start at key 0 and are this CTA's alone, the first pages are asked for along with the lengths; an
     // entry behind the sequence's end is not used.
@@ -646,13 +646,18 @@ extern "C" bool tcg_kv8_attention(void *out, const void *q, const tcg_kv8_t *c, 
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail("cuTensorMapEncodeTiled failed (%d) for the K cache", (int)r);
 
-    // Up to 8 or 16 rows (a decode step): one or two warps of 8 rows, and the CTA's other warps take other tiles. Up to 64
-    // rows share their tiles between 4 warps of 16.
+    // Warps of 8 rows (RW = 1) while the rows are few: 8, 16 or 32 rows leave 12, 6 or 3 groups of warps for other tiles.
+    // Up to 64 rows: 8 such warps where the device is not filled (17 sequences of 50 rows over a window of 1024: 13.0 us,
+    // against 15.1 with 4 warps of 16 rows), else 4 warps of 16 rows, two CTAs an SM (64 sequences of 64 rows over 2048
+    // tokens, bf16: 124 us against 153).
     const bool big = p.D > 64;
     auto go = [&](auto digits) {
         constexpr int NP = decltype(digits)::value;
         if (R <= 8) return big ? attn_launch<4, NP, 1, 1, 12, 2, 1>(p, map, R, tiles) : attn_launch<2, NP, 1, 1, 12, 4, 1>(p, map, R, tiles);
         if (R <= 16) return big ? attn_launch<4, NP, 1, 2, 6, 4, 1>(p, map, R, tiles) : attn_launch<2, NP, 1, 2, 6, 8, 1>(p, map, R, tiles);
+        if (R <= 32) return big ? attn_launch<4, NP, 1, 4, 3, 6, 1>(p, map, R, tiles) : attn_launch<2, NP, 1, 4, 3, 8, 1>(p, map, R, tiles);
+        if ((long long)p.n_kv * p.n_seq < ctx().sms)
+            return big ? attn_launch<4, NP, 1, 8, 1, 8, 1>(p, map, R, tiles) : attn_launch<2, NP, 1, 8, 1, 8, 1>(p, map, R, tiles);
         return big ? attn_launch<4, NP, 2, 4, 1, 6, 2>(p, map, R, tiles) : attn_launch<2, NP, 2, 4, 1, 8, 2>(p, map, R, tiles);
     };
     return t == GGML_TYPE_F32 ? go(std::integral_constant<int, 3>()) : go(std::integral_constant<int, 2>());

@@ -21,6 +21,7 @@ struct AttnArgs {
     float scale_log2;
     int causal, window;
     int ntile, S;                        // blocks of rows a sequence; CTAs (a cluster) that share one's keys
+    int brief;                           // a few rounds of tiles at most
     int *err;
 };
 
@@ -161,13 +162,14 @@ bool attn_grid(AttnArgs &p, dim3 block, size_t smem, int rows, int per_sm, long 
     const long long full = ((long long)p.step.n_tok * p.G + rows - 1) / rows + p.n_seq;   // blocks with rows in them, at most
     const long long ctas = all * p.n_kv, busy = (all < full ? all : full) * p.n_kv;
     p.S = 1;
-    long long best = 0;
+    long long best = 0, last = 0;
     for (int S = 1; S <= MAX_SPLIT; S++) {
         if (!sms[S] || (S > 1 && tiles < (long long)S * groups)) continue;
         const long long n = (busy * S + sms[S] - 1) / sms[S];
         const long long rounds = ((tiles + S - 1) / S + groups - 1) / groups, t = n * (rounds + 2) * (n > 1 && per_sm > 1 ? 3 : 4);
-        if (S == 1 || t < best) best = t, p.S = S;
+        if (S == 1 || t < best) best = t, p.S = S, last = rounds;
     }
+    p.brief = last <= 4;
     if (ctas * p.S > 0x7fffffffll)
         return fail("tcg_kv8_attention: %d sequences of %d row blocks and %d key heads are too many for one call", p.n_seq,
                     p.ntile, p.n_kv);

@@ -124,7 +124,7 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
     const int rank = blockIdx.x % p.S, task = blockIdx.x / p.S, head = task % p.n_kv, b = task / p.n_kv % p.n_seq;
     const int block_of = task / (p.n_kv * p.n_seq);
 
-    lm_begin();
+    lm_begin(p.brief);
     kv8_seq_t seq;
     if (!kv_seq(p.step, b, seq, p.err, tid == 0)) return;
     const int R = seq.n * p.G, r0 = (p.ntile - 1 - block_of) * TC_ROWS;

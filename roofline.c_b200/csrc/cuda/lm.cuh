@@ -46,15 +46,16 @@ template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 // Wait for the kernels before this one (programmatic dependent launch), then
-// let the next one be scheduled: where this grid leaves SMs free, the next
-// one's start overlaps this one's work. It waits in turn for this grid's
-// completion before it reads anything. A larger grid lets it come as its own
-// CTAs retire, which keeps the next grid's CTAs evenly spread.
+// let the next one be scheduled if this one is `brief`: where a short grid
+// leaves SMs free, the next one's start overlaps its work (the next one waits
+// in turn for this grid's completion before it reads anything). After a larger
+// grid it comes as the CTAs retire, which keeps its own evenly spread.
 constexpr unsigned LM_SMALL_GRID = 148;
-__device__ __forceinline__ void lm_begin()
+__device__ __forceinline__ void lm_begin(bool brief = true)
 {
     pdl_wait();
-    if (gridDim.x * gridDim.y * gridDim.z <= LM_SMALL_GRID) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (brief && gridDim.x * gridDim.y * gridDim.z <= LM_SMALL_GRID)
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
 // V consecutive elements as one access of V * sizeof(T) bytes (at most 16).
