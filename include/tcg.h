@@ -201,6 +201,7 @@ bool tcg_scale(float *out, const float *x, float s, size_t n);
  * (tcg_device_error): */
 #define TCG_ERR_KV8_LENGTHS 64  /* a sequence's rows or lengths: the whole sequence is skipped */
 #define TCG_ERR_KV8_PAGE    65  /* a page number: its tokens are not written, read as 0, and masked in attention */
+#define TCG_ERR_KV8_WAIT    66  /* a bounded wait inside attention gave up: the call's output is not valid */
 
 /* ---- rotary positions. A plain host struct, filled by tcg_rope_init and
  * the tcg_rope_scale_* calls (all host only, no GPU), passed by pointer and
@@ -289,8 +290,9 @@ typedef struct {
  * page's scale grows to max(scale, |largest new value| / 127); when it grows
  * the page's older codes become round(code * (old / new)). Codes are
  * round(x / scale), ties to even, all in fp32; a NaN is stored as 0, an
- * infinity as the largest finite value. A page that a call writes must belong
- * to one sequence of it only (pages that are only read may be shared). */
+ * infinity as the largest finite value. A page that a call writes must stand
+ * in its tables once, for one sequence (pages that are only read may be
+ * shared); otherwise what that page holds afterwards is not defined. */
 bool tcg_kv8_append(const tcg_kv8_t *c, const tcg_kv8_step_t *s, const void *k, const void *v,
                     int64_t ld_k, int64_t ld_v, ggml_type_t t);
 /* Read the step's rows back as values (code * scale, rounded to t). */

@@ -26,10 +26,25 @@
 // ring of slots, each with an mbarrier. The last warp to release a slot issues
 // the copy that refills it, so there is no producer warp.
 //
-// Work split: WM warps take 16 rows each of the same tiles, WN groups of warps
+// Rows of a warp: 16 (RW = 2), or 8 (RW = 1) with the two upper digits of Q,
+// and of P, as rows g and g + 8 of one A operand (a second one holds the third
+// digit). A decode step has few rows (G, often 4 or 8): 8 of them then cost
+// half the MMAs, accumulators and registers (64 sequences up to 8192 tokens,
+// bf16: 137 -> 109 us; one token over 131071: 88 -> 61 us).
+//
+// Work split: WM warps take their rows of the same tiles, WN groups of warps
 // take alternate tiles, and a cluster of S CTAs takes S consecutive shares of
 // the keys; partial results (m, l, O) meet in shared memory, then over
-// distributed shared memory, in a fixed order. No workspace, one launch.
+// distributed shared memory, in a fixed order. No workspace, one launch. 12
+// warps an SM with two slots each beat 8 with three (131071 tokens at S = 8:
+// 53.3 against 61.1 us): the warps' own latency, not the copies in flight,
+// was the limit.
+//
+// Bound by memory on large decode batches: 64 sequences up to 8192 tokens (32
+// query heads, 8 key heads, D = 128) 104 us, 6.2 TB/s. One token over 131071:
+// 51 us, 5.3 TB/s: clusters of 10 use 80 of 148 SMs. One token over a few
+// hundred: 6.8 us (bf16) to 8.4 us (fp32), dependent loads (lengths, page,
+// scale and tile) and the launch.
 #include "kv8_attn.cuh"
 #include "tc05.cuh"
 
@@ -206,8 +221,10 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
         odd = odd | __shfl_xor_sync(0xFFFFFFFFu, (int)odd, 1);
         odd = odd | __shfl_xor_sync(0xFFFFFFFFu, (int)odd, 2);
         constexpr float Q = NP == 3 ? 8300000.0f : 32512.0f; // the digits' largest sums
-        const float up = Q / fmaxf(m, 1e-30f);
-        qs[i] = odd ? __int_as_float(0x7FC00000) : fmaxf(m, 1e-30f) * (p.scale_log2 / Q);
+        const float lift = m < 1e-20f ? 0x1p80f : 1.0f;      // keeps Q / m finite
+        m = fmaxf(m * lift, 1e-21f);
+        const float up = Q / m;
+        qs[i] = odd ? __int_as_float(0x7FC00000) : (float)((double)m / lift * p.scale_log2 / Q);
 #pragma unroll
         for (int c = 0; c < KS / 2; c++)
 #pragma unroll
@@ -215,7 +232,7 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
                 uint32_t d[NP] = {};
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    int v = __float2int_rn(x[c][4 * w + e] * up);
+                    int v = __float2int_rn(x[c][4 * w + e] * lift * up);
 #pragma unroll
                     for (int n = 0; n < NP; n++) {
                         const int dig = (int)(int8_t)v;

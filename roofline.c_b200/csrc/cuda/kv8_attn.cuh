@@ -7,7 +7,7 @@
 namespace tcg {
 
 constexpr int PAGE = TCG_KV8_PAGE;
-constexpr int ERR_WAIT = 66;             // device error word: a tile's copy did not land in time
+constexpr int ERR_WAIT = TCG_ERR_KV8_WAIT;
 
 struct AttnArgs {
     const void *q;

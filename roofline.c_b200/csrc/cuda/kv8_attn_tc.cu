@@ -220,7 +220,8 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
         __syncthreads();
         m = fmaxf(xmax[r], xmax[r + 128]);
         odd = !(m <= 3.402823466e38f);
-        const int e = f16_scale_exp(m);
+        const int E = (__float_as_int(m) >> 23) & 0xFF;      // the largest magnitude goes to [2^14, 2^15)
+        const int e = m == 0.0f ? 0 : max(-126, min(141 - E, 126));
         const float f = odd ? 0.0f : __int_as_float((127 + e) << 23);
         // a row with a NaN or an infinity: zeros here, and a NaN factor
         cs0 = odd ? __int_as_float(0x7FC00000) : p.scale_log2 * __int_as_float((127 - e) << 23);

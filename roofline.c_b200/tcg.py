@@ -93,7 +93,7 @@ class Roofline(C.Structure):          # include/tcg.h tc_roofline_t
 
 ROPE_INTERLEAVED, ROPE_HALF, ROPE_MAX_DIM = 0, 1, 256
 KV8_PAGE = 64
-ERR_KV8_LENGTHS, ERR_KV8_PAGE = 64, 65
+ERR_KV8_LENGTHS, ERR_KV8_PAGE, ERR_KV8_WAIT = 64, 65, 66
 
 
 class Rope(C.Structure):              # include/tcg.h tcg_rope_t

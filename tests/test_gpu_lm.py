@@ -363,6 +363,8 @@ ATTN = [  # n_kv, group, d, [(new, kv)], causal, window
     (1, 32, 128, [(1, 900), (1, 2)], False, 0), (2, 4, 128, [(100, 100), (33, 200), (64, 64)], True, 0),
     (1, 1, 64, [(130, 130), (1, 1), (0, 0), (65, 1000)], True, 0), (1, 3, 112, [(70, 300)], True, 64),
     (2, 2, 64, [(40, 333), (7, 65)], False, 0), (1, 4, 48, [(257, 257)], True, 1), (1, 7, 128, [(20, 2100)], True, 0),
+    (1, 1, 128, [(65, 65), (128, 129), (129, 400)], True, 0), (2, 3, 64, [(22, 3000), (1, 5)], True, 0),
+    (150, 1, 64, [(33, 90)], True, 0), (1, 2, 32, [(16, 1000), (9, 64)], True, 100), (3, 24, 80, [(1, 1), (1, 1500)], True, 0),
 ]
 
 
@@ -389,6 +391,57 @@ def test_attention_of_peaked_and_huge_scores(lib, t):
     check_attention(lib, pool, [1, 60], 4, t, spread=30.0, seed=6)
     pool.ks[:], pool.vs[:] = 0.0, 1e-3                                   # keys of a page of zeros: equal weights
     check_attention(lib, pool, [3, 40], 4, t)
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("rows", [[1, 1], [12, 5], [70, 33]])
+def test_attention_of_pages_of_unlike_scales(lib, rows, t):
+    """Scales spread over decades from page to page, some of them zero."""
+    pool = Pool(gen(60), 2, 64, [1500, 700])
+    g = gen(61)
+    pool.ks = (10.0 ** (torch.rand(pool.ks.shape, generator=g) * 3 - 3)).cuda()
+    pool.vs = (10.0 ** (torch.rand(pool.vs.shape, generator=g) * 5 - 3)).cuda()
+    zero = pool.table[:, 3].long()
+    pool.ks[zero[0]], pool.vs[zero[1]] = 0.0, 0.0
+    check_attention(lib, pool, rows, 8, t, scale=0.02)
+    pool.vs[pool.table[0, :24].long()] = 0.0                             # nothing but zeros to add up
+    check_attention(lib, pool, rows, 8, t, scale=0.02)
+
+
+@pytest.mark.parametrize("magnitude", [1e-36, 1e-25, 1e25, 1e36])
+@pytest.mark.parametrize("rows", [[1, 1], [12, 5], [70, 33]])
+def test_attention_of_tiny_and_huge_queries(lib, rows, magnitude):
+    """Queries at the ends of fp32's range, with a scale that brings the scores back to ones of ordinary size."""
+    pool = Pool(gen(62), 2, 64, [300, 200])
+    if magnitude > 1:
+        check_attention(lib, pool, rows, 4, "f32", spread=magnitude, scale=float(np.float32(0.125 / magnitude)))
+    else:                                                                # the largest scale that is taken is 1e30
+        pool.ks *= 1e6
+        check_attention(lib, pool, rows, 4, "f32", spread=magnitude, scale=float(np.float32(min(1e30, 1e-7 / magnitude))))
+
+
+def test_a_cache_past_32_bit_offsets(lib):
+    """Pages behind the first 4 GB of codes."""
+    n_pages, n_kv, d, n = 66100, 8, 128, 200                             # 4.3 GB of K codes, as much of V
+    pool = Pool(gen(63), n_kv, d, [n])
+    small = pool.k, pool.v, pool.ks, pool.vs, pool.table.clone()
+    pool.k, pool.v = (torch.empty((n_pages,) + x.shape[1:], dtype=torch.int8, device="cuda") for x in small[:2])
+    pool.ks, pool.vs = (torch.full((n_pages, n_kv), float("nan"), device="cuda") for _ in range(2))
+    old = small[4][0, :4].long()
+    far = torch.tensor([n_pages - 1, 65600, n_pages - 3, 65536], device="cuda")
+    pool.k[far], pool.v[far], pool.ks[far], pool.vs[far] = (x[old] for x in small[:4])
+    pool.table[0, :4], pool.n = far.to(torch.int32), n_pages
+    assert int(far.min()) * n_kv * 64 * d >= 2 ** 32
+    for rows in ([1], [30]):
+        check_attention(lib, pool, rows, 16, "f32")
+    x = randn(gen(64), 70, n_kv * d)
+    s = pool.step([70])
+    call(lib.tcg_kv8_append, C.byref(pool.cache()), C.byref(s), x.data_ptr(), x.data_ptr(), n_kv * d, n_kv * d, tcg.F32)
+    out = [torch.empty_like(x) for _ in range(2)]
+    call(lib.tcg_kv8_read, out[0].data_ptr(), out[1].data_ptr(), C.byref(pool.cache()), C.byref(s), n_kv * d, n_kv * d, tcg.F32)
+    for o, sc in zip(out, (pool.ks, pool.vs)):
+        assert ((o - x).abs() <= sc[far].max() * 0.5001).all()          # half a step of the page's scale
+    check_attention(lib, pool, [70], 16, "bf16")
 
 
 def test_attention_contains_odd_queries(lib):
