@@ -46,7 +46,8 @@ void *tcg_get_stream(void);                 /* cudaStream_t                  */
 bool  tcg_set_stream(void *stream);         /* NULL: back to the library's   */
 
 /* Device-side failure flag shared by every kernel that waits on a barrier:
- * non-zero after a bounded wait gave up. Reading it synchronizes. Clearing it
+ * non-zero after a bounded wait gave up, or after a language-model operator
+ * met lengths or pages that cannot be (below). Reading it synchronizes. Clearing it
  * also resets the op API's GEMM stream-K flags; a ViT model (tcg_vit_*) that
  * saw a device error is released and uploaded again. */
 int   tcg_device_error(void);
@@ -206,9 +207,9 @@ bool tcg_scale(float *out, const float *x, float s, size_t n);
 /* ---- rotary positions. A plain host struct, filled by tcg_rope_init and
  * the tcg_rope_scale_* calls (all host only, no GPU), passed by pointer and
  * copied into each launch. Pair i of a token at position p turns by
- * p * turns[i] revolutions, reduced in 64 bits (exact to 2^-50 of a
- * revolution up to position 2^20); the rotated values are multiplied by
- * mscale. Dims from n_rot on are not rotated. */
+ * p * turns[i] revolutions, reduced in 64 bits (good to 2^-35 of a
+ * revolution at position 2^20); the rotated values are multiplied by mscale.
+ * Dims from n_rot on are not rotated. */
 #define TCG_ROPE_INTERLEAVED 0          /* pair i: dims 2i and 2i + 1             */
 #define TCG_ROPE_HALF        1          /* pair i: dims i and i + n_rot / 2       */
 #define TCG_ROPE_MAX_DIM     256

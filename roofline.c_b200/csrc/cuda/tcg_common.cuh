@@ -44,9 +44,10 @@ inline unsigned ceil_div(size_t a, size_t b) { return (unsigned)((a + b - 1) / b
 // of after that kernel's completion has been processed; it does its local
 // prologue (shared-memory barriers, TMEM allocation), then pdl_wait(), which
 // returns once every earlier kernel of the stream has completed with its
-// writes visible, before its first global load or store. No kernel signals
-// its dependents early (griddepcontrol.launch_dependents): dependents that
-// start during a tail crowd onto the few idle SMs and then run unbalanced.
+// writes visible, before its first global load or store. Large grids do not
+// signal their dependents early (griddepcontrol.launch_dependents): dependents
+// that start during a tail crowd onto the few idle SMs and then run unbalanced.
+// The language-model operators' brief grids do (lm_begin in lm.cuh).
 // Without the launch attribute pdl_wait() does nothing.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
