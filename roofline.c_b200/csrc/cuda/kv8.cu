@@ -419,7 +419,7 @@ bool rows_go(const char *who, const tcg_kv8_t *c, const tcg_kv8_step_t *s, const
     p.n_pages = c->n_pages, p.n_kv = c->n_kv_head, p.D = c->head_dim;
     const int longest = s->max_new < s->n_tok ? s->max_new : s->n_tok;
     p.reach = kv8_reach(longest);
-    p.err = ctx().d_err;
+    p.err = lm_error_word();
     const long long gx = (long long)s->n_seq * p.reach;
     if (gx > 0x7fffffffll) return fail("%s: %d sequences of up to %d tokens are too many for one call", who, s->n_seq, longest);
     const dim3 grid((unsigned)gx, (unsigned)c->n_kv_head, 2), block(ROWS_THREADS);

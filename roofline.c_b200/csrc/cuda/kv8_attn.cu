@@ -644,7 +644,7 @@ extern "C" bool tcg_kv8_attention(void *out, const void *q, const tcg_kv8_t *c, 
     p.step = kv_step(*s);
     p.n_pages = c->n_pages, p.n_kv = c->n_kv_head, p.n_seq = s->n_seq, p.D = c->head_dim, p.G = G;
     p.scale_log2 = scale * 1.44269504088896340736f;
-    p.causal = causal, p.window = window, p.err = ctx().d_err;
+    p.causal = causal, p.window = window, p.err = lm_error_word();
 
     long long keys = s->max_kv;
     if (window && keys > (long long)window + longest) keys = (long long)window + longest;

@@ -23,6 +23,9 @@ inline bool lm_ready(const char *who)
     return true;
 }
 
+// Their own device error word, apart from the one that makes a host-buffer op abort.
+inline int *lm_error_word() { return ctx().d_err + 2; }
+
 inline size_t lm_type_size(ggml_type_t t)
 {
     return t == GGML_TYPE_F32 ? 4 : t == GGML_TYPE_F16 || t == GGML_TYPE_BF16 ? 2 : 0;

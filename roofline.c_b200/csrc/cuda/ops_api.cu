@@ -10,6 +10,7 @@
 // an error.
 #include "tcg_common.cuh"
 #include "ops.h"
+#include "tcg_internal.h"
 
 #include <stdio.h>
 #include <stdlib.h>
@@ -65,7 +66,7 @@ struct Call {
     {
         if (floats && !tcg_d2h(h, dev[i], floats * sizeof(float))) die(what, tcg_last_error());
         if (!tcg_sync()) die(what, tcg_last_error());
-        const int e = tcg_device_error();
+        const int e = device_wait_error();
         if (e != 0) {
             char msg[96];
             snprintf(msg, sizeof msg, "a bounded device wait gave up (code %d)", e);

@@ -109,7 +109,7 @@ bool tcg_init(int device)
     TCG_CUDA(cudaGetDeviceProperties(&p, device));
     if (p.major != 10) return tcg::fail("device %d is sm_%d%d; libtcg is built for sm_100a", device, p.major, p.minor);
     TCG_CUDA(cudaStreamCreateWithFlags(&c.own, cudaStreamNonBlocking));
-    TCG_CUDA(cudaMalloc(&c.d_err, 4 * sizeof(int)));      // the error word, then scratch words
+    TCG_CUDA(cudaMalloc(&c.d_err, 4 * sizeof(int)));      // the error word, a scratch word, the language-model operators' error word
     TCG_CUDA(cudaMemset(c.d_err, 0, 4 * sizeof(int)));
     for (auto &e : c.ev) TCG_CUDA(cudaEventCreate(&e));
     c.device = device;
@@ -154,7 +154,7 @@ bool tcg_set_stream(void *stream)
     return true;
 }
 
-int tcg_device_error(void)
+int device_wait_error(void)
 {
     if (!ctx().ready) return -1;
     int v = 0;
@@ -166,10 +166,22 @@ int tcg_device_error(void)
     return v;
 }
 
+int tcg_device_error(void)
+{
+    if (!ctx().ready) return -1;
+    int v[3] = {};
+    if (cudaMemcpyAsync(v, ctx().d_err, sizeof v, cudaMemcpyDeviceToHost, ctx().cur) != cudaSuccess ||
+        cudaStreamSynchronize(ctx().cur) != cudaSuccess) {
+        cudaGetLastError();
+        return -1;
+    }
+    return v[0] ? v[0] : v[2];
+}
+
 bool tcg_clear_device_error(void)
 {
     if (!tcg::need_ctx()) return false;
-    TCG_CUDA(cudaMemsetAsync(ctx().d_err, 0, sizeof(int), ctx().cur));
+    TCG_CUDA(cudaMemsetAsync(ctx().d_err, 0, 3 * sizeof(int), ctx().cur));
     // a GEMM that gave up may have left stream-K flags raised
     if (ctx().gemm_work && !tcg::gemm_work_reset(*(tcg::GemmWork *)ctx().gemm_work, ctx().cur)) return false;
     return true;

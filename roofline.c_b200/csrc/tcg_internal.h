@@ -12,6 +12,11 @@ extern "C" {
 /* Sets tcg_last_error() from the C host layer; returns false. */
 bool host_fail(const char *fmt, ...) __attribute__((format(printf, 1, 2)));
 
+/* The error word of the kernels that wait on barriers alone: what a
+ * host-buffer op, which can only abort, has to heed (not the lengths or pages
+ * that a language-model operator met). Synchronizes. */
+int device_wait_error(void);
+
 /* tc_dequant's device path: host src -> device, convert, -> host dst. */
 bool tcg_dequant_host(float *dst, const void *src, size_t n, ggml_type_t t);
 

@@ -540,6 +540,27 @@ def test_device_side_refusals(gpu):
     assert (out == 0).all()
 
 
+def test_a_reported_page_leaves_other_operators_alone(gpu):
+    """The word stays raised until it is cleared, and a host-buffer op, which would abort on a failed wait, still runs."""
+    L = tcg.lib()
+    tcg.check(L.tcg_clear_device_error())
+    pool = Pool(gen(50), 1, 64, [10])
+    pool.table[0, 0] = pool.n
+    q = randn(gen(51), 1, 1, 64)
+    out = torch.empty_like(q)
+    s = pool.step([1])
+    call(L.tcg_kv8_attention, out.data_ptr(), q.data_ptr(), C.byref(pool.cache()), C.byref(s), 1, 64, 64, 0.125, True, 0, tcg.F32)
+    assert L.tcg_device_error() == tcg.ERR_KV8_PAGE
+    a, b, y = np.arange(8, dtype=np.float32), np.ones(8, np.float32), np.zeros(8, np.float32)
+    L.tc_ref_add.restype = None
+    L.tc_ref_add.argtypes = [C.c_void_p] * 3 + [C.c_size_t]
+    L.tc_ref_add(y.ctypes.data, a.ctypes.data, b.ctypes.data, 8)
+    assert np.array_equal(y, a + b)
+    assert L.tcg_device_error() == tcg.ERR_KV8_PAGE
+    tcg.check(L.tcg_clear_device_error())
+    assert L.tcg_device_error() == 0
+
+
 # ------------------------------------------------------------------ together
 
 def test_a_run_of_them_in_a_graph(lib):
