@@ -105,9 +105,6 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int wm = warp % WM, wn = warp / WM;
-    // grid: (rows from the last, sequence, head, rank), so that the blocks of rows with the most keys start first
-    const int rank = blockIdx.x % p.S, task = blockIdx.x / p.S, head = task % p.n_kv, b = task / p.n_kv % p.n_seq;
-    const int block_of = task / (p.n_kv * p.n_seq);
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < WN * NSLOT; i++) {
@@ -120,6 +117,7 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
     }
     __syncthreads();
     lm_begin(p.brief);
+    const int rank = blockIdx.x % p.S, head = blockIdx.x / p.S % p.n_kv, b = blockIdx.x / p.S / p.n_kv;
 
     // Where the tiles start at key 0 and are this CTA's alone, the first pages are asked for along with the lengths; an
     // entry behind the sequence's end is not used.
@@ -128,12 +126,12 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
     kv8_seq_t seq;
     const bool report = threadIdx.x == 0;
     if (!kv_seq(p.step, b, seq, p.err, report)) return;      // the same for the whole cluster
-    const int R = seq.n * p.G, r0 = (p.ntile - 1 - block_of) * Sh::ROWS;
-    if (r0 >= R) return;
+    const int R = seq.n * p.G;                               // one block holds them: the host picks a shape by the longest
+    if (R == 0 || R > Sh::ROWS) return;
     auto hi_of = [&](int tok) { return kv8_hi(&seq, tok, p.causal); };
     auto lo_of = [&](int tok) { return kv8_lo(&seq, tok, p.window); };
     int t0;                                                  // this warp group's tiles: t0, t0 + WN, ...
-    const int mine = kv8_tiles(&seq, r0 / p.G, (min(r0 + Sh::ROWS, R) - 1) / p.G, p.causal, p.window, rank, p.S, wn, WN, &t0);
+    const int mine = kv8_tiles(&seq, 0, (R - 1) / p.G, p.causal, p.window, rank, p.S, wn, WN, &t0);
 
     // This thread's rows.
     constexpr int RPW = 8 * RW;                              // rows of a warp
@@ -141,12 +139,12 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
     long long row_off[RW];
 #pragma unroll
     for (int i = 0; i < RW; i++) {
-        const int r = min(r0 + RPW * wm + g + 8 * i, R - 1), tok = r / p.G;
+        const int r = min(RPW * wm + g + 8 * i, R - 1), tok = r / p.G;
         hi[i] = hi_of(tok);
         lo[i] = lo_of(tok);
         row_off[i] = (long long)(head * p.G + r % p.G) * p.D;
     }
-    const int row_a = min(r0 + RPW * wm, R - 1) / p.G, row_z = min(r0 + RPW * wm + RPW - 1, R - 1) / p.G;
+    const int row_a = min(RPW * wm, R - 1) / p.G, row_z = min(RPW * wm + RPW - 1, R - 1) / p.G;
     const int all_hi = hi_of(row_a), all_lo = lo_of(row_z);  // keys that every row of the warp sees
     const int any_hi = hi_of(row_z), any_lo = lo_of(row_a);  // keys that some row of the warp sees
 
@@ -203,7 +201,7 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
     for (int i = 0; i < RW; i++) {
         float x[KS / 2][16], m = 0.0f;
         bool odd = false;                                    // a NaN or an infinity
-        const int r = min(r0 + RPW * wm + g + 8 * i, R - 1);
+        const int r = min(RPW * wm + g + 8 * i, R - 1);
         const long long off = (seq.row0 + r / p.G) * p.ld_q + row_off[i];
 #pragma unroll
         for (int c = 0; c < KS / 2; c++) {
@@ -490,7 +488,7 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
     if (WN == 1 && p.S == 1) {
 #pragma unroll
         for (int r = 0; r < RW; r++) {
-            const int row = r0 + RPW * wm + g + 8 * r;
+            const int row = RPW * wm + g + 8 * r;
             if (row >= R) continue;
             const float inv = inverse(l[r]);
             const long long off = (seq.row0 + row / p.G) * p.ld_out + row_off[r];
@@ -511,7 +509,7 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
     float *const pl = pm + WN * Sh::ROWS;
     float *const pw = pl + WN * Sh::ROWS;                    // [16][ROWS] weights of the cluster's CTAs
     float *const ps = pw + 16 * Sh::ROWS;                    // [ROWS] 1 / sum
-    const int rows = min(Sh::ROWS, R - r0), d4 = p.D / 4;
+    const int rows = R, d4 = p.D / 4;
 #pragma unroll
     for (int r = 0; r < RW; r++) {
         const int at = wn * Sh::ROWS + RPW * wm + g + 8 * r;
@@ -576,8 +574,7 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
         }
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] *= ps[r];
-        const int row = r0 + r;
-        store_out<4>(p, (seq.row0 + row / p.G) * p.ld_out + (long long)(head * p.G + row % p.G) * p.D + d, v);
+        store_out<4>(p, (seq.row0 + r / p.G) * p.ld_out + (long long)(head * p.G + r % p.G) * p.D + d, v);
     }
     if (p.S > 1) cluster_sync();                             // no CTA leaves while another reads its shared memory
 }
@@ -602,10 +599,10 @@ EncodeFn attn_encode_fn()
 }
 
 template <int KS, int NP, int RW, int WM, int WN, int NSLOT, int MINB>
-bool attn_launch(AttnArgs &p, const CUtensorMap &map, long long R, long long tiles)
+bool attn_launch(AttnArgs &p, const CUtensorMap &map, long long tiles)
 {
     using Sh = Shape<KS, RW, WM, WN, NSLOT>;
-    p.ntile = (int)((R + Sh::ROWS - 1) / Sh::ROWS);
+    p.ntile = 1;
     return attn_grid<kv8_attn_kernel<KS, NP, RW, WM, WN, NSLOT, MINB>>(p, dim3(32 * WM * WN), Sh::SMEM, Sh::ROWS, MINB, tiles, WN, map);
 }
 
@@ -649,7 +646,17 @@ extern "C" bool tcg_kv8_attention(void *out, const void *q, const tcg_kv8_t *c, 
     long long keys = s->max_kv;
     if (window && keys > (long long)window + longest) keys = (long long)window + longest;
     const long long tiles = (keys + PAGE - 1) / PAGE;
-    if (R > 64) return launch_kv8_attn_tc(p, c->k, R, tiles);
+    // More than 64 rows: 128 at a time on tcgen05. A batch whose longest sequence has twice the rows of the mean may be a
+    // prompt among decode steps: sequences of one token, or of as many rows as the shape for one token holds, go to the
+    // kernel for few rows, in a launch of their own.
+    const bool many = R > 64, mixed = many && G <= 64 && s->n_seq >= 4 && 2ll * s->n_tok < (long long)s->n_seq * longest;
+    const long long rows = !mixed ? R : G <= 8 ? 8 : G <= 16 ? 16 : G <= 32 ? 32 : 64;
+    if (many) {
+        p.row_min = mixed ? (int)rows : 0;
+        if (!launch_kv8_attn_tc(p, c->k, R, tiles)) return false;
+        if (!mixed) return true;
+        p.row_min = 0;
+    }
 
     // K as [pages x heads x 64, D] bytes; a box is 64 keys of 64 dims, zeros past D
     EncodeFn fn = attn_encode_fn();
@@ -670,12 +677,12 @@ extern "C" bool tcg_kv8_attention(void *out, const void *q, const tcg_kv8_t *c, 
     const bool big = p.D > 64;
     auto go = [&](auto digits) {
         constexpr int NP = decltype(digits)::value;
-        if (R <= 8) return big ? attn_launch<4, NP, 1, 1, 12, 2, 1>(p, map, R, tiles) : attn_launch<2, NP, 1, 1, 12, 4, 1>(p, map, R, tiles);
-        if (R <= 16) return big ? attn_launch<4, NP, 1, 2, 6, 4, 1>(p, map, R, tiles) : attn_launch<2, NP, 1, 2, 6, 8, 1>(p, map, R, tiles);
-        if (R <= 32) return big ? attn_launch<4, NP, 1, 4, 3, 6, 1>(p, map, R, tiles) : attn_launch<2, NP, 1, 4, 3, 8, 1>(p, map, R, tiles);
+        if (rows <= 8) return big ? attn_launch<4, NP, 1, 1, 12, 2, 1>(p, map, tiles) : attn_launch<2, NP, 1, 1, 12, 4, 1>(p, map, tiles);
+        if (rows <= 16) return big ? attn_launch<4, NP, 1, 2, 6, 4, 1>(p, map, tiles) : attn_launch<2, NP, 1, 2, 6, 8, 1>(p, map, tiles);
+        if (rows <= 32) return big ? attn_launch<4, NP, 1, 4, 3, 6, 1>(p, map, tiles) : attn_launch<2, NP, 1, 4, 3, 8, 1>(p, map, tiles);
         if ((long long)p.n_kv * p.n_seq < ctx().sms)
-            return big ? attn_launch<4, NP, 1, 8, 1, 8, 1>(p, map, R, tiles) : attn_launch<2, NP, 1, 8, 1, 8, 1>(p, map, R, tiles);
-        return big ? attn_launch<4, NP, 2, 4, 1, 6, 2>(p, map, R, tiles) : attn_launch<2, NP, 2, 4, 1, 8, 2>(p, map, R, tiles);
+            return big ? attn_launch<4, NP, 1, 8, 1, 8, 1>(p, map, tiles) : attn_launch<2, NP, 1, 8, 1, 8, 1>(p, map, tiles);
+        return big ? attn_launch<4, NP, 2, 4, 1, 6, 2>(p, map, tiles) : attn_launch<2, NP, 2, 4, 1, 8, 2>(p, map, tiles);
     };
     return t == GGML_TYPE_F32 ? go(std::integral_constant<int, 3>()) : go(std::integral_constant<int, 2>());
 }

@@ -22,6 +22,8 @@ struct AttnArgs {
     int causal, window;
     int ntile, S;                        // blocks of rows a sequence; CTAs (a cluster) that share one's keys
     int brief;                           // a few rounds of tiles at most
+    int row_min;                         // only sequences of more than row_min rows (the kernel for many rows)
+    int compact;                         // blocks of rows are dealt out by the lengths, not by (ntile, n_seq)
     int *err;
 };
 
@@ -159,12 +161,14 @@ bool attn_grid(AttnArgs &p, dim3 block, size_t smem, int rows, int per_sm, long 
     // The split: the S with the least work for the busiest SM, in tiles: its CTAs' rounds of tiles and about two more each
     // (start, merge). A second CTA on the SM fills the first one's waits: two take 1.5 times as long as one, measured.
     const long long all = (long long)p.ntile * p.n_seq;
-    const long long full = ((long long)p.step.n_tok * p.G + rows - 1) / rows + p.n_seq;   // blocks with rows in them, at most
-    const long long ctas = all * p.n_kv, busy = (all < full ? all : full) * p.n_kv;
+    const long long even = ((long long)p.step.n_tok * p.G + rows - 1) / rows, full = even + p.n_seq;   // with rows, at most
+    p.compact = all > 2 * full + 64;                         // and one block more, which sees every sequence
+    const long long ctas = (p.compact ? full + 1 : all) * p.n_kv, likely = p.row_min ? even + 1 : full;
+    const long long busy = (all < likely ? all : likely) * p.n_kv;
     p.S = 1;
     long long best = 0, last = 0;
     for (int S = 1; S <= MAX_SPLIT; S++) {
-        if (!sms[S] || (S > 1 && tiles < (long long)S * groups)) continue;
+        if (!sms[S] || (S > 1 && tiles < (long long)S * groups) || (p.compact && S > 2)) continue;   // compact: most are empty
         const long long n = (busy * S + sms[S] - 1) / sms[S];
         const long long rounds = ((tiles + S - 1) / S + groups - 1) / groups, t = n * (rounds + 2) * (n > 1 && per_sm > 1 ? 3 : 4);
         if (S == 1 || t < best) best = t, p.S = S, last = rounds;

@@ -105,6 +105,71 @@ __device__ __forceinline__ void store_codes(uint8_t *tile, int r, int c, uint4 r
     *(uint4 *)(tile + chunk_at(r, c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
 }
 
+// The block of rows that number `want` over all sequences with rows in this launch stands for, found by a warp
+// from the lengths; false behind the last one. For batches of unlike lengths (one prompt among decode steps), where a
+// grid of ntile x n_seq would be nearly empty. A warp that finds none has seen, and reported, every sequence.
+__device__ __forceinline__ bool find_block(const AttnArgs &p, int want, int &b, int &block)
+{
+    constexpr int SETS = 4;                                  // of 32 sequences, whose lengths are asked for together
+    const int lane = threadIdx.x & 31;
+    int before = 0;
+    for (int s0 = 0; s0 < p.n_seq; s0 += 32 * SETS) {
+        int n[SETS];
+#pragma unroll
+        for (int k = 0; k < SETS; k++) {
+            const int s = s0 + 32 * k + lane;
+            kv8_seq_t q;
+            n[k] = 0;
+            if (s < p.n_seq && kv_seq(p.step, s, q, p.err, true)) {
+                const int R = q.n * p.G;
+                if (R > p.row_min) n[k] = (R + TC_ROWS - 1) / TC_ROWS;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < SETS; k++) {
+            int upto = n[k];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            const unsigned past = __ballot_sync(0xFFFFFFFFu, before + upto > want);
+            if (past) {
+                const int l = __ffs((int)past) - 1;
+                b = s0 + 32 * k + l;
+                block = want - before - __shfl_sync(0xFFFFFFFFu, upto - n[k], l);
+                return true;
+            }
+            before += __shfl_sync(0xFFFFFFFFu, upto, 31);
+        }
+    }
+    return false;
+}
+
+// This CTA's sequence, block of rows, key head and rank in its cluster; `shared`: two words that nothing else uses. Grid:
+// (rows from the last, sequence, head, rank), so that the blocks with the most keys start first. False, for the whole CTA
+// and cluster, where there is none.
+__device__ __forceinline__ bool place_block(const AttnArgs &p, int *shared, int &b, int &block, int &head, int &rank)
+{
+    const int task = blockIdx.x / p.S, row_task = task / p.n_kv;
+    rank = blockIdx.x % p.S;
+    head = task % p.n_kv;
+    if (!p.compact) {
+        b = row_task % p.n_seq;
+        block = p.ntile - 1 - row_task / p.n_seq;
+        return true;
+    }
+    if (threadIdx.x < 32) {
+        int x = -1, y = 0;
+        if (!find_block(p, row_task, x, y)) x = -1;
+        if (threadIdx.x == 0) shared[0] = x, shared[1] = y;
+    }
+    __syncthreads();
+    b = shared[0];
+    block = shared[1];
+    return b >= 0;
+}
+
 template <int DP, int NP>
 __global__ void __launch_bounds__(TC_THREADS, 2)
 kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict__ kc)
@@ -120,15 +185,13 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
     float *const xsum = xmax + TC_THREADS;
     const int tid = threadIdx.x, warp = tid >> 5, r = tid & 127, h = tid >> 7;
     const uint32_t bar_s = su32(bars), bar_o = su32(bars + 1);
-    // grid: (rows from the last, sequence, head, rank), so that the blocks of rows with the most keys start first
-    const int rank = blockIdx.x % p.S, task = blockIdx.x / p.S, head = task % p.n_kv, b = task / p.n_kv % p.n_seq;
-    const int block_of = task / (p.n_kv * p.n_seq);
-
     lm_begin(p.brief);
+    int b, block_of, head, rank;
+    if (!place_block(p, (int *)tmem_slot + 2, b, block_of, head, rank)) return;
     kv8_seq_t seq;
     if (!kv_seq(p.step, b, seq, p.err, tid == 0)) return;
-    const int R = seq.n * p.G, r0 = (p.ntile - 1 - block_of) * TC_ROWS;
-    if (r0 >= R) return;
+    const int R = seq.n * p.G, r0 = block_of * TC_ROWS;
+    if (r0 >= R || R <= p.row_min) return;
     int t0;
     const int np = kv8_tiles(&seq, r0 / p.G, (min(r0 + TC_ROWS, R) - 1) / p.G, p.causal, p.window, rank, p.S, 0, 1, &t0);
 

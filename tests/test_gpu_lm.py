@@ -468,6 +468,47 @@ def test_long_cache_and_launch_hints(lib):
         check_attention(lib, pool, [30], 4, "bf16", max_kv=hint, max_new=31)
 
 
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("group,d", [(1, 64), (4, 128), (20, 64)])
+def test_attention_of_a_prompt_among_decode_steps(lib, group, d, t):
+    """Sequences of unlike lengths: blocks of rows dealt out by the lengths, short sequences in a launch of their own."""
+    g = torch.Generator().manual_seed(70)
+    seqs = [(1, int(torch.randint(1, 900, (1,), generator=g))) for _ in range(90)]
+    seqs[17], seqs[40], seqs[41], seqs[89] = (700, 900), (0, 33), (5, 70), (33, 33)
+    pool = Pool(gen(71), 1, d, [b for _, b in seqs])
+    check_attention(lib, pool, [a for a, _ in seqs], group, t, pad=3)
+    check_attention(lib, pool, [a for a, _ in seqs], group, t, window=100)
+    check_attention(lib, pool, [0] * 89 + [33], group, t, max_new=33)   # nothing but one
+
+
+def test_bad_lengths_among_unlike_sequences(gpu):
+    """A refused sequence is reported and the others are right, wherever the blocks of rows come from."""
+    L = tcg.lib()
+    tcg.check(L.tcg_clear_device_error())
+    lens = [1] * 80
+    lens[50] = 600
+    kv = [40] * 80
+    kv[50] = 640
+    pool = Pool(gen(72), 1, 64, kv)
+    q = randn(gen(73), sum(lens), 4, 64)
+    want = torch.empty_like(q)
+    s = pool.step(lens)
+    args = (4, 256, 256, 0.125, True, 0, tcg.F32)
+    call(L.tcg_kv8_attention, want.data_ptr(), q.data_ptr(), C.byref(pool.cache()), C.byref(s), *args)
+    assert L.tcg_device_error() == 0
+    for bad in (0, 50, 79):
+        kv2 = list(kv)
+        kv2[bad] = 10 ** 6
+        s, out = pool.step(lens, kv=kv2), torch.full_like(q, 7.0)
+        call(L.tcg_kv8_attention, out.data_ptr(), q.data_ptr(), C.byref(pool.cache()), C.byref(s), *args)
+        assert L.tcg_device_error() == tcg.ERR_KV8_LENGTHS
+        tcg.check(L.tcg_clear_device_error())
+        at = sum(lens[:bad])
+        mine = torch.zeros(len(q), dtype=torch.bool, device="cuda")
+        mine[at:at + lens[bad]] = True
+        assert (out[mine] == 7).all() and torch.equal(out[~mine], want[~mine])
+
+
 def test_device_side_refusals(gpu):
     """Lengths and pages that cannot be: skipped on the device, reported, and everything else is right."""
     L = tcg.lib()
