@@ -686,6 +686,47 @@ def test_a_run_of_them_in_a_graph(lib):
         tcg.check(lib.tcg_set_stream(None))
 
 
+CAPTURED_FIRST = """
+import sys, torch
+sys.path[:0] = sys.argv[1:3]
+import tcg, test_gpu_lm as T
+tcg.init(0)
+L, g = tcg.lib(), T.gen(80)
+pool = T.Pool(g, 2, 64, [300, 90])
+for new in ([1, 1], [3, 20], [40, 33]):
+    q, out = T.randn(g, sum(new), 8, 64), torch.zeros((sum(new), 8, 64), device="cuda")
+    x = T.randn(g, sum(new), 128)
+    pos, r = torch.arange(sum(new), dtype=torch.int32, device="cuda"), T.plan(64, 64, True)
+    s = pool.step(new)
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    tcg.check(L.tcg_set_stream(stream.cuda_stream))
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        tcg.check(L.tcg_rope(x.data_ptr(), x.data_ptr(), pos.data_ptr(), T.C.byref(r), sum(new), 2, 128, 128, 0))
+        tcg.check(L.tcg_kv8_append(T.C.byref(pool.cache()), T.C.byref(s), x.data_ptr(), x.data_ptr(), 128, 128, 0))
+        tcg.check(L.tcg_kv8_attention(out.data_ptr(), q.data_ptr(), T.C.byref(pool.cache()), T.C.byref(s), 8, 512, 512,
+                                      0.125, True, 0, 0))
+    graph.replay()
+    torch.cuda.synchronize()
+    tcg.check(L.tcg_set_stream(None))
+    want, tol = T.attention(pool, q, new, pool.kv, 4, 0.125, True, 0, "f32")
+    assert ((out.double().cpu() - want).abs() <= tol).all()
+assert L.tcg_device_error() == 0
+print("captured")
+"""
+
+
+def test_first_calls_inside_a_capture():
+    """A process whose first call of each operator is captured: nothing that a capture forbids happens in it."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    pkg = os.path.join(os.path.dirname(here), "roofline.c_b200")
+    out = subprocess.run([sys.executable, "-c", CAPTURED_FIRST, here, pkg], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "captured" in out.stdout, out.stderr[-2000:]
+
+
 def test_two_streams_at_once(lib):
     """The operators keep nothing between calls: two streams' calls over one cache do not disturb each other."""
     pool = Pool(gen(40), 4, 128, [5000, 3000])
