@@ -78,29 +78,53 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
-template <int KS, int RW, int WM, int WN, int NSLOT>
+// 4 consecutive values of a query row.
+__device__ __forceinline__ void load_q4(const AttnArgs &p, long long off, float (&x)[4])
+{
+    if (p.type == GGML_TYPE_F32) {
+        const float *s = (const float *)p.q + off;
+        if (p.q_vec) load_pack<float, 4>(s, x);
+        else
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = s[e];
+        return;
+    }
+    const unsigned short *s = (const unsigned short *)p.q + off;
+    ushort4 v;
+    if (p.q_vec) v = *(const ushort4 *)s;
+    else v = make_ushort4(s[0], s[1], s[2], s[3]);
+    const unsigned short h[4] = { v.x, v.y, v.z, v.w };
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        x[e] = p.type == GGML_TYPE_BF16 ? __uint_as_float((uint32_t)h[e] << 16) : __half2float(__ushort_as_half(h[e]));
+}
+
+template <int KS, int NP, int RW, int WM, int WN, int NSLOT>
 struct Shape {
     static constexpr int DP = KS * 32;                       // dims, padded
     static constexpr int SLOT = PAGE * DP;                   // bytes of a K or V tile
     static constexpr int RING = WN * NSLOT * SLOT;
     static constexpr int ROWS = 8 * RW * WM;
     static constexpr int PITCH = DP + 8;                     // floats of a partial O row
-    static constexpr int EXCH = (WN * ROWS * (PITCH + 2) + 18 * ROWS) * 4;   // partial O, m, l; weights of <= 16 CTAs, sum
+    static constexpr int EXCH = (WN * ROWS * (PITCH + 2) + 2 * ROWS) * 4;    // partial O, m, l; the CTA's m, l
     static constexpr int BODY = RING > EXCH ? RING : EXCH;
-    static_assert(BODY % 16 == 0, "the barriers follow");
-    static constexpr size_t SMEM = 128 + BODY + WN * NSLOT * 12 + 16;
+    static constexpr int Q_PITCH = DP / 4 + 4;               // words of a row of Q digits: 8 rows in 8 bank groups
+    static constexpr int QROWS = WN > 1 ? ROWS : 0;          // digits, factors, barriers
+    static constexpr int QD = BODY, QS = QD + NP * QROWS * Q_PITCH * 4, BARS = QS + QROWS * 4;
+    static_assert(BODY % 16 == 0 && BARS % 16 == 0, "alignment");
+    static constexpr size_t SMEM = 128 + BARS + WN * NSLOT * 12 + 16;
 };
 
 template <int KS, int NP, int RW, int WM, int WN, int NSLOT, int MINB>
 __global__ void __launch_bounds__(32 * WM * WN, MINB)
 kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUtensorMap kmap)
 {
-    using Sh = Shape<KS, RW, WM, WN, NSLOT>;
+    using Sh = Shape<KS, NP, RW, WM, WN, NSLOT>;
     constexpr int NT = KS * 4;                               // 8-dim output tiles
     extern __shared__ uint8_t raw[];
     uint8_t *const base = (uint8_t *)(((uintptr_t)raw + 127) & ~(uintptr_t)127);
-    const uint32_t ring = su32(base), bars = ring + Sh::BODY;
-    int *const count = (int *)(base + Sh::BODY + WN * NSLOT * 8);
+    const uint32_t ring = su32(base), bars = ring + Sh::BARS;
+    int *const count = (int *)(base + Sh::BARS + WN * NSLOT * 8);
     volatile int *const abort = (volatile int *)(count + WN * NSLOT);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -191,46 +215,101 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
     }
     scales();
 
-    // Q digits, in the k order of the tiles: k-step 2 c + s of chunk c takes bytes 64 c + 16 t + 8 s + 0..7.
-    // RW = 2: qd[n] is digit n's A fragment. RW = 1: the first fragment holds the two upper digits, as rows g and g + 8;
-    // with three digits a second one holds the lowest as row g + 8.
+    // A fragments, in the k order of the tiles: k-step 2 c + s of chunk c takes bytes 64 c + 16 t + 8 s + 0..7. RW = 2:
+    // qd[n] is digit n's. RW = 1: the first fragment holds the two upper digits, as rows g and g + 8; with three digits a
+    // second one holds the lowest as row g + 8.
     constexpr int NA = RW == 2 ? NP : NP - 1;                // A fragments, mma's per product
     uint32_t qd[NA][KS][4] = {};
     float qs[RW];
+    constexpr float Q = NP == 3 ? 8300000.0f : 32512.0f;     // the digits' largest sums
+    if constexpr (WN == 1) {
+        // each thread the digits of its own fragments
 #pragma unroll
-    for (int i = 0; i < RW; i++) {
-        float x[KS / 2][16], m = 0.0f;
-        bool odd = false;                                    // a NaN or an infinity
-        const int r = min(RPW * wm + g + 8 * i, R - 1);
-        const long long off = (seq.row0 + r / p.G) * p.ld_q + row_off[i];
+        for (int i = 0; i < RW; i++) {
+            float x[KS / 2][16], m = 0.0f;
+            bool odd = false;                                    // a NaN or an infinity
+            const int r = min(RPW * wm + g + 8 * i, R - 1);
+            const long long off = (seq.row0 + r / p.G) * p.ld_q + row_off[i];
 #pragma unroll
-        for (int c = 0; c < KS / 2; c++) {
+            for (int c = 0; c < KS / 2; c++) {
 #pragma unroll
-            for (int e = 0; e < 16; e++) x[c][e] = 0.0f;
-            if (64 * c + 16 * t < p.D) load_q16(p, off + 64 * c + 16 * t, x[c]);
+                for (int e = 0; e < 16; e++) x[c][e] = 0.0f;
+                if (64 * c + 16 * t < p.D) load_q16(p, off + 64 * c + 16 * t, x[c]);
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                odd |= !(fabsf(x[c][e]) <= 3.402823466e38f);
-                m = fmaxf(m, fabsf(x[c][e]));
+                for (int e = 0; e < 16; e++) {
+                    odd |= !(fabsf(x[c][e]) <= 3.402823466e38f);
+                    m = fmaxf(m, fabsf(x[c][e]));
+                }
             }
+            m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+            m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+            odd = odd | __shfl_xor_sync(0xFFFFFFFFu, (int)odd, 1);
+            odd = odd | __shfl_xor_sync(0xFFFFFFFFu, (int)odd, 2);
+            const float lift = m < 1e-20f ? 0x1p80f : 1.0f;      // keeps Q / m finite
+            const double back = m < 1e-20f ? 0x1p-80 : 1.0;
+            m = fmaxf(m * lift, 1e-21f);
+            const float up = Q / m;
+            qs[i] = odd ? __int_as_float(0x7FC00000) : (float)((double)m * back * (double)p.scale_log2 * (1.0 / Q));
+#pragma unroll
+            for (int c = 0; c < KS / 2; c++)
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    uint32_t d[NP] = {};
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        int v = __float2int_rn(x[c][4 * w + e] * lift * up);
+#pragma unroll
+                        for (int n = 0; n < NP; n++) {
+                            const int dig = (int)(int8_t)v;
+                            d[n] |= (uint32_t)(dig & 0xFF) << (8 * e);
+                            v = (v - dig) >> 8;
+                        }
+                    }
+                    if (RW == 2) {
+#pragma unroll
+                        for (int n = 0; n < NP; n++) qd[n % NA][2 * c + (w >> 1)][2 * (w & 1) + i] = d[n];
+                    } else {
+                        qd[0][2 * c + (w >> 1)][2 * (w & 1)] = d[NP - 1];
+                        qd[0][2 * c + (w >> 1)][2 * (w & 1) + 1] = d[NP - 2];
+                        if (NP == 3) qd[NA - 1][2 * c + (w >> 1)][2 * (w & 1) + 1] = d[0];
+                    }
+                }
         }
-        m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-        m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
-        odd = odd | __shfl_xor_sync(0xFFFFFFFFu, (int)odd, 1);
-        odd = odd | __shfl_xor_sync(0xFFFFFFFFu, (int)odd, 2);
-        constexpr float Q = NP == 3 ? 8300000.0f : 32512.0f; // the digits' largest sums
-        const float lift = m < 1e-20f ? 0x1p80f : 1.0f;      // keeps Q / m finite
-        m = fmaxf(m * lift, 1e-21f);
-        const float up = Q / m;
-        qs[i] = odd ? __int_as_float(0x7FC00000) : (float)((double)m / lift * p.scale_log2 / Q);
+    } else {
+        // The WN groups need the same digits: a warp a row, 4 dims a lane, through shared memory (one token over 513, fp32:
+        // 8.5 -> 7.1 us). With one group the shuffles cost more than they save (64 x 16 rows, bf16: 148 against 123 us).
+        uint32_t *const sq = (uint32_t *)(base + Sh::QD);        // [NP][ROWS][Q_PITCH], lowest digit first
+        float *const sqs = (float *)(base + Sh::QS);
+        constexpr int EACH = (Sh::ROWS + WM * WN - 1) / (WM * WN), AT_ONCE = EACH < 8 ? EACH : 8;   // rows whose loads go together
+        static_assert(EACH <= 32, "a lane keeps what belongs to one of the warp's rows");
+        const int my_row = min(warp + lane * WM * WN, R - 1);    // of the warp's lane-th row: where it lies, its largest value
+        const long long my_off = (seq.row0 + my_row / p.G) * p.ld_q + (long long)(head * p.G + my_row % p.G) * p.D;
+        float my_max = 0.0f;
 #pragma unroll
-        for (int c = 0; c < KS / 2; c++)
+        for (int k0 = 0; k0 < EACH; k0 += AT_ONCE) {
+            float x[AT_ONCE][4] = {};
 #pragma unroll
-            for (int w = 0; w < 4; w++) {
+            for (int k = 0; k < AT_ONCE; k++) {
+                const long long off = __shfl_sync(0xFFFFFFFFu, my_off, k0 + k);
+                if (4 * lane < p.D) load_q4(p, off + 4 * lane, x[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; k++) {
+                const int r = warp + (k0 + k) * WM * WN;
+                float m = fmaxf(fmaxf(fabsf(x[k][0]), fabsf(x[k][1])), fmaxf(fabsf(x[k][2]), fabsf(x[k][3])));
+                // NaN where the row has a NaN or an infinity: fmaxf drops a NaN, the sum of x * 0 does not
+                m += (x[k][0] * 0.0f + x[k][1] * 0.0f) + (x[k][2] * 0.0f + x[k][3] * 0.0f);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) {
+                    const float y = __shfl_xor_sync(0xFFFFFFFFu, m, o);
+                    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(m), "f"(y));
+                }
+                my_max = lane == k0 + k ? m : my_max;
+                const float lift = m < 1e-20f ? 0x1p80f : 1.0f, up = Q / fmaxf(m * lift, 1e-21f);   // lift keeps Q / m finite
                 uint32_t d[NP] = {};
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    int v = __float2int_rn(x[c][4 * w + e] * lift * up);
+                    int v = __float2int_rn(x[k][e] * lift * up);
 #pragma unroll
                     for (int n = 0; n < NP; n++) {
                         const int dig = (int)(int8_t)v;
@@ -238,15 +317,36 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
                         v = (v - dig) >> 8;
                     }
                 }
-                if (RW == 2) {
+                if (r < Sh::ROWS && 4 * lane < Sh::DP)
 #pragma unroll
-                    for (int n = 0; n < NP; n++) qd[n % NA][2 * c + (w >> 1)][2 * (w & 1) + i] = d[n];
-                } else {
-                    qd[0][2 * c + (w >> 1)][2 * (w & 1)] = d[NP - 1];
-                    qd[0][2 * c + (w >> 1)][2 * (w & 1) + 1] = d[NP - 2];
-                    if (NP == 3) qd[NA - 1][2 * c + (w >> 1)][2 * (w & 1) + 1] = d[0];
-                }
+                    for (int n = 0; n < NP; n++) sq[(n * Sh::ROWS + r) * Sh::Q_PITCH + lane] = d[n];
             }
+        }
+        if (lane < EACH && warp + lane * WM * WN < Sh::ROWS) {
+            // the factor of the row: NaN stays NaN
+            const double m = my_max < 1e-20f ? fmax((double)my_max * 0x1p80, 1e-21) * 0x1p-80 : (double)my_max;
+            sqs[warp + lane * WM * WN] = (float)(m * (double)p.scale_log2 * (1.0 / Q));
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < RW; i++) {
+            const int r = RPW * wm + g + 8 * i;
+            qs[i] = sqs[r];
+#pragma unroll
+            for (int n = 0; n < NP; n++)
+#pragma unroll
+                for (int c = 0; c < KS / 2; c++) {
+                    const uint4 v = *(const uint4 *)(sq + (n * Sh::ROWS + r) * Sh::Q_PITCH + 16 * c + 4 * t);
+                    const uint32_t w[4] = { v.x, v.y, v.z, v.w };
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        if (RW == 2) qd[n % NA][2 * c + (k >> 1)][2 * (k & 1) + i] = w[k];
+                        else if (n == NP - 1) qd[0][2 * c + (k >> 1)][2 * (k & 1)] = w[k];
+                        else if (n == NP - 2) qd[0][2 * c + (k >> 1)][2 * (k & 1) + 1] = w[k];
+                        else qd[NA - 1][2 * c + (k >> 1)][2 * (k & 1) + 1] = w[k];
+                    }
+                }
+        }
     }
 
     float o[NT][2 * RW], m[RW], l[RW];
@@ -507,8 +607,8 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
     float *const po = (float *)base;                         // [WN][ROWS][PITCH]
     float *const pm = po + WN * Sh::ROWS * Sh::PITCH;        // [WN][ROWS]
     float *const pl = pm + WN * Sh::ROWS;
-    float *const pw = pl + WN * Sh::ROWS;                    // [16][ROWS] weights of the cluster's CTAs
-    float *const ps = pw + 16 * Sh::ROWS;                    // [ROWS] 1 / sum
+    float *const qm = pl + WN * Sh::ROWS;                    // [ROWS] the CTA's
+    float *const ql = qm + Sh::ROWS;
     const int rows = R, d4 = p.D / 4;
 #pragma unroll
     for (int r = 0; r < RW; r++) {
@@ -522,62 +622,41 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
         }
     }
     __syncthreads();
-    if (WN > 1) {
-        for (int i = threadIdx.x; i < rows * d4; i += blockDim.x) {
-            const int r = i / d4, d = 4 * (i % d4);
-            float top = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < WN; w++) top = fmaxf(top, pm[w * Sh::ROWS + r]);
-            top = top == -INFINITY ? 0.0f : top;
-            float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-            for (int w = 0; w < WN; w++) {
-                const float a = ex2(pm[w * Sh::ROWS + r] - top);
-                const float4 v = *(const float4 *)(po + (w * Sh::ROWS + r) * Sh::PITCH + d);
-                s.x = fmaf(a, v.x, s.x), s.y = fmaf(a, v.y, s.y), s.z = fmaf(a, v.z, s.z), s.w = fmaf(a, v.w, s.w);
-            }
-            *(float4 *)(po + r * Sh::PITCH + d) = s;         // group 0's place: read by this thread only
-        }
-        __syncthreads();
-        if ((int)threadIdx.x < rows) {
-            const int r = threadIdx.x;
-            float top = -INFINITY, sum = 0.0f;
-            for (int w = 0; w < WN; w++) top = fmaxf(top, pm[w * Sh::ROWS + r]);
-            for (int w = 0; w < WN; w++) sum += pl[w * Sh::ROWS + r] * ex2(pm[w * Sh::ROWS + r] - (top == -INFINITY ? 0.0f : top));
-            pm[r] = top;
-            pl[r] = sum;
-        }
-        __syncthreads();
-    }
-    const uint32_t a_po = su32(po), a_pm = su32(pm), a_pl = su32(pl);
-    if (p.S > 1) cluster_sync();
-    for (int r = threadIdx.x; r < rows; r += blockDim.x) {
-        float top = -INFINITY, sum = 0.0f;
-        for (int s = 0; s < p.S; s++) top = fmaxf(top, p.S > 1 ? ld_cluster(mapa(a_pm + 4 * r, s)) : pm[r]);
-        top = top == -INFINITY ? 0.0f : top;
-        for (int s = 0; s < p.S; s++) {
-            const float a = ex2((p.S > 1 ? ld_cluster(mapa(a_pm + 4 * r, s)) : pm[r]) - top);
-            pw[s * Sh::ROWS + r] = a;
-            sum = fmaf(a, p.S > 1 ? ld_cluster(mapa(a_pl + 4 * r, s)) : pl[r], sum);
-        }
-        ps[r] = inverse(sum);
-    }
-    __syncthreads();
-    for (int i = threadIdx.x + rank * blockDim.x; i < rows * d4; i += blockDim.x * p.S) {
+    for (int i = threadIdx.x; i < rows * d4; i += blockDim.x) {
         const int r = i / d4, d = 4 * (i % d4);
-        float v[4] = {};
-        for (int s = 0; s < p.S; s++) {
-            const uint32_t at = a_po + 4 * (r * Sh::PITCH + d);
-            const float4 x = p.S > 1 ? ld_cluster4(mapa(at, s)) : *(const float4 *)(po + r * Sh::PITCH + d);
-            const float a = pw[s * Sh::ROWS + r];
+        float top = -INFINITY, sum = 0.0f, v[4] = {};
+#pragma unroll
+        for (int w = 0; w < WN; w++) top = fmaxf(top, pm[w * Sh::ROWS + r]);
+        const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int w = 0; w < WN; w++) {
+            const float a = ex2(pm[w * Sh::ROWS + r] - ref);
+            const float4 x = *(const float4 *)(po + (w * Sh::ROWS + r) * Sh::PITCH + d);
+            sum = fmaf(a, pl[w * Sh::ROWS + r], sum);
             v[0] = fmaf(a, x.x, v[0]), v[1] = fmaf(a, x.y, v[1]), v[2] = fmaf(a, x.z, v[2]), v[3] = fmaf(a, x.w, v[3]);
         }
+        if (p.S > 1) {                                       // to group 0's place: this thread alone reads it
+            *(float4 *)(po + r * Sh::PITCH + d) = make_float4(v[0], v[1], v[2], v[3]);
+            if (d == 0) qm[r] = top, ql[r] = sum;
+            continue;
+        }
+        const float inv = inverse(sum);
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[e] *= ps[r];
+        for (int e = 0; e < 4; e++) v[e] *= inv;
         store_out<4>(p, (seq.row0 + r / p.G) * p.ld_out + (long long)(head * p.G + r % p.G) * p.D + d, v);
     }
-    if (p.S > 1) cluster_sync();                             // no CTA leaves while another reads its shared memory
+    if (p.S == 1) return;
+    const uint32_t a_po = su32(po), a_qm = su32(qm), a_ql = su32(ql);
+    cluster_sync();
+    for (int i = threadIdx.x + rank * blockDim.x; i < rows * d4; i += blockDim.x * p.S) {
+        const int r = i / d4, d = 4 * (i % d4);
+        float v[4];
+        cluster_join(a_qm + 4 * r, a_ql + 4 * r, a_po + 4 * (r * Sh::PITCH + d), p.S, v);
+        store_out<4>(p, (seq.row0 + r / p.G) * p.ld_out + (long long)(head * p.G + r % p.G) * p.D + d, v);
+    }
+    cluster_sync();                                          // no CTA leaves while another reads its shared memory
 }
+
 
 typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
                              const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
@@ -601,7 +680,7 @@ EncodeFn attn_encode_fn()
 template <int KS, int NP, int RW, int WM, int WN, int NSLOT, int MINB>
 bool attn_launch(AttnArgs &p, const CUtensorMap &map, long long tiles)
 {
-    using Sh = Shape<KS, RW, WM, WN, NSLOT>;
+    using Sh = Shape<KS, NP, RW, WM, WN, NSLOT>;
     p.ntile = 1;
     return attn_grid<kv8_attn_kernel<KS, NP, RW, WM, WN, NSLOT, MINB>>(p, dim3(32 * WM * WN), Sh::SMEM, Sh::ROWS, MINB, tiles, WN, map);
 }

@@ -4,6 +4,8 @@
 
 #include "lm.cuh"
 
+#include <math.h>
+
 namespace tcg {
 
 constexpr int PAGE = TCG_KV8_PAGE;
@@ -123,6 +125,37 @@ __device__ __forceinline__ void cluster_sync()
 }
 
 constexpr int MAX_SPLIT = 10;            // CTAs of a cluster; of 11 or more a B200 holds 7 clusters at a time
+
+// Four output values of a row from the S CTAs of a cluster: their maxima, sums and O's at these shared-memory addresses,
+// read together, joined in the CTAs' order.
+__device__ __forceinline__ void cluster_join(uint32_t a_m, uint32_t a_l, uint32_t a_o, int S, float (&v)[4])
+{
+    float m[MAX_SPLIT], l[MAX_SPLIT], top = -INFINITY, sum = 0.0f;
+    float4 x[MAX_SPLIT];
+#pragma unroll
+    for (int s = 0; s < MAX_SPLIT; s++) {
+        m[s] = -INFINITY, l[s] = 0.0f, x[s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (s < S) {
+            m[s] = ld_cluster(mapa(a_m, s));
+            l[s] = ld_cluster(mapa(a_l, s));
+            x[s] = ld_cluster4(mapa(a_o, s));
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < MAX_SPLIT; s++) top = fmaxf(top, m[s]);
+    top = top == -INFINITY ? 0.0f : top;
+    v[0] = v[1] = v[2] = v[3] = 0.0f;
+#pragma unroll
+    for (int s = 0; s < MAX_SPLIT; s++) {
+        const float w = ex2(m[s] - top);
+        sum = fmaf(w, l[s], sum);
+        v[0] = fmaf(w, x[s].x, v[0]), v[1] = fmaf(w, x[s].y, v[1]), v[2] = fmaf(w, x[s].z, v[2]), v[3] = fmaf(w, x[s].w, v[3]);
+    }
+    const float inv = inverse(sum);
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] *= inv;
+}
+
 
 // Launches FN over ntile x n_seq x n_kv blocks of rows with `tiles` tiles of keys each at most, of which `groups` are
 // taken at a time, after choosing the split of the keys over a cluster of S CTAs. rows: of a block; per_sm: CTAs an SM.

@@ -495,18 +495,8 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
         const int rows = min(TC_ROWS, R - r0), d4 = p.D / 4;
         for (int i = tid; i < (rows + p.S - 1 - rank) / p.S * d4; i += TC_THREADS) {
             const int q = rank + i / d4 * p.S, d = i % d4;
-            float top = -INFINITY, sum = 0.0f, v[4] = {};
-            for (int s = 0; s < p.S; s++) top = fmaxf(top, ld_cluster(mapa(a_m + 4 * q, s)));
-            top = top == -INFINITY ? 0.0f : top;
-            for (int s = 0; s < p.S; s++) {
-                const float w = ex2(ld_cluster(mapa(a_m + 4 * q, s)) - top);
-                const float4 x = ld_cluster4(mapa(a_po + 16 * (q * P4 + (d ^ (q & (P4 - 1)))), s));
-                sum = fmaf(w, ld_cluster(mapa(a_m + 4 * (q + 128), s)), sum);
-                v[0] = fmaf(w, x.x, v[0]), v[1] = fmaf(w, x.y, v[1]), v[2] = fmaf(w, x.z, v[2]), v[3] = fmaf(w, x.w, v[3]);
-            }
-            const float inv = inverse(sum);
-#pragma unroll
-            for (int e = 0; e < 4; e++) v[e] *= inv;
+            float v[4];
+            cluster_join(a_m + 4 * q, a_m + 4 * (q + 128), a_po + 16 * (q * P4 + (d ^ (q & (P4 - 1)))), p.S, v);
             const int row = r0 + q;
             store_out<4>(p, (seq.row0 + row / p.G) * p.ld_out + (long long)(head * p.G + row % p.G) * p.D + 4 * d, v);
         }
