@@ -152,10 +152,11 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
     if (!kv_seq(p.step, b, seq, p.err, report)) return;      // the same for the whole cluster
     const int R = seq.n * p.G;                               // one block holds them: the host picks a shape by the longest
     if (R == 0 || R > Sh::ROWS) return;
+    auto tok_of = [&](int r) { return (int)((unsigned)r * p.g_inv >> 20); };   // r / G, for r < 64
     auto hi_of = [&](int tok) { return kv8_hi(&seq, tok, p.causal); };
     auto lo_of = [&](int tok) { return kv8_lo(&seq, tok, p.window); };
     int t0;                                                  // this warp group's tiles: t0, t0 + WN, ...
-    const int mine = kv8_tiles(&seq, 0, (R - 1) / p.G, p.causal, p.window, rank, p.S, wn, WN, &t0);
+    const int mine = kv8_tiles(&seq, 0, tok_of(R - 1), p.causal, p.window, rank, p.S, wn, WN, &t0);
 
     // This thread's rows.
     constexpr int RPW = 8 * RW;                              // rows of a warp
@@ -163,12 +164,12 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
     long long row_off[RW];
 #pragma unroll
     for (int i = 0; i < RW; i++) {
-        const int r = min(RPW * wm + g + 8 * i, R - 1), tok = r / p.G;
+        const int r = min(RPW * wm + g + 8 * i, R - 1), tok = tok_of(r);
         hi[i] = hi_of(tok);
         lo[i] = lo_of(tok);
-        row_off[i] = (long long)(head * p.G + r % p.G) * p.D;
+        row_off[i] = (long long)(head * p.G + r - tok * p.G) * p.D;
     }
-    const int row_a = min(RPW * wm, R - 1) / p.G, row_z = min(RPW * wm + RPW - 1, R - 1) / p.G;
+    const int row_a = tok_of(min(RPW * wm, R - 1)), row_z = tok_of(min(RPW * wm + RPW - 1, R - 1));
     const int all_hi = hi_of(row_a), all_lo = lo_of(row_z);  // keys that every row of the warp sees
     const int any_hi = hi_of(row_z), any_lo = lo_of(row_a);  // keys that some row of the warp sees
 
@@ -229,7 +230,7 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
             float x[KS / 2][16], m = 0.0f;
             bool odd = false;                                    // a NaN or an infinity
             const int r = min(RPW * wm + g + 8 * i, R - 1);
-            const long long off = (seq.row0 + r / p.G) * p.ld_q + row_off[i];
+            const long long off = (seq.row0 + tok_of(r)) * p.ld_q + row_off[i];
 #pragma unroll
             for (int c = 0; c < KS / 2; c++) {
 #pragma unroll
@@ -283,7 +284,8 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
         constexpr int EACH = (Sh::ROWS + WM * WN - 1) / (WM * WN), AT_ONCE = EACH < 8 ? EACH : 8;   // rows whose loads go together
         static_assert(EACH <= 32, "a lane keeps what belongs to one of the warp's rows");
         const int my_row = min(warp + lane * WM * WN, R - 1);    // of the warp's lane-th row: where it lies, its largest value
-        const long long my_off = (seq.row0 + my_row / p.G) * p.ld_q + (long long)(head * p.G + my_row % p.G) * p.D;
+        const int my_tok = tok_of(my_row);
+        const long long my_off = (seq.row0 + my_tok) * p.ld_q + (long long)(head * p.G + my_row - my_tok * p.G) * p.D;
         float my_max = 0.0f;
 #pragma unroll
         for (int k0 = 0; k0 < EACH; k0 += AT_ONCE) {
@@ -591,7 +593,7 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
             const int row = RPW * wm + g + 8 * r;
             if (row >= R) continue;
             const float inv = inverse(l[r]);
-            const long long off = (seq.row0 + row / p.G) * p.ld_out + row_off[r];
+            const long long off = (seq.row0 + tok_of(row)) * p.ld_out + row_off[r];
 #pragma unroll
             for (int n = 0; n < NT; n++) {
                 if (8 * n >= p.D) break;
@@ -623,7 +625,7 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
     }
     __syncthreads();
     for (int i = threadIdx.x; i < rows * d4; i += blockDim.x) {
-        const int r = i / d4, d = 4 * (i % d4);
+        const int r = (int)((unsigned)i * p.d4_inv >> 20), d = 4 * (i - r * d4);
         float top = -INFINITY, sum = 0.0f, v[4] = {};
 #pragma unroll
         for (int w = 0; w < WN; w++) top = fmaxf(top, pm[w * Sh::ROWS + r]);
@@ -643,16 +645,16 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
         const float inv = inverse(sum);
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] *= inv;
-        store_out<4>(p, (seq.row0 + r / p.G) * p.ld_out + (long long)(head * p.G + r % p.G) * p.D + d, v);
+        store_out<4>(p, (seq.row0 + tok_of(r)) * p.ld_out + (long long)(head * p.G + r - tok_of(r) * p.G) * p.D + d, v);
     }
     if (p.S == 1) return;
     const uint32_t a_po = su32(po), a_qm = su32(qm), a_ql = su32(ql);
     cluster_sync();
     for (int i = threadIdx.x + rank * blockDim.x; i < rows * d4; i += blockDim.x * p.S) {
-        const int r = i / d4, d = 4 * (i % d4);
+        const int r = (int)((unsigned)i * p.d4_inv >> 20), d = 4 * (i - r * d4);
         float v[4];
         cluster_join(a_qm + 4 * r, a_ql + 4 * r, a_po + 4 * (r * Sh::PITCH + d), p.S, v);
-        store_out<4>(p, (seq.row0 + r / p.G) * p.ld_out + (long long)(head * p.G + r % p.G) * p.D + d, v);
+        store_out<4>(p, (seq.row0 + tok_of(r)) * p.ld_out + (long long)(head * p.G + r - tok_of(r) * p.G) * p.D + d, v);
     }
     cluster_sync();                                          // no CTA leaves while another reads its shared memory
 }
@@ -719,6 +721,7 @@ extern "C" bool tcg_kv8_attention(void *out, const void *q, const tcg_kv8_t *c, 
     p.v = c->v, p.k_scale = c->k_scale, p.v_scale = c->v_scale;
     p.step = kv_step(*s);
     p.n_pages = c->n_pages, p.n_kv = c->n_kv_head, p.n_seq = s->n_seq, p.D = c->head_dim, p.G = G;
+    p.g_inv = (1u << 20) / (unsigned)G + 1u, p.d4_inv = (1u << 20) / (unsigned)(p.D / 4) + 1u;
     p.scale_log2 = scale * 1.44269504088896340736f;
     p.causal = causal, p.window = window, p.err = lm_error_word();
 

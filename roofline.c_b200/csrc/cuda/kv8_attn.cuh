@@ -20,6 +20,7 @@ struct AttnArgs {
     const float *k_scale, *v_scale;
     KvStep step;
     int n_pages, n_kv, n_seq, D, G;
+    unsigned g_inv, d4_inv;              // n / G and n / (D / 4) are n * inv >> 20 where n times the divisor is below 2^20
     float scale_log2;
     int causal, window;
     int ntile, S;                        // blocks of rows a sequence; CTAs (a cluster) that share one's keys

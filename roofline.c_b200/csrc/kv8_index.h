@@ -74,11 +74,10 @@ KV8_FN int kv8_tiles(const kv8_seq_t *q, int tok_a, int tok_z, int causal, int w
 {
     const int first = kv8_lo(q, tok_a, window) / KV8_PAGE_TOKENS;
     const int tiles = kv8_hi(q, tok_z, causal) / KV8_PAGE_TOKENS + 1 - first, share = (tiles + ranks - 1) / ranks;
-    const long long a = first + (long long)rank * share;
-    long long z = a + share;
-    if (z > first + tiles) z = first + tiles;
-    *t0 = (int)(a + part);
-    return z > a + part ? (int)((z - a - part + parts - 1) / parts) : 0;
+    const int a = first + rank * share, end = first + tiles;     /* below 2^26: a cache has at most 2^25 tiles */
+    const int z = a + share < end ? a + share : end;
+    *t0 = a + part;
+    return z > a + part ? (z - a - part + parts - 1) / parts : 0;
 }
 
 #endif /* TCG_KV8_INDEX_H */
