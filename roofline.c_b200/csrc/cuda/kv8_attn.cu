@@ -42,8 +42,8 @@
 //
 // Bound by memory on large decode batches: 64 sequences up to 8192 tokens (32
 // query heads, 8 key heads, D = 128) 104 us, 6.2 TB/s. One token over 131071:
-// 51 us, 5.3 TB/s: clusters of 10 use 80 of 148 SMs. One token over a few
-// hundred: 6.8 us (bf16) to 8.4 us (fp32), dependent loads (lengths, page,
+// 47 us, 5.7 TB/s: clusters of 10 use 80 of 148 SMs. One token over a few
+// hundred: 5.7 us (bf16) to 6.8 us (fp32), dependent loads (lengths, page,
 // scale and tile) and the launch.
 #include "kv8_attn.cuh"
 #include "tc05.cuh"

@@ -36,10 +36,10 @@
 // products run while the other's threads compute. Every wait is bounded as in
 // attn_tc.cu.
 //
-// Measured, 32 query and 8 key heads: a 4096-token causal prompt 385 us fp32
-// and 280 us bf16 with D = 128 (357 and 491 TFLOP/s), 4096 x 4096 without a
-// mask 660 and 463 us (417 and 594 TFLOP/s), 512 tokens over 16384 with the
-// keys split over clusters of 2 346 and 245 us. The tensor pipe is busy 35% of
+// Measured, 32 query and 8 key heads: a 4096-token causal prompt 392 us fp32
+// and 279 us bf16 with D = 128 (351 and 493 TFLOP/s), 4096 x 4096 without a
+// mask 676 and 461 us (407 and 596 TFLOP/s), 512 tokens over 16384 with the
+// keys split over clusters of 2 356 and 246 us. The tensor pipe is busy 34% of
 // the time (fp32): the threads' own chain per tile is the limit. Four threads
 // a row (64 registers) spill: 616 us. O in registers, folded every tile: 883
 // us; 64-key tiles with a second S buffer: 497 us.
