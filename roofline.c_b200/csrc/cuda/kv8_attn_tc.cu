@@ -281,6 +281,9 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
 #pragma unroll
             for (int e = 0; e < 16; e++) x[c][e] = 0.0f;
             if (DH * h + 16 * c < p.D) load_q16(p, off + 16 * c, x[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < DH / 16; c++) {
 #pragma unroll
             for (int e = 0; e < 16; e++) {
                 odd |= !(fabsf(x[c][e]) <= 3.402823466e38f);
@@ -391,10 +394,13 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
 #pragma unroll
                 for (int j = 0; j < 32; j++) x[j] = __uint_as_float(s[j]);
             } else {
-                const int k0 = key0 + 32 * q;
+                // bits lo - k0 .. hi - k0, as far as there are such
+                const int a = lo - (key0 + 32 * q), z = hi - (key0 + 32 * q);
+                const uint32_t from = a <= 0 ? 0xFFFFFFFFu : a > 31 ? 0u : 0xFFFFFFFFu << a;
+                const uint32_t upto = z >= 31 ? 0xFFFFFFFFu : z < 0 ? 0u : 0xFFFFFFFFu >> (31 - z);
+                const uint32_t sees = mine >= 0 ? from & upto : 0u;
 #pragma unroll
-                for (int j = 0; j < 32; j++)
-                    x[j] = mine >= 0 && k0 + j >= lo && k0 + j <= hi ? __uint_as_float(s[j]) : -INFINITY;
+                for (int j = 0; j < 32; j++) x[j] = sees >> j & 1u ? __uint_as_float(s[j]) : -INFINITY;
             }
         };
         float top = -INFINITY;
@@ -465,30 +471,37 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
             __syncwarp();
         }
     }
-    fold(m, np > 0);
+    // The last group's P V joins O on the way out. Where the keys are split, the S CTAs of a cluster took consecutive shares
+    // of them: their O (over Q, K and V in shared memory, a row's 16-byte pieces permuted by the row against bank
+    // conflicts), m and l meet; each CTA joins every S-th row.
+    constexpr int P4 = DP / 4;                               // pieces of a row
+    float4 *const po = (float4 *)tiles;
     xsum[tid] = l;
     __syncthreads();
-    if (p.S == 1) {
-        if (ok && r0 + r < R) {
-            const float inv = inverse(xsum[r] + xsum[r + 128]);
-            const long long off = (seq.row0 + tok) * p.ld_out + head_off + DH * h;
+    const float sum = xsum[r] + xsum[r + 128], inv = inverse(sum);
+    const long long out_off = (seq.row0 + tok) * p.ld_out + head_off + DH * h;
 #pragma unroll 1
-            for (int d = 0; d < DH && DH * h + d < p.D; d += 4) {
-                const float v[4] = { o[d] * inv, o[d + 1] * inv, o[d + 2] * inv, o[d + 3] * inv };
-                store_out<4>(p, off + d, v);
+    for (int c = 0; c < DH; c += 32) {
+        uint32_t pv[32] = {};
+        if (np > 0) tmem_ld32(lane_base + 128 + DH * h + c, pv);
+#pragma unroll
+        for (int d = 0; d < 32; d += 4) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = fmaf(__uint_as_float(pv[d + e]), sv0, o[c + d + e]);
+            if (p.S > 1) {
+                po[r * P4 + ((DH * h + c + d) / 4 ^ (r & (P4 - 1)))] = make_float4(v[0], v[1], v[2], v[3]);
+            } else if (ok && r0 + r < R && DH * h + c + d < p.D) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] *= inv;
+                store_out<4>(p, out_off + c + d, v);
             }
         }
-    } else {
-        // The S CTAs of a cluster took consecutive shares of the keys: their O (over Q, K and V in shared memory, a row's
-        // 16-byte pieces permuted by the row against bank conflicts), m and l meet; each CTA joins every S-th row.
-        constexpr int P4 = DP / 4;                           // pieces of a row
-        float4 *const po = (float4 *)tiles;
-#pragma unroll 1
-        for (int d = 0; d < DH; d += 4)
-            po[r * P4 + ((DH * h + d) / 4 ^ (r & (P4 - 1)))] = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
+    }
+    if (p.S > 1) {
         if (h == 0) {
             xmax[r] = m;
-            xmax[r + 128] = xsum[r] + xsum[r + 128];
+            xmax[r + 128] = sum;
         }
         const uint32_t a_po = su32(po), a_m = su32(xmax);
         cluster_sync();
