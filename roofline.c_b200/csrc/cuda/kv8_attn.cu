@@ -653,7 +653,7 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
     for (int i = threadIdx.x + rank * blockDim.x; i < rows * d4; i += blockDim.x * p.S) {
         const int r = (int)((unsigned)i * p.d4_inv >> 20), d = 4 * (i - r * d4);
         float v[4];
-        cluster_join(a_qm + 4 * r, a_ql + 4 * r, a_po + 4 * (r * Sh::PITCH + d), p.S, v);
+        cluster_join<MAX_SPLIT>(a_qm + 4 * r, a_ql + 4 * r, a_po + 4 * (r * Sh::PITCH + d), p.S, v);
         store_out<4>(p, (seq.row0 + tok_of(r)) * p.ld_out + (long long)(head * p.G + r - tok_of(r) * p.G) * p.D + d, v);
     }
     cluster_sync();                                          // no CTA leaves while another reads its shared memory

@@ -128,13 +128,14 @@ __device__ __forceinline__ void cluster_sync()
 constexpr int MAX_SPLIT = 10;            // CTAs of a cluster; of 11 or more a B200 holds 7 clusters at a time
 
 // Four output values of a row from the S CTAs of a cluster: their maxima, sums and O's at these shared-memory addresses,
-// read together, joined in the CTAs' order.
+// read together (MAX at least S), joined in the CTAs' order.
+template <int MAX>
 __device__ __forceinline__ void cluster_join(uint32_t a_m, uint32_t a_l, uint32_t a_o, int S, float (&v)[4])
 {
-    float m[MAX_SPLIT], l[MAX_SPLIT], top = -INFINITY, sum = 0.0f;
-    float4 x[MAX_SPLIT];
+    float m[MAX], l[MAX], top = -INFINITY, sum = 0.0f;
+    float4 x[MAX];
 #pragma unroll
-    for (int s = 0; s < MAX_SPLIT; s++) {
+    for (int s = 0; s < MAX; s++) {
         m[s] = -INFINITY, l[s] = 0.0f, x[s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (s < S) {
             m[s] = ld_cluster(mapa(a_m, s));
@@ -143,11 +144,11 @@ __device__ __forceinline__ void cluster_join(uint32_t a_m, uint32_t a_l, uint32_
         }
     }
 #pragma unroll
-    for (int s = 0; s < MAX_SPLIT; s++) top = fmaxf(top, m[s]);
+    for (int s = 0; s < MAX; s++) top = fmaxf(top, m[s]);
     top = top == -INFINITY ? 0.0f : top;
     v[0] = v[1] = v[2] = v[3] = 0.0f;
 #pragma unroll
-    for (int s = 0; s < MAX_SPLIT; s++) {
+    for (int s = 0; s < MAX; s++) {
         const float w = ex2(m[s] - top);
         sum = fmaf(w, l[s], sum);
         v[0] = fmaf(w, x[s].x, v[0]), v[1] = fmaf(w, x[s].y, v[1]), v[2] = fmaf(w, x[s].z, v[2]), v[3] = fmaf(w, x[s].w, v[3]);

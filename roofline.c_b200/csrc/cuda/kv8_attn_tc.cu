@@ -36,10 +36,10 @@
 // products run while the other's threads compute. Every wait is bounded as in
 // attn_tc.cu.
 //
-// Measured, 32 query and 8 key heads: a 4096-token causal prompt 392 us fp32
-// and 279 us bf16 with D = 128 (351 and 493 TFLOP/s), 4096 x 4096 without a
-// mask 676 and 461 us (407 and 596 TFLOP/s), 512 tokens over 16384 with the
-// keys split over clusters of 2 356 and 246 us. The tensor pipe is busy 34% of
+// Measured, 32 query and 8 key heads: a 4096-token causal prompt 382 us fp32
+// and 265 us bf16 with D = 128 (360 and 518 TFLOP/s), 4096 x 4096 without a
+// mask 690 and 465 us (398 and 591 TFLOP/s), 512 tokens over 16384 with the
+// keys split over clusters of 2 361 and 245 us. The tensor pipe is busy 34% of
 // the time (fp32): the threads' own chain per tile is the limit. Four threads
 // a row (64 registers) spill: 616 us. O in registers, folded every tile: 883
 // us; 64-key tiles with a second S buffer: 497 us.
@@ -48,6 +48,8 @@
 #include "tc05.cuh"
 
 #include <math.h>
+
+#include <type_traits>
 
 namespace tcg {
 namespace {
@@ -506,13 +508,19 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
         const uint32_t a_po = su32(po), a_m = su32(xmax);
         cluster_sync();
         const int rows = min(TC_ROWS, R - r0), d4 = p.D / 4;
-        for (int i = tid; i < (rows + p.S - 1 - rank) / p.S * d4; i += TC_THREADS) {
-            const int q = rank + i / d4 * p.S, d = i % d4;
-            float v[4];
-            cluster_join(a_m + 4 * q, a_m + 4 * (q + 128), a_po + 16 * (q * P4 + (d ^ (q & (P4 - 1)))), p.S, v);
-            const int row = r0 + q;
-            store_out<4>(p, (seq.row0 + row / p.G) * p.ld_out + (long long)(head * p.G + row % p.G) * p.D + 4 * d, v);
-        }
+        auto join = [&](auto most) {
+#pragma unroll 4
+            for (int i = tid; i < (rows + p.S - 1 - rank) / p.S * d4; i += TC_THREADS) {
+                const int k = (int)((unsigned)i * p.d4_inv >> 20), q = rank + k * p.S, d = i - k * d4;
+                float v[4];
+                cluster_join<decltype(most)::value>(a_m + 4 * q, a_m + 4 * (q + 128), a_po + 16 * (q * P4 + (d ^ (q & (P4 - 1)))),
+                                                    p.S, v);
+                const int row = r0 + q;
+                store_out<4>(p, (seq.row0 + row / p.G) * p.ld_out + (long long)(head * p.G + row % p.G) * p.D + 4 * d, v);
+            }
+        };
+        if (p.S <= 3) join(std::integral_constant<int, 3>());
+        else join(std::integral_constant<int, MAX_SPLIT>());
         cluster_sync();                                      // no CTA leaves while another reads its shared memory
     }
     // MMAs that may still run (a wait gave up) must finish before TMEM is freed: thread 0 waits, bounded, for its last
