@@ -9,11 +9,19 @@
 //   Q is quantised per row, once, to a whole number of 15 bits (fp16, bf16
 //     inputs) or 23 bits (fp32): q = q_scale * (d1 256 + d0), or with d2 65536
 //     too, digits of 8 bits in -128 .. 127. The sum over dims is exact.
-//   P in [0, 1] becomes a whole number of 16 or 23 bits the same way, by one
-//     fused multiply-add whose result's mantissa is that number, and byte
-//     permutes; P V is exact per tile and folded into fp32 with sv.
-// NP = 2 digits leave 2^-16 of a row's largest |q| and 2^-17 of the largest
-// weight (below the half step of fp16, 2^-11, by 2^5); NP = 3 2^-24 of both.
+//   P is taken against the tile's own maximum, so that a tile far below the
+//     row's largest score (the rest of a cache beside one key that holds most
+//     of the weight) keeps its digits: in [0, 1], it becomes a whole number of
+//     16 or 23 bits by one fused multiply-add whose result's mantissa is that
+//     number, and byte permutes; P V is exact per tile and folded into fp32
+//     with sv 2^(m_tile - m).
+// NP = 2 digits leave 2^-16 of a row's largest |q|, NP = 3 2^-24. A weight is
+// off by 2^-24 of its tile's largest, and up to 64 of them add up. Two digits
+// of P (2^-17) do for 16-bit results only where a tile's weight is spread:
+// they are taken where every thread's 16 keys hold 1/16 of the largest weight
+// in every row (the other keys then hold 3/16 at least, their 63 roundings
+// 2^-13 of that as a rule), three elsewhere. Three always: 131071 tokens 52.9
+// us against 49.3 with scores of spread 2.7, 64 x 16 rows 136 against 133.
 //
 // Why no shuffles: the mma's k order is free as long as A and B agree. A
 // thread (row g = lane / 4, t = lane % 4) takes 16 consecutive bytes of a K
@@ -219,7 +227,8 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
     // A fragments, in the k order of the tiles: k-step 2 c + s of chunk c takes bytes 64 c + 16 t + 8 s + 0..7. RW = 2:
     // qd[n] is digit n's. RW = 1: the first fragment holds the two upper digits, as rows g and g + 8; with three digits a
     // second one holds the lowest as row g + 8.
-    constexpr int NA = RW == 2 ? NP : NP - 1;                // A fragments, mma's per product
+    constexpr int NA = RW == 2 ? NP : NP - 1;                // A fragments, mma's of Q K^T
+    constexpr int NAP = RW == 2 ? 3 : 2;                     // the same of P V, which takes up to three digits
     uint32_t qd[NA][KS][4] = {};
     float qs[RW];
     constexpr float Q = NP == 3 ? 8300000.0f : 32512.0f;     // the digits' largest sums
@@ -456,7 +465,9 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
         }
         release(2 * i);
 
-        uint32_t pd[NA][2][4] = {};
+        uint32_t pd[NAP][2][4] = {};
+        float fold[RW];                                      // factor of the tile's P V, into O
+        bool fine = true;                                    // three digits of P
         if (real) {
             if (key0 < all_lo || key0 + PAGE - 1 > all_hi) {
 #pragma unroll
@@ -467,7 +478,8 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
                         if (key > hi[e >> 1] || key < lo[e >> 1]) f[j][e] = -INFINITY;
                     }
             }
-            bool grew = false;
+            bool grew = false, even = true;
+            float up[RW];                                    // of O, where the row's maximum grew
 #pragma unroll
             for (int r = 0; r < RW; r++) {
                 float top = -INFINITY;
@@ -480,9 +492,10 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
                 cs = cs < 1e-37f ? 1e-37f : cs;
                 // raised by 2^-22 of itself, so that rounding never puts a weight above 1 (its digits would overflow)
                 float mt = top * cs;
-                mt = fmaf(fabsf(mt), 0x1p-22f, mt);
-                const float mn = fmaxf(m[r], top == -INFINITY ? -INFINITY : mt);
-                const float use = mn == -INFINITY ? 0.0f : mn, alpha = ex2(m[r] - use);
+                mt = top == -INFINITY ? top : fmaf(fabsf(mt), 0x1p-22f, mt);
+                const float mn = fmaxf(m[r], mt), use = mn == -INFINITY ? 0.0f : mn, ref = mt == -INFINITY ? 0.0f : mt;
+                const float beta = ex2(mt - use);
+                up[r] = ex2(m[r] - use);
                 grew |= mn != m[r];
                 m[r] = mn;
                 float sum = 0.0f;
@@ -491,87 +504,108 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
                         float &v = f[j][2 * r + c];
-                        v = ex2(fmaf(v, cs, -use));
+                        v = ex2(fmaf(v, cs, -ref));
                         sum += v;
-                        v = NP == 3 ? fmaf(v, 8388607.0f, 8388608.0f) : fmaf(v, 65535.0f / 65536.0f, 128.0f);
                     }
-                l[r] = fmaf(l[r], alpha, sum);
-                if (__any_sync(0xFFFFFFFFu, grew)) {
+                l[r] = fmaf(l[r], up[r], sum * beta);
+                fold[r] = tv * beta;
+                even = even && sum >= 1.0f / 16.0f;
+            }
+            fine = NP == 3 || !__all_sync(0xFFFFFFFFu, even);
+            if (__any_sync(0xFFFFFFFFu, grew)) {
+#pragma unroll
+                for (int r = 0; r < RW; r++)
 #pragma unroll
                     for (int n = 0; n < NT; n++) {
-                        o[n][2 * r] *= alpha;
-                        o[n][2 * r + 1] *= alpha;
+                        o[n][2 * r] *= up[r];
+                        o[n][2 * r + 1] *= up[r];
                     }
-                }
-                // bytes of the four weights of keys 16 t + 4 w + 0..3
-#pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    const uint32_t y0 = __float_as_uint(f[2 * w][2 * r]), y1 = __float_as_uint(f[2 * w][2 * r + 1]);
-                    const uint32_t y2 = __float_as_uint(f[2 * w + 1][2 * r]), y3 = __float_as_uint(f[2 * w + 1][2 * r + 1]);
-                    const uint32_t u = __byte_perm(y0, y1, 0x5140), v = __byte_perm(y2, y3, 0x5140);
-                    const uint32_t d0 = __byte_perm(u, v, 0x5410), d1 = __byte_perm(u, v, 0x7632);
-                    const uint32_t d2 = __byte_perm(__byte_perm(y0, y1, 0x0062), __byte_perm(y2, y3, 0x0062), 0x5410);
-                    uint32_t (&first)[4] = pd[0][w >> 1], (&last)[4] = pd[NA - 1][w >> 1];
-                    if constexpr (RW == 2) {
-                        pd[1][w >> 1][2 * (w & 1) + r] = d1;
-                        if (NP == 3) last[2 * (w & 1) + r] = d2;
-                        first[2 * (w & 1) + r] = d0;
-                    } else {
-                        first[2 * (w & 1)] = NP == 3 ? d2 : d1;
-                        first[2 * (w & 1) + 1] = NP == 3 ? d1 : d0;
-                        if (NP == 3) last[2 * (w & 1) + 1] = d0;
-                    }
-                }
             }
+            // bytes of the four weights of keys 16 t + 4 w + 0..3
+            auto digits = [&](auto three) {
+                constexpr bool THREE = decltype(three)::value;
+#pragma unroll
+                for (int r = 0; r < RW; r++) {
+                    fold[r] *= THREE ? 1.0f / 8388607.0f : 1.0f / 65535.0f;
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        uint32_t y[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const float v = f[2 * w + (e >> 1)][2 * r + (e & 1)];
+                            y[e] = __float_as_uint(THREE ? fmaf(v, 8388607.0f, 8388608.0f) : fmaf(v, 65535.0f / 65536.0f, 128.0f));
+                        }
+                        const uint32_t u = __byte_perm(y[0], y[1], 0x5140), v = __byte_perm(y[2], y[3], 0x5140);
+                        const uint32_t d0 = __byte_perm(u, v, 0x5410), d1 = __byte_perm(u, v, 0x7632);
+                        const uint32_t d2 = __byte_perm(__byte_perm(y[0], y[1], 0x0062), __byte_perm(y[2], y[3], 0x0062), 0x5410);
+                        const int at = 2 * (w & 1);
+                        if constexpr (RW == 2) {
+                            pd[0][w >> 1][at + r] = d0;
+                            pd[1][w >> 1][at + r] = d1;
+                            if (THREE) pd[NAP - 1][w >> 1][at + r] = d2;
+                        } else {
+                            pd[0][w >> 1][at] = THREE ? d2 : d1;
+                            pd[0][w >> 1][at + 1] = THREE ? d1 : d0;
+                            if (THREE) pd[1][w >> 1][at + 1] = d0;
+                        }
+                    }
+                }
+            };
+            if (NP == 3 || fine) digits(std::true_type());
+            else digits(std::false_type());
         }
 
         ok = landed();
         if (!ok) break;
         if (real) {
             const uint32_t vt = my_ring + slot * Sh::SLOT + g * 64 + 16 * t;
-            const float fs = tv * (NP == 3 ? 1.0f / 8388607.0f : 1.0f / 65535.0f);
             constexpr int B = 4;                             // output tiles side by side
+            auto product = [&](auto three) {
+                constexpr bool THREE = decltype(three)::value;
 #pragma unroll
-            for (int n0 = 0; n0 < NT; n0 += B) {
-                uint4 w[B];
-                int a[B][4] = {}, top[B][4] = {};
+                for (int n0 = 0; n0 < NT; n0 += B) {
+                    uint4 w[B];
+                    int a[B][4] = {}, top[B][4] = {};
 #pragma unroll
-                for (int n = 0; n < B; n++) w[n] = lds128(vt + (n0 + n) * 512);
-                auto keys = [&](int (&d)[B][4], const uint32_t (&q)[2][4]) {
+                    for (int n = 0; n < B; n++) w[n] = lds128(vt + (n0 + n) * 512);
+                    auto keys = [&](int (&d)[B][4], const uint32_t (&q)[2][4]) {
 #pragma unroll
-                    for (int n = 0; n < B; n++) mma_u8s8(d[n], q[0], w[n].x, w[n].y);
+                        for (int n = 0; n < B; n++) mma_u8s8(d[n], q[0], w[n].x, w[n].y);
 #pragma unroll
-                    for (int n = 0; n < B; n++) mma_u8s8(d[n], q[1], w[n].z, w[n].w);
-                };
-                if constexpr (RW == 2) {
-                    keys(a, pd[1]);
-                    if (NP == 3) keys(top, pd[NA - 1]);
+                        for (int n = 0; n < B; n++) mma_u8s8(d[n], q[1], w[n].z, w[n].w);
+                    };
+                    if constexpr (RW == 2) {
+                        keys(a, pd[1]);
+                        if (THREE) keys(top, pd[NAP - 1]);
 #pragma unroll
-                    for (int n = 0; n < B; n++)
+                        for (int n = 0; n < B; n++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) a[n][e] <<= 8;   // |a| <= 255 * 128 * 64 < 2^21
-                    keys(a, pd[0]);
+                            for (int e = 0; e < 4; e++) a[n][e] <<= 8;   // |a| <= 255 * 128 * 64 < 2^21
+                        keys(a, pd[0]);
 #pragma unroll
-                    for (int n = 0; n < B; n++)
+                        for (int n = 0; n < B; n++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            o[n0 + n][e] = fmaf(NP == 3 ? fmaf((float)top[n][e], 65536.0f, (float)a[n][e]) : (float)a[n][e],
-                                                fs, o[n0 + n][e]);
-                } else {
-                    keys(a, pd[0]);
-                    if (NP == 3) {
+                            for (int e = 0; e < 4; e++)
+                                o[n0 + n][e] = fmaf(THREE ? fmaf((float)top[n][e], 65536.0f, (float)a[n][e]) : (float)a[n][e],
+                                                    fold[e >> 1], o[n0 + n][e]);
+                    } else {
+                        keys(a, pd[0]);
+                        if (THREE) {
 #pragma unroll
-                        for (int n = 0; n < B; n++) a[n][2] <<= 8, a[n][3] <<= 8;
-                        keys(a, pd[NA - 1]);
+                            for (int n = 0; n < B; n++) a[n][2] <<= 8, a[n][3] <<= 8;
+                            keys(a, pd[1]);                  // its rows 0..7 are zero
+                        }
+#pragma unroll
+                        for (int n = 0; n < B; n++)
+#pragma unroll
+                            for (int e = 0; e < 2; e++)
+                                o[n0 + n][e] = fmaf(THREE ? fmaf((float)a[n][e], 65536.0f, (float)a[n][2 + e])
+                                                          : (float)(a[n][e] * 256 + a[n][2 + e]), fold[0], o[n0 + n][e]);
                     }
-#pragma unroll
-                    for (int n = 0; n < B; n++)
-#pragma unroll
-                        for (int e = 0; e < 2; e++)
-                            o[n0 + n][e] = fmaf(NP == 3 ? fmaf((float)a[n][e], 65536.0f, (float)a[n][2 + e])
-                                                        : (float)(a[n][e] * 256 + a[n][2 + e]), fs, o[n0 + n][e]);
                 }
-            }
+            };
+            if (NP == 3 || fine) product(std::true_type());
+            else product(std::false_type());
         }
         release(2 * i + 1);
     }

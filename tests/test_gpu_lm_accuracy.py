@@ -1,0 +1,125 @@
+"""Attention over the 8-bit cache where softmax is far from broad: one key that
+holds nearly all of the weight, a page's V beside one of another magnitude,
+scores past what 24 bits resolve. Against 64 bits, with bounds that do not grow
+with the number of keys but for the sums' own roundings.
+
+u = 2^-24 is half a step of fp32, half_step(t) that of the output type.
+"""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+import tcg
+from test_gpu_lm import PAGE, TYPES, U, Pool, call, gen, half_step, lib, randn  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def exact(pool, q, new, kv, group, scale, t, causal=True, window=0, unlike=1.0):
+    """64-bit attention of q [n, heads, d] and the bound on each value's error, on the GPU. unlike: how far apart the V
+    scales of a group of pages are (up to 64)."""
+    few = max(new) * group <= 64
+    f32 = t == "f32"
+    out, tol = torch.zeros_like(q, dtype=torch.float64), torch.zeros_like(q, dtype=torch.float64)
+    at = 0
+    for b, (n, m) in enumerate(zip(new, kv)):
+        k, v = pool.values(b, m)
+        pos, key = torch.arange(m - n, m, device="cuda")[:, None], torch.arange(m, device="cuda")[None]
+        see = (key <= pos) if causal else torch.ones((n, m), dtype=torch.bool, device="cuda")
+        if window:
+            see &= key > pos - window
+        x = q[at:at + n].double()
+        for h in range(q.shape[1]):
+            kk, vv = k[h // group], v[h // group]
+            s = (x[:, h] @ kk.T * scale).masked_fill(~see, -math.inf)
+            w = torch.exp(s - s.amax(-1, keepdim=True))
+            l = w.sum(-1, keepdim=True)
+            mass = w @ vv.abs() / l
+            big = s.masked_fill(~see, 0).abs().amax(-1, keepdim=True)
+            reach = kk.abs().sum(-1)[None].expand(n, -1).masked_fill(~see, 0).amax(-1, keepdim=True)
+            top = x[:, h].abs().amax(-1, keepdim=True)
+            # A score: few rows, half a digit of q (of its row's largest) against each |k|; many rows, q as it is (two
+            # pieces of 11 bits with fp32) and a truncating sum, 2e-8 of its magnitude for each of at most 16 MMAs. Then
+            # six roundings of the scaled score and ex2's 2^-22. Twice (weights and their sum).
+            score = top / (2 * 8300000.0 if f32 else 2 * 32512.0) if few else top * (16 * 2e-8 + 2.0 ** -22)
+            delta = score * scale * reach + 6 * U * big + 2.0 ** -22
+            rel = 2 * torch.expm1(delta) + (m / PAGE + 40) * U
+            if few:
+                # Weights are whole numbers against the largest of their own tile, half a step off each: of 23 bits, or of
+                # 16 where the inputs are and every 16 keys of the tile hold 1/16 of that weight (0.06: rounding).
+                pad = -m % PAGE
+                wt = torch.nn.functional.pad(w, (0, pad)).view(n, -1, 4, PAGE // 4)
+                vt = torch.nn.functional.pad(vv.abs(), (0, 0, 0, pad)).view(-1, PAGE, vv.shape[1]).amax(1)
+                top_w = wt.amax((-1, -2))
+                coarse = (wt.sum(-1) >= 0.06 * top_w[..., None]).all(-1) & torch.tensor(not f32, device="cuda")
+                lost = PAGE * (torch.where(coarse, 2.0 ** -17, 2.0 ** -24) * top_w) @ vt / l
+            else:
+                # Weights are fp16 under 2^8 (two of them with fp32): half a step of 11 (22) bits, and of fp16's
+                # subnormals, 2^-25 / 2^8, times what the page's V scale is below its group's.
+                rel += (2.0 ** -23 if f32 else 2.0 ** -12) + (64 if f32 else 256) * 2e-8
+                lost = torch.minimum(w, torch.full_like(w, unlike * 2.0 ** -33)) @ vv.abs() / l
+            out[at:at + n, h] = w @ vv / l
+            tol[at:at + n, h] = mass * rel + lost
+        at += n
+    return out, tol + out.abs() * half_step(TYPES[t][0])
+
+
+def run(lib, pool, q, new, heads, scale, t, causal=True, window=0, **kw):
+    out = torch.full_like(q, float("nan"))
+    s = pool.step(new, **kw)
+    ld = heads * pool.d
+    call(lib.tcg_kv8_attention, out.data_ptr(), q.data_ptr(), C.byref(pool.cache()), C.byref(s), heads, ld, ld, scale, causal,
+         window, TYPES[t][1])
+    return out
+
+
+def near(got, want, tol):
+    over = (got.double() - want).abs() - tol
+    worst = ((got.double() - want).abs() / want.abs().clamp(min=1e-300)).max().item()
+    assert (over <= 0).all(), f"{over.max():.3g} over; relative error up to {worst:.3g}"
+
+
+# ------------------------------------------------------------------ one key holds nearly all of the weight
+
+def sink(seed, n_kv, d, keys, held, group, new, t):
+    """Key 0 holds `held` of every row's weight and a V of zeros; the others' scores are normal, their V has one sign."""
+    pool, g = Pool(gen(seed), n_kv, d, [keys], spare=0), gen(seed + 1)
+    pool.ks[:], pool.vs[:] = 1 / 73.0, 0.01
+    page, dims = int(pool.table[0, 0]), 16                               # dims that the sink's score comes from
+    pool.k[..., :dims] = 0
+    pool.k[page, :, 0] = 0
+    pool.k[page, :, 0, :dims] = 127
+    pool.v.copy_(torch.randint(32, 97, tuple(pool.v.shape), generator=g, dtype=torch.int8))
+    pool.v[page, :, :, 0] = 0
+    gap = math.log(keys * math.exp(0.5 * (d - dims) / d) * held / (1 - held))
+    q = randn(g, new, n_kv * group, d, dtype=torch.float64)
+    q[..., :dims] = gap * math.sqrt(d) / (dims * 127 / 73.0)
+    return pool, q.to(TYPES[t][0])
+
+
+SINKS = [  # tokens, query heads a key head, key heads, d: the shapes for 8, 16, 32 and 64 rows, and for many
+    (1, 4, 1, 128), (4, 4, 1, 64), (7, 4, 1, 128), (5, 8, 1, 64), (16, 4, 1, 128), (16, 4, 160, 64), (70, 4, 1, 128),
+]
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("keys,held", [(2048, 0.99), (8192, 0.99), (131072, 0.9), (131072, 0.99)])
+@pytest.mark.parametrize("new,group,n_kv,d", SINKS)
+def test_attention_beside_a_sink(lib, new, group, n_kv, d, keys, held, t):
+    if n_kv > 1:
+        keys = min(keys, 2048)                                           # every SM has a key head: no split of the keys
+    pool, q = sink(100, n_kv, d, keys, held, group, new, t)
+    want, tol = exact(pool, q, [new], [keys], group, 1 / math.sqrt(d), t)
+    assert (tol < 0.02 * want.abs()).all()                               # a lost tail does not fit under the bound
+    near(run(lib, pool, q, [new], n_kv * group, 1 / math.sqrt(d), t), want, tol)
+
+
+@pytest.mark.parametrize("new,group", [(1, 4), (7, 4), (16, 4), (70, 4)])
+def test_a_row_does_not_depend_on_the_launch(lib, new, group):
+    """The same rows over the same keys, whatever the split that the launch's hint leads to: alike to the bound's size."""
+    pool, q = sink(110, 1, 64, 20000, 0.99, group, new, "bf16")
+    want, tol = exact(pool, q, [new], [20000], group, 0.125, "bf16")
+    for hint in (1, 700, 20000):
+        near(run(lib, pool, q, [new], group, 0.125, "bf16", max_kv=hint), want, tol)
