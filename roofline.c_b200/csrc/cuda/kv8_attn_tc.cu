@@ -10,15 +10,23 @@
 // memory in the K-major, 128-byte-swizzled layout the MMA reads; V is
 // dim-major in the cache, so neither is transposed. Then
 //   S = Q K^T    128 x 128 fp32 in TMEM, Q as fp16 in shared memory;
-//   softmax      x = S cs - m, cs = scale log2(e) 2^-e sk, P = exp2(x + 8);
+//   softmax      x = S cs - m_g, cs = scale log2(e) 2^-e sk, P = exp2(x + 8);
 //   P V          128 x D fp32 in TMEM, P as fp16 in TMEM over S's columns,
 //                accumulated there over a group of tiles;
-//   O = O 2^(m_old - m) + sv0 P V at a group's end.
-// Within a group the reference m and the V scale sv0 stay: a page's sv enters
-// as log2(sv / sv0) in the exponent. A group ends where a row's maximum
-// outgrows its reference by 2^7, where sv and sv0 are 2^6 apart, or after 4
-// tiles with fp32 inputs (32 otherwise): the tensor core's accumulation
-// truncates, by about 2e-8 of the result per MMA, 64 (256) of them a group.
+//   O = (O + sv0 2^(m_g - 8 - m) P V) 2^(m - m_new) at a group's end.
+// Within a group the reference m_g and the V scale sv0 stay: a page's sv enters
+// as log2(sv / sv0) in the exponent. m_g is the row's running maximum m, or 2^4
+// over the maximum of the group's first tile where that is more than 2^8 below
+// m (2^4, so that groups last: at the maximum itself, prompts of peaked scores
+// take 5% longer). A group ends where
+// a row's maximum outgrows its reference by 2^7, where sv and sv0 are 2^3
+// apart, or after 4 tiles with fp32 inputs (32 otherwise): the tensor core's
+// accumulation truncates, by about 2e-8 of the result per MMA, 64 (256) of them
+// a group. A tile whose two pages' scales are 2^3 apart is taken twice, once
+// for each page. So a weight is rounded (to 11 or 22 bits, or 2^-33 of 2^m_g)
+// against weights of its own group, times V of about its own size: neither a
+// key elsewhere that holds most of the weight nor a page of large V beside it
+// takes its bits.
 // O is used at a group's end only and lives in local memory.
 // Q is scaled by a power of two per row into [2^14, 2^15). With fp16 or bf16
 // inputs it is exact as one fp16, and P's rounding to fp16 (2^-12 of itself)
@@ -59,6 +67,8 @@ constexpr int TC_ROWS = 128;
 constexpr uint32_t TC_COLS = 256;                // S, and P over it: 0 .. 127; P V: from 128
 constexpr uint32_t Q_TILE = 128 * 128;           // [128 rows or keys x 64 fp16]
 constexpr float P_BIAS = 8.0f, GROWTH = 7.0f;    // weights are up to 2^8, and 2^15 before a group ends (fp16: below 2^16)
+constexpr float FAR_M = 8.0f, ROOM = 4.0f;       // a first maximum this far (log2) below m gets a reference of its own, ROOM above it
+constexpr float NEAR_V = 3.0f;                   // log2 of how far a group's V scales are apart at most
 
 template <int DP, int NP>
 struct TcShape {
@@ -355,37 +365,49 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
     }
     __syncwarp();
 
-    float o[DH], m = -INFINITY, l = 0.0f, sv0 = 0.0f;        // m, sv0: the group's references; l: this half's share
+    float o[DH], m = -INFINITY, l = 0.0f;                    // m: what O and l stand against; l: this half's share
+    float mg = -INFINITY, dm = 0.0f, sv0 = 0.0f;             // the group's references; dm = mg - 8 - m
 #pragma unroll 1
     for (int j = 0; j < DH; j++) o[j] = 0.0f;                // used at a group's end only: kept in local memory
     int left = 0;                                            // tiles that the group may still take
-    // The group's P V, complete, joins O; then O and l move to the reference `now`.
-    auto fold = [&](float now, bool any) {
-        const float alpha = now == m ? 1.0f : ex2(m - now);
+    // The group's P V, complete, joins O; then O and l move to the new m, and a group begins with a tile of maximum `t`.
+    auto fold = [&](float t, bool any) {
+        const float now = fmaxf(m, t), ref = t < now - FAR_M ? t + ROOM : now, alpha = now == m ? 1.0f : ex2(m - now), f = sv0 * ex2(dm);
 #pragma unroll 1
         for (int c = 0; c < DH; c += 32) {
             uint32_t pv[32];
             if (any) tmem_ld32(lane_base + 128 + DH * h + c, pv);
 #pragma unroll
-            for (int j = 0; j < 32; j++) o[c + j] = alpha * (any ? fmaf(__uint_as_float(pv[j]), sv0, o[c + j]) : o[c + j]);
+            for (int j = 0; j < 32; j++) o[c + j] = alpha * (any ? fmaf(__uint_as_float(pv[j]), f, o[c + j]) : o[c + j]);
         }
         l *= alpha;
         m = now;
+        mg = ref;
+        dm = ref == -INFINITY ? 0.0f : ref - P_BIAS - now;   // a row that sees nothing yet has weights of 0
+    };
+    // log2(s / sv0), also of scales below fp32's normal numbers
+    auto log_ratio = [&](float s) {
+        const float k = sv0 < 0x1p-60f ? 0x1p64f : 1.0f;
+        return __log2f(__fdividef(s * k, sv0 * k));
     };
 
-    // Tile kb: S(kb) is under way. V(kb) replaces K(kb) when it is done; the maxima are posted and the CTA agrees whether
-    // the tile opens a group; the weights replace S(kb) and P V(kb) is issued; when that is done K(kb + 1) replaces V(kb).
+    // Step it, on tile kb: S is under way. V replaces K when it is done; the maxima are posted and the CTA agrees whether
+    // the step opens a group; the weights replace S and P V is issued; when that is done the next step's K replaces V.
     const int tiles_n = (np + 1) / 2;
-    for (int kb = 0; kb < tiles_n; kb++) {
+    bool second = false;                                     // the tile's second page alone
+    for (int it = 0, kb = 0; kb < tiles_n; it++) {
         const int mine = h ? pb : pa, key0 = (t0 + 2 * kb + h) * PAGE;
         const long long at_a = (long long)max(pa, 0) * p.n_kv + head, at_b = (long long)max(pb, 0) * p.n_kv + head;
         const float sk = p.k_scale[h ? at_b : at_a];
         const float va = pa < 0 ? 0.0f : p.v_scale[at_a], vb = pb < 0 ? 0.0f : p.v_scale[at_b], sv = h ? vb : va;
         load_pages(raw4, p.v, pa, pb, false);
-        const float cs = cs0 * (mine < 0 ? 1.0f : sk), c = cs < 1e-37f ? 1e-37f : cs;   // not 0: a masked -inf stays -inf
-        float lr = sv == sv0 || mine < 0 ? 0.0f : __log2f(__fdividef(sv, sv0));
-        const bool whole = __all_sync(0xFFFFFFFFu, mine >= 0 && key0 >= lo && key0 + PAGE - 1 <= hi);
-        if (ok) ok = bar_wait(bar_s, (uint32_t)(kb & 1), abort, p.err, ERR_WAIT);
+        const float v_min = fminf(va, vb), v_max = fmaxf(va, vb);
+        const bool apart = v_min > 0.0f && v_max > 8.0f * v_min, again = apart && !second;   // the same for the whole CTA
+        const bool on = mine >= 0 && (!apart || second == (h != 0));
+        const float cs = cs0 * (on ? sk : 1.0f), c = cs < 1e-37f ? 1e-37f : cs;   // not 0: a masked -inf stays -inf
+        float lr = sv == sv0 || !on ? 0.0f : log_ratio(sv);
+        const bool whole = __all_sync(0xFFFFFFFFu, on && key0 >= lo && key0 + PAGE - 1 <= hi);
+        if (ok) ok = bar_wait(bar_s, (uint32_t)(it & 1), abort, p.err, ERR_WAIT);
         fence_after();
         store_v(raw4);
         // 32 scores of this thread's page, -inf where its row does not see the key
@@ -400,7 +422,7 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
                 const int a = lo - (key0 + 32 * q), z = hi - (key0 + 32 * q);
                 const uint32_t from = a <= 0 ? 0xFFFFFFFFu : a > 31 ? 0u : 0xFFFFFFFFu << a;
                 const uint32_t upto = z >= 31 ? 0xFFFFFFFFu : z < 0 ? 0u : 0xFFFFFFFFu >> (31 - z);
-                const uint32_t sees = mine >= 0 ? from & upto : 0u;
+                const uint32_t sees = on ? from & upto : 0u;
 #pragma unroll
                 for (int j = 0; j < 32; j++) x[j] = sees >> j & 1u ? __uint_as_float(s[j]) : -INFINITY;
             }
@@ -415,15 +437,15 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
         }
         top = top == -INFINITY ? top : top * c;
         xmax[tid] = top;
-        const bool group = __syncthreads_or(left == 0 || !(fabsf(lr) <= 6.0f) || top + lr > m + GROWTH);
+        const bool group = __syncthreads_or(left == 0 || !(fabsf(lr) <= NEAR_V) || top + lr > mg + GROWTH);
         if (group) {
-            fold(fmaxf(m, fmaxf(xmax[r], xmax[r + 128])), kb > 0);
-            sv0 = fmaxf(va, vb);
-            lr = sv == sv0 || mine < 0 ? 0.0f : fmaxf(__log2f(__fdividef(sv, sv0)), -60.0f);
+            fold(fmaxf(xmax[r], xmax[r + 128]), it > 0);
+            sv0 = !apart ? v_max : second ? vb : va;
+            lr = sv == sv0 || !on ? 0.0f : fmaxf(log_ratio(sv), -60.0f);     // beyond NEAR_V only where sv is 0
             left = NP == 2 ? 4 : 32;
         }
         left--;
-        const float use = P_BIAS + lr - (m == -INFINITY ? 0.0f : m);
+        const float use = P_BIAS + lr - (mg == -INFINITY ? 0.0f : mg);
         float sum = 0.0f;
 #pragma unroll
         for (int q = 0; q < 2; q++) {
@@ -445,30 +467,35 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
             tmem_st16(lane_base + 64 * h + 32 * q, p1);
             if (NP == 2) tmem_st16(lane_base + 64 * h + 32 * q + 16, p2);
         }
-        l = fmaf(sum, ex2(-lr), l);
-        if (kb + 1 < tiles_n) load_pages(raw4, kc, na, nb, true);
+        l = fmaf(sum, ex2(dm - lr), l);
+        const bool more = again || kb + 1 < tiles_n;
+        if (!again) {
+            pa = na, pb = nb;
+            na = page_at(2 * kb + 4), nb = page_at(2 * kb + 5);
+            kb++;
+        }
+        second = again;
+        if (more) load_pages(raw4, kc, pa, pb, true);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         fence_before();
-        __syncthreads();                                     // P(kb) and V(kb) in place; the maxima and a group's P V read
+        __syncthreads();                                     // P and V in place; the maxima and a group's P V read
         fence_after();
         if (tid == 0 && ok) {
             issue_o(!group);
-            last_o = kb;
+            last_o = it;
         }
         __syncwarp();
-        pa = na, pb = nb;
-        na = page_at(2 * kb + 4), nb = page_at(2 * kb + 5);
-        if (ok) ok = bar_wait(bar_o, (uint32_t)(kb & 1), abort, p.err, ERR_WAIT);
+        if (ok) ok = bar_wait(bar_o, (uint32_t)(it & 1), abort, p.err, ERR_WAIT);
         fence_after();
-        if (kb + 1 < tiles_n) {
+        if (more) {
             store_k(raw4);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             fence_before();
-            __syncthreads();                                 // K(kb + 1) in place
+            __syncthreads();                                 // the next K in place
             fence_after();
             if (tid == 0 && ok) {
                 issue_s();
-                last_s = kb + 1;
+                last_s = it + 1;
             }
             __syncwarp();
         }
@@ -480,7 +507,7 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
     float4 *const po = (float4 *)tiles;
     xsum[tid] = l;
     __syncthreads();
-    const float sum = xsum[r] + xsum[r + 128], inv = inverse(sum);
+    const float sum = xsum[r] + xsum[r + 128], inv = inverse(sum), last = sv0 * ex2(dm);
     const long long out_off = (seq.row0 + tok) * p.ld_out + head_off + DH * h;
 #pragma unroll 1
     for (int c = 0; c < DH; c += 32) {
@@ -490,7 +517,7 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
         for (int d = 0; d < 32; d += 4) {
             float v[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = fmaf(__uint_as_float(pv[d + e]), sv0, o[c + d + e]);
+            for (int e = 0; e < 4; e++) v[e] = fmaf(__uint_as_float(pv[d + e]), last, o[c + d + e]);
             if (p.S > 1) {
                 po[r * P4 + ((DH * h + c + d) / 4 ^ (r & (P4 - 1)))] = make_float4(v[0], v[1], v[2], v[3]);
             } else if (ok && r0 + r < R && DH * h + c + d < p.D) {

@@ -17,9 +17,8 @@ from test_gpu_lm import PAGE, TYPES, U, Pool, call, gen, half_step, lib, randn  
 pytestmark = pytest.mark.gpu
 
 
-def exact(pool, q, new, kv, group, scale, t, causal=True, window=0, unlike=1.0):
-    """64-bit attention of q [n, heads, d] and the bound on each value's error, on the GPU. unlike: how far apart the V
-    scales of a group of pages are (up to 64)."""
+def exact(pool, q, new, kv, group, scale, t, causal=True, window=0):
+    """64-bit attention of q [n, heads, d] and the bound on each value's error, on the GPU."""
     few = max(new) * group <= 64
     f32 = t == "f32"
     out, tol = torch.zeros_like(q, dtype=torch.float64), torch.zeros_like(q, dtype=torch.float64)
@@ -57,9 +56,14 @@ def exact(pool, q, new, kv, group, scale, t, causal=True, window=0, unlike=1.0):
                 lost = PAGE * (torch.where(coarse, 2.0 ** -17, 2.0 ** -24) * top_w) @ vt / l
             else:
                 # Weights are fp16 under 2^8 (two of them with fp32): half a step of 11 (22) bits, and of fp16's
-                # subnormals, 2^-25 / 2^8, times what the page's V scale is below its group's.
+                # subnormals, 2^-25 / 2^8 of a reference at most 2^8 over the group's largest weight, of pages whose V scales
+                # are within 2^3: six standard deviations (0.58 each) of as many roundings as a group has keys, against the
+                # row's own sum of weights times |V| (the largest key's |V| a quarter of the page's or more), or, where
+                # that key's V is 0, all of them against the key.
                 rel += (2.0 ** -23 if f32 else 2.0 ** -12) + (64 if f32 else 256) * 2e-8
-                lost = torch.minimum(w, torch.full_like(w, unlike * 2.0 ** -33)) @ vv.abs() / l
+                group_keys = min(m, 512 if f32 else 4096)
+                lost = torch.minimum(torch.minimum(w, torch.full_like(w, 2.0 ** -33)) @ vv.abs() / l,
+                                     4 * 6 * 0.58 * math.sqrt(group_keys) * 2.0 ** -22 * mass)
             out[at:at + n, h] = w @ vv / l
             tol[at:at + n, h] = mass * rel + lost
         at += n
@@ -76,6 +80,8 @@ def run(lib, pool, q, new, heads, scale, t, causal=True, window=0, **kw):
 
 
 def near(got, want, tol):
+    if not got.numel():
+        return
     over = (got.double() - want).abs() - tol
     worst = ((got.double() - want).abs() / want.abs().clamp(min=1e-300)).max().item()
     assert (over <= 0).all(), f"{over.max():.3g} over; relative error up to {worst:.3g}"
@@ -123,3 +129,49 @@ def test_a_row_does_not_depend_on_the_launch(lib, new, group):
     want, tol = exact(pool, q, [new], [20000], group, 0.125, "bf16")
     for hint in (1, 700, 20000):
         near(run(lib, pool, q, [new], group, 0.125, "bf16", max_kv=hint), want, tol)
+
+
+# ------------------------------------------------------------------ pages of unlike V scales
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("low", [2.0 ** -7, 1e-6, 1e-12, 1e-30])
+@pytest.mark.parametrize("new,group", [(1, 4), (16, 4), (250, 4)])
+@pytest.mark.parametrize("gap", [0.0, 20.0])
+def test_attention_of_rows_whose_weight_lies_in_pages_of_small_v(lib, new, group, gap, low, t):
+    """Every other page's V is `low` times its neighbours'. Rows that see the small one alone, or give it e^gap times the
+    weight, are as right as any."""
+    keys, d = 250, 128
+    for first in (0, 1):
+        pool = Pool(gen(130), 1, d, [keys])
+        pool.ks[:] = 1 / 73.0
+        for i in range(4):
+            page = int(pool.table[0, i])
+            small = i % 2 == first
+            pool.vs[page] = 0.01 * (low if small else 1.0)
+            pool.k[page, :, :, :16] = 127 if small else 0
+        q = randn(gen(131), new, group, d, dtype=torch.float64)
+        q[..., :16] = gap * math.sqrt(d) / (16 * 127 / 73.0)
+        q = q.to(TYPES[t][0])
+        want, tol = exact(pool, q, [new], [keys], group, 1 / math.sqrt(d), t)
+        near(run(lib, pool, q, [new], group, 1 / math.sqrt(d), t), want, tol)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("new,group", [(140, 1), (190, 4)])
+def test_attention_of_v_scales_at_the_ends_of_fp32(lib, new, group, t):
+    """A later page of huge V leaves the rows before it alone; scales below fp32's normal numbers are scales."""
+    pool = Pool(gen(140), 1, 64, [190])
+    pages = pool.table[0, :3].long()
+    q = randn(gen(141), new, group, 64, dtype=TYPES[t][0])
+    for huge in (1e30, 1e36):
+        pool.vs[pages] = torch.tensor([1e-3, 1e20, huge], device="cuda")[:, None]
+        want, tol = exact(pool, q, [new], [190], group, 0.125, t)
+        got = run(lib, pool, q, [new], group, 0.125, t)
+        # the sum of weights times V passes fp32's range with the second one: 60 x 1.27e38 over rows that see that page
+        sees = torch.arange(190 - new, 190) >= (128 if huge > 1e30 else 190)
+        near(got[~sees], want[~sees], tol[~sees])
+    pool.vs[pages] = torch.tensor([2e-39, 3e-40, 1e-38], device="cuda")[:, None]
+    want, tol = exact(pool, q, [new], [190], group, 0.125, t)
+    # a page's factor is rounded to 2^-150 and multiplied by its P V, below 64 * 127 * 2^23 at 2^11 for few rows, and
+    # below 128 * 127 * 2^15 for many: 2^-124 for three pages
+    near(run(lib, pool, q, [new], group, 0.125, t), want, tol + 2.0 ** -124)
