@@ -107,6 +107,10 @@ __device__ __forceinline__ void load_q4(const AttnArgs &p, long long off, float 
         x[e] = p.type == GGML_TYPE_BF16 ? __uint_as_float((uint32_t)h[e] << 16) : __half2float(__ushort_as_half(h[e]));
 }
 
+// O is kept times this, about the root of what a weight's digits count to: the factor of a tile's P V (its V scale over
+// that count) then keeps its bits down to V of 1e-33, and the sums have room up to 1e35. At 1 it lost them below 1e-29.
+constexpr float O_UNIT = 2048.0f;
+
 template <int KS, int NP, int RW, int WM, int WN, int NSLOT>
 struct Shape {
     static constexpr int DP = KS * 32;                       // dims, padded
@@ -526,7 +530,7 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
                 constexpr bool THREE = decltype(three)::value;
 #pragma unroll
                 for (int r = 0; r < RW; r++) {
-                    fold[r] *= THREE ? 1.0f / 8388607.0f : 1.0f / 65535.0f;
+                    fold[r] *= O_UNIT / (THREE ? 8388607.0f : 65535.0f);
 #pragma unroll
                     for (int w = 0; w < 4; w++) {
                         uint32_t y[4];
@@ -626,7 +630,7 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
         for (int r = 0; r < RW; r++) {
             const int row = RPW * wm + g + 8 * r;
             if (row >= R) continue;
-            const float inv = inverse(l[r]);
+            const float inv = inverse(l[r]) * (1.0f / O_UNIT);
             const long long off = (seq.row0 + tok_of(row)) * p.ld_out + row_off[r];
 #pragma unroll
             for (int n = 0; n < NT; n++) {
@@ -676,7 +680,7 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
             if (d == 0) qm[r] = top, ql[r] = sum;
             continue;
         }
-        const float inv = inverse(sum);
+        const float inv = inverse(sum) * (1.0f / O_UNIT);
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] *= inv;
         store_out<4>(p, (seq.row0 + tok_of(r)) * p.ld_out + (long long)(head * p.G + r - tok_of(r) * p.G) * p.D + d, v);
@@ -687,7 +691,7 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
     for (int i = threadIdx.x + rank * blockDim.x; i < rows * d4; i += blockDim.x * p.S) {
         const int r = (int)((unsigned)i * p.d4_inv >> 20), d = 4 * (i - r * d4);
         float v[4];
-        cluster_join<MAX_SPLIT>(a_qm + 4 * r, a_ql + 4 * r, a_po + 4 * (r * Sh::PITCH + d), p.S, v);
+        cluster_join<MAX_SPLIT>(a_qm + 4 * r, a_ql + 4 * r, a_po + 4 * (r * Sh::PITCH + d), p.S, 1.0f / O_UNIT, v);
         store_out<4>(p, (seq.row0 + tok_of(r)) * p.ld_out + (long long)(head * p.G + r - tok_of(r) * p.G) * p.D + d, v);
     }
     cluster_sync();                                          // no CTA leaves while another reads its shared memory

@@ -128,9 +128,9 @@ __device__ __forceinline__ void cluster_sync()
 constexpr int MAX_SPLIT = 10;            // CTAs of a cluster; of 11 or more a B200 holds 7 clusters at a time
 
 // Four output values of a row from the S CTAs of a cluster: their maxima, sums and O's at these shared-memory addresses,
-// read together (MAX at least S), joined in the CTAs' order.
+// read together (MAX at least S), joined in the CTAs' order, times `unit`.
 template <int MAX>
-__device__ __forceinline__ void cluster_join(uint32_t a_m, uint32_t a_l, uint32_t a_o, int S, float (&v)[4])
+__device__ __forceinline__ void cluster_join(uint32_t a_m, uint32_t a_l, uint32_t a_o, int S, float unit, float (&v)[4])
 {
     float m[MAX], l[MAX], top = -INFINITY, sum = 0.0f;
     float4 x[MAX];
@@ -153,7 +153,7 @@ __device__ __forceinline__ void cluster_join(uint32_t a_m, uint32_t a_l, uint32_
         sum = fmaf(w, l[s], sum);
         v[0] = fmaf(w, x[s].x, v[0]), v[1] = fmaf(w, x[s].y, v[1]), v[2] = fmaf(w, x[s].z, v[2]), v[3] = fmaf(w, x[s].w, v[3]);
     }
-    const float inv = inverse(sum);
+    const float inv = inverse(sum) * unit;
 #pragma unroll
     for (int e = 0; e < 4; e++) v[e] *= inv;
 }

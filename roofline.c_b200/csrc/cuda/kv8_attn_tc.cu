@@ -541,7 +541,7 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
                 const int k = (int)((unsigned)i * p.d4_inv >> 20), q = rank + k * p.S, d = i - k * d4;
                 float v[4];
                 cluster_join<decltype(most)::value>(a_m + 4 * q, a_m + 4 * (q + 128), a_po + 16 * (q * P4 + (d ^ (q & (P4 - 1)))),
-                                                    p.S, v);
+                                                    p.S, 1.0f, v);
                 const int row = r0 + q;
                 store_out<4>(p, (seq.row0 + row / p.G) * p.ld_out + (long long)(head * p.G + row % p.G) * p.D + 4 * d, v);
             }
