@@ -111,6 +111,10 @@ __device__ __forceinline__ void load_q4(const AttnArgs &p, long long off, float 
 // that count) then keeps its bits down to V of 1e-33, and the sums have room up to 1e35. At 1 it lost them below 1e-29.
 constexpr float O_UNIT = 2048.0f;
 
+// What a weight of 1 is as a whole number of 23 and 16 bits. Below 2^23 by more than ex2's error and the product's
+// rounding up to FAR_SCORE, 2^-12 of the weight at most, can put it above 1: a weight past the last number would be 0.
+constexpr float P3 = 8386000.0f, P2 = 65516.0f;
+
 template <int KS, int NP, int RW, int WM, int WN, int NSLOT>
 struct Shape {
     static constexpr int DP = KS * 32;                       // dims, padded
@@ -263,7 +267,7 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
             const double back = m < 1e-20f ? 0x1p-80 : 1.0;
             m = fmaxf(m * lift, 1e-21f);
             const float up = Q / m;
-            qs[i] = odd ? __int_as_float(0x7FC00000) : (float)((double)m * back * (double)p.scale_log2 * (1.0 / Q));
+            qs[i] = odd ? __int_as_float(0x7FC00000) : (float)fmin((double)m * back * (double)p.scale_log2 * (1.0 / Q), 3e38);
 #pragma unroll
             for (int c = 0; c < KS / 2; c++)
 #pragma unroll
@@ -340,7 +344,8 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
         if (lane < EACH && warp + lane * WM * WN < Sh::ROWS) {
             // the factor of the row: NaN stays NaN
             const double m = my_max < 1e-20f ? fmax((double)my_max * 0x1p80, 1e-21) * 0x1p-80 : (double)my_max;
-            sqs[warp + lane * WM * WN] = (float)(m * (double)p.scale_log2 * (1.0 / Q));
+            const double s = m * (double)p.scale_log2 * (1.0 / Q);
+            sqs[warp + lane * WM * WN] = (float)(s > 3e38 ? 3e38 : s);
         }
         __syncthreads();
 #pragma unroll
@@ -491,17 +496,22 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
                 for (int j = 0; j < 8; j++) top = fmaxf(top, fmaxf(f[j][2 * r], f[j][2 * r + 1]));
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-                // a zero factor would turn a masked -inf into NaN; a NaN factor (a NaN query) has to stay
-                float cs = qs[r] * tk;
-                cs = cs < 1e-37f ? 1e-37f : cs;
-                // raised by 2^-22 of itself, so that rounding never puts a weight above 1 (its digits would overflow)
-                float mt = top * cs;
-                mt = top == -INFINITY ? top : fmaf(fabsf(mt), 0x1p-22f, mt);
-                const float mn = fmaxf(m[r], mt), use = mn == -INFINITY ? 0.0f : mn, ref = mt == -INFINITY ? 0.0f : mt;
+                float cs = tame(qs[r] * tk);
+                const bool none = top == -INFINITY, far = !none && fabsf(top * cs) > FAR_SCORE;
+                const float mt = none ? top : in_range(top * cs);
+                float ref = none ? 0.0f : mt;
+                const float mn = fmaxf(m[r], mt), use = mn == -INFINITY ? 0.0f : mn;
                 const float beta = ex2(mt - use);
                 up[r] = ex2(m[r] - use);
                 grew |= mn != m[r];
                 m[r] = mn;
+                if (far) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+#pragma unroll
+                        for (int c = 0; c < 2; c++) f[j][2 * r + c] = (f[j][2 * r + c] - top) * cs;
+                    cs = 1.0f, ref = 0.0f;
+                }
                 float sum = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 8; j++)
@@ -513,7 +523,7 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
                     }
                 l[r] = fmaf(l[r], up[r], sum * beta);
                 fold[r] = tv * beta;
-                even = even && sum >= 1.0f / 16.0f;
+                even = even && !(sum < 1.0f / 16.0f);
             }
             fine = NP == 3 || !__all_sync(0xFFFFFFFFu, even);
             if (__any_sync(0xFFFFFFFFu, grew)) {
@@ -530,14 +540,14 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
                 constexpr bool THREE = decltype(three)::value;
 #pragma unroll
                 for (int r = 0; r < RW; r++) {
-                    fold[r] *= O_UNIT / (THREE ? 8388607.0f : 65535.0f);
+                    fold[r] *= O_UNIT / (THREE ? P3 : P2);
 #pragma unroll
                     for (int w = 0; w < 4; w++) {
                         uint32_t y[4];
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             const float v = f[2 * w + (e >> 1)][2 * r + (e & 1)];
-                            y[e] = __float_as_uint(THREE ? fmaf(v, 8388607.0f, 8388608.0f) : fmaf(v, 65535.0f / 65536.0f, 128.0f));
+                            y[e] = __float_as_uint(THREE ? fmaf(v, P3, 8388608.0f) : fmaf(v, P2 / 65536.0f, 128.0f));
                         }
                         const uint32_t u = __byte_perm(y[0], y[1], 0x5140), v = __byte_perm(y[2], y[3], 0x5140);
                         const uint32_t d0 = __byte_perm(u, v, 0x5410), d1 = __byte_perm(u, v, 0x7632);

@@ -36,6 +36,16 @@ __device__ __forceinline__ float ex2(float x)
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// A score's factor without the values that would turn 0 or a masked -inf times it into NaN; a NaN (a query with a NaN or
+// an infinity) stays.
+__device__ __forceinline__ float tame(float c) { return c < 1e-37f ? 1e-37f : c > 3e38f ? 3e38f : c; }
+// A scaled score within fp32's range, which differences of two of them pass to -inf only.
+__device__ __forceinline__ float in_range(float x) { return fminf(fmaxf(x, -3e38f), 3e38f); }
+
+// Scaled scores beyond this are subtracted before they are scaled: fp32's rounding of the product, 2^-24 of it, would
+// otherwise enter the exponent (at 2^27 the row's largest weight came out as 2^-32).
+constexpr float FAR_SCORE = 4096.0f;
+
 // 16 consecutive values of a query row.
 __device__ __forceinline__ void load_q16(const AttnArgs &p, long long off, float (&x)[16])
 {

@@ -366,12 +366,12 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
     __syncwarp();
 
     float o[DH], m = -INFINITY, l = 0.0f;                    // m: what O and l stand against; l: this half's share
-    float mg = -INFINITY, dm = 0.0f, sv0 = 0.0f;             // the group's references; dm = mg - 8 - m
+    float mg = -INFINITY, rest = 0.0f, dm = 0.0f, sv0 = 0.0f;   // the group's references, mg + rest and sv0; dm = mg - 8 - m
 #pragma unroll 1
     for (int j = 0; j < DH; j++) o[j] = 0.0f;                // used at a group's end only: kept in local memory
     int left = 0;                                            // tiles that the group may still take
-    // The group's P V, complete, joins O; then O and l move to the new m, and a group begins with a tile of maximum `t`.
-    auto fold = [&](float t, bool any) {
+    // The group's P V, complete, joins O; then O and l move to the new m, and a group begins with a tile of maximum t + low.
+    auto fold = [&](float t, float low, bool any) {
         const float now = fmaxf(m, t), ref = t < now - FAR_M ? t + ROOM : now, alpha = now == m ? 1.0f : ex2(m - now), f = sv0 * ex2(dm);
 #pragma unroll 1
         for (int c = 0; c < DH; c += 32) {
@@ -383,7 +383,8 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
         l *= alpha;
         m = now;
         mg = ref;
-        dm = ref == -INFINITY ? 0.0f : ref - P_BIAS - now;   // a row that sees nothing yet has weights of 0
+        rest = ref == t ? low : 0.0f;
+        dm = ref == -INFINITY ? 0.0f : ref - now - P_BIAS;   // a row that sees nothing yet has weights of 0
     };
     // log2(s / sv0), also of scales below fp32's normal numbers
     auto log_ratio = [&](float s) {
@@ -404,7 +405,7 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
         const float v_min = fminf(va, vb), v_max = fmaxf(va, vb);
         const bool apart = v_min > 0.0f && v_max > 8.0f * v_min, again = apart && !second;   // the same for the whole CTA
         const bool on = mine >= 0 && (!apart || second == (h != 0));
-        const float cs = cs0 * (on ? sk : 1.0f), c = cs < 1e-37f ? 1e-37f : cs;   // not 0: a masked -inf stays -inf
+        const float c = tame(cs0 * (on ? sk : 1.0f));
         float lr = sv == sv0 || !on ? 0.0f : log_ratio(sv);
         const bool whole = __all_sync(0xFFFFFFFFu, on && key0 >= lo && key0 + PAGE - 1 <= hi);
         if (ok) ok = bar_wait(bar_s, (uint32_t)(it & 1), abort, p.err, ERR_WAIT);
@@ -435,38 +436,53 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
 #pragma unroll
             for (int j = 0; j < 32; j++) top = fmaxf(top, x[j]);
         }
-        top = top == -INFINITY ? top : top * c;
-        xmax[tid] = top;
-        const bool group = __syncthreads_or(left == 0 || !(fabsf(lr) <= NEAR_V) || top + lr > mg + GROWTH);
+        // The maximum, scaled, is high + low: the product and what its rounding left, which counts where scores pass what
+        // 24 bits resolve. A NaN (a NaN query) opens no group.
+        const float high = top == -INFINITY ? top : in_range(top * c), low = fabsf(high) < 3e38f ? fmaf(top, c, -high) : 0.0f;
+        xmax[tid] = high;
+        xsum[tid] = low;
+        const bool group = __syncthreads_or(left == 0 || !(fabsf(lr) <= NEAR_V) || high - mg + (low - rest) + lr > GROWTH);
         if (group) {
-            fold(fmaxf(xmax[r], xmax[r + 128]), it > 0);
+            const float a = xmax[r], z = xmax[r + 128];
+            fold(fmaxf(a, z), a > z ? xsum[r] : a < z ? xsum[r + 128] : fmaxf(xsum[r], xsum[r + 128]), it > 0);
             sv0 = !apart ? v_max : second ? vb : va;
             lr = sv == sv0 || !on ? 0.0f : fmaxf(log_ratio(sv), -60.0f);     // beyond NEAR_V only where sv is 0
             left = NP == 2 ? 4 : 32;
         }
         left--;
-        const float use = P_BIAS + lr - (mg == -INFINITY ? 0.0f : mg);
+        const bool far = fabsf(mg) > FAR_SCORE && mg != -INFINITY;
+        const float ref = mg == -INFINITY ? 0.0f : mg, use = P_BIAS + lr - ref;
         float sum = 0.0f;
+        auto weights = [&](auto some_far) {
 #pragma unroll
-        for (int q = 0; q < 2; q++) {
-            float x[32];
-            uint32_t p1[16], p2[16];
-            scores(q, x);
+            for (int q = 0; q < 2; q++) {
+                float x[32];
+                uint32_t p1[16], p2[16];
+                scores(q, x);
+                auto weight = [&](float s) {
+                    if (!decltype(some_far)::value || !far) return ex2(fmaf(s, c, use));
+                    const float y = fmaf(s, c, -ref) - rest;
+                    return ex2((y > GROWTH - lr ? GROWTH - lr : y) + (P_BIAS + lr));    // above only past fp32's range
+                };
 #pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-                const float a = ex2(fmaf(x[j], c, use)), z = ex2(fmaf(x[j + 1], c, use));
-                sum += a + z;
-                const __half2 u = __floats2half2_rn(a, z);
-                p1[j / 2] = *(const uint32_t *)&u;
-                if (NP == 2) {
-                    const float2 w = __half22float2(u);
-                    const __half2 v = __floats2half2_rn(a - w.x, z - w.y);
-                    p2[j / 2] = *(const uint32_t *)&v;
+                for (int j = 0; j < 32; j += 2) {
+                    const float a = weight(x[j]), z = weight(x[j + 1]);
+                    sum += a + z;
+                    const __half2 u = __floats2half2_rn(a, z);
+                    p1[j / 2] = *(const uint32_t *)&u;
+                    if (NP == 2) {
+                        const float2 w = __half22float2(u);
+                        const __half2 v = __floats2half2_rn(a - w.x, z - w.y);
+                        p2[j / 2] = *(const uint32_t *)&v;
+                    }
                 }
+                if (decltype(some_far)::value) __syncwarp();
+                tmem_st16(lane_base + 64 * h + 32 * q, p1);
+                if (NP == 2) tmem_st16(lane_base + 64 * h + 32 * q + 16, p2);
             }
-            tmem_st16(lane_base + 64 * h + 32 * q, p1);
-            if (NP == 2) tmem_st16(lane_base + 64 * h + 32 * q + 16, p2);
-        }
+        };
+        if (__any_sync(0xFFFFFFFFu, far)) weights(std::true_type());
+        else weights(std::false_type());
         l = fmaf(sum, ex2(dm - lr), l);
         const bool more = again || kb + 1 < tiles_n;
         if (!again) {

@@ -175,3 +175,34 @@ def test_attention_of_v_scales_at_the_ends_of_fp32(lib, new, group, t):
     # a page's factor is rounded to 2^-150 and multiplied by its P V, below 64 * 127 * 2^23 at 2^11 for few rows, and
     # below 128 * 127 * 2^15 for many: 2^-123 for three pages
     near(run(lib, pool, q, [new], group, 0.125, t), want, tol + 2.0 ** -123)
+
+
+# ------------------------------------------------------------------ scores past what 24 bits resolve
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("size", [3e2, 1e4, 1e6, 1e8, 1e10, 1e20])
+@pytest.mark.parametrize("new,group", [(1, 4), (7, 4), (16, 4), (70, 4)])
+def test_attention_of_scores_of_any_size(lib, new, group, size, t):
+    """Where the largest score is ahead by more than its own rounding, softmax is one: the row is that key's V."""
+    keys, d = 1000, 64
+    pool = Pool(gen(120), 2, d, [keys])
+    pool.ks *= size / (100.0 * 73 * 0.025 * 8)                           # |q| about 100, |k| 73 codes, 8 = sqrt(d)
+    q = randn(gen(121), new, 2 * group, d, dtype=TYPES[t][0], spread=100.0)
+    got = run(lib, pool, q, [new], 2 * group, 1.0, t).double()
+    k, v = pool.values(0, keys)
+    hide = torch.arange(keys, device="cuda")[None] > torch.arange(keys - new, keys, device="cuda")[:, None]
+    sure = 0
+    for h in range(2 * group):
+        s = (q[:, h].double() @ k[h // group].T).masked_fill(hide, -math.inf)
+        two, at = s.topk(2, -1)
+        # half a digit of q against each |k|, as in exact(), and eight roundings of the largest score; the keys e^40 behind
+        # leave what `others` says of them
+        slack = q[:, h].double().abs().amax(-1) / 65024 * k[h // group].abs().sum(-1).max() + 8 * U * s.masked_fill(hide, 0).abs().amax(-1)
+        ahead = two[:, 0] - two[:, 1] > 2 * slack + 40
+        sure += int(ahead.sum())
+        want = v[h // group][at[:, 0]]
+        others = keys * math.exp(-40) * v.abs().max()
+        bad = (got[:, h] - want).abs() > want.abs() * (half_step(TYPES[t][0]) + 2.0 ** -11) + others
+        assert not bad[ahead].any(), f"{int(bad[ahead].any(-1).sum())} of {int(ahead.sum())} rows"
+        assert got[:, h].isfinite().all()
+    assert size < 1e4 or sure > new * group                              # half of the rows and more
