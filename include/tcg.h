@@ -291,12 +291,14 @@ typedef struct {
  * page's scale grows to max(scale, |largest new value| / 127); when it grows
  * the page's older codes become round(code * (old / new)). Codes are
  * round(x / scale), ties to even, all in fp32; a NaN is stored as 0, an
- * infinity as the largest finite value. A page that a call writes must stand
+ * infinity as fp32's largest finite value (which reads back as an infinity in
+ * the 16-bit types, as any value beyond their range does). A page that a call writes must stand
  * in its tables once, for one sequence (pages that are only read may be
  * shared); otherwise what that page holds afterwards is not defined. */
 bool tcg_kv8_append(const tcg_kv8_t *c, const tcg_kv8_step_t *s, const void *k, const void *v,
                     int64_t ld_k, int64_t ld_v, ggml_type_t t);
-/* Read the step's rows back as values (code * scale, rounded to t). */
+/* Read the step's rows back as values (code * scale in fp32, at most its
+ * largest finite value, rounded to t). */
 bool tcg_kv8_read(void *k, void *v, const tcg_kv8_t *c, const tcg_kv8_step_t *s, int64_t ld_k, int64_t ld_v,
                   ggml_type_t t);
 /* Attention of the step's queries (n_head heads, a multiple of n_kv_head;

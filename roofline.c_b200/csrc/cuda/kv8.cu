@@ -57,6 +57,13 @@ __device__ __forceinline__ float finite(float x)
     return x == x ? fminf(fmaxf(x, -3.402823466e38f), 3.402823466e38f) : 0.0f;
 }
 
+// A product of a code and a scale, which rounds to an infinity for the largest ones (127 * fl(largest / 127)); NaN stays.
+__device__ __forceinline__ float at_most_finite(float x)
+{
+    asm("min.NaN.xorsign.abs.f32 %0, %0, %1;" : "+f"(x) : "f"(3.402823466e38f));
+    return x;
+}
+
 // The format's code for x at scale s, as it is defined. The clamp is for the quotients of a subnormal scale.
 __device__ __forceinline__ int code_of(float x, float s)
 {
@@ -394,7 +401,7 @@ __global__ void __launch_bounds__(ROWS_THREADS) read_kernel(const RowsArgs p)
             if (!my.in || slot < at.lo || slot >= at.hi) continue;
             float v[V];
 #pragma unroll
-            for (int e = 0; e < V; e++) v[e] = bad ? 0.0f : (float)c[k][j].v[e] * scale;
+            for (int e = 0; e < V; e++) v[e] = bad ? 0.0f : at_most_finite((float)c[k][j].v[e] * scale);
             store_pack<T, V>(y + slot * ld, v);
         }
 }

@@ -206,3 +206,51 @@ def test_attention_of_scores_of_any_size(lib, new, group, size, t):
         assert not bad[ahead].any(), f"{int(bad[ahead].any(-1).sum())} of {int(ahead.sum())} rows"
         assert got[:, h].isfinite().all()
     assert size < 1e4 or sure > new * group                              # half of the rows and more
+
+
+# ------------------------------------------------------------------ infinities
+
+@pytest.mark.parametrize("n", [2, 70])
+def test_an_infinity_is_read_back_as_the_largest_finite_value(lib, n):
+    """Stored by both forms of the append (few rows, many), with fp32's largest value itself, in K and in V."""
+    biggest = torch.finfo(torch.float32).max
+    pool = Pool(gen(150), 1, 64, [n])
+    x = [randn(gen(151 + i), n, 64) for i in range(2)]
+    for i in range(2):
+        x[i][0, 3], x[i][n - 1, 5 + i], x[i][n - 1, 9] = math.inf, -math.inf, -biggest
+    s = pool.step([n])
+    call(lib.tcg_kv8_append, C.byref(pool.cache()), C.byref(s), x[0].data_ptr(), x[1].data_ptr(), 64, 64, tcg.F32)
+    for dt, code in TYPES.values():
+        out = [torch.empty((n, 64), dtype=dt, device="cuda") for _ in range(2)]
+        call(lib.tcg_kv8_read, out[0].data_ptr(), out[1].data_ptr(), C.byref(pool.cache()), C.byref(s), 64, 64, code)
+        want = torch.tensor(biggest, device="cuda").to(dt)
+        for i in range(2):
+            assert out[i][0, 3] == want and out[i][n - 1, 5 + i] == -want and out[i][n - 1, 9] == -want
+            rest = out[i].clone()
+            rest[0, 3] = rest[n - 1, 5 + i] = rest[n - 1, 9] = 0
+            assert (rest == 0).all()                                     # half a step of those pages is 1.3e36
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("new,group", [(1, 4), (30, 2), (90, 4)])
+def test_attention_over_an_infinite_key(lib, new, group, t):
+    """A K with an infinity decides each row that sees it, one way or the other; the rows before it never see it."""
+    pool = Pool(gen(160), 1, 64, [200])
+    x = randn(gen(161), 1, 64)
+    x[0, 7] = math.inf
+    v = pool.values(0, 200)[1].clone()
+    kv = torch.tensor([171], dtype=torch.int32, device="cuda")
+    start = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    s = tcg.Kv8Step(start.data_ptr(), kv.data_ptr(), pool.table.data_ptr(), pool.ld, 1, 1, 1, 171)
+    call(lib.tcg_kv8_append, C.byref(pool.cache()), C.byref(s), x.data_ptr(), x.data_ptr(), 64, 64, tcg.F32)
+    pool.v[pool.table[0, 2].long()], pool.vs[pool.table[0, 2].long()] = 0, 0.01      # its V too was infinite
+    v = pool.values(0, 200)[1]
+    q = randn(gen(162), new, group, 64, dtype=TYPES[t][0])
+    q[..., 7] = torch.where(q[..., 7] >= 0, 1.0, -1.0).to(q.dtype)
+    got = run(lib, pool, q, [new], group, 0.125, t).double()
+    assert got.isfinite().all()
+    for i in range(new):
+        pos = 200 - new + i
+        for h in range(group):
+            if pos >= 170 and q[i, h, 7] > 0:                            # the older keys of its page moved to codes of 0
+                assert (got[i, h] - v[0, 170]).abs().max() <= 1e-6
