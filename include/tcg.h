@@ -241,8 +241,10 @@ bool tcg_rope_scale_factors(tcg_rope_t *r, const float *f, int n);
  * (10000 when absent), .rope.dimension_count, .attention.key_length (or
  * embedding_length / attention.head_count), .rope.scaling.type (none,
  * linear, yarn) with .factor, .original_context_length and .attn_factor, and
- * the F32 tensor rope_freqs.weight. The pair layout is the architecture's;
- * the file does not record it. */
+ * the F32 tensor rope_freqs.weight. Anything else that a file says of
+ * positions (another key under <arch>.rope., another rope_ tensor, a factor
+ * without a scaling type) is refused, unless its value changes nothing. The
+ * pair layout is the architecture's; the file does not record it. */
 bool tcg_rope_from_gguf(tcg_rope_t *r, const gguf_t *g, int layout);
 
 /* out = x rotated: n_tok rows of n_head heads, token i at position pos[i]

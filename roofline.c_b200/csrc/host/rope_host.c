@@ -113,6 +113,60 @@ bool tcg_rope_scale_factors(tcg_rope_t *r, const float *f, int n)
     return true;
 }
 
+/* A number of the metadata, of any scalar type; `fallback` when the key is absent, false when it holds something else. */
+static bool number(const gguf_t *g, const char *key, double fallback, double *out)
+{
+    const gguf_kv_t *kv = gguf_find(g, key);
+    int64_t i;
+    float f;
+    *out = fallback;
+    if (!kv) return true;
+    if (kv->type == GGUF_T_FLOAT64) *out = kv->v.f64;
+    else if (gguf_get_f32(g, key, &f)) *out = (double)f;
+    else if (kv->type != GGUF_T_BOOL && gguf_get_i64(g, key, &i)) *out = (double)i;
+    else return false;
+    return true;
+}
+
+/* What else a file says of positions must not be passed over, since it changes the angles or the magnitude: every key
+ * under <arch>.rope. is one that the plan follows, says nothing (the value beside it), or is refused, and so is every
+ * tensor of rotary factors but rope_freqs.weight. False names the first one that is refused. */
+static bool all_known(const gguf_t *g, const char *arch, const char *who)
+{
+    static const char *const followed[] = { "dimension_count", "freq_base", "scaling.type", "scaling.factor",
+                                            "scaling.original_context_length", "scaling.attn_factor",
+                                            "scaling.finetuned" };       /* of the weights: it changes no angle */
+    static const struct { const char *name; double neutral; } idle[] = {
+        { "scale_linear", 1.0 }, { "scaling.yarn_ext_factor", 1.0 }, { "scaling.yarn_attn_factor", 1.0 },
+        { "scaling.yarn_beta_fast", 32.0 }, { "scaling.yarn_beta_slow", 1.0 }, { "scaling.yarn_log_multiplier", 0.0 } };
+    char start[80];
+    const size_t skip = (size_t)snprintf(start, sizeof start, "%s.rope.", arch);
+    for (uint64_t i = 0; i < g->n_kv; i++) {
+        const gguf_str_t key = g->kv[i].key;
+        if (!key.ptr || key.len < skip || memcmp(key.ptr, start, skip)) continue;
+        const gguf_str_t name = { key.ptr + skip, key.len - skip };
+        bool known = false;
+        for (size_t j = 0; j < sizeof followed / sizeof *followed; j++) known = known || gguf_str_eq(name, followed[j]);
+        for (size_t j = 0; j < sizeof idle / sizeof *idle; j++) {
+            char full[160];
+            double v;
+            snprintf(full, sizeof full, "%s%s", start, idle[j].name);
+            known = known || (gguf_str_eq(name, idle[j].name) && number(g, full, 0.0, &v) && v == idle[j].neutral);
+        }
+        if (!known) return host_fail("%s: '%.*s' is not followed here (tcg_rope_init and tcg_rope_scale_* take any rule)", who,
+                                     (int)(key.len < 100 ? key.len : 100), key.ptr);
+    }
+    for (uint64_t i = 0; i < g->n_tensors; i++) {
+        const gguf_str_t name = g->tensors[i].name;
+        if (!name.ptr || gguf_str_eq(name, "rope_freqs.weight")) continue;
+        for (uint64_t at = 0; at + 5 <= name.len; at++)
+            if (!memcmp(name.ptr + at, "rope_", 5))
+                return host_fail("%s: the tensor '%.*s' is not followed here", who, (int)(name.len < 100 ? name.len : 100),
+                                 name.ptr);
+    }
+    return true;
+}
+
 bool tcg_rope_from_gguf(tcg_rope_t *r, const gguf_t *g, int layout)
 {
     const char *who = "tcg_rope_from_gguf";
@@ -130,9 +184,13 @@ bool tcg_rope_from_gguf(tcg_rope_t *r, const gguf_t *g, int layout)
     const uint64_t n_rot = gguf_u64_or(g, KEY("rope.dimension_count"), d);
     if (d > TCG_ROPE_MAX_DIM || n_rot > d) return host_fail("%s: head length %llu, %llu of it rotated", who,
                                                                  (unsigned long long)d, (unsigned long long)n_rot);
+    if (!all_known(g, arch, who)) return false;
+    double base, factor, attn;
+    if (!number(g, KEY("rope.freq_base"), 10000.0, &base) || !number(g, KEY("rope.scaling.factor"), 0.0, &factor) ||
+        !number(g, KEY("rope.scaling.attn_factor"), 1.0, &attn))
+        return host_fail("%s: %s is not a number", who, key);
     tcg_rope_t plan;                            /* *r changes only when everything is read */
-    if (!tcg_rope_init(&plan, (int)d, (int)n_rot, layout, (double)gguf_f32_or(g, KEY("rope.freq_base"), 10000.0f)))
-        return false;
+    if (!tcg_rope_init(&plan, (int)d, (int)n_rot, layout, base)) return false;
     const gguf_tensor_t *t = gguf_tensor(g, "rope_freqs.weight");
     if (t) {
         if (t->type != GGML_TYPE_F32 || !t->data || t->n_elem != n_rot / 2)
@@ -141,17 +199,21 @@ bool tcg_rope_from_gguf(tcg_rope_t *r, const gguf_t *g, int layout)
         memcpy(f, t->data, (size_t)t->n_elem * sizeof(float));
         if (!tcg_rope_scale_factors(&plan, f, (int)t->n_elem)) return false;
     }
-    gguf_str_t kind;
-    if (gguf_get_str(g, KEY("rope.scaling.type"), &kind) && !gguf_str_eq(kind, "none")) {
-        const double factor = (double)gguf_f32_or(g, KEY("rope.scaling.factor"), 0.0f);
+    gguf_str_t kind = { NULL, 0 };
+    if (gguf_find(g, KEY("rope.scaling.type")) && !gguf_get_str(g, key, &kind)) return host_fail("%s: %s is not a text", who, key);
+    const bool yarn = gguf_str_eq(kind, "yarn");
+    if (!yarn && attn != 1.0) return host_fail("%s: attn_factor %g without a rope.scaling.type of yarn", who, attn);
+    if (!kind.ptr) {
+        /* some readers take a factor without a type as linear, some as none */
+        if (factor != 0.0 && factor != 1.0) return host_fail("%s: a rope.scaling.factor of %g without a type", who, factor);
+    } else if (!gguf_str_eq(kind, "none")) {
         if (gguf_str_eq(kind, "linear")) {
             if (!tcg_rope_scale_linear(&plan, factor)) return false;
-        } else if (gguf_str_eq(kind, "yarn")) {
+        } else if (yarn) {
             const uint64_t ctx = gguf_u64_or(g, KEY("rope.scaling.original_context_length"),
                                              gguf_u64_or(g, KEY("context_length"), 0));
             if (ctx > 0x7fffffffu) return host_fail("%s: original context %llu", who, (unsigned long long)ctx);
             /* a positive attn_factor scales the rule's own 0.1 ln(factor) + 1 */
-            const double attn = (double)gguf_f32_or(g, KEY("rope.scaling.attn_factor"), 1.0f);
             if (!(attn > 0.0)) return host_fail("%s: attn_factor %g", who, attn);
             if (!tcg_rope_scale_yarn(&plan, factor, (int)ctx, 32.0, 1.0, 0.0)) return false;
             plan.mscale *= (float)attn;

@@ -148,6 +148,40 @@ def test_plan_from_gguf(tmp_path):
     assert not _from_gguf(tmp_path, base, [("rope_freqs.weight", f, G.F32, (16,))])[0]      # 16 factors for 32 pairs
 
 
+def test_plan_from_gguf_passes_nothing_over(tmp_path):
+    """What changes the angles or the magnitude is followed or refused; what changes nothing is taken."""
+    base = {"general.architecture": "lm", "lm.embedding_length": 512, "lm.attention.head_count": 8}
+    yarn = {**base, "lm.rope.scaling.type": "yarn", "lm.rope.scaling.factor": 4.0,
+            "lm.rope.scaling.original_context_length": 2048}
+    f = np.full(32, 2.0, np.float32)
+    for kvs in ({"lm.rope.scale_linear": 4.0}, {"lm.rope.freq_base_swa": 1e5}, {"lm.rope.dimension_sections": [16.0, 24.0]},
+                {"lm.rope.scaling.factor": 4.0}, {"lm.rope.scaling.attn_factor": 1.2}, {"lm.rope.scaling.alpha": 2.0},
+                {"lm.rope.scaling.type": "linear", "lm.rope.scaling.factor": 2.0, "lm.rope.scaling.attn_factor": 0.5},
+                {"lm.rope.scaling.type": 1}, {"lm.rope.freq_base": "10000"}, {"lm.rope.scaling.yarn_log_multiplier": 0.1}):
+        ok, r = _from_gguf(tmp_path, {**base, **kvs})
+        assert not ok and "tcg_rope_from_gguf" in tcg.err() and r.n_rot == 0, kvs
+    for kvs in ({"lm.rope.scaling.yarn_log_multiplier": 0.1}, {"lm.rope.scaling.yarn_beta_fast": 16.0},
+                {"lm.rope.scaling.yarn_beta_slow": 2.0}, {"lm.rope.scaling.yarn_ext_factor": 0.0},
+                {"lm.rope.scaling.yarn_attn_factor": 2.0}):
+        assert not _from_gguf(tmp_path, {**yarn, **kvs})[0], kvs
+    for name in ("rope_factors_long.weight", "rope_factors_short.weight", "blk.0.rope_freqs.weight"):
+        ok, r = _from_gguf(tmp_path, base, [(name, f, G.F32, (32,))])
+        assert not ok and name in tcg.err() and r.n_rot == 0
+
+    plain, scaled = (_from_gguf(tmp_path, x)[1] for x in (base, yarn))
+    for kvs in ({"lm.rope.scale_linear": 1.0}, {"lm.rope.scaling.finetuned": True}, {"lm.rope.scaling.factor": 1.0},
+                {"lm.rope.scaling.attn_factor": 1.0}, {"lm.rope.scaling.type": "none", "lm.rope.scaling.factor": 4.0},
+                {"lm.rope.freq_base": 10000}, {"other.rope.scale_linear": 4.0}, {"lm.ropes": 1}):
+        ok, r = _from_gguf(tmp_path, {**base, **kvs})
+        assert ok and bytes(r) == bytes(plain), kvs
+    for kvs in ({"lm.rope.scaling.yarn_beta_fast": 32.0, "lm.rope.scaling.yarn_beta_slow": 1.0},
+                {"lm.rope.scaling.yarn_ext_factor": 1.0, "lm.rope.scaling.yarn_log_multiplier": 0.0}):
+        ok, r = _from_gguf(tmp_path, {**yarn, **kvs})
+        assert ok and bytes(r) == bytes(scaled), kvs
+    ok, r = _from_gguf(tmp_path, {**base, "lm.rope.freq_base": 500000})  # a whole number is a number
+    assert ok and r.base == 500000.0
+
+
 # ------------------------------------------------------------------ refusals
 
 P = 1 << 20          # an aligned address that is never dereferenced: every call here is refused before any launch
