@@ -205,7 +205,7 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
     float *const xsum = xmax + TC_THREADS;
     const int tid = threadIdx.x, warp = tid >> 5, r = tid & 127, h = tid >> 7;
     const uint32_t bar_s = su32(bars), bar_o = su32(bars + 1);
-    lm_begin(p.brief);
+    pdl_wait();
     int b, block_of, head, rank;
     if (!place_block(p, (int *)tmem_slot + 2, b, block_of, head, rank)) return;
     kv8_seq_t seq;
@@ -225,6 +225,10 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(su32(tmem_slot)), "r"(TC_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        // Only now, with its TMEM columns taken, does this CTA let the next kernel start (one thread's signal is the CTA's):
+        // a kernel that allocates before it waits for this grid, as the GEMMs do, would otherwise hold columns that this
+        // grid waits for. A CTA that returned above needs none.
+        lm_signal(p.brief);
     }
 
     // This thread's row (the last one again where there are fewer) and its keys lo .. hi.

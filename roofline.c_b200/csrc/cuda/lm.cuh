@@ -54,11 +54,15 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(flo
 // in turn for this grid's completion before it reads anything). After a larger
 // grid it comes as the CTAs retire, which keeps its own evenly spread.
 constexpr unsigned LM_SMALL_GRID = 148;
+__device__ __forceinline__ void lm_signal(bool brief = true)
+{
+    if (brief && gridDim.x * gridDim.y * gridDim.z <= LM_SMALL_GRID)
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
 __device__ __forceinline__ void lm_begin(bool brief = true)
 {
     pdl_wait();
-    if (brief && gridDim.x * gridDim.y * gridDim.z <= LM_SMALL_GRID)
-        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    lm_signal(brief);
 }
 
 // V consecutive elements as one access of V * sizeof(T) bytes (at most 16).

@@ -254,3 +254,36 @@ def test_attention_over_an_infinite_key(lib, new, group, t):
         for h in range(group):
             if pos >= 170 and q[i, h, 7] > 0:                            # the older keys of its page moved to codes of 0
                 assert (got[i, h] - v[0, 170]).abs().max() <= 1e-6
+
+
+# ------------------------------------------------------------------ beside other kernels
+
+def test_attention_between_gemms(lib):
+    """Chunks of few blocks, whose kernel lets the next one start early, between GEMMs that take TMEM before they wait for
+    it: the chain finishes and gives what the calls give one by one."""
+    rows, heads, d = 150, 4, 128
+    pool = Pool(gen(170), 1, d, [600])
+    s = pool.step([rows])
+    w = randn(gen(171), heads * d, heads * d) * 0.05
+    x = randn(gen(172), rows, heads * d)
+    out, y = torch.empty_like(x), torch.empty_like(x)
+
+    def step(src, sync):
+        tcg.check(lib.tcg_kv8_attention(out.data_ptr(), src.data_ptr(), C.byref(pool.cache()), C.byref(s), heads, heads * d,
+                                        heads * d, 0.09, True, 0, tcg.F32))
+        if sync:
+            tcg.check(lib.tcg_sync())
+        tcg.check(lib.tcg_linear(y.data_ptr(), out.data_ptr(), w.data_ptr(), None, rows, heads * d, heads * d))
+        if sync:
+            tcg.check(lib.tcg_sync())
+
+    torch.cuda.synchronize()
+    got = []
+    for sync in (True, False):
+        y.copy_(x)
+        torch.cuda.synchronize()
+        for i in range(40):
+            step(y, sync)
+        tcg.check(lib.tcg_sync())
+        got.append(y.clone())
+    assert torch.equal(*got) and got[0].isfinite().all() and got[0].abs().sum() > 0
