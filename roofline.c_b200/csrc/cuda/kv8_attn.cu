@@ -58,6 +58,7 @@
 
 #include <math.h>
 
+#include <atomic>
 #include <type_traits>
 
 namespace tcg {
@@ -714,13 +715,14 @@ typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, voi
 
 EncodeFn attn_encode_fn()
 {
-    static EncodeFn fn = nullptr;
+    static std::atomic<EncodeFn> known{nullptr};             // threads that come first together find the same
+    EncodeFn fn = known.load(std::memory_order_acquire);
     if (!fn) {
         void *p = nullptr;
         cudaDriverEntryPointQueryResult q;
         if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
             q == cudaDriverEntryPointSuccess)
-            fn = (EncodeFn)p;
+            known.store(fn = (EncodeFn)p, std::memory_order_release);
         else
             cudaGetLastError();
     }

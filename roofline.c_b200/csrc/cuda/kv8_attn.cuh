@@ -6,6 +6,8 @@
 
 #include <math.h>
 
+#include <atomic>
+
 namespace tcg {
 
 constexpr int PAGE = TCG_KV8_PAGE;
@@ -181,10 +183,11 @@ bool attn_grid(AttnArgs &p, dim3 block, size_t smem, int rows, int per_sm, long 
     lc.stream = ctx().cur;
     lc.attrs = attrs;
     // SMs that clusters of a size can use at once (a property of the device: its SMs come in groups that a cluster does not
-    // cross); the first call prepares the kernel, too.
-    static int usable[64][MAX_SPLIT + 1];
-    int *const sms = usable[ctx().device & 63];
-    if (!sms[1]) {
+    // cross); the first call prepares the kernel, too. Threads that come first together write the same; sms[1] says that
+    // the others are there.
+    static std::atomic<int> usable[64][MAX_SPLIT + 1];
+    std::atomic<int> *const sms = usable[ctx().device & 63];
+    if (!sms[1].load(std::memory_order_acquire)) {
         TCG_CUDA(cudaFuncSetAttribute(FN, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         TCG_CUDA(cudaFuncSetAttribute(FN, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         attrs[0].id = cudaLaunchAttributeClusterDimension;
@@ -199,9 +202,9 @@ bool attn_grid(AttnArgs &p, dim3 block, size_t smem, int rows, int per_sm, long 
                 cudaGetLastError();
                 n = 0;
             }
-            sms[S] = n * S < ctx().sms ? n * S : ctx().sms;
+            sms[S].store(n * S < ctx().sms ? n * S : ctx().sms, std::memory_order_relaxed);
         }
-        sms[1] = ctx().sms;
+        sms[1].store(ctx().sms, std::memory_order_release);
     }
     // The split: the S with the least work for the busiest SM, in tiles: its CTAs' rounds of tiles and about two more each
     // (start, merge). A second CTA on the SM fills the first one's waits: two take 1.5 times as long as one, measured.
@@ -213,8 +216,9 @@ bool attn_grid(AttnArgs &p, dim3 block, size_t smem, int rows, int per_sm, long 
     p.S = 1;
     long long best = 0, last = 0;
     for (int S = 1; S <= MAX_SPLIT; S++) {
-        if (!sms[S] || (S > 1 && tiles < (long long)S * groups) || (p.compact && S > 2)) continue;   // compact: most are empty
-        const long long n = (busy * S + sms[S] - 1) / sms[S];
+        const int at_once = sms[S].load(std::memory_order_relaxed);
+        if (!at_once || (S > 1 && tiles < (long long)S * groups) || (p.compact && S > 2)) continue;   // compact: most are empty
+        const long long n = (busy * S + at_once - 1) / at_once;
         const long long rounds = ((tiles + S - 1) / S + groups - 1) / groups, t = n * (rounds + 2) * (n > 1 && per_sm > 1 ? 3 : 4);
         if (S == 1 || t < best) best = t, p.S = S, last = rounds;
     }

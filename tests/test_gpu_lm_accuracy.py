@@ -287,3 +287,57 @@ def test_attention_between_gemms(lib):
         tcg.check(lib.tcg_sync())
         got.append(y.clone())
     assert torch.equal(*got) and got[0].isfinite().all() and got[0].abs().sum() > 0
+
+
+THREADS_FIRST = """
+import sys, threading, torch
+sys.path[:0] = sys.argv[1:3]
+import tcg, test_gpu_lm as T
+L, g, N = tcg.lib(), T.gen(180), 8
+tcg.init(0)
+pool = T.Pool(g, 2, 64, [700, 90])
+news = ([1, 1], [3, 20], [40, 33])
+steps = [pool.step(new) for new in news]
+keep = []
+for new, s in zip(news, steps):                    # each step's lengths in memory of its own
+    keep.append((torch.tensor([0, new[0], sum(new)], dtype=torch.int32).cuda(), torch.tensor(pool.kv, dtype=torch.int32).cuda()))
+    s.tok_start, s.kv_len = (x.data_ptr() for x in keep[-1])
+qs = [T.randn(g, sum(new), 8, 64) for new in news]
+outs = [[torch.zeros_like(q) for q in qs] for _ in range(N)]
+cache, wall, bad = pool.cache(), threading.Barrier(N), []
+torch.cuda.synchronize()
+
+def work(i):
+    try:
+        tcg.init(0)
+        for q, s, o in zip(qs, steps, outs[i]):
+            wall.wait(60)
+            tcg.check(L.tcg_kv8_attention(o.data_ptr(), q.data_ptr(), T.C.byref(cache), T.C.byref(s), 8, 512, 512, 0.125, True,
+                                          0, 0))
+        tcg.check(L.tcg_sync())
+    except Exception as e:
+        bad.append(e)
+        wall.abort()
+
+threads = [threading.Thread(target=work, args=(i,)) for i in range(N)]
+[t.start() for t in threads]
+[t.join() for t in threads]
+torch.cuda.synchronize()
+assert not bad, bad
+for q, s, new, *got in zip(qs, steps, news, *outs):
+    want, tol = T.attention(pool, q, new, pool.kv, 4, 0.125, True, 0, "f32")
+    for o in got:
+        assert torch.equal(o, got[0]) and ((o.double().cpu() - want).abs() <= tol).all()
+print("together")
+"""
+
+
+def test_first_calls_of_several_threads_at_once():
+    """What a kernel's first call on a device finds out is found by threads that come together, and none of them runs without."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    pkg = os.path.join(os.path.dirname(here), "roofline.c_b200")
+    out = subprocess.run([sys.executable, "-c", THREADS_FIRST, here, pkg], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "together" in out.stdout, out.stderr[-2000:]
