@@ -191,8 +191,9 @@ bool tcg_scale(float *out, const float *x, float s, size_t n);
  * head norms, an 8-bit key/value cache and the attention that reads it.
  * Rows are tokens; a row's heads lie side by side (head h at h * head_dim)
  * and successive rows are ld elements apart, so the parts of a fused QKV row
- * are passed as pointers into it. Types: GGML_TYPE_F32, F16 and BF16, the
- * arithmetic is fp32 and each result is rounded once. No call allocates or
+ * are passed as pointers into it. Types: GGML_TYPE_F32, F16 and BF16; norms,
+ * rotations, softmax statistics and sums are fp32 and each result is rounded
+ * once (attention's products take fewer bits, see there). No call allocates or
  * keeps anything between calls: all of them can be captured into CUDA graphs
  * and run on several streams at once, as long as they do not write the same
  * rows or pages.
@@ -308,8 +309,18 @@ bool tcg_kv8_read(void *k, void *v, const tcg_kv8_t *c, const tcg_kv8_step_t *s,
  * already holds the step's own tokens: out = sum_j softmax_j(scale q.k_j) v_j.
  * causal: a query sees the positions up to its own, and with window > 0 only
  * the last `window` of them; not causal: all kv_len positions (window 0). A
- * query that sees nothing gets zeros. Rows from tok_start[n_seq] on are left
- * as they were. scale > 0. out must not overlap q. */
+ * query that sees nothing gets zeros; one with a NaN or an infinity gets NaN.
+ * Rows from tok_start[n_seq] on are left as they were. scale > 0. out must not
+ * overlap q.
+ * What the products hold, by the largest max_new x n_head / n_kv_head:
+ *   up to 64 rows: a query's values to 2^-16 of the head's largest (2^-24 with
+ *     F32), so a score to that times scale sum |k|; a weight to 2^-24 of the
+ *     largest among its 64 keys (2^-17 with F16 and BF16, where those keys'
+ *     weight is spread);
+ *   more: queries in full (to 2^-23 with F32), weights to 2^-12 of themselves
+ *     (2^-23 with F32), the smallest to 2^-25 of the largest of their group of
+ *     keys at worst.
+ * V and its sums may be anything that fp32 holds up to 1e32. */
 bool tcg_kv8_attention(void *out, const void *q, const tcg_kv8_t *c, const tcg_kv8_step_t *s, int n_head,
                        int64_t ld_out, int64_t ld_q, float scale, bool causal, int window, ggml_type_t t);
 

@@ -341,3 +341,37 @@ def test_first_calls_of_several_threads_at_once():
     pkg = os.path.join(os.path.dirname(here), "roofline.c_b200")
     out = subprocess.run([sys.executable, "-c", THREADS_FIRST, here, pkg], capture_output=True, text=True, timeout=300)
     assert out.returncode == 0 and "together" in out.stdout, out.stderr[-2000:]
+
+
+# ------------------------------------------------------------------ in place
+
+@pytest.mark.parametrize("d,n_rot,half,heads,kv,n,t", [(128, 128, True, 32, 8, 3, "f32"), (64, 32, False, 5, 1, 129, "bf16"),
+                                                      (80, 80, True, 7, 2, 17, "f16"), (256, 256, False, 3, 3, 40, "f32"),
+                                                      (6, 4, True, 2, 1, 5, "bf16"), (128, 64, True, 40, 8, 6001, "bf16")])
+def test_norm_and_rotation_in_place(lib, d, n_rot, half, heads, kv, n, t):
+    """Over a fused row's queries and keys, where they lie: the bits of the call out of place, and the values beside them kept."""
+    dt, code = TYPES[t]
+    g = gen(190)
+    r = tcg.Rope()
+    tcg.check(lib.tcg_rope_init(C.byref(r), d, n_rot, int(half), 10000.0))
+    for ld in ((heads + 2 * kv) * d, (heads + 2 * kv) * d + 3):
+        rows = randn(g, n, ld, dtype=dt)
+        wq, wk = randn(g, d) + 1, randn(g, d) + 1
+        pos = torch.randint(0, 1 << 17, (n,), generator=g, dtype=torch.int32).cuda()
+        at, size = heads * d, rows.element_size()
+        apart = [torch.empty((n, h * d), dtype=dt, device="cuda") for h in (heads, kv)]
+        x = rows.data_ptr()
+        call(lib.tcg_qk_norm_rope, apart[0].data_ptr(), apart[1].data_ptr(), x, x + at * size, wq.data_ptr(), wk.data_ptr(), 1e-6,
+             pos.data_ptr(), C.byref(r), n, heads, kv, heads * d, kv * d, ld, ld, code)
+        place = rows.clone()
+        x = place.data_ptr()
+        call(lib.tcg_qk_norm_rope, x, x + at * size, x, x + at * size, wq.data_ptr(), wk.data_ptr(), 1e-6, pos.data_ptr(),
+             C.byref(r), n, heads, kv, ld, ld, ld, ld, code)
+        if ld % 4 == 0:                                                  # else by single values, in another order of sums
+            assert torch.equal(place[:, :at], apart[0]) and torch.equal(place[:, at:at + kv * d], apart[1])
+        else:
+            # two sums of d squares in fp32 and the steps after them, twice: 2 x 25 u of each value, and a step of the type
+            for a, b in ((place[:, :at], apart[0]), (place[:, at:at + kv * d], apart[1])):
+                pair = b.double().abs().view(n, -1, d).amax(-1, keepdim=True).expand(-1, -1, d).reshape(n, -1)
+                assert ((a.double() - b.double()).abs() <= 50 * U * pair + 2 * half_step(dt) * b.double().abs() + 2.0 ** -23 * (t == "f16")).all()
+        assert torch.equal(place[:, at + kv * d:], rows[:, at + kv * d:])
