@@ -18,9 +18,10 @@
 // NP = 2 digits leave 2^-16 of a row's largest |q|, NP = 3 2^-24. A weight is
 // off by 2^-24 of its tile's largest, and up to 64 of them add up. Two digits
 // of P (2^-17) do for 16-bit results only where a tile's weight is spread:
-// they are taken where every thread's 16 keys hold 1/16 of the largest weight
-// in every row (the other keys then hold 3/16 at least, their 63 roundings
-// 2^-13 of that as a rule), three elsewhere. Three always: 131071 tokens 52.9
+// a row takes them where each of its threads' 16 keys hold 1/16 of its largest
+// weight (the other keys then hold 3/16 at least, their 63 roundings 2^-13 of
+// that as a rule), three elsewhere, and a warp the third product where one of
+// its rows does. Three always: 131071 tokens 52.9
 // us against 49.3 with scores of spread 2.7, 64 x 16 rows 136 against 133.
 //
 // Why no shuffles: the mma's k order is free as long as A and B agree. A
@@ -488,7 +489,8 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
                         if (key > hi[e >> 1] || key < lo[e >> 1]) f[j][e] = -INFINITY;
                     }
             }
-            bool grew = false, even = true;
+            bool grew = false;
+            uint32_t spread[RW];                             // lanes whose 16 keys hold 1/16 of their row's largest weight
             float up[RW];                                    // of O, where the row's maximum grew
 #pragma unroll
             for (int r = 0; r < RW; r++) {
@@ -524,9 +526,9 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
                     }
                 l[r] = fmaf(l[r], up[r], sum * beta);
                 fold[r] = tv * beta;
-                even = even && !(sum < 1.0f / 16.0f);
+                spread[r] = NP == 3 ? 0 : __ballot_sync(0xFFFFFFFFu, !(sum < 1.0f / 16.0f));
             }
-            fine = NP == 3 || !__all_sync(0xFFFFFFFFu, even);
+            fine = (spread[0] & spread[RW - 1]) != 0xFFFFFFFFu;
             if (__any_sync(0xFFFFFFFFu, grew)) {
 #pragma unroll
                 for (int r = 0; r < RW; r++)
@@ -541,14 +543,17 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
                 constexpr bool THREE = decltype(three)::value;
 #pragma unroll
                 for (int r = 0; r < RW; r++) {
-                    fold[r] *= O_UNIT / (THREE ? P3 : P2);
+                    // each row its own digits, whatever its neighbours need: two of them are three with a zero
+                    const bool mine = THREE && (NP == 3 || (spread[r] >> (lane & 28) & 15u) != 15u);
+                    const float one = mine ? P3 : P2 / 65536.0f, base_of = mine ? 8388608.0f : 128.0f;
+                    fold[r] *= mine ? O_UNIT / P3 : O_UNIT / P2;
 #pragma unroll
                     for (int w = 0; w < 4; w++) {
                         uint32_t y[4];
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             const float v = f[2 * w + (e >> 1)][2 * r + (e & 1)];
-                            y[e] = __float_as_uint(THREE ? fmaf(v, P3, 8388608.0f) : fmaf(v, P2 / 65536.0f, 128.0f));
+                            y[e] = __float_as_uint(fmaf(v, one, base_of));
                         }
                         const uint32_t u = __byte_perm(y[0], y[1], 0x5140), v = __byte_perm(y[2], y[3], 0x5140);
                         const uint32_t d0 = __byte_perm(u, v, 0x5410), d1 = __byte_perm(u, v, 0x7632);

@@ -375,3 +375,44 @@ def test_norm_and_rotation_in_place(lib, d, n_rot, half, heads, kv, n, t):
                 pair = b.double().abs().view(n, -1, d).amax(-1, keepdim=True).expand(-1, -1, d).reshape(n, -1)
                 assert ((a.double() - b.double()).abs() <= 50 * U * pair + 2 * half_step(dt) * b.double().abs() + 2.0 ** -23 * (t == "f16")).all()
         assert torch.equal(place[:, at + kv * d:], rows[:, at + kv * d:])
+
+
+# ------------------------------------------------------------------ the shape for a device full of rows, and NaN beside others
+
+@pytest.mark.parametrize("t", list(TYPES))
+def test_many_key_heads_of_huge_scores_and_small_v(lib, t):
+    """40 rows of each of 150 key heads: warps of 16 rows. As above, one key decides; then V below fp32's normal numbers."""
+    pool = Pool(gen(200), 150, 64, [300])
+    q = randn(gen(201), 40, 150, 64, dtype=TYPES[t][0], spread=100.0)
+    pool.ks *= 1e8 / (100.0 * 73 * 0.025 * 8)
+    got = run(lib, pool, q, [40], 150, 1.0, t).double()
+    k, v = pool.values(0, 300)
+    hide = torch.arange(300, device="cuda")[None] > torch.arange(260, 300, device="cuda")[:, None]
+    s = torch.einsum("nhd,hkd->hnk", q.double(), k).masked_fill(hide, -math.inf)
+    two, at = s.topk(2, -1)
+    slack = (q.double().abs().amax(-1).T / 65024 * k.abs().sum(-1).amax(-1)[:, None]
+             + 8 * U * s.masked_fill(hide, 0).abs().amax(-1))            # as in the test of scores of any size
+    ahead = two[..., 0] - two[..., 1] > 2 * slack + 40
+    want = torch.gather(v, 1, at[..., :1].expand(-1, -1, 64))
+    bad = (got.transpose(0, 1) - want).abs() > want.abs() * (half_step(TYPES[t][0]) + 2.0 ** -11) + 300 * math.exp(-40) * v.abs().max()
+    assert ahead.float().mean() > 0.8 and not bad[ahead].any()
+    if t != "f16":
+        pool = Pool(gen(202), 150, 64, [150])
+        pool.vs *= 1e-37
+        q = randn(gen(203), 40, 150, 64, dtype=TYPES[t][0])
+        want, tol = exact(pool, q, [40], [150], 1, 0.125, t)
+        near(run(lib, pool, q, [40], 150, 0.125, t), want, tol + 2.0 ** -123)
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("new,group", [(2, 4), (4, 4), (8, 4), (16, 4), (40, 4)])
+def test_a_nan_query_leaves_the_rows_beside_it_alone(lib, new, group, t):
+    pool = Pool(gen(210), 1, 64, [300])
+    q = randn(gen(211), new, group, 64, dtype=TYPES[t][0])
+    clean = run(lib, pool, q, [new], group, 0.125, t)
+    odd = q.clone()
+    odd[0, 1, 5], odd[new - 1, 2, 63] = math.nan, -math.inf
+    got = run(lib, pool, odd, [new], group, 0.125, t)
+    hit = torch.zeros((new, group), dtype=torch.bool, device="cuda")
+    hit[0, 1] = hit[new - 1, 2] = True
+    assert got[hit].isnan().all() and torch.equal(got[~hit], clean[~hit]) and not clean.isnan().any()
