@@ -11,9 +11,10 @@
 // write the same bytes; its new rows are read once, into registers. Bound by
 // memory for prompts in principle (4 or 2 bytes in, 1 out per element); as it
 // is, by instructions, about 22 a value: five f16 prompts up to 2048 tokens
-// (8 heads of 128) 17 us, and 14 us to read them back as fp32. A decode step
+// (8 heads of 128) 14 us, and 11 us to read them back as fp32. A decode step
 // is bound by the latency of dependent loads (lengths, page, scale): 33 tokens
-// 5.5 us, their pages read back 8.8 us, 8.5 us for both in a row.
+// 3.8 us, their pages read back 6.1 us, 8.7 us for both in a row (back to back;
+// an empty kernel launched the same way 2.6 us).
 #include "lm.cuh"
 
 namespace tcg {

@@ -50,9 +50,10 @@
 // was the limit.
 //
 // Bound by memory on large decode batches: 64 sequences up to 8192 tokens (32
-// query heads, 8 key heads, D = 128) 104 us, 6.2 TB/s. One token over 131071:
-// 47 us, 5.7 TB/s: clusters of 10 use 80 of 148 SMs. One token over a few
-// hundred: 5.7 us (bf16) to 6.8 us (fp32), dependent loads (lengths, page,
+// query heads, 8 key heads, D = 128) 105 us, 6.1 TB/s. One token over 131071:
+// 48 us, 5.5 TB/s: clusters of 10 use 80 of 148 SMs. One token over a few
+// hundred: 6.3 us (bf16) to 6.8 us (fp32), an empty kernel launched the same
+// way 2.6 us; dependent loads (lengths, page,
 // scale and tile) and the launch.
 #include "kv8_attn.cuh"
 #include "tc05.cuh"
@@ -808,9 +809,9 @@ extern "C" bool tcg_kv8_attention(void *out, const void *q, const tcg_kv8_t *c, 
     if (r != CUDA_SUCCESS) return fail("cuTensorMapEncodeTiled failed (%d) for the K cache", (int)r);
 
     // Warps of 8 rows (RW = 1) while the rows are few: 8, 16 or 32 rows leave 12, 6 or 3 groups of warps for other tiles.
-    // Up to 64 rows: 8 such warps where the device is not filled (17 sequences of 50 rows over a window of 1024: 13.0 us,
-    // against 15.1 with 4 warps of 16 rows), else 4 warps of 16 rows, two CTAs an SM (64 sequences of 64 rows over 2048
-    // tokens, bf16: 124 us against 153).
+    // Up to 64 rows: 8 such warps where the device is not filled (17 sequences of 50 rows over a window of 1024: 12.3 us,
+    // against 15.0 with 4 warps of 16 rows), else 4 warps of 16 rows, two CTAs an SM (64 sequences of up to 64 rows over 2048
+    // tokens, bf16: 131 us against 157).
     const bool big = p.D > 64;
     auto go = [&](auto digits) {
         constexpr int NP = decltype(digits)::value;

@@ -44,13 +44,14 @@
 // products run while the other's threads compute. Every wait is bounded as in
 // attn_tc.cu.
 //
-// Measured, 32 query and 8 key heads: a 4096-token causal prompt 382 us fp32
-// and 265 us bf16 with D = 128 (360 and 518 TFLOP/s), 4096 x 4096 without a
-// mask 690 and 465 us (398 and 591 TFLOP/s), 512 tokens over 16384 with the
-// keys split over clusters of 2 361 and 245 us. The tensor pipe is busy 34% of
+// Measured, 32 query and 8 key heads: a 4096-token causal prompt 406 us fp32
+// and 276 us bf16 with D = 128 (339 and 499 TFLOP/s), 4096 x 4096 without a
+// mask 731 and 510 us (376 and 539 TFLOP/s), 512 tokens over 16384 with the
+// keys split over clusters of 2 379 and 254 us. The tensor pipe is busy 33% of
 // the time (fp32): the threads' own chain per tile is the limit. Four threads
 // a row (64 registers) spill: 616 us. O in registers, folded every tile: 883
-// us; 64-key tiles with a second S buffer: 497 us.
+// us; 64-key tiles with a second S buffer: 497 us. (The last three when the
+// kernel took 438 us.)
 #include "kv8_attn.cuh"
 #include "numerics.cuh"
 #include "tc05.cuh"

@@ -11,7 +11,7 @@
 // sum of squares in fp32 over the lanes of a head.
 //
 // Bound by memory: 2 * 4 bytes an element (fp32) for ~10 operations (4096 rows
-// of 40 heads of 128 with norms, fp32: 30.1 us, 5.6 TB/s; 6001 rows of 36
+// of 40 heads of 128 with norms, fp32: 30.3 us, 5.5 TB/s; 6001 rows of 36
 // heads, half of each rotated, bf16: 23.3 us, 4.7 TB/s). A lane
 // owns one "unit" of 2 V dims of a head, two vectors of V: V pairs of the
 // rotated part, or 2 V dims of the rest. The warp computes its token's sines
