@@ -317,8 +317,8 @@ bool tcg_kv8_read(void *k, void *v, const tcg_kv8_t *c, const tcg_kv8_step_t *s,
  *     F32), so a score to that times scale sum |k|; a weight to 2^-24 of the
  *     largest among its 64 keys (2^-17 with F16 and BF16, where those keys'
  *     weight is spread);
- *   more: queries in full (to 2^-23 with F32), weights to 2^-12 of themselves
- *     (2^-23 with F32), the smallest to 2^-25 of the largest of their group of
+ *   more: queries in full (to 2^-22 with F32), weights to 2^-11 of themselves
+ *     (2^-22 with F32), the smallest to 2^-25 of the largest of their group of
  *     keys at worst.
  * V and its sums may be anything that fp32 holds up to 1e32. */
 bool tcg_kv8_attention(void *out, const void *q, const tcg_kv8_t *c, const tcg_kv8_step_t *s, int n_head,

@@ -20,7 +20,7 @@
 // m (2^4, so that groups last: at the maximum itself, prompts of peaked scores
 // take 5% longer). A group ends where
 // a row's maximum outgrows its reference by 2^7, where sv and sv0 are 2^3
-// apart, or after 4 tiles with fp32 inputs (32 otherwise): the tensor core's
+// apart (a V of zeros is far from any), or after 4 tiles with fp32 inputs (32 otherwise): the tensor core's
 // accumulation truncates, by about 2e-8 of the result per MMA, 64 (256) of them
 // a group. A tile whose two pages' scales are 2^3 apart is taken twice, once
 // for each page. So a weight is rounded (to 11 or 22 bits, or 2^-33 of 2^m_g)
@@ -29,9 +29,11 @@
 // takes its bits.
 // O is used at a group's end only and lives in local memory.
 // Q is scaled by a power of two per row into [2^14, 2^15). With fp16 or bf16
-// inputs it is exact as one fp16, and P's rounding to fp16 (2^-12 of itself)
-// is below the output's; with fp32 inputs Q and P are two fp16 pieces of 11
-// bits each (NP = 2), the small piece's products first.
+// inputs it is exact as one fp16, and P's rounding to fp16 (2^-11 of itself) is
+// that of an fp16 output and below bf16's (over 2000 keys an fp16 result is off
+// by 2.4e-4 to 2.9e-4, 2.1e-4 by its own rounding alone); with fp32 inputs Q
+// and P are two fp16 pieces of 11 bits each (NP = 2), the small piece's
+// products first.
 //
 // Why fp16 and not the 8-bit integers of the cache, as the kernel for few rows
 // does: with one thread a row the integer path is bound by the threads' work
@@ -408,7 +410,7 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
         const float va = pa < 0 ? 0.0f : p.v_scale[at_a], vb = pb < 0 ? 0.0f : p.v_scale[at_b], sv = h ? vb : va;
         load_pages(raw4, p.v, pa, pb, false);
         const float v_min = fminf(va, vb), v_max = fmaxf(va, vb);
-        const bool apart = v_min > 0.0f && v_max > 8.0f * v_min, again = apart && !second;   // the same for the whole CTA
+        const bool apart = pa >= 0 && pb >= 0 && v_max > 8.0f * v_min, again = apart && !second;   // the same for the whole CTA
         const bool on = mine >= 0 && (!apart || second == (h != 0));
         const float c = tame(cs0 * (on ? sk : 1.0f));
         float lr = sv == sv0 || !on ? 0.0f : log_ratio(sv);
@@ -451,7 +453,7 @@ kv8_attn_tc_kernel(const __grid_constant__ AttnArgs p, const int8_t *__restrict_
             const float a = xmax[r], z = xmax[r + 128];
             fold(fmaxf(a, z), a > z ? xsum[r] : a < z ? xsum[r + 128] : fmaxf(xsum[r], xsum[r + 128]), it > 0);
             sv0 = !apart ? v_max : second ? vb : va;
-            lr = sv == sv0 || !on ? 0.0f : fmaxf(log_ratio(sv), -60.0f);     // beyond NEAR_V only where sv is 0
+            lr = sv == sv0 || !on ? 0.0f : log_ratio(sv);
             left = NP == 2 ? 4 : 32;
         }
         left--;

@@ -55,12 +55,12 @@ def exact(pool, q, new, kv, group, scale, t, causal=True, window=0):
                 coarse = (wt.sum(-1) >= 0.06 * top_w[..., None]).all(-1) & torch.tensor(not f32, device="cuda")
                 lost = PAGE * (torch.where(coarse, 2.0 ** -17, 2.0 ** -24) * top_w) @ vt / l
             else:
-                # Weights are fp16 under 2^8 (two of them with fp32): half a step of 11 (22) bits, and of fp16's
+                # Weights are fp16 under 2^8 (two of them with fp32): half a step, 2^-11 (2^-22), and that of fp16's
                 # subnormals, 2^-25 / 2^8 of a reference at most 2^8 over the group's largest weight, of pages whose V scales
                 # are within 2^3: six standard deviations (0.58 each) of as many roundings as a group has keys, against the
                 # row's own sum of weights times |V| (the largest key's |V| a quarter of the page's or more), or, where
                 # that key's V is 0, all of them against the key.
-                rel += (2.0 ** -23 if f32 else 2.0 ** -12) + (64 if f32 else 256) * 2e-8
+                rel += (2.0 ** -22 if f32 else 2.0 ** -11) + (64 if f32 else 256) * 2e-8
                 group_keys = min(m, 512 if f32 else 4096)
                 lost = torch.minimum(torch.minimum(w, torch.full_like(w, 2.0 ** -33)) @ vv.abs() / l,
                                      4 * 6 * 0.58 * math.sqrt(group_keys) * 2.0 ** -22 * mass)
@@ -134,7 +134,7 @@ def test_a_row_does_not_depend_on_the_launch(lib, new, group):
 # ------------------------------------------------------------------ pages of unlike V scales
 
 @pytest.mark.parametrize("t", ["f32", "bf16"])
-@pytest.mark.parametrize("low", [2.0 ** -7, 1e-6, 1e-12, 1e-30])
+@pytest.mark.parametrize("low", [2.0 ** -7, 1e-6, 1e-12, 1e-30, 0.0])
 @pytest.mark.parametrize("new,group", [(1, 4), (16, 4), (250, 4)])
 @pytest.mark.parametrize("gap", [0.0, 20.0])
 def test_attention_of_rows_whose_weight_lies_in_pages_of_small_v(lib, new, group, gap, low, t):
