@@ -18,11 +18,11 @@
 // as log2(sv / sv0) in the exponent. m_g is the row's running maximum m, or 2^4
 // over the maximum of the group's first tile where that is more than 2^8 below
 // m (2^4, so that groups last: at the maximum itself, prompts of peaked scores
-// take 5% longer). A group ends where
-// a row's maximum outgrows its reference by 2^7, where sv and sv0 are 2^3
-// apart (a V of zeros is far from any), or after 4 tiles with fp32 inputs (32 otherwise): the tensor core's
-// accumulation truncates, by about 2e-8 of the result per MMA, 64 (256) of them
-// a group. A tile whose two pages' scales are 2^3 apart is taken twice, once
+// take 5% longer). A group ends where a row's maximum outgrows its reference by
+// 2^7, where sv and sv0 are 2^3 apart (a V of zeros is far from any), or after
+// 4 tiles with fp32 inputs (32 otherwise): the tensor core's accumulation
+// truncates, by about 2e-8 of the result per MMA, 64 (256) of them a group. A
+// tile whose two pages' scales are 2^3 apart is taken twice, once
 // for each page. So a weight is rounded (to 11 or 22 bits, or 2^-33 of 2^m_g)
 // against weights of its own group, times V of about its own size: neither a
 // key elsewhere that holds most of the weight nor a page of large V beside it
