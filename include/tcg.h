@@ -204,6 +204,7 @@ bool tcg_scale(float *out, const float *x, float s, size_t n);
 #define TCG_ERR_KV8_LENGTHS 64  /* a sequence's rows or lengths: the whole sequence is skipped */
 #define TCG_ERR_KV8_PAGE    65  /* a page number: its tokens are not written, read as 0, and masked in attention */
 #define TCG_ERR_KV8_WAIT    66  /* a bounded wait inside attention gave up: the call's output is not valid */
+#define TCG_ERR_MX_WAIT     67  /* a bounded wait inside tcg_mx_linear gave up: the call's output is not valid */
 
 /* ---- rotary positions. A plain host struct, filled by tcg_rope_init and
  * the tcg_rope_scale_* calls (all host only, no GPU), passed by pointer and
@@ -323,6 +324,51 @@ bool tcg_kv8_read(void *k, void *v, const tcg_kv8_t *c, const tcg_kv8_step_t *s,
  * V and its sums may be anything that fp32 holds up to 1e32. */
 bool tcg_kv8_attention(void *out, const void *q, const tcg_kv8_t *c, const tcg_kv8_step_t *s, int n_head,
                        int64_t ld_out, int64_t ld_q, float scale, bool causal, int window, ggml_type_t t);
+
+/* ---- microscaled matrices (MX, the Open Compute Project's format): codes in
+ * 4 (E2M1) or 8 bits (E4M3), one power of two for 32 columns of a row.
+ *   codes  [rows, P] codes, P = cols rounded up to 128; in 4 bits two in a
+ *      byte, the even column in the low half. Columns behind cols are 0
+ *   scales one byte s for 32 columns: value = code * 2^(s - 127), and NaN with
+ *      s = 255. The bytes of 128 rows and 128 columns stand together, as the
+ *      tensor core reads them: row r, block b = column / 32 at
+ *      (r / 128 * P / 128 + b / 4) * 512 + r % 32 * 16 + r / 32 % 4 * 4 + b % 4
+ * A block's scale is 2^(floor(log2(largest magnitude)) - m), m = 2 (E2M1) or 8
+ * (E4M3), at least 2^-127; codes are the values nearest to x / scale, ties to
+ * the even code, at most the format's largest (6 or 448). A block that holds a
+ * NaN or an infinity is NaN, one of zeros is zero. The caller owns the memory
+ * (DEVICE, codes on a 32-byte and scales on a 16-byte boundary); rows and
+ * blocks that are written need no initialisation. */
+#define TCG_MX_MAX_ROWS (1 << 30)
+#define TCG_MX_MAX_COLS (1 << 24)
+#define TCG_NORM_MAX_COLS 32768
+typedef struct {
+    uint8_t *codes, *scales;
+    int rows, cols, bits;
+} tcg_mx_t;
+/* Bytes of a matrix's codes and of its scales (host only; 0 for sizes that cannot be). */
+size_t tcg_mx_code_bytes(int rows, int cols, int bits);
+size_t tcg_mx_scale_bytes(int rows, int cols);
+
+/* m = x quantised: x [m->rows, m->cols], rows ld elements apart. */
+bool tcg_mx_quantize(const tcg_mx_t *m, const void *x, int64_t ld, ggml_type_t t);
+/* y = m's values, rounded to t (bf16 and fp32 hold every one exactly, down to
+ * bf16's smallest). Elements between the rows are left as they were. */
+bool tcg_mx_dequantize(void *y, const tcg_mx_t *m, int64_t ld, ggml_type_t t);
+/* y = x w^T + bias: x [rows, cols] in 8 or 4 bits, w [outs, cols] in 4 bits,
+ * bias fp32 [outs] or NULL, y [rows, outs]. Products are exact and summed in
+ * fp32 (F32 results: in groups of columns that keep the sum's error at
+ * fp32's), the sum is rounded once to t. y must not overlap x or w. */
+bool tcg_mx_linear(void *y, const tcg_mx_t *x, const tcg_mx_t *w, const float *bias, int64_t ld_y, ggml_type_t t);
+/* The residual's addition and the root-mean-square norm of the sum, in one
+ * pass over n_tok rows of cols columns (at most TCG_NORM_MAX_COLS):
+ *   h = x + r, rounded to t (r NULL: h = x),
+ *   v = h / sqrt(mean(h^2) + eps) * w (w fp32 [cols]),
+ * out as y (rounded to t) and/or as mx (quantised, from v itself). Each of h,
+ * y and mx may be NULL, not all of them. h and y may be x or r in place (the
+ * same pointer and stride), not each other; otherwise nothing overlaps. */
+bool tcg_add_rms_norm(void *h, void *y, const tcg_mx_t *mx, const void *x, const void *r, const float *w, float eps,
+                      int n_tok, int cols, int64_t ld_h, int64_t ld_y, int64_t ld_x, int64_t ld_r, ggml_type_t t);
 
 /* ------------------------------------------------- batched ViT (new)
  * The forward of tc_vit_encode (src/vit.c:305-391) over a batch of images.

@@ -1,0 +1,339 @@
+// mx_linear.cu -- tcg_mx_linear: y = x w^T + bias, x in 8 (E4M3) or 4 bits (E2M1), w in 4 bits, a power of two for each 32
+// columns of a row, on the tensor core's block-scaled products (tcgen05 kind::mxf8f6f4 and kind::mxf4).
+#include "mx.cuh"
+#include "tc05.cuh"
+
+#include <type_traits>
+
+namespace tcg {
+namespace {
+
+constexpr int ERR_WAIT = TCG_ERR_MX_WAIT;
+constexpr int TILE_N = 128;             // weight rows of a tile: the MMA's M, a TMEM lane each
+constexpr int MAX_SPLIT = 8;            // portable cluster size
+
+// What differs between rows in 4 and in 8 bits. A stage is 128 bytes of a row of x; the weights' 4-bit codes next to 8-bit
+// rows are spread by the copy itself to 16 bytes for 16 codes, as kind::mxf8f6f4 reads them.
+template <int BITS>
+struct Fmt {
+    static constexpr int K = BITS == 4 ? 256 : 128;         // columns of a stage
+    static constexpr int ATOMS = K / MX_ATOM;               // scale groups of a stage
+    static constexpr int STEPS = 4;                         // MMAs of a stage: 32 bytes of a row each
+    static constexpr int STEP_K = K / STEPS;
+    static constexpr uint32_t A_TX = BITS == 4 ? TILE_N * 128 : TILE_N * 64;     // bytes of w that the copy counts
+};
+
+// Instruction descriptor: formats (E2M1 is 1 of kind::mxf4, 5 of kind::mxf8f6f4; E4M3 is 0), N / 8 at 17, scales E8M0 at
+// 23, M / 128 at 27; the bytes of the scale words that a step takes go to bits 29 (A) and 4 (B).
+template <int BITS>
+__device__ __forceinline__ uint32_t mx_idesc(int n, int m)
+{
+    const uint32_t a = BITS == 4 ? 1 : 5, b = BITS == 4 ? 1 : 0;
+    return a << 7 | b << 10 | (uint32_t)(n / 8) << 17 | 1u << 23 | (uint32_t)(m / 128) << 27;
+}
+
+template <int BITS>
+__device__ __forceinline__ void mma_mx(uint32_t d, unsigned long long a, unsigned long long b, uint32_t id, uint32_t sa,
+                                       uint32_t sb, uint32_t acc)
+{
+    if (BITS == 4)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+                     "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(sa), "r"(sb), "r"(acc));
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+                     "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(sa), "r"(sb), "r"(acc));
+}
+
+// 512 bytes of scales (32 lanes of 16 bytes) to four TMEM columns, the same in each warp's 32 lanes.
+__device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint32_t smem)
+{
+    const unsigned long long d = (unsigned long long)((smem & 0x3FFFFu) >> 4) | ((unsigned long long)(128 >> 4) << 32) | (1ull << 46);
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+}
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float peer_f32(uint32_t addr, uint32_t rank)
+{
+    uint32_t at;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+
+struct LinArgs {
+    const uint8_t *xs, *ws;             // scales
+    const float *bias;
+    void *y;
+    long long ldy;
+    int *err;
+    int rows, outs, atoms;              // of x, of w, scale groups of a row
+    int stages_k;                       // stages of the whole K
+    int tiles_n, split, per;            // CTAs of a tile, stages of each
+    int accs, acc_stages;               // accumulators of a CTA, stages of each
+    int depth;                          // stages in shared memory
+    int type;
+};
+
+template <typename T>
+__device__ __forceinline__ void put(const LinArgs &p, long long row, int n, float v)
+{
+    ((T *)p.y)[row * p.ldy + n] = from_f32<T>(v);
+}
+__device__ __forceinline__ void store_y(const LinArgs &p, long long row, int n, float v)
+{
+    if (p.type == GGML_TYPE_F32) put<float>(p, row, n, v);
+    else if (p.type == GGML_TYPE_F16) put<__half>(p, row, n, v);
+    else put<__nv_bfloat16>(p, row, n, v);
+}
+
+template <int BITS, int BN>
+struct Stream {
+    static constexpr int A = TILE_N * 128, B = BN * 128, SF = Fmt<BITS>::ATOMS * 512;
+    static constexpr int STAGE = A + B + 2 * SF;            // SF is a multiple of 512; A and B of 1024
+    static constexpr int COLS = BN <= 32 ? 256 : 512;       // TMEM: accumulators, then the scales
+    static constexpr int SF_COL = COLS - 2 * Fmt<BITS>::ATOMS * 4;
+    static constexpr int MAX_ACC = SF_COL / BN;
+};
+
+// One tile of 128 weight rows x BN rows of x a cluster, its K dealt out to the cluster's CTAs.
+template <int BITS, int BN>
+__global__ void __launch_bounds__(128) mx_stream_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap mx,
+                                                        const __grid_constant__ LinArgs p)
+{
+    using F = Fmt<BITS>;
+    using S = Stream<BITS, BN>;
+    extern __shared__ unsigned char raw[];
+    __shared__ __align__(8) unsigned long long bars[2 * 16 + 1];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort;
+    unsigned char *const smem = (unsigned char *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t base = su32(smem), full = su32(bars), empty = full + 8 * 16, done = full + 8 * 32;
+    const int rank = blockIdx.x % p.split, tile = blockIdx.x / p.split;
+    const int n0 = tile % p.tiles_n * TILE_N, m0 = tile / p.tiles_n * BN;
+    const int k_begin = rank * p.per, k_end = min(p.stages_k, k_begin + p.per), count = max(0, k_end - k_begin);
+    if (tid == 0) {
+        for (int i = 0; i < p.depth; i++) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
+        bar_init(done, 1);
+        s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(&s_tmem)), "r"(S::COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = s_tmem;
+    volatile int *abort = &s_abort;
+    bool ok = true;
+    pdl_wait();
+    lm_signal();
+    auto at = [&](int slot) { return base + slot * S::STAGE; };
+    auto atoms_of = [&](int k) { return min(F::ATOMS, p.atoms - k * F::ATOMS); };
+    if (warp == 0 && lane == 0) {
+        int k = 0;
+        for (; k < count && ok; k++) {
+            const int slot = k % p.depth, kk = k_begin + k, na = atoms_of(kk);
+            if (k >= p.depth) ok = bar_wait(empty + 8 * slot, (k / p.depth - 1) & 1, abort, p.err, ERR_WAIT);
+            if (!ok) break;
+            const uint32_t bar = full + 8 * slot, a = at(slot), b = a + S::A, sa = b + S::B, sb = sa + S::SF;
+            bar_expect_tx(bar, F::A_TX + S::B + 2 * 512 * na);
+            tma_load(a, &mw, bar, kk * 128, n0);
+            tma_load(b, &mx, bar, kk * 128, m0);
+            bulk_load(sa, p.ws + ((size_t)(n0 / MX_ATOM) * p.atoms + (size_t)kk * F::ATOMS) * 512, 512 * na, bar);
+            bulk_load(sb, p.xs + ((size_t)(m0 / MX_ATOM) * p.atoms + (size_t)kk * F::ATOMS) * 512, 512 * na, bar);
+        }
+        // copies in flight land before the CTA ends
+        if (!ok)
+            for (int j = max(0, k - p.depth); j < k; j++)
+                bar_wait(full + 8 * (j % p.depth), (j / p.depth) & 1, abort, p.err, ERR_WAIT, false);
+    } else if (warp == 1 && lane == 0) {
+        const uint32_t id = mx_idesc<BITS>(BN, TILE_N), sfa = tmem + S::SF_COL, sfb = sfa + 4 * F::ATOMS;
+        const uint32_t b_off = m0 % MX_ATOM / 32;           // the tile's first column of its group of 128 rows
+        for (int k = 0; k < count; k++) {
+            const int slot = k % p.depth, na = atoms_of(k_begin + k);
+            ok = bar_wait(full + 8 * slot, (k / p.depth) & 1, abort, p.err, ERR_WAIT);
+            if (!ok) break;
+            fence_after();
+            const uint32_t a = at(slot), b = a + S::A, sa = b + S::B, sb = sa + S::SF;
+            for (int i = 0; i < na; i++) {
+                scales_to_tmem(sfa + 4 * i, sa + 512 * i);
+                scales_to_tmem(sfb + 4 * i, sb + 512 * i);
+            }
+            const uint32_t d = tmem + k / p.acc_stages * BN;
+            const unsigned long long da = sdesc<128>(a), db = sdesc<128>(b);
+#pragma unroll
+            for (int j = 0; j < F::STEPS; j++) {
+                const int atom = j * F::STEP_K / MX_ATOM, byte = j * F::STEP_K / MX_BLOCK % 4;
+                if (atom < na)
+                    mma_mx<BITS>(d, da + 2 * j, db + 2 * j, id | byte << 29 | byte << 4, sfa + 4 * atom, sfb + 4 * atom + b_off,
+                                 k % p.acc_stages != 0 || j != 0);
+            }
+            mma_commit(empty + 8 * slot);
+        }
+        mma_commit(done);
+    }
+    __syncwarp();
+    ok = bar_wait(done, 0, abort, p.err, ERR_WAIT, false) && ok && !*abort;
+    fence_after();
+    const int accs = count ? (count - 1) / p.acc_stages + 1 : 0;
+    const uint32_t lane_base = tmem + ((uint32_t)warp << 21);
+    const int n = n0 + tid;
+    float *const part = (float *)smem;                      // [BN][128], over the stages: their MMAs are done
+    const float bias = p.bias && n < p.outs ? p.bias[n] : 0.0f;
+    constexpr int STEP = 8;
+#pragma unroll 1
+    for (int c = 0; c < BN; c += STEP) {
+        if (m0 + c >= p.rows) break;
+        float v[STEP] = {};
+        for (int i = 0; i < accs; i++) {
+            uint32_t r[STEP];
+            tmem_ld8(lane_base + i * BN + c, r);
+#pragma unroll
+            for (int j = 0; j < STEP; j++) v[j] += __uint_as_float(r[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < STEP; j++) {
+            if (p.split > 1) part[(c + j) * TILE_N + tid] = v[j];
+            else if (ok && n < p.outs && m0 + c + j < p.rows) store_y(p, m0 + c + j, n, v[j] + bias);
+        }
+    }
+    if (p.split > 1) {
+        cluster_sync();
+        const int rows = min(BN, p.rows - m0);
+        for (int c = rank; c < rows; c += p.split) {
+            float v[MAX_SPLIT], sum = 0.0f;
+#pragma unroll
+            for (int s = 0; s < MAX_SPLIT; s++) v[s] = s < p.split ? peer_f32(su32(part + c * TILE_N + tid), s) : 0.0f;
+#pragma unroll
+            for (int s = 0; s < MAX_SPLIT; s++) sum += v[s];
+            if (ok && n < p.outs) store_y(p, m0 + c, n, sum + bias);
+        }
+        cluster_sync();                                     // no CTA leaves while another reads its shared memory
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::COLS) : "memory");
+    }
+}
+
+// ------------------------------------------------------------------ launch
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                  const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn()
+{
+    static const EncodeTiledFn fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            return (EncodeTiledFn)p;
+        cudaGetLastError();
+        return (EncodeTiledFn) nullptr;
+    }();
+    return fn;
+}
+
+// Boxes of 128 bytes of shared memory x box_rows in the 128-byte swizzle. spread: 4-bit codes, 16 of them to 16 bytes.
+bool encode_mx(CUtensorMap *map, const tcg_mx_t &m, int box_rows, bool spread)
+{
+    const EncodeTiledFn fn = encode_fn();
+    if (!fn) return fail("cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint64_t pitch = (cuuint64_t)mx_pitch(m.cols, m.bits);
+    cuuint64_t dims[2] = { spread ? (cuuint64_t)mx_wide(m.cols) : pitch, (cuuint64_t)m.rows };
+    cuuint64_t strides[1] = { pitch };
+    cuuint32_t box[2] = { 128, (cuuint32_t)box_rows };
+    cuuint32_t estr[2] = { 1, 1 };
+    const CUresult r = fn(map, spread ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void *)m.codes,
+                          dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail("cuTensorMapEncodeTiled failed (%d) for [%d x %d] in %d bits", (int)r, m.rows, m.cols, m.bits);
+    return true;
+}
+
+template <int BITS, int BN>
+bool stream_launch(LinArgs &p, const tcg_mx_t &x, const tcg_mx_t &w)
+{
+    using S = Stream<BITS, BN>;
+    CUtensorMap mw, mx;
+    if (!encode_mx(&mw, w, TILE_N, BITS == 8) || !encode_mx(&mx, x, BN, false)) return false;
+    p.tiles_n = (p.outs + TILE_N - 1) / TILE_N;
+    p.stages_k = (p.atoms + Fmt<BITS>::ATOMS - 1) / Fmt<BITS>::ATOMS;
+    const long long tiles = (long long)p.tiles_n * ((p.rows + BN - 1) / BN);
+    p.split = 1;
+    while (p.split < MAX_SPLIT && tiles * (p.split + 1) <= ctx().sms + ctx().sms / 8 && p.split * 4 < p.stages_k) p.split++;
+    p.per = (p.stages_k + p.split - 1) / p.split;
+    p.split = (p.stages_k + p.per - 1) / p.per;
+    // accumulators of at most 1024 (512) columns, as many as TMEM holds
+    p.acc_stages = max((p.per + S::MAX_ACC - 1) / S::MAX_ACC, 4);
+    const int room = 200 * 1024 / (BN <= 32 ? 2 : 1), part = p.split > 1 ? BN * TILE_N * 4 : 0;
+    p.depth = min(16, min(max(p.per, 2), room / S::STAGE));
+    const size_t smem = 1024 + max(p.depth * S::STAGE, part);
+    if (tiles * p.split > 0x7fffffffll) return fail("tcg_mx_linear: %d rows and %d outputs are too many for one call", p.rows, p.outs);
+    void (*fn)(const CUtensorMap, const CUtensorMap, const LinArgs) = mx_stream_kernel<BITS, BN>;
+    TCG_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 512));
+    cudaLaunchAttribute attrs[2];
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3((unsigned)(tiles * p.split));
+    lc.blockDim = dim3(128);
+    lc.dynamicSmemBytes = smem;
+    lc.stream = ctx().cur;
+    lc.attrs = attrs;
+    lc.numAttrs = pdl_attr(attrs);
+    attrs[lc.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attrs[lc.numAttrs].val.clusterDim = { (unsigned)p.split, 1, 1 };
+    lc.numAttrs++;
+    TCG_CUDA(cudaLaunchKernelEx(&lc, fn, mw, mx, (const LinArgs)p));
+    return true;
+}
+
+template <int BITS>
+bool linear_go(LinArgs &p, const tcg_mx_t &x, const tcg_mx_t &w)
+{
+    if (p.rows <= 8) return stream_launch<BITS, 8>(p, x, w);
+    if (p.rows <= 16) return stream_launch<BITS, 16>(p, x, w);
+    if (p.rows <= 32) return stream_launch<BITS, 32>(p, x, w);
+    if (p.rows <= 64) return stream_launch<BITS, 64>(p, x, w);
+    return stream_launch<BITS, 128>(p, x, w);
+}
+
+}  // namespace
+}  // namespace tcg
+
+using namespace tcg;
+
+extern "C" bool tcg_mx_linear(void *y, const tcg_mx_t *x, const tcg_mx_t *w, const float *bias, int64_t ld_y, ggml_type_t t)
+{
+    const char *who = "tcg_mx_linear";
+    if (!lm_type_size(t)) return fail("%s: type %d is not F32, F16 or BF16", who, (int)t);
+    if (!mx_check(who, "x", x) || !mx_check(who, "w", w)) return false;
+    if (w->bits != 4) return fail("%s: weights in %d bits: 4", who, w->bits);
+    if (x->cols != w->cols) return fail("%s: rows of %d columns and weights of %d", who, x->cols, w->cols);
+    if (w->rows && !mx_rows(who, "y", y, x->rows, w->rows, ld_y, t)) return false;
+    if ((uintptr_t)bias % 4) return fail("%s: misaligned bias", who);
+    if (!lm_ready(who)) return false;
+    if (!x->rows || !w->rows) return true;
+    LinArgs p = {};
+    p.xs = x->scales, p.ws = w->scales, p.bias = bias, p.y = y, p.ldy = ld_y, p.err = lm_error_word();
+    p.rows = x->rows, p.outs = w->rows, p.atoms = (int)(mx_wide(x->cols) / MX_ATOM), p.type = t;
+    return x->bits == 4 ? linear_go<4>(p, *x, *w) : linear_go<8>(p, *x, *w);
+}

@@ -93,7 +93,8 @@ class Roofline(C.Structure):          # include/tcg.h tc_roofline_t
 
 ROPE_INTERLEAVED, ROPE_HALF, ROPE_MAX_DIM = 0, 1, 256
 KV8_PAGE = 64
-ERR_KV8_LENGTHS, ERR_KV8_PAGE, ERR_KV8_WAIT = 64, 65, 66
+ERR_KV8_LENGTHS, ERR_KV8_PAGE, ERR_KV8_WAIT, ERR_MX_WAIT = 64, 65, 66, 67
+MX_MAX_ROWS, MX_MAX_COLS, NORM_MAX_COLS = 1 << 30, 1 << 24, 32768
 
 
 class Rope(C.Structure):              # include/tcg.h tcg_rope_t
@@ -109,6 +110,10 @@ class Kv8(C.Structure):               # include/tcg.h tcg_kv8_t
 class Kv8Step(C.Structure):           # include/tcg.h tcg_kv8_step_t
     _fields_ = [(n, vp) for n in ("tok_start", "kv_len", "table")] + \
                [(n, C.c_int) for n in ("table_ld", "n_seq", "n_tok", "max_new", "max_kv")]
+
+
+class Mx(C.Structure):                # include/tcg.h tcg_mx_t
+    _fields_ = [(n, vp) for n in ("codes", "scales")] + [(n, C.c_int) for n in ("rows", "cols", "bits")]
 
 
 # (name, restype, argtypes) of every entry point the binding uses
@@ -221,6 +226,11 @@ _SIGS = [
     ("tcg_kv8_read", boolean, [vp, vp, C.POINTER(Kv8), C.POINTER(Kv8Step), i64, i64, C.c_int]),
     ("tcg_kv8_attention", boolean, [vp, vp, C.POINTER(Kv8), C.POINTER(Kv8Step), i32, i64, i64, f32, boolean, i32,
                                     C.c_int]),
+    ("tcg_mx_code_bytes", sz, [i32, i32, i32]), ("tcg_mx_scale_bytes", sz, [i32, i32]),
+    ("tcg_mx_quantize", boolean, [C.POINTER(Mx), vp, i64, C.c_int]),
+    ("tcg_mx_dequantize", boolean, [vp, C.POINTER(Mx), i64, C.c_int]),
+    ("tcg_mx_linear", boolean, [vp, C.POINTER(Mx), C.POINTER(Mx), vp, i64, C.c_int]),
+    ("tcg_add_rms_norm", boolean, [vp, vp, C.POINTER(Mx), vp, vp, vp, f32, i32, i32, i64, i64, i64, i64, C.c_int]),
     ("tcg_nccl_unique_id", boolean, [C.c_char_p]),
     ("tcg_vit_upload_bcast", vp, [C.POINTER(Vit), i32, i32, i32, C.c_char_p]),
 ]
