@@ -59,6 +59,16 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
+// One lane of a converged warp. The role loops below run in whole warps and issue under this, so that what they issue is
+// known to be the same in all lanes: descriptors then live in uniform registers, where a branch to lane 0 moves each of them
+// there (105 cycles a product, which takes 64).
+__device__ __forceinline__ bool elect()
+{
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+
 __device__ __forceinline__ void cluster_sync()
 {
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
@@ -72,6 +82,21 @@ __device__ __forceinline__ float peer_f32(uint32_t addr, uint32_t rank)
     return v;
 }
 
+// Wait for the phase of parity `parity`. Gives up (false) when another role has (abort), or after WAIT_TRIES tests, each of
+// which the hardware may hold for a while: between 0.1 s and minutes. bar_wait (tc05.cuh) bounds its waits by a timer,
+// whose reading costs as much as a stage of this kernel.
+constexpr int WAIT_TRIES = 1 << 23;
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int *abort, int *err, bool heed_abort = true)
+{
+    for (int i = 0; i < WAIT_TRIES; i++) {
+        if (bar_test(bar, parity)) return true;
+        if ((i & 1023) == 1023 && heed_abort && *abort) return false;
+    }
+    *abort = 1;
+    atomicExch(err, ERR_WAIT);
+    return false;
+}
+
 struct LinArgs {
     const uint8_t *xs, *ws;             // scales
     const float *bias;
@@ -80,7 +105,7 @@ struct LinArgs {
     int *err;
     int rows, outs, atoms;              // of x, of w, scale groups of a row
     int stages_k;                       // stages of the whole K
-    int tiles_n, split, per;            // CTAs of a tile, stages of each
+    int tiles_n, tiles_m, split, per;   // CTAs of a tile, stages of each
     int accs, acc_stages;               // accumulators of a CTA, stages of each
     int depth;                          // stages in shared memory
     int type;
@@ -144,51 +169,65 @@ __global__ void __launch_bounds__(128) mx_stream_kernel(const __grid_constant__ 
     lm_signal();
     auto at = [&](int slot) { return base + slot * S::STAGE; };
     auto atoms_of = [&](int k) { return min(F::ATOMS, p.atoms - k * F::ATOMS); };
-    if (warp == 0 && lane == 0) {
-        int k = 0;
-        for (; k < count && ok; k++) {
-            const int slot = k % p.depth, kk = k_begin + k, na = atoms_of(kk);
-            if (k >= p.depth) ok = bar_wait(empty + 8 * slot, (k / p.depth - 1) & 1, abort, p.err, ERR_WAIT);
+    // warp indices as the compiler can see them to be uniform
+    const int role = __shfl_sync(0xFFFFFFFFu, warp, 0);
+    if (role == 0) {
+        int k = 0, slot = 0, phase = 1;
+        for (; k < count; k++) {
+            const int kk = k_begin + k, na = atoms_of(kk);
+            ok = wait_for(empty + 8 * slot, phase, abort, p.err);
             if (!ok) break;
             const uint32_t bar = full + 8 * slot, a = at(slot), b = a + S::A, sa = b + S::B, sb = sa + S::SF;
-            bar_expect_tx(bar, F::A_TX + S::B + 2 * 512 * na);
-            tma_load(a, &mw, bar, kk * 128, n0);
-            tma_load(b, &mx, bar, kk * 128, m0);
-            bulk_load(sa, p.ws + ((size_t)(n0 / MX_ATOM) * p.atoms + (size_t)kk * F::ATOMS) * 512, 512 * na, bar);
-            bulk_load(sb, p.xs + ((size_t)(m0 / MX_ATOM) * p.atoms + (size_t)kk * F::ATOMS) * 512, 512 * na, bar);
+            if (elect()) {
+                bar_expect_tx(bar, F::A_TX + S::B + 2 * 512 * na);
+                tma_load(a, &mw, bar, kk * 128, n0);
+                tma_load(b, &mx, bar, kk * 128, m0);
+                bulk_load(sa, p.ws + ((size_t)(n0 / MX_ATOM) * p.atoms + (size_t)kk * F::ATOMS) * 512, 512 * na, bar);
+                bulk_load(sb, p.xs + ((size_t)(m0 / MX_ATOM) * p.atoms + (size_t)kk * F::ATOMS) * 512, 512 * na, bar);
+            }
+            __syncwarp();
+            if (++slot == p.depth) slot = 0, phase ^= 1;
         }
         // copies in flight land before the CTA ends
         if (!ok)
             for (int j = max(0, k - p.depth); j < k; j++)
-                bar_wait(full + 8 * (j % p.depth), (j / p.depth) & 1, abort, p.err, ERR_WAIT, false);
-    } else if (warp == 1 && lane == 0) {
+                wait_for(full + 8 * (j % p.depth), (j / p.depth) & 1, abort, p.err, false);
+    } else if (role == 1) {
         const uint32_t id = mx_idesc<BITS>(BN, TILE_N), sfa = tmem + S::SF_COL, sfb = sfa + 4 * F::ATOMS;
         const uint32_t b_off = m0 % MX_ATOM / 32;           // the tile's first column of its group of 128 rows
+        int slot = 0, phase = 0, in_acc = 0;
+        uint32_t d = tmem;
         for (int k = 0; k < count; k++) {
-            const int slot = k % p.depth, na = atoms_of(k_begin + k);
-            ok = bar_wait(full + 8 * slot, (k / p.depth) & 1, abort, p.err, ERR_WAIT);
+            const int na = atoms_of(k_begin + k);
+            ok = wait_for(full + 8 * slot, phase, abort, p.err);
             if (!ok) break;
             fence_after();
             const uint32_t a = at(slot), b = a + S::A, sa = b + S::B, sb = sa + S::SF;
-            for (int i = 0; i < na; i++) {
-                scales_to_tmem(sfa + 4 * i, sa + 512 * i);
-                scales_to_tmem(sfb + 4 * i, sb + 512 * i);
-            }
-            const uint32_t d = tmem + k / p.acc_stages * BN;
-            const unsigned long long da = sdesc<128>(a), db = sdesc<128>(b);
+            if (elect()) {
 #pragma unroll
-            for (int j = 0; j < F::STEPS; j++) {
-                const int atom = j * F::STEP_K / MX_ATOM, byte = j * F::STEP_K / MX_BLOCK % 4;
-                if (atom < na)
-                    mma_mx<BITS>(d, da + 2 * j, db + 2 * j, id | byte << 29 | byte << 4, sfa + 4 * atom, sfb + 4 * atom + b_off,
-                                 k % p.acc_stages != 0 || j != 0);
+                for (int i = 0; i < F::ATOMS; i++)
+                    if (i < na) {
+                        scales_to_tmem(sfa + 4 * i, sa + 512 * i);
+                        scales_to_tmem(sfb + 4 * i, sb + 512 * i);
+                    }
+                const unsigned long long da = sdesc<128>(a), db = sdesc<128>(b);
+#pragma unroll
+                for (int j = 0; j < F::STEPS; j++) {
+                    const int atom = j * F::STEP_K / MX_ATOM, byte = j * F::STEP_K / MX_BLOCK % 4;
+                    if (atom < na)
+                        mma_mx<BITS>(d, da + 2 * j, db + 2 * j, id | byte << 29 | byte << 4, sfa + 4 * atom,
+                                     sfb + 4 * atom + b_off, in_acc != 0 || j != 0);
+                }
+                mma_commit(empty + 8 * slot);
             }
-            mma_commit(empty + 8 * slot);
+            __syncwarp();
+            if (++slot == p.depth) slot = 0, phase ^= 1;
+            if (++in_acc == p.acc_stages) in_acc = 0, d += BN;
         }
-        mma_commit(done);
+        if (elect()) mma_commit(done);
     }
     __syncwarp();
-    ok = bar_wait(done, 0, abort, p.err, ERR_WAIT, false) && ok && !*abort;
+    ok = wait_for(done, 0, abort, p.err, false) && ok && !*abort;
     fence_after();
     const int accs = count ? (count - 1) / p.acc_stages + 1 : 0;
     const uint32_t lane_base = tmem + ((uint32_t)warp << 21);
@@ -233,6 +272,247 @@ __global__ void __launch_bounds__(128) mx_stream_kernel(const __grid_constant__ 
     }
 }
 
+// ------------------------------------------------------------------ many rows: CTA pairs
+
+// A cluster of two CTAs computes tiles of 256 weight rows x 256 rows of x, one after the other: CTA r holds weight rows
+// 128 r .. 128 r + 127 (in its shared memory, and as the lanes of its accumulators) and half of x's rows; the pair's
+// products read both halves. Each CTA has the scales of its weight rows and of all 256 rows of x.
+template <int BITS>
+struct Pair {
+    static constexpr int ROWS = 256;                        // of x
+    static constexpr int A = TILE_N * 128, B = ROWS / 2 * 128, SF = Fmt<BITS>::ATOMS * 512;
+    static constexpr int STAGE = (A + B + 3 * SF + 1023) / 1024 * 1024;
+    static constexpr int STAGES = 6;
+    static constexpr uint32_t TX = 2 * (Fmt<BITS>::A_TX + B + 3 * SF);
+    // Two accumulators of 256 columns and the scales do not fit 512 columns; the second starts 32 columns before the first
+    // one's end. Those 32 are drained before anything else, so the next tile's products wait for an eighth of a drain.
+    static constexpr int ACC1 = 224, SF_COL = 480, COLS = 512;
+    static constexpr int SMEM = 1024 + STAGES * STAGE;
+    static_assert(SF_COL + 3 * 4 * Fmt<BITS>::ATOMS <= COLS, "the scales fit behind the accumulators");
+};
+
+constexpr int PAIR_EPI = 8, PAIR_THREADS = 32 * (2 + PAIR_EPI);
+
+__device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank)
+{
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar)
+{
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// A copy into this CTA's shared memory whose bytes complete on the leader's barrier.
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y)
+{
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+                 " [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"((unsigned long long)map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+template <int BITS>
+__device__ __forceinline__ void mma_mx_pair(uint32_t d, unsigned long long a, unsigned long long b, uint32_t id, uint32_t sa,
+                                            uint32_t sb, uint32_t acc)
+{
+    if (BITS == 4)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+                     "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(sa), "r"(sb), "r"(acc));
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+                     "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(sa), "r"(sb), "r"(acc));
+}
+__device__ __forceinline__ void scales_to_tmem_pair(uint32_t taddr, uint32_t smem)
+{
+    const unsigned long long d = (unsigned long long)((smem & 0x3FFFFu) >> 4) | ((unsigned long long)(128 >> 4) << 32) | (1ull << 46);
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+}
+// The pair's products so far, to the barrier at this offset in both CTAs.
+__device__ __forceinline__ void commit_pair(uint32_t bar)
+{
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(bar), "h"((unsigned short)3) : "memory");
+}
+
+template <typename T, int BITS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
+mx_pair_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap msw,
+               const __grid_constant__ CUtensorMap msx, const __grid_constant__ LinArgs p)
+{
+    using F = Fmt<BITS>;
+    using S = Pair<BITS>;
+    extern __shared__ unsigned char raw[];
+    // full, empty a stage; full, free, overlap free an accumulator; the end
+    __shared__ __align__(8) unsigned long long bars[2 * S::STAGES + 7];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort;
+    const uint32_t base = (su32(raw) + 1023) & ~1023u;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
+    const uint32_t rank = blockIdx.x & 1;
+    const uint32_t full = su32(bars), empty = full + 8 * S::STAGES, acc_full = empty + 8 * S::STAGES, acc_free = acc_full + 16,
+                   lap_free = acc_free + 16, end = lap_free + 16;
+    if (tid == 0) {
+        for (int i = 0; i < S::STAGES; i++) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
+        for (int i = 0; i < 2; i++) {
+            bar_init(acc_full + 8 * i, 1);
+            bar_init(acc_free + 8 * i, 2 * PAIR_EPI);       // every draining warp of both CTAs
+            bar_init(lap_free + 8 * i, PAIR_EPI);           // those that hold the shared columns
+        }
+        bar_init(end, 1);
+        s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(&s_tmem)), "r"(S::COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
+    fence_before();
+    __syncthreads();
+    cluster_sync();                                         // barriers and TMEM are there in both CTAs
+    fence_after();
+    const uint32_t tmem = s_tmem;
+    volatile int *abort = &s_abort;
+    bool ok = true;
+    pdl_wait();
+    const int tiles = p.tiles_n * p.tiles_m, first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    // Units: a tile's K, or with F32 results a part of it at a time.
+    if (warp == 0) {
+        int slot = 0, phase = 1, issued = 0;
+        for (int tile = first; tile < tiles && ok; tile += step) {
+            const int n0 = tile % p.tiles_n * 256 + rank * 128, m0 = tile / p.tiles_n * S::ROWS;
+            for (int k = 0; k < p.stages_k; k++) {
+                ok = wait_for(empty + 8 * slot, phase, abort, p.err);
+                if (!ok) break;
+                const uint32_t a = base + slot * S::STAGE, b = a + S::A, sa = b + S::B, sb = sa + S::SF;
+                const uint32_t bar = peer_addr(full + 8 * slot, 0);
+                if (elect()) {
+                    if (rank == 0) bar_expect_tx(full + 8 * slot, S::TX);
+                    tma_load_pair(a, &mw, bar, k * 128, n0);
+                    tma_load_pair(b, &mx, bar, k * 128, m0 + rank * 128);
+                    tma_load_pair(sa, &msw, bar, k * (F::ATOMS * 64), n0 / 128);
+                    tma_load_pair(sb, &msx, bar, k * (F::ATOMS * 64), m0 / 128);
+                }
+                __syncwarp();
+                issued++;
+                if (++slot == S::STAGES) slot = 0, phase ^= 1;
+            }
+        }
+        // copies in flight land before the CTAs end (both CTAs' complete on the leader's barriers)
+        if (rank == 0)
+            for (int i = 1; i <= S::STAGES && i <= issued; i++) {
+                const int at = slot - i, wrapped = at < 0;
+                wait_for(full + 8 * (wrapped ? at + S::STAGES : at), phase ^ 1 ^ wrapped, abort, p.err, false);
+            }
+    } else if (warp == 1 && rank == 0) {
+        const uint32_t id = mx_idesc<BITS>(S::ROWS, 256), sfa = tmem + S::SF_COL, sfb = sfa + 4 * F::ATOMS;
+        int slot = 0, phase = 0;
+        uint32_t unit = 0;
+        for (int tile = first; tile < tiles && ok; tile += step) {
+            for (int k0 = 0; k0 < p.stages_k && ok; k0 += p.acc_stages, unit++) {
+                const uint32_t buf = unit & 1, d = tmem + (buf ? S::ACC1 : 0);
+                ok = wait_for(acc_free + 8 * buf, (unit >> 1 & 1) ^ 1, abort, p.err) &&
+                     (unit == 0 || wait_for(lap_free + 8 * (buf ^ 1), (unit - 1) >> 1 & 1, abort, p.err));
+                fence_after();
+                const int k1 = min(p.stages_k, k0 + p.acc_stages);
+                for (int k = k0; k < k1 && ok; k++) {
+                    const int na = min(F::ATOMS, p.atoms - k * F::ATOMS);
+                    ok = wait_for(full + 8 * slot, phase, abort, p.err);
+                    if (!ok) break;
+                    fence_after();
+                    const uint32_t a = base + slot * S::STAGE, b = a + S::A, sa = b + S::B, sb = sa + S::SF;
+                    if (elect()) {
+#pragma unroll
+                        for (int i = 0; i < F::ATOMS; i++) {
+                            scales_to_tmem_pair(sfa + 4 * i, sa + 512 * i);
+                            scales_to_tmem_pair(sfb + 8 * i, sb + 512 * i);
+                            scales_to_tmem_pair(sfb + 8 * i + 4, sb + S::SF + 512 * i);
+                        }
+                        const unsigned long long da = sdesc<128>(a), db = sdesc<128>(b);
+#pragma unroll
+                        for (int j = 0; j < F::STEPS; j++) {
+                            const int atom = j * F::STEP_K / MX_ATOM, byte = j * F::STEP_K / MX_BLOCK % 4;
+                            if (atom < na)
+                                mma_mx_pair<BITS>(d, da + 2 * j, db + 2 * j, id | byte << 29 | byte << 4, sfa + 4 * atom,
+                                                  sfb + 8 * atom, k != k0 || j != 0);
+                        }
+                        commit_pair(empty + 8 * slot);
+                    }
+                    __syncwarp();
+                    if (++slot == S::STAGES) slot = 0, phase ^= 1;
+                }
+                if (ok && elect()) commit_pair(acc_full + 8 * buf);
+                __syncwarp();
+            }
+        }
+        // every product issued above has ended once this flips
+        if (elect())
+            asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(end) : "memory");
+        __syncwarp();
+        wait_for(end, 0, abort, p.err, false);
+    } else if (warp >= 2) {
+        const int q = warp & 3, h = (warp - 2) >> 2;        // TMEM lanes 32 q .., columns 128 h ..
+        const uint32_t at = tmem + ((uint32_t)q << 21) + 128 * h;
+        const uint32_t free_bar = peer_addr(acc_free, 0), lap_bar = peer_addr(lap_free, 0);
+        uint32_t unit = 0;
+        for (int tile = first; tile < tiles && ok; tile += step) {
+            const int n = tile % p.tiles_n * 256 + rank * 128 + 32 * q + lane, m0 = tile / p.tiles_n * S::ROWS + 128 * h;
+            const float bias = p.bias && n < p.outs ? p.bias[n] : 0.0f;
+            float acc[4][32];
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < 32; j++) acc[i][j] = bias;
+            for (int k0 = 0; k0 < p.stages_k; k0 += p.acc_stages, unit++) {
+                const uint32_t buf = unit & 1;
+                ok = wait_for(acc_full + 8 * buf, unit >> 1 & 1, abort, p.err);
+                if (!ok) break;
+                fence_after();
+                auto drain = [&](float (&v)[32], uint32_t col) {
+                    uint32_t r[32];
+                    tmem_ld32(at + col, r);
+#pragma unroll
+                    for (int j = 0; j < 32; j++) v[j] += __uint_as_float(r[j]);
+                };
+                auto shared_columns = [&](bool mine) {
+                    fence_before();
+                    __syncwarp();
+                    if (mine && lane == 0) arrive_cluster(lap_bar + 8 * buf);
+                };
+                if (buf == 0) {                             // the shared columns are the last 32 of 256
+                    drain(acc[3], 96);
+                    shared_columns(h == 1);
+                    drain(acc[0], 0), drain(acc[1], 32), drain(acc[2], 64);
+                } else {                                    // the first 32
+                    drain(acc[0], S::ACC1);
+                    shared_columns(h == 0);
+                    drain(acc[1], S::ACC1 + 32), drain(acc[2], S::ACC1 + 64), drain(acc[3], S::ACC1 + 96);
+                }
+                fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_cluster(free_bar + 8 * buf);
+            }
+            if (!ok) break;
+            T *y = (T *)p.y + m0 * p.ldy + n;
+            const int rows = n < p.outs ? p.rows - m0 : 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < 32; j++) {
+                    if (32 * i + j < rows) *y = from_f32<T>(acc[i][j]);
+                    y += p.ldy;
+                }
+        }
+    }
+    fence_before();
+    __syncthreads();
+    cluster_sync();                                         // the leader's products into this CTA's TMEM have ended
+    if (warp == 1) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::COLS) : "memory");
+    }
+}
+
 // ------------------------------------------------------------------ launch
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
@@ -267,6 +547,45 @@ bool encode_mx(CUtensorMap *map, const tcg_mx_t &m, int box_rows, bool spread)
                           dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail("cuTensorMapEncodeTiled failed (%d) for [%d x %d] in %d bits", (int)r, m.rows, m.cols, m.bits);
+    return true;
+}
+
+// The scales as rows of 64-bit words, a row for each 128 rows of the matrix; boxes of a stage's scales of `blocks` rows.
+bool encode_scales(CUtensorMap *map, const tcg_mx_t &m, int atoms, int blocks)
+{
+    const EncodeTiledFn fn = encode_fn();
+    if (!fn) return fail("cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint64_t wide = (cuuint64_t)mx_wide(m.cols) / MX_ATOM * 64;
+    cuuint64_t dims[2] = { wide, ((cuuint64_t)m.rows + MX_ATOM - 1) / MX_ATOM };
+    cuuint64_t strides[1] = { wide * 8 };
+    cuuint32_t box[2] = { (cuuint32_t)atoms * 64, (cuuint32_t)blocks };
+    cuuint32_t estr[2] = { 1, 1 };
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT64, 2, (void *)m.scales, dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail("cuTensorMapEncodeTiled failed (%d) for the scales of [%d x %d]", (int)r, m.rows, m.cols);
+    return true;
+}
+
+template <typename T, int BITS>
+bool pair_launch(LinArgs &p, const tcg_mx_t &x, const tcg_mx_t &w)
+{
+    using S = Pair<BITS>;
+    using F = Fmt<BITS>;
+    CUtensorMap mw, mx, msw, msx;
+    if (!encode_mx(&mw, w, TILE_N, BITS == 8) || !encode_mx(&mx, x, S::ROWS / 2, false) ||
+        !encode_scales(&msw, w, F::ATOMS, 1) || !encode_scales(&msx, x, F::ATOMS, 2))
+        return false;
+    p.tiles_n = (p.outs + 255) / 256;
+    p.tiles_m = (p.rows + S::ROWS - 1) / S::ROWS;
+    p.stages_k = (p.atoms + F::ATOMS - 1) / F::ATOMS;
+    p.acc_stages = sizeof(T) == 4 ? 2048 / F::K : p.stages_k;
+    const long long tiles = (long long)p.tiles_n * p.tiles_m;
+    if (tiles > 0x7fffff00ll) return fail("tcg_mx_linear: %d rows and %d outputs are too many for one call", p.rows, p.outs);
+    const int pairs = (int)min(tiles, (long long)ctx().sms / 2);
+    void (*fn)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const CUtensorMap, const LinArgs) = mx_pair_kernel<T, BITS>;
+    TCG_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+    TCG_CUDA(launch_pdl(fn, dim3(2 * pairs), dim3(PAIR_THREADS), S::SMEM, ctx().cur, mw, mx, msw, msx, (const LinArgs)p));
     return true;
 }
 
@@ -313,6 +632,8 @@ bool linear_go(LinArgs &p, const tcg_mx_t &x, const tcg_mx_t &w)
     if (p.rows <= 16) return stream_launch<BITS, 16>(p, x, w);
     if (p.rows <= 32) return stream_launch<BITS, 32>(p, x, w);
     if (p.rows <= 64) return stream_launch<BITS, 64>(p, x, w);
+    if ((long long)((p.rows + 255) / 256) * ((p.outs + 255) / 256) >= ctx().sms / 4)
+        return lm_by_type((ggml_type_t)p.type, [&](auto v) { return pair_launch<decltype(v), BITS>(p, x, w); });
     return stream_launch<BITS, 128>(p, x, w);
 }
 
