@@ -3,6 +3,7 @@
 #include "mx.cuh"
 #include "tc05.cuh"
 
+#include <string.h>
 #include <type_traits>
 
 namespace tcg {
@@ -109,6 +110,7 @@ struct LinArgs {
     int accs, acc_stages;               // accumulators of a CTA, stages of each
     int depth;                          // stages in shared memory
     int type;
+    bool pairs;                         // two 16-bit results of a row as one word
 };
 
 template <typename T>
@@ -291,7 +293,7 @@ struct Pair {
     static_assert(SF_COL + 3 * 4 * Fmt<BITS>::ATOMS <= COLS, "the scales fit behind the accumulators");
 };
 
-constexpr int PAIR_EPI = 8, PAIR_THREADS = 32 * (2 + PAIR_EPI);
+constexpr int PAIR_EPI = 16, PAIR_THREADS = 32 * (2 + PAIR_EPI);
 
 __device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank)
 {
@@ -335,6 +337,23 @@ __device__ __forceinline__ void commit_pair(uint32_t bar)
                  ::"r"(bar), "h"((unsigned short)3) : "memory");
 }
 
+// Tile `i` in the order they are taken: eight blocks of x's rows at a time, so that the tiles under way together share both.
+__device__ __forceinline__ void tile_at(const LinArgs &p, int i, int &tn, int &tm)
+{
+    const int group = i / (8 * p.tiles_n), in = i - group * 8 * p.tiles_n, high = min(8, p.tiles_m - 8 * group);
+    tn = in / high;
+    tm = 8 * group + in - tn * high;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b)
+{
+    const T v[2] = { from_f32<T>(a), from_f32<T>(b) };
+    uint32_t w;
+    memcpy(&w, v, sizeof w);
+    return w;
+}
+
 template <typename T, int BITS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
 mx_pair_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap msw,
@@ -357,7 +376,7 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ C
         for (int i = 0; i < 2; i++) {
             bar_init(acc_full + 8 * i, 1);
             bar_init(acc_free + 8 * i, 2 * PAIR_EPI);       // every draining warp of both CTAs
-            bar_init(lap_free + 8 * i, PAIR_EPI);           // those that hold the shared columns
+            bar_init(lap_free + 8 * i, 8);                  // those that hold the shared columns
         }
         bar_init(end, 1);
         s_abort = 0;
@@ -380,7 +399,9 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ C
     if (warp == 0) {
         int slot = 0, phase = 1, issued = 0;
         for (int tile = first; tile < tiles && ok; tile += step) {
-            const int n0 = tile % p.tiles_n * 256 + rank * 128, m0 = tile / p.tiles_n * S::ROWS;
+            int tn, tm;
+            tile_at(p, tile, tn, tm);
+            const int n0 = tn * 256 + rank * 128, m0 = tm * S::ROWS;
             for (int k = 0; k < p.stages_k; k++) {
                 ok = wait_for(empty + 8 * slot, phase, abort, p.err);
                 if (!ok) break;
@@ -451,57 +472,73 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ C
         __syncwarp();
         wait_for(end, 0, abort, p.err, false);
     } else if (warp >= 2) {
-        const int q = warp & 3, h = (warp - 2) >> 2;        // TMEM lanes 32 q .., columns 128 h ..
-        const uint32_t at = tmem + ((uint32_t)q << 21) + 128 * h;
+        const int q = warp & 3, h = (warp - 2) >> 2;        // TMEM lanes 32 q .., columns 64 h ..
+        const uint32_t at = tmem + ((uint32_t)q << 21) + 64 * h;
         const uint32_t free_bar = peer_addr(acc_free, 0), lap_bar = peer_addr(lap_free, 0);
         uint32_t unit = 0;
         for (int tile = first; tile < tiles && ok; tile += step) {
-            const int n = tile % p.tiles_n * 256 + rank * 128 + 32 * q + lane, m0 = tile / p.tiles_n * S::ROWS + 128 * h;
+            int tn, tm;
+            tile_at(p, tile, tn, tm);
+            const int n = tn * 256 + rank * 128 + 32 * q + lane, m0 = tm * S::ROWS + 64 * h;
+            // the order of 16-column pieces: the shared columns are the last 32 of the first accumulator, the first of the second
+            auto piece = [&](int i) { return (i ^ (h == 3 ? 2 : 0)) * 16; };
             const float bias = p.bias && n < p.outs ? p.bias[n] : 0.0f;
-            float acc[4][32];
+            // 64 columns: fp32 results are summed here over the tile's units; 16-bit ones have one unit and are packed at once
+            constexpr bool WIDE = sizeof(T) == 4;
+            constexpr int WORDS = WIDE ? 16 : 8;            // of 16 columns
+            uint32_t acc[4][WORDS];
+            if (WIDE)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 32; j++) acc[i][j] = bias;
+                for (int i = 0; i < 4 * WORDS; i++) acc[i / WORDS][i % WORDS] = __float_as_uint(bias);
             for (int k0 = 0; k0 < p.stages_k; k0 += p.acc_stages, unit++) {
                 const uint32_t buf = unit & 1;
                 ok = wait_for(acc_full + 8 * buf, unit >> 1 & 1, abort, p.err);
                 if (!ok) break;
                 fence_after();
-                auto drain = [&](float (&v)[32], uint32_t col) {
-                    uint32_t r[32];
-                    tmem_ld32(at + col, r);
 #pragma unroll
-                    for (int j = 0; j < 32; j++) v[j] += __uint_as_float(r[j]);
-                };
-                auto shared_columns = [&](bool mine) {
-                    fence_before();
-                    __syncwarp();
-                    if (mine && lane == 0) arrive_cluster(lap_bar + 8 * buf);
-                };
-                if (buf == 0) {                             // the shared columns are the last 32 of 256
-                    drain(acc[3], 96);
-                    shared_columns(h == 1);
-                    drain(acc[0], 0), drain(acc[1], 32), drain(acc[2], 64);
-                } else {                                    // the first 32
-                    drain(acc[0], S::ACC1);
-                    shared_columns(h == 0);
-                    drain(acc[1], S::ACC1 + 32), drain(acc[2], S::ACC1 + 64), drain(acc[3], S::ACC1 + 96);
+                for (int i = 0; i < 4; i++) {
+                    uint32_t r[16];
+                    tmem_ld16(at + (buf ? S::ACC1 : 0) + piece(i), r);
+#pragma unroll
+                    for (int j = 0; j < 16; j += WIDE ? 1 : 2) {
+                        if constexpr (WIDE) acc[i][j] = __float_as_uint(__uint_as_float(acc[i][j]) + __uint_as_float(r[j]));
+                        else acc[i][j / 2] = pack2<T>(__uint_as_float(r[j]) + bias, __uint_as_float(r[j + 1]) + bias);
+                    }
+                    if (i == 1) {                           // the shared columns are drained
+                        fence_before();
+                        __syncwarp();
+                        if (h == (buf ? 0 : 3) && lane == 0) arrive_cluster(lap_bar + 8 * buf);
+                    }
                 }
                 fence_before();
                 __syncwarp();
                 if (lane == 0) arrive_cluster(free_bar + 8 * buf);
             }
             if (!ok) break;
-            T *y = (T *)p.y + m0 * p.ldy + n;
-            const int rows = n < p.outs ? p.rows - m0 : 0;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int i = 0; i < 4; i++) {
+                const int m = m0 + piece(i), rows = n < p.outs ? p.rows - m : 0;
+                if constexpr (WIDE) {
+                    T *y = (T *)p.y + m * p.ldy + n;
 #pragma unroll
-                for (int j = 0; j < 32; j++) {
-                    if (32 * i + j < rows) *y = from_f32<T>(acc[i][j]);
-                    y += p.ldy;
+                    for (int j = 0; j < 16; j++, y += p.ldy)
+                        if (j < rows) *y = __uint_as_float(acc[i][j]);
+                } else if (p.pairs) {
+                    // a lane trades with its neighbour: two features of one row instead of one feature of two
+                    T *y = (T *)p.y + (m + (lane & 1)) * p.ldy + (n & ~1);
+#pragma unroll
+                    for (int j = 0; j < 8; j++, y += 2 * p.ldy) {
+                        const uint32_t own = acc[i][j], other = __shfl_xor_sync(0xFFFFFFFFu, own, 1);
+                        if (2 * j + (lane & 1) < rows)
+                            *(uint32_t *)y = lane & 1 ? __byte_perm(other, own, 0x7632) : __byte_perm(own, other, 0x5410);
+                    }
+                } else {
+                    unsigned short *y = (unsigned short *)p.y + m * p.ldy + n;
+#pragma unroll
+                    for (int j = 0; j < 16; j++, y += p.ldy)
+                        if (j < rows) *y = (unsigned short)(acc[i][j / 2] >> (j & 1) * 16);
                 }
+            }
         }
     }
     fence_before();
@@ -579,6 +616,7 @@ bool pair_launch(LinArgs &p, const tcg_mx_t &x, const tcg_mx_t &w)
     p.tiles_n = (p.outs + 255) / 256;
     p.tiles_m = (p.rows + S::ROWS - 1) / S::ROWS;
     p.stages_k = (p.atoms + F::ATOMS - 1) / F::ATOMS;
+    p.pairs = p.ldy % 2 == 0 && (uintptr_t)p.y % 4 == 0 && p.outs % 2 == 0;
     p.acc_stages = sizeof(T) == 4 ? 2048 / F::K : p.stages_k;
     const long long tiles = (long long)p.tiles_n * p.tiles_m;
     if (tiles > 0x7fffff00ll) return fail("tcg_mx_linear: %d rows and %d outputs are too many for one call", p.rows, p.outs);
