@@ -10,8 +10,12 @@ namespace tcg {
 namespace {
 
 constexpr int ERR_WAIT = TCG_ERR_MX_WAIT;
+constexpr int STREAM_THREADS = 256, MAX_DEPTH = 16;
+constexpr int HALF_SM = 108 * 1024;
+constexpr int SUM_K = 4096;             // columns that the tensor core sums before fp32 results are added up outside
 constexpr int TILE_N = 128;             // weight rows of a tile: the MMA's M, a TMEM lane each
 constexpr int MAX_SPLIT = 8;            // portable cluster size
+constexpr int MIN_STAGES = 2;           // of a CTA, where K is split: 4096 -> 1024 3.8 us, with 4 4.4, with 8 4.8
 
 // What differs between rows in 4 and in 8 bits. A stage is 128 bytes of a row of x; the weights' 4-bit codes next to 8-bit
 // rows are spread by the copy itself to 16 bytes for 16 codes, as kind::mxf8f6f4 reads them.
@@ -60,6 +64,11 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *map)
+{
+    asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)map) : "memory");
+}
+
 // One lane of a converged warp. The role loops below run in whole warps and issue under this, so that what they issue is
 // known to be the same in all lanes: descriptors then live in uniform registers, where a branch to lane 0 moves each of them
 // there (105 cycles a product, which takes 64).
@@ -74,22 +83,30 @@ __device__ __forceinline__ void cluster_sync()
 {
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float peer_f32(uint32_t addr, uint32_t rank)
+__device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank)
 {
-    uint32_t at;
-    float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-    return v;
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+// Bytes from this CTA's shared memory to a peer's, counted by its barrier.
+__device__ __forceinline__ void push(uint32_t to, uint32_t from, uint32_t bytes, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(to), "r"(from), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar)
+{
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-// Wait for the phase of parity `parity`. Gives up (false) when another role has (abort), or after WAIT_TRIES tests, each of
-// which the hardware may hold for a while: between 0.1 s and minutes. bar_wait (tc05.cuh) bounds its waits by a timer,
-// whose reading costs as much as a stage of this kernel.
+// Wait for the phase of parity `parity`. Gives up (false) when another role has (abort), or after `tries` tests, each of
+// which the hardware may hold for a while: between 0.1 s and minutes. bar_wait (tc05.cuh) bounds its waits by a timer.
 constexpr int WAIT_TRIES = 1 << 23;
-__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int *abort, int *err, bool heed_abort = true)
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int *abort, int *err, bool heed_abort = true,
+                                         int tries = WAIT_TRIES)
 {
-    for (int i = 0; i < WAIT_TRIES; i++) {
+    for (int i = 0; i < tries; i++) {
         if (bar_test(bar, parity)) return true;
         if ((i & 1023) == 1023 && heed_abort && *abort) return false;
     }
@@ -107,55 +124,65 @@ struct LinArgs {
     int rows, outs, atoms;              // of x, of w, scale groups of a row
     int stages_k;                       // stages of the whole K
     int tiles_n, tiles_m, split, per;   // CTAs of a tile, stages of each
-    int accs, acc_stages;               // accumulators of a CTA, stages of each
+    int acc_stages;                     // stages of an accumulator
     int depth;                          // stages in shared memory
     int type;
     bool pairs;                         // two 16-bit results of a row as one word
 };
 
-template <typename T>
-__device__ __forceinline__ void put(const LinArgs &p, long long row, int n, float v)
+// Results of rows row, row + 1 .. of x (as far as there are such rows) for weight row n.
+template <int STEP, typename T>
+__device__ __forceinline__ void put_columns(const LinArgs &p, int row, int n, float bias, const float (&v)[STEP])
 {
-    ((T *)p.y)[row * p.ldy + n] = from_f32<T>(v);
+    T *y = (T *)p.y + row * p.ldy + n;
+    const int rows = n < p.outs ? p.rows - row : 0;
+#pragma unroll
+    for (int j = 0; j < STEP; j++, y += p.ldy)
+        if (j < rows) *y = from_f32<T>(v[j] + bias);
 }
-__device__ __forceinline__ void store_y(const LinArgs &p, long long row, int n, float v)
-{
-    if (p.type == GGML_TYPE_F32) put<float>(p, row, n, v);
-    else if (p.type == GGML_TYPE_F16) put<__half>(p, row, n, v);
-    else put<__nv_bfloat16>(p, row, n, v);
-}
+// ------------------------------------------------------------------ few rows: K split over clusters
 
+// A stage is 256 columns: 128 bytes of a row in 4 bits, two times 128 next to and in 8 bits. (Four warps that spread the
+// weights' codes in shared memory, from boxes of whole 128-byte rows, in place of the copy: one token 4096 -> 14336
+// 14.5 us against 10.5.)
 template <int BITS, int BN>
 struct Stream {
-    static constexpr int A = TILE_N * 128, B = BN * 128, SF = Fmt<BITS>::ATOMS * 512;
-    static constexpr int STAGE = A + B + 2 * SF;            // SF is a multiple of 512; A and B of 1024
+    static constexpr int SUBS = BITS == 8 ? 2 : 1, K = 256, ATOMS = 2;
+    static constexpr int A1 = TILE_N * 128, A = SUBS * A1, B1 = BN * 128, B = SUBS * B1, SF = ATOMS * 512;
+    static constexpr int STAGE = A + B + 2 * SF;            // every part starts on 1024 bytes
+    static constexpr int TX = TILE_N * 128 + B;             // bytes that the copies of codes count: weights as they are held
     static constexpr int COLS = BN <= 32 ? 256 : 512;       // TMEM: accumulators, then the scales
-    static constexpr int SF_COL = COLS - 2 * Fmt<BITS>::ATOMS * 4;
+    static constexpr int SF_COL = COLS - 2 * ATOMS * 4;
     static constexpr int MAX_ACC = SF_COL / BN;
 };
 
-// One tile of 128 weight rows x BN rows of x a cluster, its K dealt out to the cluster's CTAs.
+// One tile of 128 weight rows x BN rows of x a cluster, its K dealt out to the cluster's CTAs. Warp 0 loads, warp 1 issues the
+// products; then all of them take the results.
 template <int BITS, int BN>
-__global__ void __launch_bounds__(128) mx_stream_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap mx,
-                                                        const __grid_constant__ LinArgs p)
+__global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap mx,
+                                                                   const __grid_constant__ LinArgs p)
 {
-    using F = Fmt<BITS>;
     using S = Stream<BITS, BN>;
     extern __shared__ unsigned char raw[];
-    __shared__ __align__(8) unsigned long long bars[2 * 16 + 1];
+    __shared__ __align__(8) unsigned long long bars[2 * MAX_DEPTH + 2];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
     unsigned char *const smem = (unsigned char *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t base = su32(smem), full = su32(bars), empty = full + 8 * 16, done = full + 8 * 32;
+    const uint32_t base = su32(smem), full = su32(bars), empty = full + 8 * MAX_DEPTH, done = empty + 8 * MAX_DEPTH, join = done + 8;
     const int rank = blockIdx.x % p.split, tile = blockIdx.x / p.split;
     const int n0 = tile % p.tiles_n * TILE_N, m0 = tile / p.tiles_n * BN;
-    const int k_begin = rank * p.per, k_end = min(p.stages_k, k_begin + p.per), count = max(0, k_end - k_begin);
+    const int k_begin = rank * p.per, k_end = min(p.stages_k, k_begin + p.per), count = k_end - k_begin;
+    // Where a tile's K is split, its results meet by fours of x's rows: the CTA of rank g % split adds up group g.
+    const int groups = (min(BN, p.rows - m0) + 3) / 4, mine = p.split > 1 && groups > rank ? (groups - rank + p.split - 1) / p.split : 0;
     if (tid == 0) {
+        prefetch_map(&mw), prefetch_map(&mx);
         for (int i = 0; i < p.depth; i++) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
         bar_init(done, 1);
+        bar_init(join, 1);
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        if (mine) bar_expect_tx(join, p.split * mine * TILE_N * 16);
     }
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(&s_tmem)), "r"(S::COLS) : "memory");
@@ -164,28 +191,34 @@ __global__ void __launch_bounds__(128) mx_stream_kernel(const __grid_constant__ 
     fence_before();
     __syncthreads();
     fence_after();
+    if (p.split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     const uint32_t tmem = s_tmem;
     volatile int *abort = &s_abort;
     bool ok = true;
     pdl_wait();
     lm_signal();
+    const int n = n0 + (tid & 127);
+    const float bias = p.bias && n < p.outs ? p.bias[n] : 0.0f;
     auto at = [&](int slot) { return base + slot * S::STAGE; };
-    auto atoms_of = [&](int k) { return min(F::ATOMS, p.atoms - k * F::ATOMS); };
+    auto atoms_of = [&](int k) { return min(S::ATOMS, p.atoms - (k_begin + k) * S::ATOMS); };
     // warp indices as the compiler can see them to be uniform
     const int role = __shfl_sync(0xFFFFFFFFu, warp, 0);
     if (role == 0) {
         int k = 0, slot = 0, phase = 1;
         for (; k < count; k++) {
-            const int kk = k_begin + k, na = atoms_of(kk);
+            const int kk = k_begin + k, na = atoms_of(k);
             ok = wait_for(empty + 8 * slot, phase, abort, p.err);
             if (!ok) break;
             const uint32_t bar = full + 8 * slot, a = at(slot), b = a + S::A, sa = b + S::B, sb = sa + S::SF;
             if (elect()) {
-                bar_expect_tx(bar, F::A_TX + S::B + 2 * 512 * na);
-                tma_load(a, &mw, bar, kk * 128, n0);
-                tma_load(b, &mx, bar, kk * 128, m0);
-                bulk_load(sa, p.ws + ((size_t)(n0 / MX_ATOM) * p.atoms + (size_t)kk * F::ATOMS) * 512, 512 * na, bar);
-                bulk_load(sb, p.xs + ((size_t)(m0 / MX_ATOM) * p.atoms + (size_t)kk * F::ATOMS) * 512, 512 * na, bar);
+                bar_expect_tx(bar, S::TX + 2 * 512 * na);
+#pragma unroll
+                for (int i = 0; i < S::SUBS; i++) {
+                    tma_load(a + i * S::A1, &mw, bar, (kk * S::SUBS + i) * 128, n0);
+                    tma_load(b + i * S::B1, &mx, bar, (kk * S::SUBS + i) * 128, m0);
+                }
+                bulk_load(sa, p.ws + ((size_t)(n0 / MX_ATOM) * p.atoms + (size_t)kk * S::ATOMS) * 512, 512 * na, bar);
+                bulk_load(sb, p.xs + ((size_t)(m0 / MX_ATOM) * p.atoms + (size_t)kk * S::ATOMS) * 512, 512 * na, bar);
             }
             __syncwarp();
             if (++slot == p.depth) slot = 0, phase ^= 1;
@@ -195,29 +228,29 @@ __global__ void __launch_bounds__(128) mx_stream_kernel(const __grid_constant__ 
             for (int j = max(0, k - p.depth); j < k; j++)
                 wait_for(full + 8 * (j % p.depth), (j / p.depth) & 1, abort, p.err, false);
     } else if (role == 1) {
-        const uint32_t id = mx_idesc<BITS>(BN, TILE_N), sfa = tmem + S::SF_COL, sfb = sfa + 4 * F::ATOMS;
+        const uint32_t id = mx_idesc<BITS>(BN, TILE_N), sfa = tmem + S::SF_COL, sfb = sfa + 4 * S::ATOMS;
         const uint32_t b_off = m0 % MX_ATOM / 32;           // the tile's first column of its group of 128 rows
         int slot = 0, phase = 0, in_acc = 0;
         uint32_t d = tmem;
         for (int k = 0; k < count; k++) {
-            const int na = atoms_of(k_begin + k);
+            const int na = atoms_of(k);
             ok = wait_for(full + 8 * slot, phase, abort, p.err);
             if (!ok) break;
             fence_after();
             const uint32_t a = at(slot), b = a + S::A, sa = b + S::B, sb = sa + S::SF;
             if (elect()) {
 #pragma unroll
-                for (int i = 0; i < F::ATOMS; i++)
+                for (int i = 0; i < S::ATOMS; i++)
                     if (i < na) {
                         scales_to_tmem(sfa + 4 * i, sa + 512 * i);
                         scales_to_tmem(sfb + 4 * i, sb + 512 * i);
                     }
-                const unsigned long long da = sdesc<128>(a), db = sdesc<128>(b);
 #pragma unroll
-                for (int j = 0; j < F::STEPS; j++) {
-                    const int atom = j * F::STEP_K / MX_ATOM, byte = j * F::STEP_K / MX_BLOCK % 4;
+                for (int j = 0; j < 4 * S::SUBS; j++) {     // 32 bytes of a row each: 64 or 32 columns
+                    const int atom = BITS == 8 ? j / 4 : j / 2, byte = BITS == 8 ? j % 4 : j % 2 * 2;
+                    const unsigned long long da = sdesc<128>(a + j / 4 * S::A1), db = sdesc<128>(b + j / 4 * S::B1);
                     if (atom < na)
-                        mma_mx<BITS>(d, da + 2 * j, db + 2 * j, id | byte << 29 | byte << 4, sfa + 4 * atom,
+                        mma_mx<BITS>(d, da + 2 * (j % 4), db + 2 * (j % 4), id | byte << 29 | byte << 4, sfa + 4 * atom,
                                      sfb + 4 * atom + b_off, in_acc != 0 || j != 0);
                 }
                 mma_commit(empty + 8 * slot);
@@ -231,41 +264,64 @@ __global__ void __launch_bounds__(128) mx_stream_kernel(const __grid_constant__ 
     __syncwarp();
     ok = wait_for(done, 0, abort, p.err, false) && ok && !*abort;
     fence_after();
-    const int accs = count ? (count - 1) / p.acc_stages + 1 : 0;
-    const uint32_t lane_base = tmem + ((uint32_t)warp << 21);
-    const int n = n0 + tid;
-    float *const part = (float *)smem;                      // [BN][128], over the stages: their MMAs are done
-    const float bias = p.bias && n < p.outs ? p.bias[n] : 0.0f;
-    constexpr int STEP = 8;
+    const int accs = (count - 1) / p.acc_stages + 1;
+    const uint32_t lane_base = tmem + ((uint32_t)(warp & 3) << 21);
+    // Two warps share 32 TMEM lanes (weight rows) and take every second step of columns (x's rows).
+    const int t = tid & 127, half = tid >> 7;
+    auto finish = [&](auto type) {
+        using T = decltype(type);
+        // [split][ceil(BN / 4 / split)][128] words of four columns: by owner, over the stages (whose products are done), what
+        // this CTA sends; by sender, behind the stages, what the cluster's CTAs send here
+        const int per_rank = (BN / 4 + p.split - 1) / p.split;
+        float4 *const sent = (float4 *)smem;
+        const float4 *const part = (const float4 *)(smem + p.depth * S::STAGE);
+        constexpr int STEP = BN < 32 ? 8 : 16;
 #pragma unroll 1
-    for (int c = 0; c < BN; c += STEP) {
-        if (m0 + c >= p.rows) break;
-        float v[STEP] = {};
-        for (int i = 0; i < accs; i++) {
-            uint32_t r[STEP];
-            tmem_ld8(lane_base + i * BN + c, r);
+        for (int c = half * STEP; c < BN && m0 + c < p.rows; c += 2 * STEP) {
+            float v[STEP] = {};
+            for (int i = 0; i < accs; i++) {
+                uint32_t r[STEP];
+                if constexpr (STEP == 8) tmem_ld8(lane_base + i * BN + c, r);
+                else tmem_ld16(lane_base + i * BN + c, r);
 #pragma unroll
-            for (int j = 0; j < STEP; j++) v[j] += __uint_as_float(r[j]);
+                for (int j = 0; j < STEP; j++) v[j] += __uint_as_float(r[j]);
+            }
+            if (p.split > 1) {
+#pragma unroll
+                for (int j = 0; j < STEP; j += 4) {
+                    const int g = (c + j) / 4, i = g / p.split, owner = g - i * p.split;
+                    sent[(owner * per_rank + i) * TILE_N + t] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                }
+            } else if (ok) {
+                put_columns<STEP, T>(p, m0 + c, n, bias, v);
+            }
         }
+        if (p.split == 1) return;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncthreads();
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");     // the peers' barriers are there
+        if (tid < p.split && tid < groups)
+            push(peer_addr(su32(part + rank * per_rank * TILE_N), tid), su32(sent + tid * per_rank * TILE_N),
+                 (groups - tid + p.split - 1) / p.split * TILE_N * 16, peer_addr(join, tid));
+        __syncwarp();
+        if (mine) ok = wait_for(join, 0, abort, p.err, false) && ok;
+        asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+#pragma unroll 2
+        for (int i = half; i < mine; i += 2) {
+            float sum[4] = {};
 #pragma unroll
-        for (int j = 0; j < STEP; j++) {
-            if (p.split > 1) part[(c + j) * TILE_N + tid] = v[j];
-            else if (ok && n < p.outs && m0 + c + j < p.rows) store_y(p, m0 + c + j, n, v[j] + bias);
+            for (int s = 0; s < MAX_SPLIT; s++) {
+                const float4 v = s < p.split ? part[(s * per_rank + i) * TILE_N + t] : make_float4(0, 0, 0, 0);
+                sum[0] += v.x, sum[1] += v.y, sum[2] += v.z, sum[3] += v.w;
+            }
+            if (ok) put_columns<4, T>(p, m0 + 4 * (rank + i * p.split), n, bias, sum);
         }
-    }
-    if (p.split > 1) {
-        cluster_sync();
-        const int rows = min(BN, p.rows - m0);
-        for (int c = rank; c < rows; c += p.split) {
-            float v[MAX_SPLIT], sum = 0.0f;
-#pragma unroll
-            for (int s = 0; s < MAX_SPLIT; s++) v[s] = s < p.split ? peer_f32(su32(part + c * TILE_N + tid), s) : 0.0f;
-#pragma unroll
-            for (int s = 0; s < MAX_SPLIT; s++) sum += v[s];
-            if (ok && n < p.outs) store_y(p, m0 + c, n, sum + bias);
-        }
-        cluster_sync();                                     // no CTA leaves while another reads its shared memory
-    }
+        // A CTA leaves when all that it sent has arrived: when every CTA of the cluster has received.
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    };
+    if (p.type == GGML_TYPE_F32) finish(float());
+    else if (p.type == GGML_TYPE_F16) finish(__half());
+    else finish(__nv_bfloat16());
     fence_before();
     __syncthreads();
     if (warp == 0) {
@@ -295,16 +351,6 @@ struct Pair {
 
 constexpr int PAIR_EPI = 16, PAIR_THREADS = 32 * (2 + PAIR_EPI);
 
-__device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank)
-{
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ void arrive_cluster(uint32_t bar)
-{
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
 // A copy into this CTA's shared memory whose bytes complete on the leader's barrier.
 __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y)
 {
@@ -372,6 +418,7 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ C
     const uint32_t full = su32(bars), empty = full + 8 * S::STAGES, acc_full = empty + 8 * S::STAGES, acc_free = acc_full + 16,
                    lap_free = acc_free + 16, end = lap_free + 16;
     if (tid == 0) {
+        prefetch_map(&mw), prefetch_map(&mx), prefetch_map(&msw), prefetch_map(&msx);
         for (int i = 0; i < S::STAGES; i++) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
         for (int i = 0; i < 2; i++) {
             bar_init(acc_full + 8 * i, 1);
@@ -617,7 +664,7 @@ bool pair_launch(LinArgs &p, const tcg_mx_t &x, const tcg_mx_t &w)
     p.tiles_m = (p.rows + S::ROWS - 1) / S::ROWS;
     p.stages_k = (p.atoms + F::ATOMS - 1) / F::ATOMS;
     p.pairs = p.ldy % 2 == 0 && (uintptr_t)p.y % 4 == 0 && p.outs % 2 == 0;
-    p.acc_stages = sizeof(T) == 4 ? 2048 / F::K : p.stages_k;
+    p.acc_stages = sizeof(T) == 4 ? SUM_K / F::K : p.stages_k;
     const long long tiles = (long long)p.tiles_n * p.tiles_m;
     if (tiles > 0x7fffff00ll) return fail("tcg_mx_linear: %d rows and %d outputs are too many for one call", p.rows, p.outs);
     const int pairs = (int)min(tiles, (long long)ctx().sms / 2);
@@ -634,24 +681,29 @@ bool stream_launch(LinArgs &p, const tcg_mx_t &x, const tcg_mx_t &w)
     CUtensorMap mw, mx;
     if (!encode_mx(&mw, w, TILE_N, BITS == 8) || !encode_mx(&mx, x, BN, false)) return false;
     p.tiles_n = (p.outs + TILE_N - 1) / TILE_N;
-    p.stages_k = (p.atoms + Fmt<BITS>::ATOMS - 1) / Fmt<BITS>::ATOMS;
+    p.stages_k = (p.atoms + S::ATOMS - 1) / S::ATOMS;
     const long long tiles = (long long)p.tiles_n * ((p.rows + BN - 1) / BN);
     p.split = 1;
-    while (p.split < MAX_SPLIT && tiles * (p.split + 1) <= ctx().sms + ctx().sms / 8 && p.split * 4 < p.stages_k) p.split++;
+    while (p.split < MAX_SPLIT && tiles * (p.split + 1) <= ctx().sms && (p.split + 1) * MIN_STAGES <= p.stages_k) p.split++;
     p.per = (p.stages_k + p.split - 1) / p.split;
     p.split = (p.stages_k + p.per - 1) / p.per;
-    // accumulators of at most 1024 (512) columns, as many as TMEM holds
-    p.acc_stages = max((p.per + S::MAX_ACC - 1) / S::MAX_ACC, 4);
-    const int room = 200 * 1024 / (BN <= 32 ? 2 : 1), part = p.split > 1 ? BN * TILE_N * 4 : 0;
-    p.depth = min(16, min(max(p.per, 2), room / S::STAGE));
-    const size_t smem = 1024 + max(p.depth * S::STAGE, part);
+    // fp32 results: accumulators of SUM_K columns
+    p.acc_stages = p.type == GGML_TYPE_F32 ? max((p.per + S::MAX_ACC - 1) / S::MAX_ACC, SUM_K / S::K) : p.per;
+    // Half an SM's shared memory a CTA: one wave leaves room for the next kernel's CTAs to start in (one token 4096 -> 14336
+    // in 4 bits 7.2 us, with all of it 8.3), several waves run two CTAs an SM (60000 outputs 27 us, with one CTA 36). Not
+    // where that leaves fewer than four stages of one wave: 14336 -> 4096 in 8 bits 8.6 us, with half 11.4.
+    const bool half = BN <= 32 && (tiles * p.split > ctx().sms || 4 * S::STAGE + 16 * 1024 <= HALF_SM);
+    const int room = half ? HALF_SM : 200 * 1024;
+    const int part = p.split > 1 ? p.split * ((BN / 4 + p.split - 1) / p.split) * TILE_N * 16 : 0;
+    p.depth = min(MAX_DEPTH, min(max(p.per, 2), (room - part) / S::STAGE));
+    const size_t smem = 1024 + p.depth * S::STAGE + part;
     if (tiles * p.split > 0x7fffffffll) return fail("tcg_mx_linear: %d rows and %d outputs are too many for one call", p.rows, p.outs);
     void (*fn)(const CUtensorMap, const CUtensorMap, const LinArgs) = mx_stream_kernel<BITS, BN>;
     TCG_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 512));
     cudaLaunchAttribute attrs[2];
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3((unsigned)(tiles * p.split));
-    lc.blockDim = dim3(128);
+    lc.blockDim = dim3(STREAM_THREADS);
     lc.dynamicSmemBytes = smem;
     lc.stream = ctx().cur;
     lc.attrs = attrs;
