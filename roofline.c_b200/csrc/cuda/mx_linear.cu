@@ -15,7 +15,7 @@ constexpr int HALF_SM = 108 * 1024;
 constexpr int SUM_K = 4096;             // columns that the tensor core sums before fp32 results are added up outside
 constexpr int TILE_N = 128;             // weight rows of a tile: the MMA's M, a TMEM lane each
 constexpr int MAX_SPLIT = 8;            // portable cluster size
-constexpr int MIN_STAGES = 2;           // of a CTA, where K is split: 4096 -> 1024 3.8 us, with 4 4.4, with 8 4.8
+constexpr int MIN_STAGES = 2;           // of a CTA, where K is split (one token 4096 -> 1024: 3.8 us, with 4 4.4, with 8 4.8)
 
 // What differs between rows in 4 and in 8 bits. A stage is 128 bytes of a row of x; the weights' 4-bit codes next to 8-bit
 // rows are spread by the copy itself to 16 bytes for 16 codes, as kind::mxf8f6f4 reads them.
@@ -156,7 +156,8 @@ struct Stream {
     static constexpr int MAX_ACC = SF_COL / BN;
 };
 
-// One tile of 128 weight rows x BN rows of x a cluster, its K dealt out to the cluster's CTAs. Warp 0 loads, warp 1 issues the
+// One tile of 128 weight rows x BN rows of x a cluster (a tile starts with a group of 128 rows of x, whose scales are four
+// TMEM columns: with BN < 128 there is one tile of rows), its K dealt out to the cluster's CTAs. Warp 0 loads, warp 1 issues the
 // products; then all of them take the results.
 template <int BITS, int BN>
 __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap mx,
@@ -229,7 +230,6 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
                 wait_for(full + 8 * (j % p.depth), (j / p.depth) & 1, abort, p.err, false);
     } else if (role == 1) {
         const uint32_t id = mx_idesc<BITS>(BN, TILE_N), sfa = tmem + S::SF_COL, sfb = sfa + 4 * S::ATOMS;
-        const uint32_t b_off = m0 % MX_ATOM / 32;           // the tile's first column of its group of 128 rows
         int slot = 0, phase = 0, in_acc = 0;
         uint32_t d = tmem;
         for (int k = 0; k < count; k++) {
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
                     const unsigned long long da = sdesc<128>(a + j / 4 * S::A1), db = sdesc<128>(b + j / 4 * S::B1);
                     if (atom < na)
                         mma_mx<BITS>(d, da + 2 * (j % 4), db + 2 * (j % 4), id | byte << 29 | byte << 4, sfa + 4 * atom,
-                                     sfb + 4 * atom + b_off, in_acc != 0 || j != 0);
+                                     sfb + 4 * atom, in_acc != 0 || j != 0);
                 }
                 mma_commit(empty + 8 * slot);
             }
@@ -674,17 +674,49 @@ bool pair_launch(LinArgs &p, const tcg_mx_t &x, const tcg_mx_t &w)
     return true;
 }
 
+// What a call takes, estimated: ns measured on a B200, as in
+//   rows, columns -> outputs, bits     stream            pair
+//   512, 4096 -> 4096, 4               8.9               11.3 us
+//   1000, 4096 -> 4096, 4              17.2              11.9
+//   200, 1100 -> 5003, 8               6.0               9.2
+//   200, 4096 -> 14336, 8              22.6              17.4
+//   200, 14336 -> 4096, 4              18.0 (split 2)    22.8
+// A stage of 256 columns; where K is split, the join takes 45 ns a row of the tile (70 rows of 4096 -> 4096 in 4 bits: 8.2 us
+// in four parts; 200 rows, two parts: 11.9, undivided 8.8).
+struct StreamPlan {
+    int split;
+    double ns;
+};
+template <int BITS>
+StreamPlan stream_plan(int rows, long long tiles, int stages, int bn)
+{
+    const double stage = BITS == 4 ? (bn <= 64 ? 250 : 310) : (bn <= 64 ? 400 : 460), join = 300 + 45 * min(bn, rows);
+    const double start = 3700 * (double)((tiles + ctx().sms - 1) / ctx().sms);
+    StreamPlan best = { 1, start + stages * stage * (double)((tiles + ctx().sms - 1) / ctx().sms) };
+    for (int s = 2; s <= MAX_SPLIT && tiles * s <= ctx().sms && s * MIN_STAGES <= stages; s++) {
+        const double ns = start + (stages + s - 1) / s * stage + join;
+        if (ns < best.ns) best = { s, ns };
+    }
+    return best;
+}
+template <int BITS>
+double pair_ns(long long tiles, int stages)
+{
+    const long long pairs = ctx().sms / 2, rounds = (tiles + pairs - 1) / pairs;
+    return 3700 + (double)rounds * (2100 + stages * (BITS == 4 ? 290 : 590));
+}
+
 template <int BITS, int BN>
 bool stream_launch(LinArgs &p, const tcg_mx_t &x, const tcg_mx_t &w)
 {
     using S = Stream<BITS, BN>;
+    if (BN < MX_ATOM && p.rows > BN) return fail("tcg_mx_linear: %d rows in tiles of %d", p.rows, BN);
     CUtensorMap mw, mx;
     if (!encode_mx(&mw, w, TILE_N, BITS == 8) || !encode_mx(&mx, x, BN, false)) return false;
     p.tiles_n = (p.outs + TILE_N - 1) / TILE_N;
     p.stages_k = (p.atoms + S::ATOMS - 1) / S::ATOMS;
     const long long tiles = (long long)p.tiles_n * ((p.rows + BN - 1) / BN);
-    p.split = 1;
-    while (p.split < MAX_SPLIT && tiles * (p.split + 1) <= ctx().sms && (p.split + 1) * MIN_STAGES <= p.stages_k) p.split++;
+    p.split = stream_plan<BITS>(p.rows, tiles, p.stages_k, BN).split;
     p.per = (p.stages_k + p.split - 1) / p.split;
     p.split = (p.stages_k + p.per - 1) / p.per;
     // fp32 results: accumulators of SUM_K columns
@@ -722,7 +754,10 @@ bool linear_go(LinArgs &p, const tcg_mx_t &x, const tcg_mx_t &w)
     if (p.rows <= 16) return stream_launch<BITS, 16>(p, x, w);
     if (p.rows <= 32) return stream_launch<BITS, 32>(p, x, w);
     if (p.rows <= 64) return stream_launch<BITS, 64>(p, x, w);
-    if ((long long)((p.rows + 255) / 256) * ((p.outs + 255) / 256) >= ctx().sms / 4)
+    const int stages = (p.atoms + 1) / 2;
+    const long long wide = (long long)((p.rows + 255) / 256) * ((p.outs + 255) / 256);
+    const long long tiles = (long long)((p.rows + 127) / 128) * ((p.outs + 127) / 128);
+    if (pair_ns<BITS>(wide, stages) < stream_plan<BITS>(p.rows, tiles, stages, 128).ns)
         return lm_by_type((ggml_type_t)p.type, [&](auto v) { return pair_launch<decltype(v), BITS>(p, x, w); });
     return stream_launch<BITS, 128>(p, x, w);
 }
