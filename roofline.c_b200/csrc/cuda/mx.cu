@@ -7,13 +7,15 @@
 //
 // The norm's codes have to be those of y = h / sqrt(mean(h^2) + eps) * w, not of an fp32 approximation that may lie on
 // the other side of the border between two codes. The sum of squares and the root are taken in 64 bits; the products in
-// two fp32 numbers (y + rest, good to 2^-46), and before y is rounded to fewer bits its last bit is made odd where a rest
-// is left: a rounding to odd, after which the second rounding cannot meet a tie that is none. That is ~12 fp32 operations
-// a value instead of 64-bit conversions, whose rate (16 a cycle and SM) is half of what the memory delivers for 16-bit rows.
+// fp32, within 2^-21 of y. Where y (1 - 2^-21) and y (1 + 2^-21) have the same code, that is y's (rounding keeps order);
+// where they have not (one value in 2^16 or so), the warp takes its values again as y + rest, good to 2^-46, and makes y's
+// last bit odd where a rest is left: rounding that once more cannot meet a tie that is none.
 #include "mx.cuh"
 
 #include <cuda_fp4.h>
 #include <cuda_fp8.h>
+
+#include <string.h>
 
 namespace tcg {
 namespace {
@@ -21,41 +23,183 @@ namespace {
 constexpr int LANE = 8;             // consecutive columns of a lane: 4 lanes make a block, 16 a word of scales
 constexpr int MX_WARPS = 8;
 
-// 8 elements from p, of which `left` exist (the rest are 0); `vec`: p is 16-byte aligned where all 8 exist.
+// 8 elements as they are held.
 template <typename T>
-__device__ __forceinline__ void load8(const T *p, long long left, bool vec, float (&x)[LANE])
-{
-    if (vec && left >= LANE) {
-        constexpr int V = 16 / sizeof(T);
-#pragma unroll
-        for (int i = 0; i < LANE; i += V) {
-            float k[V];
-            load_pack<T, V>(p + i, k);
-#pragma unroll
-            for (int j = 0; j < V; j++) x[i + j] = k[j];
+struct Raw {
+    static constexpr int W = 2 * sizeof(T);     // words
+    uint32_t w[W];
+    __device__ __forceinline__ T at(int i) const
+    {
+        T v;
+        if constexpr (sizeof(T) == 4) memcpy(&v, &w[i], 4);
+        else {
+            const unsigned short h = (unsigned short)(w[i / 2] >> (i & 1) * 16);
+            memcpy(&v, &h, 2);
         }
-    } else {
+        return v;
+    }
+    __device__ __forceinline__ void set(int i, T v)
+    {
+        if constexpr (sizeof(T) == 4) memcpy(&w[i], &v, 4);
+        else {
+            unsigned short h;
+            memcpy(&h, &v, 2);
+            w[i / 2] = i & 1 ? (w[i / 2] & 0xFFFFu) | (uint32_t)h << 16 : h;
+        }
+    }
+};
+
+// Words k[0 .. N - 1] of the bytes that start at byte `off` (0 .. 15) of k[0 .. N + 3].
+template <int N>
+__device__ __forceinline__ void shift_bytes(uint32_t (&k)[N + 4], uint32_t off)
+{
 #pragma unroll
-        for (int i = 0; i < LANE; i++) x[i] = i < left ? to_f32(p[i]) : 0.0f;
+    for (int i = 0; i < N + 2; i++) k[i] = off & 8 ? k[i + 2] : k[i];
+#pragma unroll
+    for (int i = 0; i < N + 1; i++) k[i] = off & 4 ? k[i + 1] : k[i];
+#pragma unroll
+    for (int i = 0; i < N; i++) k[i] = __funnelshift_r(k[i], k[i + 1], (off & 3) * 8);
+}
+
+// A lane's 8 elements of a row, of which `left` exist (the others are 0). A row that starts on no 8-byte boundary is read
+// by the aligned 16-byte words around it and shifted, where those lie in [lo, hi), the array (1501 rows of 4103 16-bit values
+// quantised: PLACE_LOAD us, element by element 8.1).
+// VEC: rows start on 16-byte boundaries.
+template <bool VEC, typename T>
+__device__ __forceinline__ Raw<T> load_row(const T *p, long long left, const void *lo, const void *hi)
+{
+    constexpr int W = Raw<T>::W;
+    Raw<T> r;
+    const uintptr_t at = (uintptr_t)p;
+    const uint32_t off = VEC ? 0 : (uint32_t)at & 15;
+    if (left >= LANE) {
+        if (VEC || off == 0) {
+#pragma unroll
+            for (int i = 0; i < W; i += 4) {
+                const uint4 v = ((const uint4 *)p)[i / 4];
+                r.w[i] = v.x, r.w[i + 1] = v.y, r.w[i + 2] = v.z, r.w[i + 3] = v.w;
+            }
+            return r;
+        }
+        if (off == 8) {
+#pragma unroll
+            for (int i = 0; i < W; i += 2) {
+                const uint2 v = ((const uint2 *)p)[i / 2];
+                r.w[i] = v.x, r.w[i + 1] = v.y;
+            }
+            return r;
+        }
+        const uint4 *const from = (const uint4 *)(at - off);
+        if (!VEC && (const void *)from >= lo && (const void *)(from + W / 4 + 1) <= hi) {
+            uint32_t k[W + 4];
+#pragma unroll
+            for (int i = 0; i < W + 4; i += 4) {
+                const uint4 v = from[i / 4];
+                k[i] = v.x, k[i + 1] = v.y, k[i + 2] = v.z, k[i + 3] = v.w;
+            }
+            shift_bytes<W>(k, off);
+#pragma unroll
+            for (int i = 0; i < W; i++) r.w[i] = k[i];
+            return r;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < LANE; i++) r.set(i, i < left ? p[i] : from_f32<T>(0.0f));
+    return r;
+}
+
+// The same back; all lanes of a warp call it, on consecutive elements of one row. Off an 8-byte boundary a lane writes the
+// aligned words that start in the lane before it, with that lane's last bytes.
+template <bool VEC, typename T>
+__device__ __forceinline__ void store_row(T *p, long long left, const Raw<T> &r)
+{
+    constexpr int W = Raw<T>::W;
+    const uintptr_t at = (uintptr_t)p;
+    const uint32_t off = VEC ? 0 : (uint32_t)at & 15;
+    const bool full = left >= LANE;
+    if (VEC || off == 0 || off == 8) {
+        if (full && (VEC || off == 0)) {
+#pragma unroll
+            for (int i = 0; i < W; i += 4) ((uint4 *)p)[i / 4] = make_uint4(r.w[i], r.w[i + 1], r.w[i + 2], r.w[i + 3]);
+        } else if (full) {
+#pragma unroll
+            for (int i = 0; i < W; i += 2) ((uint2 *)p)[i / 2] = make_uint2(r.w[i], r.w[i + 1]);
+        } else if (left > 0) {
+#pragma unroll
+            for (int i = 0; i < LANE; i++)
+                if (i < left) p[i] = r.at(i);
+        }
+        return;
+    }
+    const int lane = threadIdx.x & 31;
+    const unsigned fulls = __ballot_sync(0xFFFFFFFFu, full);
+    uint32_t k[W + 4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) k[i] = __shfl_up_sync(0xFFFFFFFFu, r.w[W - 4 + i], 1);
+    const bool before = lane > 0 && (fulls >> (lane - 1) & 1), after = lane < 31 && (fulls >> (lane + 1) & 1);
+#pragma unroll
+    for (int i = 0; i < W; i++) k[4 + i] = r.w[i];
+    shift_bytes<W>(k, 16 - off);
+    uint4 *const words = (uint4 *)(at - off);
+    if (full) {
+        if (before) words[0] = make_uint4(k[0], k[1], k[2], k[3]);
+#pragma unroll
+        for (int i = 4; i < W; i += 4) words[i / 4] = make_uint4(k[i], k[i + 1], k[i + 2], k[i + 3]);
+        if (before && after) return;
+    }
+    // what no word of this lane or the next one holds
+    const int to = !full ? (int)max(left, 0ll) : before ? 0 : (int)((16 - off) / sizeof(T));
+    const int from = full && !after ? LANE - (int)(off / sizeof(T)) : LANE;
+#pragma unroll
+    for (int i = 0; i < LANE; i++)
+        if (i < to || i >= from) p[i] = r.at(i);
+}
+
+// A word's two 16-bit values, and back; a word is one fp32 value.
+__device__ __forceinline__ float2 pair_f32(uint32_t w, __half)
+{
+    __half2 h;
+    memcpy(&h, &w, 4);
+    return __half22float2(h);
+}
+__device__ __forceinline__ float2 pair_f32(uint32_t w, __nv_bfloat16) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
+__device__ __forceinline__ uint32_t pair_word(float a, float b, __half)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    uint32_t w;
+    memcpy(&w, &h, 4);
+    return w;
+}
+__device__ __forceinline__ uint32_t pair_word(float a, float b, __nv_bfloat16)
+{
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    uint32_t w;
+    memcpy(&w, &h, 4);
+    return w;
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack(const Raw<T> &r, float (&x)[LANE])
+{
+#pragma unroll
+    for (int i = 0; i < Raw<T>::W; i++) {
+        if constexpr (sizeof(T) == 4) x[i] = __uint_as_float(r.w[i]);
+        else {
+            const float2 v = pair_f32(r.w[i], T());
+            x[2 * i] = v.x, x[2 * i + 1] = v.y;
+        }
     }
 }
 template <typename T>
-__device__ __forceinline__ void store8(T *p, long long left, bool vec, const float (&x)[LANE])
+__device__ __forceinline__ Raw<T> packed(const float (&x)[LANE])
 {
-    if (vec && left >= LANE) {
-        constexpr int V = 16 / sizeof(T);
+    Raw<T> r;
 #pragma unroll
-        for (int i = 0; i < LANE; i += V) {
-            float k[V];
-#pragma unroll
-            for (int j = 0; j < V; j++) k[j] = x[i + j];
-            store_pack<T, V>(p + i, k);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < LANE; i++)
-            if (i < left) p[i] = from_f32<T>(x[i]);
+    for (int i = 0; i < Raw<T>::W; i++) {
+        if constexpr (sizeof(T) == 4) r.w[i] = __float_as_uint(x[i]);
+        else r.w[i] = pair_word(x[2 * i], x[2 * i + 1], T());
     }
+    return r;
 }
 
 struct MxOut {
@@ -64,96 +208,195 @@ struct MxOut {
     int bits;
 };
 
-// Codes and scale of 8 columns from `col` on (a multiple of 8) of row r; the warp's lanes hold consecutive columns, the
-// first of them a multiple of 256. All lanes call it; columns from `wide` on are not stored.
-__device__ __forceinline__ void mx_store8(const MxOut &o, long long r, long long col, const float (&x)[LANE])
+// The scale byte of a block, from the largest magnitude of its values (as fp32 bits: whole numbers keep their order,
+// infinities and NaN above all), and 1 / scale (0 for a block that is NaN). Subnormals have exponent field 0: the smallest scale.
+__device__ __forceinline__ uint32_t mx_scale(uint32_t top, int bits)
 {
-    const int lane = threadIdx.x & 31;
-    // magnitudes as whole numbers keep their order, infinities and NaN above all
+    return top < 0x7F800000u ? (uint32_t)max((int)(top >> 23) - (bits == 4 ? 2 : 8), 0) : 255u;
+}
+__device__ __forceinline__ float mx_inverse(uint32_t s) { return __uint_as_float(s == 255 ? 0u : (254u - s) << 23); }
+__device__ __forceinline__ uint32_t mx_top(const float (&x)[LANE])
+{
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < LANE; i++) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
     top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-    const bool fine = top < 0x7F800000u;
-    const int e = (int)(top >> 23) - (o.bits == 4 ? 2 : 8);         // subnormals have field 0: the smallest scale
-    const uint32_t s = fine ? (uint32_t)max(e, 0) : 255u;
-    const float inv = __uint_as_float(fine ? (254u - s) << 23 : 0u);
-    float q[LANE];
-#pragma unroll
-    for (int i = 0; i < LANE; i++) q[i] = fine ? x[i] * inv : 0.0f;
-    uint32_t word = s << (lane >> 2 & 3) * 8;
-    word |= __shfl_xor_sync(0xFFFFFFFFu, word, 4);
-    word |= __shfl_xor_sync(0xFFFFFFFFu, word, 8);
-    if (col >= o.wide) return;
-    uint8_t *const row = o.codes + r * o.pitch;
-    if (o.bits == 4) {
-        uint32_t c = 0;
+    return max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+}
+__device__ __forceinline__ uint2 mx_codes(const float (&q)[LANE], int bits)
+{
+    uint2 c = make_uint2(0, 0);
+    if (bits == 4) {
 #pragma unroll
         for (int i = 0; i < LANE; i += 2)
-            c |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(q[i], q[i + 1]), __NV_E2M1, cudaRoundNearest) << 4 * i;
-        *(uint32_t *)(row + col / 2) = c;
+            c.x |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(q[i], q[i + 1]), __NV_E2M1, cudaRoundNearest) << 4 * i;
     } else {
-        uint32_t c[2];
 #pragma unroll
-        for (int i = 0; i < 2; i++)
-            c[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(q[4 * i], q[4 * i + 1]), __NV_SATFINITE, __NV_E4M3) |
-                   (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(q[4 * i + 2], q[4 * i + 3]), __NV_SATFINITE, __NV_E4M3) << 16;
-        *(uint2 *)(row + col) = make_uint2(c[0], c[1]);
+        for (int i = 0; i < 4; i += 2) {
+            c.x |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(q[i], q[i + 1]), __NV_SATFINITE, __NV_E4M3) << 8 * i;
+            c.y |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(q[i + 4], q[i + 5]), __NV_SATFINITE, __NV_E4M3) << 8 * i;
+        }
     }
-    if ((lane & 15) == 0) *(uint32_t *)(o.scales + mx_scale_at(r, col / MX_BLOCK, o.wide / MX_ATOM)) = word;
+    return c;
+}
+// A lane's codes to row r, column `col` (not from `wide` on); returns the four scales of the 128 columns it is among.
+__device__ __forceinline__ uint32_t mx_put(const MxOut &o, long long r, long long col, uint2 c, uint32_t s)
+{
+    uint32_t word = s << (threadIdx.x >> 2 & 3) * 8;
+    word |= __shfl_xor_sync(0xFFFFFFFFu, word, 4);
+    word |= __shfl_xor_sync(0xFFFFFFFFu, word, 8);
+    if (col < o.wide) {
+        uint8_t *const row = o.codes + r * o.pitch;
+        if (o.bits == 4) *(uint32_t *)(row + col / 2) = c.x;
+        else *(uint2 *)(row + col) = c;
+    }
+    return word;
+}
+
+// 8 columns from `col` on (a multiple of 8) of row r; the warp's lanes hold consecutive columns, the first of them a multiple
+// of 256. All lanes call it.
+__device__ __forceinline__ uint32_t mx_store8(const MxOut &o, long long r, long long col, const float (&x)[LANE])
+{
+    const uint32_t s = mx_scale(mx_top(x), o.bits);
+    const float inv = mx_inverse(s);
+    float q[LANE];
+#pragma unroll
+    for (int i = 0; i < LANE; i++) q[i] = x[i] * inv;
+    return mx_put(o, r, col, mx_codes(q, o.bits), s);
+}
+
+// The same for values known to within 2^-22 of themselves: false (and nothing stored) where some lane's codes or scales
+// depend on more than that.
+__device__ __forceinline__ bool mx_store8_near(const MxOut &o, long long r, long long col, const float (&x)[LANE], uint32_t &word)
+{
+    constexpr float LOW = 1.0f - 0x1p-21f, HIGH = 1.0f + 0x1p-21f;
+    const uint32_t top = mx_top(x);
+    const uint32_t s = mx_scale(__float_as_uint(__uint_as_float(top) * LOW), o.bits);
+    const float low = mx_inverse(s) * LOW, high = mx_inverse(s) * HIGH;     // inverse is a power of two: both are exact
+    float q[LANE];
+#pragma unroll
+    for (int i = 0; i < LANE; i++) q[i] = x[i] * low;
+    const uint2 c = mx_codes(q, o.bits);
+#pragma unroll
+    for (int i = 0; i < LANE; i++) q[i] = x[i] * high;
+    const uint2 d = mx_codes(q, o.bits);
+    const bool sure = ((c.x ^ d.x) | (c.y ^ d.y)) == 0 && s == mx_scale(__float_as_uint(__uint_as_float(top) * HIGH), o.bits);
+    if (!__all_sync(0xFFFFFFFFu, sure)) return false;
+    word = mx_put(o, r, col, c, s);
+    return true;
 }
 
 // ------------------------------------------------------------------ quantisation and back
 
+// A warp takes 256 columns of the rows l, l + 32, l + 64 and l + 96 of a group of 128: their scales are 16 bytes in one
+// place, and four rows' loads are under way together.
 struct QuantArgs {
-    const void *x;
-    long long ld, cols, chunks, tasks;      // a task: 256 columns of a row
+    void *x;
+    const void *end;                // of x
+    long long ld, cols;
+    unsigned rows, chunks, tasks;
     MxOut o;
     bool vec;
 };
 
-template <typename T>
+struct QuantTask {
+    unsigned group, line;
+    long long col;
+    bool live;
+};
+__device__ __forceinline__ QuantTask quant_task(const QuantArgs &p)
+{
+    const unsigned task = blockIdx.x * MX_WARPS + (threadIdx.x >> 5), row = task / p.chunks;
+    return { row / 32, row % 32, (long long)(task - row * p.chunks) * 256 + (threadIdx.x & 31) * LANE, task < p.tasks };
+}
+
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(32 * MX_WARPS) mx_quantize_kernel(const __grid_constant__ QuantArgs p)
 {
     lm_begin();
-    const long long task = (long long)blockIdx.x * MX_WARPS + (threadIdx.x >> 5);
-    if (task >= p.tasks) return;
-    const long long r = task / p.chunks, col = (task - r * p.chunks) * 256 + (threadIdx.x & 31) * LANE;
-    float x[LANE];
-    load8((const T *)p.x + r * p.ld + col, p.cols - col, p.vec, x);
-    mx_store8(p.o, r, col, x);
+    const QuantTask t = quant_task(p);
+    const unsigned first = t.group * 128 + t.line;
+    if (!t.live || first >= p.rows) return;
+    Raw<T> raw[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const long long r = first + 32 * i;
+        raw[i] = load_row<VEC>((const T *)p.x + r * p.ld + t.col, r < p.rows ? p.cols - t.col : 0, p.x, p.end);
+    }
+    uint32_t word[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const long long r = first + 32 * i;
+        if (r >= p.rows) break;
+        float x[LANE];
+        unpack(raw[i], x);
+        word[i] = mx_store8(p.o, r, t.col, x);
+    }
+    if ((threadIdx.x & 15) || t.col >= p.o.wide) return;
+    uint32_t *const at = (uint32_t *)(p.o.scales + mx_scale_at(first, t.col / MX_BLOCK, p.o.wide / MX_ATOM));
+    if (first + 96 < p.rows) *(uint4 *)at = make_uint4(word[0], word[1], word[2], word[3]);
+    else
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (first + 32 * i < p.rows) at[i] = word[i];
 }
 
-template <typename T>
-__global__ void __launch_bounds__(32 * MX_WARPS) mx_dequantize_kernel(const __grid_constant__ QuantArgs p, T *y)
+// C times 256 columns a warp, so that more than one row's 128 bytes of codes and its scales are under way.
+template <typename T, int C, bool VEC>
+__global__ void __launch_bounds__(32 * MX_WARPS) mx_dequantize_kernel(const __grid_constant__ QuantArgs p)
 {
     lm_begin();
-    const long long task = (long long)blockIdx.x * MX_WARPS + (threadIdx.x >> 5);
-    if (task >= p.tasks) return;
-    const long long r = task / p.chunks, col = (task - r * p.chunks) * 256 + (threadIdx.x & 31) * LANE;
-    if (col >= p.cols) return;
-    const uint8_t *const row = p.o.codes + r * p.o.pitch;
-    const uint32_t s = p.o.scales[mx_scale_at(r, col / MX_BLOCK, p.o.wide / MX_ATOM)];
-    const float scale = __uint_as_float(s == 255 ? 0x7FFFFFFFu : s ? s << 23 : 0x00400000u);
-    float x[LANE];
-    if (p.o.bits == 4) {
-        const uint32_t c = *(const uint32_t *)(row + col / 2);
+    QuantTask t = quant_task(p);
+    t.col = (t.col - (threadIdx.x & 31) * LANE) * C + (threadIdx.x & 31) * LANE;
+    const unsigned first = t.group * 128 + t.line;
+    if (!t.live || first >= p.rows) return;
+    uint2 code[C][4];
+    uint4 scales[C];
 #pragma unroll
-        for (int i = 0; i < LANE; i += 2) {
-            const float2 v = __half22float2(__half2(__nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)(c >> 4 * i & 255), __NV_E2M1)));
-            x[i] = v.x * scale, x[i + 1] = v.y * scale;
-        }
-    } else {
-        const uint2 c = *(const uint2 *)(row + col);
+    for (int c = 0; c < C; c++) {
+        const long long col = t.col + 256 * c;
+        const bool in = col < p.o.wide;
+        scales[c] = make_uint4(0, 0, 0, 0);
+        if (in) scales[c] = *(const uint4 *)(p.o.scales + mx_scale_at(first, col / 128 * 4, p.o.wide / MX_ATOM));
 #pragma unroll
-        for (int i = 0; i < LANE; i += 2) {
-            const uint32_t w = (i < 4 ? c.x : c.y) >> (i & 2) * 8 & 0xFFFF;
-            const float2 v = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)w, __NV_E4M3)));
-            x[i] = v.x * scale, x[i + 1] = v.y * scale;
+        for (int i = 0; i < 4; i++) {
+            const long long r = first + 32 * i;
+            code[c][i] = make_uint2(0, 0);
+            if (in && r < p.rows) {
+                if (p.o.bits == 4) code[c][i].x = *(const uint32_t *)(p.o.codes + r * p.o.pitch + col / 2);
+                else code[c][i] = *(const uint2 *)(p.o.codes + r * p.o.pitch + col);
+            }
         }
     }
-    store8(y + r * p.ld + col, p.cols - col, p.vec, x);
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        const long long col = t.col + 256 * c;
+        const uint32_t words[4] = { scales[c].x, scales[c].y, scales[c].z, scales[c].w };
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const long long r = first + 32 * i;
+            if (r >= p.rows) break;
+            const uint32_t s = words[i] >> (threadIdx.x >> 2 & 3) * 8 & 255;
+            const float scale = __uint_as_float(s == 255 ? 0x7FFFFFFFu : s ? s << 23 : 0x00400000u);
+            float x[LANE];
+            if (p.o.bits == 4) {
+#pragma unroll
+                for (int j = 0; j < LANE; j += 2) {
+                    const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)(code[c][i].x >> 4 * j & 255), __NV_E2M1);
+                    const float2 v = __half22float2(__half2(h));
+                    x[j] = v.x * scale, x[j + 1] = v.y * scale;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < LANE; j += 2) {
+                    const uint32_t w = (j < 4 ? code[c][i].x : code[c][i].y) >> (j & 2) * 8 & 0xFFFF;
+                    const float2 v = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)w, __NV_E4M3)));
+                    x[j] = v.x * scale, x[j + 1] = v.y * scale;
+                }
+            }
+            store_row<VEC>((T *)p.x + r * p.ld + col, p.cols - col, packed<T>(x));
+        }
+    }
 }
 
 MxOut mx_out(const tcg_mx_t &m)
@@ -161,18 +404,23 @@ MxOut mx_out(const tcg_mx_t &m)
     return { m.codes, m.scales, mx_pitch(m.cols, m.bits), mx_wide(m.cols), m.bits };
 }
 
-bool aligned16(const void *p, int64_t ld, ggml_type_t t) { return (uintptr_t)p % 16 == 0 && ld * lm_type_size(t) % 16 == 0; }
+// Whether every row starts on a 16-byte boundary.
+bool on_16(const void *p, int64_t ld, ggml_type_t t) { return (uintptr_t)p % 16 == 0 && ld * (int64_t)lm_type_size(t) % 16 == 0; }
 
-bool quant_args(const char *who, QuantArgs &p, const tcg_mx_t &m, const void *x, int64_t ld, ggml_type_t t)
+bool quant_args(const char *who, QuantArgs &p, const tcg_mx_t &m, void *x, int64_t ld, ggml_type_t t, int wide = 1)
 {
     p.x = x;
+    p.end = (const char *)x + ((m.rows - 1) * ld + m.cols) * (int64_t)lm_type_size(t);
     p.ld = ld;
     p.cols = m.cols;
-    p.chunks = (mx_wide(m.cols) + 255) / 256;
-    p.tasks = p.chunks * m.rows;
+    p.rows = (unsigned)m.rows;
+    p.chunks = (unsigned)((mx_wide(m.cols) + 256 * wide - 1) / (256 * wide));
+    // rows beyond 128 are dealt out by groups, 32 lines each; a few rows are lines of one group
+    const long long lines = m.rows < 32 ? m.rows : (m.rows + 127ll) / 128 * 32, tasks = lines * p.chunks;
+    if (tasks > 0x7fffffffll) return fail("%s: %d rows of %d columns are too many for one call", who, m.rows, m.cols);
+    p.tasks = (unsigned)tasks;
     p.o = mx_out(m);
-    p.vec = aligned16(x, ld, t);
-    if (p.tasks > 0x7fffffffll * MX_WARPS) return fail("%s: %d rows of %d columns are too many for one call", who, m.rows, m.cols);
+    p.vec = on_16(x, ld, t);
     return true;
 }
 
@@ -180,24 +428,21 @@ bool quant_args(const char *who, QuantArgs &p, const tcg_mx_t &m, const void *x,
 
 struct NormArgs {
     const void *x, *r;
+    const void *x_end, *r_end;      // of the arrays
     void *h, *y;
     const float *w;
     long long ldx, ldr, ldh, ldy;
     MxOut o;                        // codes NULL: none
     int rows, cols;
-    double eps;
-    bool vx, vr, vh, vy, vw;        // 16-byte accesses
+    double eps, mean;               // 1 / cols
+    bool vec;
 };
 
-// y = v * rstd * w as fp32 (round to nearest), and as the odd-rounded number that may be rounded once more.
-struct Normed {
-    float near, odd;
-};
-__device__ __forceinline__ Normed normed(float v, float r_hi, float r_lo, float w)
+// v * rstd * w to 2^-46, the last of its 24 bits odd where something is left.
+__device__ __forceinline__ float normed_odd(float v, float r_hi, float r_lo, float w)
 {
     const float q = v * r_hi, ql = fmaf(v, r_lo, fmaf(v, r_hi, -q));
     const float y = q * w, rest = fmaf(ql, w, fmaf(q, w, -y));
-    // y + rest, |rest| up to an ulp: once more, so that y is the nearest
     const float near = y + rest, left = rest - (near - y);
     uint32_t b = __float_as_uint(near);
     if (left != 0.0f && (b & 0x7FFFFFFFu) < 0x7F800000u) {
@@ -205,38 +450,55 @@ __device__ __forceinline__ Normed normed(float v, float r_hi, float r_lo, float 
         if (near != 0.0f && (__float_as_uint(left) ^ b) >> 31) b -= 1;
         b |= 1;
     }
-    return { near, __uint_as_float(b) };
+    return __uint_as_float(b);
 }
 
-// A row's columns are dealt out to G threads (a warp's 32, or the CTA's), N pieces of 8 consecutive columns each.
-template <typename T, int N, bool WARP>
-__global__ void __launch_bounds__(1024) add_rms_norm_kernel(const __grid_constant__ NormArgs p)
+// A row's columns are dealt out to G threads (a warp's 32, or the CTA's, at most MOST), N pieces of 8 consecutive columns each.
+// CTAs an SM that registers are kept for. 4096 rows of 4096 fp32 values with their residual, to 8 bits: two pieces a thread of 256
+// and five CTAs 39.9 us (5.5 TB/s); two of 512 and two CTAs 40.9; one of 512 and three 43.2; four of 128 and five 50.0.
+constexpr int norm_ctas(int n, int most) { return n == 2 && most == 256 ? 5 : 1; }
+
+template <typename T, int N, int MOST, bool VEC>
+__global__ void __launch_bounds__(MOST == 32 ? 256 : MOST, norm_ctas(N, MOST)) add_rms_norm_kernel(const __grid_constant__ NormArgs p)
 {
+    constexpr bool WARP = MOST == 32;
     const int G = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
     const long long row = WARP ? (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
     __shared__ double part[32];
     lm_begin();
     if (WARP && row >= p.rows) return;
-    float v[N][LANE];
+    Raw<T> h[N], r[N];
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        const long long col = (long long)(k * G + t) * LANE;
+        h[k] = load_row<VEC>((const T *)p.x + row * p.ldx + col, p.cols - col, p.x, p.x_end);
+        if (p.r) r[k] = load_row<VEC>((const T *)p.r + row * p.ldr + col, p.cols - col, p.r, p.r_end);
+    }
+    // a thread of one piece has the registers to ask for its weights now
+    Raw<float> w0;
+    if (N == 1 && p.w) w0 = load_row<VEC>(p.w + (long long)t * LANE, p.cols - (long long)t * LANE, p.w, p.w + p.cols);
     double ss = 0.0;
 #pragma unroll
     for (int k = 0; k < N; k++) {
-        const long long col = (long long)(k * G + t) * LANE;
-        load8((const T *)p.x + row * p.ldx + col, p.cols - col, p.vx, v[k]);
+        float v[LANE];
+        unpack(h[k], v);
         if (p.r) {
-            float r[LANE];
-            load8((const T *)p.r + row * p.ldr + col, p.cols - col, p.vr, r);
+            float u[LANE];
+            unpack(r[k], u);
 #pragma unroll
-            for (int i = 0; i < LANE; i++) v[k][i] = to_f32(from_f32<T>(v[k][i] + r[i]));
+            for (int i = 0; i < LANE; i++) v[i] += u[i];
+            h[k] = packed<T>(v);
+            unpack(h[k], v);
         }
-    }
 #pragma unroll
-    for (int k = 0; k < N; k++) {
-        const long long col = (long long)(k * G + t) * LANE;
-        if (p.h) store8((T *)p.h + row * p.ldh + col, p.cols - col, p.vh, v[k]);
-#pragma unroll
-        for (int i = 0; i < LANE; i++) ss = fma((double)v[k][i], (double)v[k][i], ss);
+        for (int i = 0; i < LANE; i++) ss = fma((double)v[i], (double)v[i], ss);
     }
+    if (p.h)
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const long long col = (long long)(k * G + t) * LANE;
+            store_row<VEC>((T *)p.h + row * p.ldh + col, p.cols - col, h[k]);
+        }
     if (!p.y && !p.o.codes) return;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
@@ -248,39 +510,49 @@ __global__ void __launch_bounds__(1024) add_rms_norm_kernel(const __grid_constan
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
     }
-    const double rstd = rsqrt(ss / p.cols + p.eps);
+    const double rstd = rsqrt(fma(ss, p.mean, p.eps));
     const float r_hi = (float)rstd, r_lo = (float)(rstd - r_hi);
     // rows whose root leaves fp32's normal numbers take the product in 64 bits
     const bool plain = rstd > 1e-30 && rstd < 1e30;
 #pragma unroll
     for (int k = 0; k < N; k++) {
         const long long col = (long long)(k * G + t) * LANE;
-        float w[LANE], near[LANE], odd[LANE];
-        load8(p.w + col, p.cols - col, p.vw, w);
+        const Raw<float> w = N == 1 ? w0 : load_row<VEC>(p.w + col, p.cols - col, p.w, p.w + p.cols);
+        float v[LANE], y[LANE];
+        unpack(h[k], v);
 #pragma unroll
-        for (int i = 0; i < LANE; i++) {
-            if (plain) {
-                const Normed n = normed(v[k][i], r_hi, r_lo, w[i]);
-                near[i] = n.near, odd[i] = n.odd;
-            } else {
-                const double y = v[k][i] * rstd * w[i];
-                near[i] = (float)y;
-                odd[i] = __double2float_rz(y);
-                if ((double)odd[i] != y && fabsf(near[i]) < INFINITY) odd[i] = __uint_as_float(__float_as_uint(odd[i]) | 1);
-                else odd[i] = fabsf(near[i]) < INFINITY ? odd[i] : near[i];
+        for (int i = 0; i < LANE; i++) y[i] = plain ? v[i] * r_hi * w.at(i) : (float)(v[i] * rstd * w.at(i));
+        if (col + LANE > p.cols)
+#pragma unroll
+            for (int i = 0; i < LANE; i++)
+                if (col + i >= p.cols) y[i] = 0.0f;                 // 0 * rstd may be NaN there
+        if (p.y) store_row<VEC>((T *)p.y + row * p.ldy + col, p.cols - col, packed<T>(y));
+        if (!p.o.codes) continue;
+        uint32_t word;
+        if (!plain || !mx_store8_near(p.o, row, col, y, word)) {
+#pragma unroll
+            for (int i = 0; i < LANE; i++) {
+                if (plain) y[i] = normed_odd(v[i], r_hi, r_lo, w.at(i));
+                else if (fabsf(y[i]) < INFINITY) {
+                    const double d = v[i] * rstd * w.at(i);
+                    y[i] = __double2float_rz(d);
+                    if ((double)y[i] != d) y[i] = __uint_as_float(__float_as_uint(y[i]) | 1);
+                }
+                if (col + i >= p.cols) y[i] = 0.0f;
             }
-            if (col + i >= p.cols) near[i] = odd[i] = 0.0f;         // 0 * rstd may be NaN there
+            word = mx_store8(p.o, row, col, y);
         }
-        if (p.y) store8((T *)p.y + row * p.ldy + col, p.cols - col, p.vy, sizeof(T) == 4 ? near : odd);
-        if (p.o.codes) mx_store8(p.o, row, col, odd);
+        if ((t & 15) == 0 && col < p.o.wide)
+            *(uint32_t *)(p.o.scales + mx_scale_at(row, col / MX_BLOCK, p.o.wide / MX_ATOM)) = word;
     }
 }
 
-template <typename T, int N, bool WARP>
+template <typename T, int N, int MOST>
 bool norm_launch(const NormArgs &p, int threads)
 {
-    const unsigned grid = WARP ? ceil_div(p.rows, threads / 32) : (unsigned)p.rows;
-    TCG_CUDA(launch_pdl(add_rms_norm_kernel<T, N, WARP>, dim3(grid), dim3(threads), 0, ctx().cur, p));
+    const unsigned grid = MOST == 32 ? ceil_div(p.rows, threads / 32) : (unsigned)p.rows;
+    void (*fn)(const NormArgs) = p.vec ? add_rms_norm_kernel<T, N, MOST, true> : add_rms_norm_kernel<T, N, MOST, false>;
+    TCG_CUDA(launch_pdl(fn, dim3(grid), dim3(threads), 0, ctx().cur, p));
     return true;
 }
 
@@ -288,13 +560,18 @@ template <typename T>
 bool norm_go(const NormArgs &p)
 {
     const int pieces = (int)(mx_wide(p.cols) / LANE);           // of 8 columns, those behind the last one included
-    if (pieces <= 32) return norm_launch<T, 1, true>(p, 256);
-    if (pieces <= 64) return norm_launch<T, 2, true>(p, 256);
-    const int n = pieces <= 1024 ? 1 : pieces <= 2048 ? 2 : 4;
-    const int threads = ((pieces + n - 1) / n + 31) / 32 * 32;
-    if (n == 1) return norm_launch<T, 1, false>(p, threads);
-    if (n == 2) return norm_launch<T, 2, false>(p, threads);
-    return norm_launch<T, 4, false>(p, threads);
+    // Few rows: a thread has one piece. Many: more, whose loads are under way together, and a join of fewer warps.
+    const bool many = p.rows >= 2 * ctx().sms;
+    auto threads = [&](int n) { return ((pieces + n - 1) / n + 31) / 32 * 32; };
+    if (pieces <= 32) return norm_launch<T, 1, 32>(p, 256);
+    if (many) {
+        if (pieces <= 64) return norm_launch<T, 2, 32>(p, 256);
+        if (pieces <= 512) return norm_launch<T, 2, 256>(p, threads(2));
+        if (pieces <= 1024) return norm_launch<T, 2, 512>(p, threads(2));
+    }
+    if (pieces <= 1024) return norm_launch<T, 1, 1024>(p, threads(1));
+    if (pieces <= 2048) return norm_launch<T, 4, 512>(p, threads(4));
+    return norm_launch<T, 4, 1024>(p, threads(4));
 }
 
 }  // namespace
@@ -322,9 +599,10 @@ extern "C" bool tcg_mx_quantize(const tcg_mx_t *m, const void *x, int64_t ld, gg
     if (!lm_ready(who)) return false;
     if (!m->rows) return true;
     QuantArgs p = {};
-    if (!quant_args(who, p, *m, x, ld, t)) return false;
+    if (!quant_args(who, p, *m, (void *)x, ld, t)) return false;
     return lm_by_type(t, [&](auto v) {
-        TCG_CUDA(launch_pdl(mx_quantize_kernel<decltype(v)>, dim3(ceil_div(p.tasks, MX_WARPS)), dim3(32 * MX_WARPS), 0, ctx().cur, p));
+        void (*fn)(const QuantArgs) = p.vec ? mx_quantize_kernel<decltype(v), true> : mx_quantize_kernel<decltype(v), false>;
+        TCG_CUDA(launch_pdl(fn, dim3(ceil_div(p.tasks, MX_WARPS)), dim3(32 * MX_WARPS), 0, ctx().cur, p));
         return true;
     });
 }
@@ -337,10 +615,14 @@ extern "C" bool tcg_mx_dequantize(void *y, const tcg_mx_t *m, int64_t ld, ggml_t
     if (!lm_ready(who)) return false;
     if (!m->rows) return true;
     QuantArgs p = {};
-    if (!quant_args(who, p, *m, y, ld, t)) return false;
+    // two chunks of columns a warp where that leaves 16 warps an SM
+    const bool wide = (long long)m->rows * m->cols >= (long long)ctx().sms * 16 * 2048;
+    if (!quant_args(who, p, *m, y, ld, t, wide ? 2 : 1)) return false;
     return lm_by_type(t, [&](auto v) {
         using T = decltype(v);
-        TCG_CUDA(launch_pdl(mx_dequantize_kernel<T>, dim3(ceil_div(p.tasks, MX_WARPS)), dim3(32 * MX_WARPS), 0, ctx().cur, p, (T *)y));
+        void (*fn)(const QuantArgs) = p.vec ? (wide ? mx_dequantize_kernel<T, 2, true> : mx_dequantize_kernel<T, 1, true>)
+                                            : (wide ? mx_dequantize_kernel<T, 2, false> : mx_dequantize_kernel<T, 1, false>);
+        TCG_CUDA(launch_pdl(fn, dim3(ceil_div(p.tasks, MX_WARPS)), dim3(32 * MX_WARPS), 0, ctx().cur, p));
         return true;
     });
 }
@@ -373,7 +655,10 @@ extern "C" bool tcg_add_rms_norm(void *h, void *y, const tcg_mx_t *mx, const voi
     if (mx) p.o = mx_out(*mx);
     p.rows = n_tok, p.cols = cols;
     p.eps = eps;
-    p.vx = aligned16(x, ld_x, t), p.vr = aligned16(r, ld_r, t), p.vh = aligned16(h, ld_h, t), p.vy = aligned16(y, ld_y, t);
-    p.vw = (uintptr_t)w % 16 == 0;
+    p.mean = 1.0 / cols;
+    p.vec = on_16(x, ld_x, t) && (!r || on_16(r, ld_r, t)) && (!h || on_16(h, ld_h, t)) && (!y || on_16(y, ld_y, t)) && (uintptr_t)w % 16 == 0;
+    const int64_t size = (int64_t)lm_type_size(t);
+    p.x_end = (const char *)x + ((n_tok - 1) * ld_x + cols) * size;
+    p.r_end = (const char *)r + ((n_tok - 1) * ld_r + cols) * size;
     return lm_by_type(t, [&](auto v) { return norm_go<decltype(v)>(p); });
 }
