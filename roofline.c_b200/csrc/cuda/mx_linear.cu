@@ -4,6 +4,8 @@
 #include "tc05.cuh"
 
 #include <string.h>
+
+#include <atomic>
 #include <type_traits>
 
 namespace tcg {
@@ -11,7 +13,7 @@ namespace {
 
 constexpr int ERR_WAIT = TCG_ERR_MX_WAIT;
 constexpr int STREAM_THREADS = 256, MAX_DEPTH = 16;
-constexpr int HALF_SM = 108 * 1024;
+constexpr int HALF_SM = 108 * 1024, MOST_SMEM = 226 * 1024;     // of dynamic shared memory; the static part is below 1 KB
 constexpr int SUM_K = 4096;             // columns that the tensor core sums before fp32 results are added up outside
 constexpr int TILE_N = 128;             // weight rows of a tile: the MMA's M, a TMEM lane each
 constexpr int MAX_SPLIT = 8;            // portable cluster size
@@ -268,6 +270,15 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
     const uint32_t lane_base = tmem + ((uint32_t)(warp & 3) << 21);
     // Two warps share 32 TMEM lanes (weight rows) and take every second step of columns (x's rows).
     const int t = tid & 127, half = tid >> 7;
+    // Before any wait for a peer: a CTA that waits must hold no TMEM that another cluster's CTA on its SM, for which that
+    // cluster's other CTAs wait in turn, has asked for.
+    auto free_tmem = [&] {
+        fence_before();
+        __syncthreads();
+        if (warp != 0) return;
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::COLS) : "memory");
+    };
     auto finish = [&](auto type) {
         using T = decltype(type);
         // [split][ceil(BN / 4 / split)][128] words of four columns: by owner, over the stages (whose products are done), what
@@ -296,15 +307,16 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
                 put_columns<STEP, T>(p, m0 + c, n, bias, v);
             }
         }
-        if (p.split == 1) return;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncthreads();
+        free_tmem();
+        if (p.split == 1) return;
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");     // the peers' barriers are there
         if (tid < p.split && tid < groups)
             push(peer_addr(su32(part + rank * per_rank * TILE_N), tid), su32(sent + tid * per_rank * TILE_N),
                  (groups - tid + p.split - 1) / p.split * TILE_N * 16, peer_addr(join, tid));
         __syncwarp();
-        if (mine) ok = wait_for(join, 0, abort, p.err, false) && ok;
+        const bool came = !mine || wait_for(join, 0, abort, p.err, false);
+        ok = ok && came;
         asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 #pragma unroll 2
         for (int i = half; i < mine; i += 2) {
@@ -318,16 +330,11 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
         }
         // A CTA leaves when all that it sent has arrived: when every CTA of the cluster has received.
         asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+        if (!came) wait_for(join, 0, abort, p.err, false);      // sent late, but sent by now
     };
     if (p.type == GGML_TYPE_F32) finish(float());
     else if (p.type == GGML_TYPE_F16) finish(__half());
     else finish(__nv_bfloat16());
-    fence_before();
-    __syncthreads();
-    if (warp == 0) {
-        fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::COLS) : "memory");
-    }
 }
 
 // ------------------------------------------------------------------ many rows: CTA pairs
@@ -651,6 +658,19 @@ bool encode_scales(CUtensorMap *map, const tcg_mx_t &m, int atoms, int blocks)
     return true;
 }
 
+// The shared memory that a kernel may ask for, set at its first call on each device. (Calls that come first together set the
+// same.)
+template <auto FN>
+bool allow_smem(int bytes)
+{
+    static std::atomic<bool> done[64];
+    std::atomic<bool> &here = done[ctx().device & 63];
+    if (here.load(std::memory_order_acquire)) return true;
+    TCG_CUDA(cudaFuncSetAttribute(FN, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    here.store(true, std::memory_order_release);
+    return true;
+}
+
 template <typename T, int BITS>
 bool pair_launch(LinArgs &p, const tcg_mx_t &x, const tcg_mx_t &w)
 {
@@ -668,8 +688,8 @@ bool pair_launch(LinArgs &p, const tcg_mx_t &x, const tcg_mx_t &w)
     const long long tiles = (long long)p.tiles_n * p.tiles_m;
     if (tiles > 0x7fffff00ll) return fail("tcg_mx_linear: %d rows and %d outputs are too many for one call", p.rows, p.outs);
     const int pairs = (int)min(tiles, (long long)ctx().sms / 2);
-    void (*fn)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const CUtensorMap, const LinArgs) = mx_pair_kernel<T, BITS>;
-    TCG_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+    constexpr auto fn = mx_pair_kernel<T, BITS>;
+    if (!allow_smem<fn>(S::SMEM)) return false;
     TCG_CUDA(launch_pdl(fn, dim3(2 * pairs), dim3(PAIR_THREADS), S::SMEM, ctx().cur, mw, mx, msw, msx, (const LinArgs)p));
     return true;
 }
@@ -730,8 +750,8 @@ bool stream_launch(LinArgs &p, const tcg_mx_t &x, const tcg_mx_t &w)
     p.depth = min(MAX_DEPTH, min(max(p.per, 2), (room - part) / S::STAGE));
     const size_t smem = 1024 + p.depth * S::STAGE + part;
     if (tiles * p.split > 0x7fffffffll) return fail("tcg_mx_linear: %d rows and %d outputs are too many for one call", p.rows, p.outs);
-    void (*fn)(const CUtensorMap, const CUtensorMap, const LinArgs) = mx_stream_kernel<BITS, BN>;
-    TCG_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 512));
+    constexpr auto fn = mx_stream_kernel<BITS, BN>;
+    if (!allow_smem<fn>(MOST_SMEM)) return false;
     cudaLaunchAttribute attrs[2];
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3((unsigned)(tiles * p.split));
