@@ -13,7 +13,7 @@ namespace {
 
 constexpr int ERR_WAIT = TCG_ERR_MX_WAIT;
 constexpr int STREAM_THREADS = 256, MAX_DEPTH = 16;
-constexpr int HALF_SM = 108 * 1024, MOST_SMEM = 226 * 1024;     // of dynamic shared memory; the static part is below 1 KB
+constexpr int HALF_SM = 112 * 1024, MOST_SMEM = 226 * 1024;     // of dynamic shared memory; the static part is below 1 KB
 constexpr int SUM_K = 4096;             // columns that the tensor core sums before fp32 results are added up outside
 constexpr int TILE_N = 128;             // weight rows of a tile: the MMA's M, a TMEM lane each
 constexpr int MAX_SPLIT = 8;            // portable cluster size
@@ -81,6 +81,18 @@ __device__ __forceinline__ bool elect()
     return one != 0;
 }
 
+__device__ __forceinline__ int special_rank()
+{
+    int r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ int special_cluster()
+{
+    int r;
+    asm volatile("mov.u32 %0, %%clusterid.x;" : "=r"(r));
+    return r;
+}
 __device__ __forceinline__ void cluster_sync()
 {
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
@@ -126,6 +138,7 @@ struct LinArgs {
     int rows, outs, atoms;              // of x, of w, scale groups of a row
     int stages_k;                       // stages of the whole K
     int tiles_n, tiles_m, split, per;   // CTAs of a tile, stages of each
+    unsigned split_inv;                 // 2^16 / split, rounded up
     int acc_stages;                     // stages of an accumulator
     int depth;                          // stages in shared memory
     int type;
@@ -173,11 +186,14 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
     unsigned char *const smem = (unsigned char *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t base = su32(smem), full = su32(bars), empty = full + 8 * MAX_DEPTH, done = empty + 8 * MAX_DEPTH, join = done + 8;
-    const int rank = blockIdx.x % p.split, tile = blockIdx.x / p.split;
-    const int n0 = tile % p.tiles_n * TILE_N, m0 = tile / p.tiles_n * BN;
+    // a cluster a tile; a division costs as much as a few dozen instructions, so none where there is one tile of rows
+    const int rank = special_rank(), tile = special_cluster(), tm = BN < MX_ATOM ? 0 : tile / p.tiles_n;
+    const int n0 = (tile - tm * p.tiles_n) * TILE_N, m0 = tm * BN;
     const int k_begin = rank * p.per, k_end = min(p.stages_k, k_begin + p.per), count = k_end - k_begin;
     // Where a tile's K is split, its results meet by fours of x's rows: the CTA of rank g % split adds up group g.
-    const int groups = (min(BN, p.rows - m0) + 3) / 4, mine = p.split > 1 && groups > rank ? (groups - rank + p.split - 1) / p.split : 0;
+    const int groups = (min(BN, p.rows - m0) + 3) / 4;
+    auto over_split = [&](int i) { return (int)((unsigned)i * p.split_inv >> 16); };        // i / split, of i up to 40
+    const int mine = p.split > 1 && groups > rank ? over_split(groups - rank + p.split - 1) : 0;
     if (tid == 0) {
         prefetch_map(&mw), prefetch_map(&mx);
         for (int i = 0; i < p.depth; i++) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
@@ -185,7 +201,7 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
         bar_init(join, 1);
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        if (mine) bar_expect_tx(join, p.split * mine * TILE_N * 16);
+        if (mine) bar_expect_tx(join, (p.split - 1) * mine * TILE_N * 16);
     }
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(&s_tmem)), "r"(S::COLS) : "memory");
@@ -281,9 +297,11 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
     };
     auto finish = [&](auto type) {
         using T = decltype(type);
-        // [split][ceil(BN / 4 / split)][128] words of four columns: by owner, over the stages (whose products are done), what
-        // this CTA sends; by sender, behind the stages, what the cluster's CTAs send here
-        const int per_rank = (BN / 4 + p.split - 1) / p.split;
+        // [owner][ceil(BN / 4 / split)][128] words of four columns over the stages (whose products are done): what this CTA
+        // adds up itself or sends. [sender][..][128] behind the stages: what the cluster's other CTAs send here. (The second
+        // over the stages as well leaves room for more of them, but has to wait for the peers' stages: one token 4096 ->
+        // 4096 in 4 bits 4.9 us against 4.2.)
+        const int per_rank = over_split(BN / 4 + p.split - 1);
         float4 *const sent = (float4 *)smem;
         const float4 *const part = (const float4 *)(smem + p.depth * S::STAGE);
         constexpr int STEP = BN < 32 ? 8 : 16;
@@ -300,7 +318,7 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
             if (p.split > 1) {
 #pragma unroll
                 for (int j = 0; j < STEP; j += 4) {
-                    const int g = (c + j) / 4, i = g / p.split, owner = g - i * p.split;
+                    const int g = (c + j) / 4, i = over_split(g), owner = g - i * p.split;
                     sent[(owner * per_rank + i) * TILE_N + t] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
                 }
             } else if (ok) {
@@ -311,9 +329,9 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
         free_tmem();
         if (p.split == 1) return;
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");     // the peers' barriers are there
-        if (tid < p.split && tid < groups)
-            push(peer_addr(su32(part + rank * per_rank * TILE_N), tid), su32(sent + tid * per_rank * TILE_N),
-                 (groups - tid + p.split - 1) / p.split * TILE_N * 16, peer_addr(join, tid));
+        if (tid < p.split && tid < groups && tid != rank)
+            push(peer_addr(su32(part + (rank - (rank > tid)) * per_rank * TILE_N), tid), su32(sent + tid * per_rank * TILE_N),
+                 over_split(groups - tid + p.split - 1) * TILE_N * 16, peer_addr(join, tid));
         __syncwarp();
         const bool came = !mine || wait_for(join, 0, abort, p.err, false);
         ok = ok && came;
@@ -323,7 +341,8 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
             float sum[4] = {};
 #pragma unroll
             for (int s = 0; s < MAX_SPLIT; s++) {
-                const float4 v = s < p.split ? part[(s * per_rank + i) * TILE_N + t] : make_float4(0, 0, 0, 0);
+                const float4 *const from = s == rank ? sent + rank * per_rank * TILE_N : part + (s - (s > rank)) * per_rank * TILE_N;
+                const float4 v = s < p.split ? from[i * TILE_N + t] : make_float4(0, 0, 0, 0);
                 sum[0] += v.x, sum[1] += v.y, sum[2] += v.z, sum[3] += v.w;
             }
             if (ok) put_columns<4, T>(p, m0 + 4 * (rank + i * p.split), n, bias, sum);
@@ -745,8 +764,9 @@ bool stream_launch(LinArgs &p, const tcg_mx_t &x, const tcg_mx_t &w)
     // in 4 bits 7.2 us, with all of it 8.3), several waves run two CTAs an SM (60000 outputs 27 us, with one CTA 36). Not
     // where that leaves fewer than four stages of one wave: 14336 -> 4096 in 8 bits 8.6 us, with half 11.4.
     const bool half = BN <= 32 && (tiles * p.split > ctx().sms || 4 * S::STAGE + 16 * 1024 <= HALF_SM);
-    const int room = half ? HALF_SM : 200 * 1024;
-    const int part = p.split > 1 ? p.split * ((BN / 4 + p.split - 1) / p.split) * TILE_N * 16 : 0;
+    const int room = (half ? HALF_SM : MOST_SMEM) - 1024;
+    p.split_inv = (65536 + p.split - 1) / p.split;
+    const int part = p.split > 1 ? (p.split - 1) * ((BN / 4 + p.split - 1) / p.split) * TILE_N * 16 : 0;
     p.depth = min(MAX_DEPTH, min(max(p.per, 2), (room - part) / S::STAGE));
     const size_t smem = 1024 + p.depth * S::STAGE + part;
     if (tiles * p.split > 0x7fffffffll) return fail("tcg_mx_linear: %d rows and %d outputs are too many for one call", p.rows, p.outs);
