@@ -139,6 +139,7 @@ struct LinArgs {
     int stages_k;                       // stages of the whole K
     int tiles_n, tiles_m, split, per;   // CTAs of a tile, stages of each
     unsigned split_inv;                 // 2^16 / split, rounded up
+    int tiles, whole;                   // of the pairs: how many, from which on halves
     int acc_stages;                     // stages of an accumulator
     int depth;                          // stages in shared memory
     int type;
@@ -409,12 +410,19 @@ __device__ __forceinline__ void commit_pair(uint32_t bar)
                  ::"r"(bar), "h"((unsigned short)3) : "memory");
 }
 
-// Tile `i` in the order they are taken: eight blocks of x's rows at a time, so that the tiles under way together share both.
-__device__ __forceinline__ void tile_at(const LinArgs &p, int i, int &tn, int &tm)
+// The i-th tile, in the order they are taken: eight blocks of x's rows at a time, so that the tiles under way together share
+// both operands. What is left for the last round goes by halves of 128 rows of x where each pair gets at most one.
+struct PairTile {
+    int n0, m0, rows;                                       // first weight row, first row of x, 256 or 128 of them
+};
+__device__ __forceinline__ PairTile tile_at(const LinArgs &p, int i)
 {
-    const int group = i / (8 * p.tiles_n), in = i - group * 8 * p.tiles_n, high = min(8, p.tiles_m - 8 * group);
-    tn = in / high;
-    tm = 8 * group + in - tn * high;
+    const bool half = i >= p.whole;
+    if (half) i -= p.whole;
+    const int tile = half ? p.whole + i / 2 : i;
+    const int group = tile / (8 * p.tiles_n), in = tile - group * 8 * p.tiles_n, high = min(8, p.tiles_m - 8 * group);
+    const int tn = in / high, tm = 8 * group + in - tn * high;
+    return { tn * 256, tm * 256 + (half ? i % 2 * 128 : 0), half ? 128 : 256 };
 }
 
 template <typename T>
@@ -467,14 +475,13 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ C
     volatile int *abort = &s_abort;
     bool ok = true;
     pdl_wait();
-    const int tiles = p.tiles_n * p.tiles_m, first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
     // Units: a tile's K, or with F32 results a part of it at a time.
     if (warp == 0) {
         int slot = 0, phase = 1, issued = 0;
-        for (int tile = first; tile < tiles && ok; tile += step) {
-            int tn, tm;
-            tile_at(p, tile, tn, tm);
-            const int n0 = tn * 256 + rank * 128, m0 = tm * S::ROWS;
+        for (int tile = first; tile < p.tiles && ok; tile += step) {
+            const PairTile at = tile_at(p, tile);
+            const int n0 = at.n0 + rank * 128, m0 = at.m0, mine = m0 + rank * (at.rows / 2);    // a half's box brings 64 rows too many
             for (int k = 0; k < p.stages_k; k++) {
                 ok = wait_for(empty + 8 * slot, phase, abort, p.err);
                 if (!ok) break;
@@ -483,7 +490,7 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ C
                 if (elect()) {
                     if (rank == 0) bar_expect_tx(full + 8 * slot, S::TX);
                     tma_load_pair(a, &mw, bar, k * 128, n0);
-                    tma_load_pair(b, &mx, bar, k * 128, m0 + rank * 128);
+                    tma_load_pair(b, &mx, bar, k * 128, mine);
                     tma_load_pair(sa, &msw, bar, k * (F::ATOMS * 64), n0 / 128);
                     tma_load_pair(sb, &msx, bar, k * (F::ATOMS * 64), m0 / 128);
                 }
@@ -499,10 +506,11 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ C
                 wait_for(full + 8 * (wrapped ? at + S::STAGES : at), phase ^ 1 ^ wrapped, abort, p.err, false);
             }
     } else if (warp == 1 && rank == 0) {
-        const uint32_t id = mx_idesc<BITS>(S::ROWS, 256), sfa = tmem + S::SF_COL, sfb = sfa + 4 * F::ATOMS;
+        const uint32_t sfa = tmem + S::SF_COL, sfb = sfa + 4 * F::ATOMS;
         int slot = 0, phase = 0;
         uint32_t unit = 0;
-        for (int tile = first; tile < tiles && ok; tile += step) {
+        for (int tile = first; tile < p.tiles && ok; tile += step) {
+            const uint32_t id = mx_idesc<BITS>(tile_at(p, tile).rows, 256);
             for (int k0 = 0; k0 < p.stages_k && ok; k0 += p.acc_stages, unit++) {
                 const uint32_t buf = unit & 1, d = tmem + (buf ? S::ACC1 : 0);
                 ok = wait_for(acc_free + 8 * buf, (unit >> 1 & 1) ^ 1, abort, p.err) &&
@@ -549,10 +557,8 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ C
         const uint32_t at = tmem + ((uint32_t)q << 21) + 64 * h;
         const uint32_t free_bar = peer_addr(acc_free, 0), lap_bar = peer_addr(lap_free, 0);
         uint32_t unit = 0;
-        for (int tile = first; tile < tiles && ok; tile += step) {
-            int tn, tm;
-            tile_at(p, tile, tn, tm);
-            const int n = tn * 256 + rank * 128 + 32 * q + lane, m0 = tm * S::ROWS + 64 * h;
+        for (int tile = first; tile < p.tiles && ok; tile += step) {
+            const int n = tile_at(p, tile).n0 + rank * 128 + 32 * q + lane;
             // the order of 16-column pieces: the shared columns are the last 32 of the first accumulator, the first of the second
             auto piece = [&](int i) { return (i ^ (h == 3 ? 2 : 0)) * 16; };
             const float bias = p.bias && n < p.outs ? p.bias[n] : 0.0f;
@@ -588,9 +594,13 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ C
                 if (lane == 0) arrive_cluster(free_bar + 8 * buf);
             }
             if (!ok) break;
+            int again = tile;                               // taken anew: the registers are the accumulators' until here
+            asm volatile("" : "+r"(again));
+            const PairTile here = tile_at(p, again);
+            const int m0 = here.m0 + 64 * h, end = min(p.rows, here.m0 + here.rows);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int m = m0 + piece(i), rows = n < p.outs ? p.rows - m : 0;
+                const int m = m0 + piece(i), rows = n < p.outs ? end - m : 0;
                 if constexpr (WIDE) {
                     T *y = (T *)p.y + m * p.ldy + n;
 #pragma unroll
@@ -704,9 +714,13 @@ bool pair_launch(LinArgs &p, const tcg_mx_t &x, const tcg_mx_t &w)
     p.stages_k = (p.atoms + F::ATOMS - 1) / F::ATOMS;
     p.pairs = p.ldy % 2 == 0 && (uintptr_t)p.y % 4 == 0 && p.outs % 2 == 0;
     p.acc_stages = sizeof(T) == 4 ? SUM_K / F::K : p.stages_k;
-    const long long tiles = (long long)p.tiles_n * p.tiles_m;
+    const long long tiles = (long long)p.tiles_n * p.tiles_m, most = ctx().sms / 2;
     if (tiles > 0x7fffff00ll) return fail("tcg_mx_linear: %d rows and %d outputs are too many for one call", p.rows, p.outs);
-    const int pairs = (int)min(tiles, (long long)ctx().sms / 2);
+    const int left = (int)(tiles % most);
+    const bool halve = 2 * left <= most;
+    p.whole = (int)(halve ? tiles - left : tiles);
+    p.tiles = p.whole + (halve ? 2 * left : 0);
+    const int pairs = (int)min((long long)p.tiles, most);
     constexpr auto fn = mx_pair_kernel<T, BITS>;
     if (!allow_smem<fn>(S::SMEM)) return false;
     TCG_CUDA(launch_pdl(fn, dim3(2 * pairs), dim3(PAIR_THREADS), S::SMEM, ctx().cur, mw, mx, msw, msx, (const LinArgs)p));
@@ -741,8 +755,9 @@ StreamPlan stream_plan(int rows, long long tiles, int stages, int bn)
 template <int BITS>
 double pair_ns(long long tiles, int stages)
 {
-    const long long pairs = ctx().sms / 2, rounds = (tiles + pairs - 1) / pairs;
-    return 3700 + (double)rounds * (2100 + stages * (BITS == 4 ? 290 : 590));
+    const long long pairs = ctx().sms / 2, left = tiles % pairs;
+    const double rounds = (double)(tiles / pairs) + (left == 0 ? 0 : 2 * left <= pairs ? 0.8 : 1);
+    return 3700 + rounds * (2100 + stages * (BITS == 4 ? 290 : 590));
 }
 
 template <int BITS, int BN>
