@@ -188,7 +188,9 @@ bool tcg_scale(float *out, const float *x, float s, size_t n);
 /* ------------------------------- language-model operators (new)
  * What a decode or prefill step of a GGUF language model needs between the
  * projections (tcg_matvec_q, tcg_linear_q, tcg_linear): rotary positions,
- * head norms, an 8-bit key/value cache and the attention that reads it.
+ * head norms, an 8-bit key/value cache and the attention that reads it; and
+ * projections in 4 bits on the block-scaled tensor path, with the norm that
+ * feeds them.
  * Rows are tokens; a row's heads lie side by side (head h at h * head_dim)
  * and successive rows are ld elements apart, so the parts of a fused QKV row
  * are passed as pointers into it. Types: GGML_TYPE_F32, F16 and BF16; norms,
@@ -200,7 +202,7 @@ bool tcg_scale(float *out, const float *x, float s, size_t n);
  *
  * Lengths and page numbers are read on the device. What is out of range
  * there is skipped, without any access, and raises the device error word
- * (tcg_device_error): */
+ * (tcg_device_error); so does a wait that gives up: */
 #define TCG_ERR_KV8_LENGTHS 64  /* a sequence's rows or lengths: the whole sequence is skipped */
 #define TCG_ERR_KV8_PAGE    65  /* a page number: its tokens are not written, read as 0, and masked in attention */
 #define TCG_ERR_KV8_WAIT    66  /* a bounded wait inside attention gave up: the call's output is not valid */
@@ -356,15 +358,18 @@ bool tcg_mx_quantize(const tcg_mx_t *m, const void *x, int64_t ld, ggml_type_t t
  * bf16's smallest). Elements between the rows are left as they were. */
 bool tcg_mx_dequantize(void *y, const tcg_mx_t *m, int64_t ld, ggml_type_t t);
 /* y = x w^T + bias: x [rows, cols] in 8 or 4 bits, w [outs, cols] in 4 bits,
- * bias fp32 [outs] or NULL, y [rows, outs]. Products are exact and summed in
- * fp32 (F32 results: in groups of columns that keep the sum's error at
- * fp32's), the sum is rounded once to t. y must not overlap x or w. */
+ * bias fp32 [outs] or NULL, y [rows, outs]. Products are exact; the tensor core
+ * adds 32 columns (x in 8 bits) or 64 (4 bits) at a time to a sum of 24 bits,
+ * cutting what lies below (F32 results are summed in parts of 4096 columns);
+ * the sum is rounded once to t. What stands behind cols in the codes must be
+ * 0, with any scale but 255. y must not overlap x or w. */
 bool tcg_mx_linear(void *y, const tcg_mx_t *x, const tcg_mx_t *w, const float *bias, int64_t ld_y, ggml_type_t t);
 /* The residual's addition and the root-mean-square norm of the sum, in one
  * pass over n_tok rows of cols columns (at most TCG_NORM_MAX_COLS):
  *   h = x + r, rounded to t (r NULL: h = x),
  *   v = h / sqrt(mean(h^2) + eps) * w (w fp32 [cols]),
- * out as y (rounded to t) and/or as mx (quantised, from v itself). Each of h,
+ * out as y (v to 4 roundings of fp32, rounded to t) and/or as mx (the codes of
+ * v itself, where v is of fp32's normal numbers). Each of h,
  * y and mx may be NULL, not all of them. h and y may be x or r in place (the
  * same pointer and stride), not each other; otherwise nothing overlaps. */
 bool tcg_add_rms_norm(void *h, void *y, const tcg_mx_t *mx, const void *x, const void *r, const float *w, float eps,

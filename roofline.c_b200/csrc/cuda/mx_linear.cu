@@ -1,5 +1,23 @@
 // mx_linear.cu -- tcg_mx_linear: y = x w^T + bias, x in 8 (E4M3) or 4 bits (E2M1), w in 4 bits, a power of two for each 32
 // columns of a row, on the tensor core's block-scaled products (tcgen05 kind::mxf8f6f4 and kind::mxf4).
+//
+//   y[i, n] = sum_b 2^(sx[i, b] + sw[n, b] - 254) sum_{k in block b} cx[i, k] cw[n, k] + bias[n]
+//
+// Products of codes are exact (at most 6 significant bits), the scales add to the exponent, and the tensor core adds 32 (8
+// bits) or 64 columns (4 bits) at a time to an fp32 sum that it cuts after 24 bits; fp32 results are summed in parts of 4096
+// columns. Against 64 bits, normally distributed rows: 5e-8 over 14336 columns in 8 bits (an fp32 library product on the
+// decoded values: 6e-8), nothing in 4 bits, whose sums fit 24 bits.
+//
+// The weights are the MMA's first operand: 128 weight rows are TMEM lanes, x's rows columns, so that a warp's 32 lanes hold
+// neighbouring results of one row of y and store them as they come, and one token costs 8 columns and not 128 rows.
+//   Few rows (mx_stream_kernel): bound by reading the weights. One wave of CTAs, K split over the CTAs of a cluster where the
+//     tiles are fewer than the SMs; parts meet in shared memory. One token 4096 -> 14336, x in 8 bits 8.7 us (31.2 MB: 3.6
+//     TB/s, of which ~4 us are start, first bytes and end), in 4 bits 7.1; 60000 outputs in 4 bits 25 us (5.2 TB/s); 64 rows
+//     of 14336 -> 4096 in 8 bits 11.3 us.
+//   Many (mx_pair_kernel): bound by the tensor core and the power that it takes. CTA pairs on tiles of 256 x 256, two
+//     accumulators. 4096 rows of 4096 -> 14336 in 4 bits 98 us (4.9 PFLOP/s at ~1.6 GHz: 60% of the cycles; the last round
+//     is 8 of 74 pairs' worth), 8192^3 189 us (5.8); 2048 rows of 14336 -> 4096 in 8 bits, fp32 results, 93 us (2.6: two
+//     rounds of which the second is three quarters full), 8192^3 363 us (3.0).
 #include "mx.cuh"
 #include "tc05.cuh"
 
@@ -114,19 +132,32 @@ __device__ __forceinline__ void arrive_cluster(uint32_t bar)
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-// Wait for the phase of parity `parity`. Gives up (false) when another role has (abort), or after `tries` tests, each of
-// which the hardware may hold for a while: between 0.1 s and minutes. bar_wait (tc05.cuh) bounds its waits by a timer.
-constexpr int WAIT_TRIES = 1 << 23;
-__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int *abort, int *err, bool heed_abort = true,
-                                         int tries = WAIT_TRIES)
+// Wait for the phase of parity `parity`. Gives up when another role has (abort), or WAIT_NS after its first thousand tests
+// (bar_wait, tc05.cuh, reads the timer at its start). wait_lane: a warp's lanes may come to differ; they agree again after
+// the elected lane has issued what it waited for. wait_for: they agree at once.
+__device__ __forceinline__ bool wait_lane(uint32_t bar, uint32_t parity, volatile int *abort, int *err, bool heed_abort = true)
 {
-    for (int i = 0; i < tries; i++) {
-        if (bar_test(bar, parity)) return true;
-        if ((i & 1023) == 1023 && heed_abort && *abort) return false;
+    bool here = bar_test(bar, parity);
+    unsigned long long since = 0;
+    for (uint32_t i = 1; !here; i++) {
+        here = bar_test(bar, parity);
+        if (!here && (i & 1023) == 0) {
+            const unsigned long long now = now_ns();
+            if (since == 0) since = now;
+            if (now - since > WAIT_NS) {
+                *abort = 1;
+                atomicExch(err, ERR_WAIT);
+                break;
+            }
+            if (heed_abort && *abort) break;
+        }
     }
-    *abort = 1;
-    atomicExch(err, ERR_WAIT);
-    return false;
+    return here;
+}
+__device__ __forceinline__ bool agree(bool ok) { return __all_sync(0xFFFFFFFFu, ok); }
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int *abort, int *err, bool heed_abort = true)
+{
+    return agree(wait_lane(bar, parity, abort, err, heed_abort));
 }
 
 struct LinArgs {
@@ -227,10 +258,9 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
         int k = 0, slot = 0, phase = 1;
         for (; k < count; k++) {
             const int kk = k_begin + k, na = atoms_of(k);
-            ok = wait_for(empty + 8 * slot, phase, abort, p.err);
-            if (!ok) break;
+            ok = wait_lane(empty + 8 * slot, phase, abort, p.err);
             const uint32_t bar = full + 8 * slot, a = at(slot), b = a + S::A, sa = b + S::B, sb = sa + S::SF;
-            if (elect()) {
+            if (elect() && ok) {
                 bar_expect_tx(bar, S::TX + 2 * 512 * na);
 #pragma unroll
                 for (int i = 0; i < S::SUBS; i++) {
@@ -240,12 +270,13 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
                 bulk_load(sa, p.ws + ((size_t)(n0 / MX_ATOM) * p.atoms + (size_t)kk * S::ATOMS) * 512, 512 * na, bar);
                 bulk_load(sb, p.xs + ((size_t)(m0 / MX_ATOM) * p.atoms + (size_t)kk * S::ATOMS) * 512, 512 * na, bar);
             }
-            __syncwarp();
+            ok = agree(ok);
+            if (!ok) break;
             if (++slot == p.depth) slot = 0, phase ^= 1;
         }
-        // copies in flight land before the CTA ends
+        // copies in flight land before the CTA ends (the one that it gave up on may have been issued, too)
         if (!ok)
-            for (int j = max(0, k - p.depth); j < k; j++)
+            for (int j = max(0, k - p.depth); j <= k; j++)
                 wait_for(full + 8 * (j % p.depth), (j / p.depth) & 1, abort, p.err, false);
     } else if (role == 1) {
         const uint32_t id = mx_idesc<BITS>(BN, TILE_N), sfa = tmem + S::SF_COL, sfb = sfa + 4 * S::ATOMS;
@@ -253,11 +284,10 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
         uint32_t d = tmem;
         for (int k = 0; k < count; k++) {
             const int na = atoms_of(k);
-            ok = wait_for(full + 8 * slot, phase, abort, p.err);
-            if (!ok) break;
+            ok = wait_lane(full + 8 * slot, phase, abort, p.err);
             fence_after();
             const uint32_t a = at(slot), b = a + S::A, sa = b + S::B, sb = sa + S::SF;
-            if (elect()) {
+            if (elect() && ok) {
 #pragma unroll
                 for (int i = 0; i < S::ATOMS; i++)
                     if (i < na) {
@@ -274,7 +304,8 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
                 }
                 mma_commit(empty + 8 * slot);
             }
-            __syncwarp();
+            ok = agree(ok);
+            if (!ok) break;
             if (++slot == p.depth) slot = 0, phase ^= 1;
             if (++in_acc == p.acc_stages) in_acc = 0, d += BN;
         }
@@ -483,20 +514,20 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ C
             const PairTile at = tile_at(p, tile);
             const int n0 = at.n0 + rank * 128, m0 = at.m0, mine = m0 + rank * (at.rows / 2);    // a half's box brings 64 rows too many
             for (int k = 0; k < p.stages_k; k++) {
-                ok = wait_for(empty + 8 * slot, phase, abort, p.err);
-                if (!ok) break;
+                ok = wait_lane(empty + 8 * slot, phase, abort, p.err);
                 const uint32_t a = base + slot * S::STAGE, b = a + S::A, sa = b + S::B, sb = sa + S::SF;
                 const uint32_t bar = peer_addr(full + 8 * slot, 0);
-                if (elect()) {
+                if (elect() && ok) {
                     if (rank == 0) bar_expect_tx(full + 8 * slot, S::TX);
                     tma_load_pair(a, &mw, bar, k * 128, n0);
                     tma_load_pair(b, &mx, bar, k * 128, mine);
                     tma_load_pair(sa, &msw, bar, k * (F::ATOMS * 64), n0 / 128);
                     tma_load_pair(sb, &msx, bar, k * (F::ATOMS * 64), m0 / 128);
                 }
-                __syncwarp();
-                issued++;
+                ok = agree(ok);
+                issued++;                                   // or perhaps not, where it gave up
                 if (++slot == S::STAGES) slot = 0, phase ^= 1;
+                if (!ok) break;
             }
         }
         // copies in flight land before the CTAs end (both CTAs' complete on the leader's barriers)
@@ -519,11 +550,10 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ C
                 const int k1 = min(p.stages_k, k0 + p.acc_stages);
                 for (int k = k0; k < k1 && ok; k++) {
                     const int na = min(F::ATOMS, p.atoms - k * F::ATOMS);
-                    ok = wait_for(full + 8 * slot, phase, abort, p.err);
-                    if (!ok) break;
+                    ok = wait_lane(full + 8 * slot, phase, abort, p.err);
                     fence_after();
                     const uint32_t a = base + slot * S::STAGE, b = a + S::A, sa = b + S::B, sb = sa + S::SF;
-                    if (elect()) {
+                    if (elect() && ok) {
 #pragma unroll
                         for (int i = 0; i < F::ATOMS; i++) {
                             scales_to_tmem_pair(sfa + 4 * i, sa + 512 * i);
@@ -540,7 +570,8 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ C
                         }
                         commit_pair(empty + 8 * slot);
                     }
-                    __syncwarp();
+                    ok = agree(ok);
+                    if (!ok) break;
                     if (++slot == S::STAGES) slot = 0, phase ^= 1;
                 }
                 if (ok && elect()) commit_pair(acc_full + 8 * buf);
