@@ -66,8 +66,8 @@ __device__ __forceinline__ void shift_bytes(uint32_t (&k)[N + 4], uint32_t off)
 }
 
 // A lane's 8 elements of a row, of which `left` exist (the others are 0). A row that starts on no 8-byte boundary is read
-// by the aligned 16-byte words around it and shifted, where those lie in [lo, hi), the array (1501 rows of 4103 16-bit values
-// of 4100 columns quantised: 6.4 us, element by element 8.1).
+// by the aligned 16-byte words around it and shifted, where those lie in [lo, hi), the array (1501 rows of 4100 16-bit values,
+// 4103 apart, quantised: 6.4 us, element by element 8.1).
 // VEC: rows start on 16-byte boundaries.
 template <bool VEC, typename T>
 __device__ __forceinline__ Raw<T> load_row(const T *p, long long left, const void *lo, const void *hi)
