@@ -212,34 +212,51 @@ struct MxOut {
     int bits;
 };
 
-// The scale byte of a block, from the largest magnitude of its values (as fp32 bits: whole numbers keep their order,
-// infinities and NaN above all), and 1 / scale (0 for a block that is NaN). Subnormals have exponent field 0: the smallest scale.
+// The scale byte of a block, from the bits of its largest magnitude (infinities and NaN above all), and 1 / scale (0 for a
+// block that is NaN). Subnormals have exponent field 0: the smallest scale.
 __device__ __forceinline__ uint32_t mx_scale(uint32_t top, int bits)
 {
     return top < 0x7F800000u ? (uint32_t)max((int)(top >> 23) - (bits == 4 ? 2 : 8), 0) : 255u;
 }
 __device__ __forceinline__ float mx_inverse(uint32_t s) { return __uint_as_float(s == 255 ? 0u : (254u - s) << 23); }
+// maxima that a NaN wins
+__device__ __forceinline__ float max_nan(float a, float b)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ uint32_t mx_top(const float (&x)[LANE])
 {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < LANE; i++) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-    return max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+    float t = max_nan(fabsf(x[0]), fabsf(x[1]), fabsf(x[2]));
+    t = max_nan(t, fabsf(x[3]), fabsf(x[4]));
+    t = max_nan(t, fabsf(x[5]), fabsf(x[6]));
+    t = max_nan(t, fabsf(x[7]));
+    t = max_nan(t, __shfl_xor_sync(0xFFFFFFFFu, t, 1));
+    return __float_as_uint(max_nan(t, __shfl_xor_sync(0xFFFFFFFFu, t, 2))) & 0x7FFFFFFFu;
 }
 __device__ __forceinline__ uint2 mx_codes(const float (&q)[LANE], int bits)
 {
     uint2 c = make_uint2(0, 0);
     if (bits == 4) {
-#pragma unroll
-        for (int i = 0; i < LANE; i += 2)
-            c.x |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(q[i], q[i + 1]), __NV_E2M1, cudaRoundNearest) << 4 * i;
+        asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+            "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+            "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+            "mov.b32 %0, {a, b, c, d};\n\t}"
+            : "=r"(c.x) : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]), "f"(q[4]), "f"(q[5]), "f"(q[6]), "f"(q[7]));
     } else {
-#pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-            c.x |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(q[i], q[i + 1]), __NV_SATFINITE, __NV_E4M3) << 8 * i;
-            c.y |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(q[i + 4], q[i + 5]), __NV_SATFINITE, __NV_E4M3) << 8 * i;
-        }
+        asm("{\n\t.reg .b16 a, b, c, d;\n\t"
+            "cvt.rn.satfinite.e4m3x2.f32 a, %3, %2;\n\tcvt.rn.satfinite.e4m3x2.f32 b, %5, %4;\n\t"
+            "cvt.rn.satfinite.e4m3x2.f32 c, %7, %6;\n\tcvt.rn.satfinite.e4m3x2.f32 d, %9, %8;\n\t"
+            "mov.b32 %0, {a, b};\n\tmov.b32 %1, {c, d};\n\t}"
+            : "=r"(c.x), "=r"(c.y)
+            : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]), "f"(q[4]), "f"(q[5]), "f"(q[6]), "f"(q[7]));
     }
     return c;
 }
