@@ -5,15 +5,15 @@
 //
 // Products of codes are exact (at most 6 significant bits), the scales add to the exponent, and the tensor core adds 32 (8
 // bits) or 64 columns (4 bits) at a time to an fp32 sum that it cuts after 24 bits; fp32 results are summed in parts of 4096
-// columns. Against 64 bits, normally distributed rows: 5e-8 over 14336 columns in 8 bits (an fp32 library product on the
-// decoded values: 6e-8), nothing in 4 bits, whose sums fit 24 bits.
+// columns as far as TMEM holds them. Against 64 bits, normally distributed rows: 5e-8 over 14336 columns in 8 bits (an fp32
+// library product on the decoded values: 6e-8), nothing in 4 bits, whose sums fit 24 bits.
 //
 // The weights are the MMA's first operand: 128 weight rows are TMEM lanes, x's rows columns, so that a warp's 32 lanes hold
 // neighbouring results of one row of y and store them as they come, and one token costs 8 columns and not 128 rows.
 //   Few rows (mx_stream_kernel): bound by reading the weights. One wave of CTAs, K split over the CTAs of a cluster where the
-//     tiles are fewer than the SMs; parts meet in shared memory. One token 4096 -> 14336, x in 8 bits 8.7 us (31.2 MB: 3.6
-//     TB/s, of which ~4 us are start, first bytes and end), in 4 bits 7.1; 60000 outputs in 4 bits 25 us (5.2 TB/s); 64 rows
-//     of 14336 -> 4096 in 8 bits 11.3 us.
+//     tiles are fewer than the SMs; parts meet in shared memory. One token 4096 -> 14336, x in 8 bits 7.6 us (31.2 MB: 4.1
+//     TB/s, of which ~4 us are start, first bytes and end), in 4 bits 6.8; 60000 outputs in 4 bits 25 us (5.2 TB/s); 64 rows
+//     of 14336 -> 4096 in 8 bits 11.4 us.
 //   Many (mx_pair_kernel): bound by the tensor core and the power that it takes. CTA pairs on tiles of 256 x 256, two
 //     accumulators. 4096 rows of 4096 -> 14336 in 4 bits 98 us (4.9 PFLOP/s at ~1.6 GHz: 60% of the cycles; the last round
 //     is 8 of 74 pairs' worth), 8192^3 189 us (5.8); 2048 rows of 14336 -> 4096 in 8 bits, fp32 results, 93 us (2.6: two
@@ -30,7 +30,7 @@ namespace tcg {
 namespace {
 
 constexpr int ERR_WAIT = TCG_ERR_MX_WAIT;
-constexpr int STREAM_THREADS = 256, MAX_DEPTH = 16;
+constexpr int STREAM_THREADS = 256, MAX_DEPTH = 16, ISSUERS = 2;
 constexpr int HALF_SM = 112 * 1024, MOST_SMEM = 226 * 1024;     // of dynamic shared memory; the static part is below 1 KB
 constexpr int SUM_K = 4096;             // columns that the tensor core sums before fp32 results are added up outside
 constexpr int TILE_N = 128;             // weight rows of a tile: the MMA's M, a TMEM lane each
@@ -171,7 +171,7 @@ struct LinArgs {
     int tiles_n, tiles_m, split, per;   // CTAs of a tile, stages of each
     unsigned split_inv;                 // 2^16 / split, rounded up
     int tiles, whole;                   // of the pairs: how many, from which on halves
-    int acc_stages;                     // stages of an accumulator
+    int acc_stages, accs;               // stages of an accumulator; accumulators of an issuing warp
     int depth;                          // stages in shared memory
     int type;
     bool pairs;                         // two 16-bit results of a row as one word
@@ -199,13 +199,22 @@ struct Stream {
     static constexpr int STAGE = A + B + 2 * SF;            // every part starts on 1024 bytes
     static constexpr int TX = TILE_N * 128 + B;             // bytes that the copies of codes count: weights as they are held
     static constexpr int COLS = BN <= 32 ? 256 : 512;       // TMEM: accumulators, then the scales
-    static constexpr int SF_COL = COLS - 2 * ATOMS * 4;
-    static constexpr int MAX_ACC = SF_COL / BN;
+    static constexpr int SF_COLS = 2 * ATOMS * 4, SF_COL = COLS - ISSUERS * SF_COLS;
+    static constexpr int MAX_ACC = SF_COL / BN / ISSUERS;   // of an issuing warp
 };
 
+// Of a CTA's stages those that the second issuing warp takes: slots are 0 .. depth - 1 in turn, the odd ones are its.
+__host__ __device__ __forceinline__ int second_issuer(int stages, int depth)
+{
+    const int cycles = stages / depth;
+    return cycles * (depth / 2) + (stages - cycles * depth) / 2;
+}
+
 // One tile of 128 weight rows x BN rows of x a cluster (a tile starts with a group of 128 rows of x, whose scales are four
-// TMEM columns: with BN < 128 there is one tile of rows), its K dealt out to the cluster's CTAs. Warp 0 loads, warp 1 issues the
-// products; then all of them take the results.
+// TMEM columns: with BN < 128 there is one tile of rows), its K dealt out to the cluster's CTAs. Warp 0 loads, warps 1 and 2
+// issue the products, by turns, each on accumulators and scales of its own: what a warp spends on a stage (waiting, copying
+// scales, committing: about 500 cycles) is more than the copies need for one (with one issuing warp: one token 4096 ->
+// 14336 in 8 bits 8.8 us, with two 7.6; 64 rows of 14336 -> 4096 in 4 bits 9.8 and 9.2). Then all of them take the results.
 template <int BITS, int BN>
 __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap mx,
                                                                    const __grid_constant__ LinArgs p)
@@ -229,7 +238,7 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
     if (tid == 0) {
         prefetch_map(&mw), prefetch_map(&mx);
         for (int i = 0; i < p.depth; i++) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
-        bar_init(done, 1);
+        bar_init(done, ISSUERS);
         bar_init(join, 1);
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -278,11 +287,14 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
         if (!ok)
             for (int j = max(0, k - p.depth); j <= k; j++)
                 wait_for(full + 8 * (j % p.depth), (j / p.depth) & 1, abort, p.err, false);
-    } else if (role == 1) {
-        const uint32_t id = mx_idesc<BITS>(BN, TILE_N), sfa = tmem + S::SF_COL, sfb = sfa + 4 * S::ATOMS;
-        int slot = 0, phase = 0, in_acc = 0;
-        uint32_t d = tmem;
-        for (int k = 0; k < count; k++) {
+    } else if (role <= ISSUERS) {
+        const int turn = role - 1;
+        const uint32_t id = mx_idesc<BITS>(BN, TILE_N), sfa = tmem + S::SF_COL + turn * S::SF_COLS, sfb = sfa + 4 * S::ATOMS;
+        int slot = turn, phase = 0, in_acc = 0;
+        uint32_t d = tmem + turn * p.accs * BN;
+        // By slots, not by stages: a slot's phases are then waited for by one warp, one after the other. (A warp that waited
+        // for a phase while the one before it, another warp's, was still to come would take the one before that for it.)
+        for (int k = turn; k < count;) {
             const int na = atoms_of(k);
             ok = wait_lane(full + 8 * slot, phase, abort, p.err);
             fence_after();
@@ -306,7 +318,8 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
             }
             ok = agree(ok);
             if (!ok) break;
-            if (++slot == p.depth) slot = 0, phase ^= 1;
+            if (slot + ISSUERS < p.depth) slot += ISSUERS, k += ISSUERS;
+            else k += p.depth - slot + turn, slot = turn, phase ^= 1;
             if (++in_acc == p.acc_stages) in_acc = 0, d += BN;
         }
         if (elect()) mma_commit(done);
@@ -314,7 +327,9 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
     __syncwarp();
     ok = wait_for(done, 0, abort, p.err, false) && ok && !*abort;
     fence_after();
-    const int accs = (count - 1) / p.acc_stages + 1;
+    // accumulators that hold something: the first warp's, then the second's
+    const int own1 = second_issuer(count, p.depth), accs0 = (count - own1 - 1) / p.acc_stages + 1;
+    const int accs = accs0 + (own1 + p.acc_stages - 1) / p.acc_stages;
     const uint32_t lane_base = tmem + ((uint32_t)(warp & 3) << 21);
     // Two warps share 32 TMEM lanes (weight rows) and take every second step of columns (x's rows).
     const int t = tid & 127, half = tid >> 7;
@@ -342,8 +357,9 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
             float v[STEP] = {};
             for (int i = 0; i < accs; i++) {
                 uint32_t r[STEP];
-                if constexpr (STEP == 8) tmem_ld8(lane_base + i * BN + c, r);
-                else tmem_ld16(lane_base + i * BN + c, r);
+                const int acc = i < accs0 ? i : p.accs + i - accs0;
+                if constexpr (STEP == 8) tmem_ld8(lane_base + acc * BN + c, r);
+                else tmem_ld16(lane_base + acc * BN + c, r);
 #pragma unroll
                 for (int j = 0; j < STEP; j++) v[j] += __uint_as_float(r[j]);
             }
@@ -758,37 +774,76 @@ bool pair_launch(LinArgs &p, const tcg_mx_t &x, const tcg_mx_t &w)
     return true;
 }
 
-// What a call takes, estimated: ns measured on a B200, as in
-//   rows, columns -> outputs, bits     stream            pair
-//   512, 4096 -> 4096, 4               8.9               11.3 us
-//   1000, 4096 -> 4096, 4              17.2              11.9
-//   200, 1100 -> 5003, 8               6.0               9.2
-//   200, 4096 -> 14336, 8              22.6              17.4
-//   200, 14336 -> 4096, 4              18.0 (split 2)    22.8
-// A stage of 256 columns; where K is split, the join takes 45 ns a row of the tile (70 rows of 4096 -> 4096 in 4 bits: 8.2 us
-// in four parts; 200 rows, two parts: 11.9, undivided 8.8).
+// What a call takes, estimated in ns from B200 measurements, to choose between the kernels and the number of parts of K:
+//   rows, columns -> outputs, bits     stream (us)                         pair
+//   1, 14336 -> 4096, 8                13.9, 4 parts 7.2
+//   64, 4096 -> 4096, 4                6.4, 2 parts 6.8, 4 parts 6.8
+//   128, 14336 -> 4096, 8              24.2, 2 parts 22.5, 4 parts 15.8    25.6
+//   512, 4096 -> 4096, 4               8.2                                 10.0
+//   300, 14336 -> 4096, 8              31.0                                29.2
+//   200, 4096 -> 14336, 8              23.2                                17.4
+//   1000, 4096 -> 4096, 4              15.8                                11.9
+// A CTA of the stream kernel starts and ends in 3 us and 11 ns a row of x's tile; a stage of 256 columns takes what its MMAs
+// and waits take, and more the more CTAs read; the join of parts takes 600 ns and 20 a row, and with 128 rows in 8 bits
+// leaves room for only two stages in flight.
+template <int BITS, int BN>
+double stream_ns(int rows, long long tiles, int stages, int split)
+{
+    const double waves = (double)((tiles * split + ctx().sms - 1) / ctx().sms), r = min(BN, rows);
+    const double stage = (BITS == 4 ? 165 : BN <= 64 ? 220 : split == 1 ? 340 : 440)
+        + (double)min(tiles * split, (long long)ctx().sms) * Stream<BITS, BN>::STAGE * 1.8e-5;
+    return waves * (3000 + 11 * r + (stages + split - 1) / split * stage) + (split > 1 ? 600 + 20 * r : 0);
+}
+
+// Clusters of `split` CTAs that run at once. Those of eight with an SM's shared memory each are 15 on a B200, not 148 / 8: 16
+// of them take two rounds (200 rows of 4096 -> 1024 in 8 bits in eight parts 13.1 us, in five 9.1). 0 after an error.
+template <int BITS, int BN>
+int clusters_at_once(int split)
+{
+    static std::atomic<int> known[MAX_SPLIT + 1];
+    int n = known[split].load(std::memory_order_relaxed);
+    if (n) return n;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim = { (unsigned)split, 1, 1 };
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3((unsigned)split);
+    lc.blockDim = dim3(STREAM_THREADS);
+    lc.dynamicSmemBytes = MOST_SMEM;
+    lc.attrs = &attr;
+    lc.numAttrs = 1;
+    constexpr auto fn = mx_stream_kernel<BITS, BN>;
+    if (!allow_smem<fn>(MOST_SMEM)) return 0;
+    if (cudaOccupancyMaxActiveClusters(&n, fn, &lc) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    known[split].store(n, std::memory_order_relaxed);
+    return n;
+}
+
 struct StreamPlan {
     int split;
     double ns;
 };
-template <int BITS>
-StreamPlan stream_plan(int rows, long long tiles, int stages, int bn)
+template <int BITS, int BN>
+StreamPlan stream_plan(int rows, long long tiles, int stages)
 {
-    const double stage = BITS == 4 ? (bn <= 64 ? 250 : 310) : (bn <= 64 ? 400 : 460), join = 300 + 45 * min(bn, rows);
-    const double start = 3700 * (double)((tiles + ctx().sms - 1) / ctx().sms);
-    StreamPlan best = { 1, start + stages * stage * (double)((tiles + ctx().sms - 1) / ctx().sms) };
+    StreamPlan best = { 1, stream_ns<BITS, BN>(rows, tiles, stages, 1) };
     for (int s = 2; s <= MAX_SPLIT && tiles * s <= ctx().sms && s * MIN_STAGES <= stages; s++) {
-        const double ns = start + (stages + s - 1) / s * stage + join;
-        if (ns < best.ns) best = { s, ns };
+        const double ns = stream_ns<BITS, BN>(rows, tiles, stages, s);
+        if (ns < best.ns && tiles <= clusters_at_once<BITS, BN>(s)) best = { s, ns };
     }
     return best;
 }
+
+// Rounds of the pairs; the last one's tiles are halved where each pair gets at most one half.
 template <int BITS>
 double pair_ns(long long tiles, int stages)
 {
     const long long pairs = ctx().sms / 2, left = tiles % pairs;
-    const double rounds = (double)(tiles / pairs) + (left == 0 ? 0 : 2 * left <= pairs ? 0.8 : 1);
-    return 3700 + rounds * (2100 + stages * (BITS == 4 ? 290 : 590));
+    const double round = 2100 + stages * (BITS == 4 ? 290 : 590), last = 2400 + stages * (BITS == 4 ? 240 : 400);
+    return 3700 + (double)(tiles / pairs) * round + (left == 0 ? 0 : 2 * left <= pairs ? min(last, round) : round);
 }
 
 template <int BITS, int BN>
@@ -801,20 +856,23 @@ bool stream_launch(LinArgs &p, const tcg_mx_t &x, const tcg_mx_t &w)
     p.tiles_n = (p.outs + TILE_N - 1) / TILE_N;
     p.stages_k = (p.atoms + S::ATOMS - 1) / S::ATOMS;
     const long long tiles = (long long)p.tiles_n * ((p.rows + BN - 1) / BN);
-    p.split = stream_plan<BITS>(p.rows, tiles, p.stages_k, BN).split;
+    p.split = stream_plan<BITS, BN>(p.rows, tiles, p.stages_k).split;
     p.per = (p.stages_k + p.split - 1) / p.split;
     p.split = (p.stages_k + p.per - 1) / p.per;
-    // fp32 results: accumulators of SUM_K columns
-    p.acc_stages = p.type == GGML_TYPE_F32 ? max((p.per + S::MAX_ACC - 1) / S::MAX_ACC, SUM_K / S::K) : p.per;
-    // Half an SM's shared memory a CTA: one wave leaves room for the next kernel's CTAs to start in (one token 4096 -> 14336
-    // in 4 bits 7.2 us, with all of it 8.3), several waves run two CTAs an SM (60000 outputs 27 us, with one CTA 36). Not
-    // where that leaves fewer than four stages of one wave: 14336 -> 4096 in 8 bits 8.6 us, with half 11.4.
-    const bool half = BN <= 32 && (tiles * p.split > ctx().sms || 4 * S::STAGE + 16 * 1024 <= HALF_SM);
+    // Half an SM's shared memory a CTA: undivided, one wave leaves room for the next kernel's CTAs to start in (one token
+    // 4096 -> 14336 in 4 bits 6.8 us, with all of it 7.6), several waves run two CTAs an SM (60000 outputs 25 us, with one
+    // CTA 31). Not where one wave would have fewer than four stages (4096 -> 14336 in 8 bits 7.5 us, with half 9.1) or K is
+    // split (14336 -> 4096 in 4 bits 7.0 us, with half 7.3).
+    const bool half = BN <= 32 && (tiles * p.split > ctx().sms || (p.split == 1 && 4 * S::STAGE + 16 * 1024 <= HALF_SM));
     const int room = (half ? HALF_SM : MOST_SMEM) - 1024;
     p.split_inv = (65536 + p.split - 1) / p.split;
     const int part = p.split > 1 ? (p.split - 1) * ((BN / 4 + p.split - 1) / p.split) * TILE_N * 16 : 0;
     p.depth = min(MAX_DEPTH, min(max(p.per, 2), (room - part) / S::STAGE));
     const size_t smem = 1024 + p.depth * S::STAGE + part;
+    // fp32 results: accumulators of SUM_K columns, or as many as TMEM holds
+    const int own = p.per - second_issuer(p.per, p.depth);  // stages of the first issuing warp, which has more
+    p.acc_stages = p.type == GGML_TYPE_F32 ? max((own + S::MAX_ACC - 1) / S::MAX_ACC, SUM_K / S::K) : own;
+    p.accs = (own + p.acc_stages - 1) / p.acc_stages;
     if (tiles * p.split > 0x7fffffffll) return fail("tcg_mx_linear: %d rows and %d outputs are too many for one call", p.rows, p.outs);
     constexpr auto fn = mx_stream_kernel<BITS, BN>;
     if (!allow_smem<fn>(MOST_SMEM)) return false;
@@ -843,7 +901,7 @@ bool linear_go(LinArgs &p, const tcg_mx_t &x, const tcg_mx_t &w)
     const int stages = (p.atoms + 1) / 2;
     const long long wide = (long long)((p.rows + 255) / 256) * ((p.outs + 255) / 256);
     const long long tiles = (long long)((p.rows + 127) / 128) * ((p.outs + 127) / 128);
-    if (pair_ns<BITS>(wide, stages) < stream_plan<BITS>(p.rows, tiles, stages, 128).ns)
+    if (pair_ns<BITS>(wide, stages) < stream_plan<BITS, 128>(p.rows, tiles, stages).ns)
         return lm_by_type((ggml_type_t)p.type, [&](auto v) { return pair_launch<decltype(v), BITS>(p, x, w); });
     return stream_launch<BITS, 128>(p, x, w);
 }
