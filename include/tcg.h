@@ -361,8 +361,9 @@ bool tcg_mx_dequantize(void *y, const tcg_mx_t *m, int64_t ld, ggml_type_t t);
  * bias fp32 [outs] or NULL, y [rows, outs]. Products are exact; the tensor core
  * adds 32 columns (x in 8 bits) or 64 (4 bits) at a time to a sum of 24 bits,
  * cutting what lies below (F32 results: such sums of 4096 columns each, or of
- * more where they have no room, are added up); the sum is rounded once to t. What stands behind cols in the codes must be
- * 0, with any scale but 255. y must not overlap x or w. */
+ * more where they have no room, are added up); the sum is rounded once to t.
+ * What stands behind cols in the codes must be 0, with any scale but 255.
+ * y must not overlap x or w. */
 bool tcg_mx_linear(void *y, const tcg_mx_t *x, const tcg_mx_t *w, const float *bias, int64_t ld_y, ggml_type_t t);
 /* The residual's addition and the root-mean-square norm of the sum, in one
  * pass over n_tok rows of cols columns (at most TCG_NORM_MAX_COLS):

@@ -666,6 +666,12 @@ extern "C" bool tcg_add_rms_norm(void *h, void *y, const tcg_mx_t *mx, const voi
         if (!mx_rows(who, "x", x, n_tok, cols, ld_x, t) || (r && !mx_rows(who, "r", r, n_tok, cols, ld_r, t)) ||
             (h && !mx_rows(who, "h", h, n_tok, cols, ld_h, t)) || (y && !mx_rows(who, "y", y, n_tok, cols, ld_y, t)))
             return false;
+        // In place, a row's results must fall on the row itself.
+        const auto in_place = [&](const void *o, int64_t ld) {
+            return !o || n_tok == 1 || ((o != x || ld == ld_x) && (o != r || ld == ld_r));
+        };
+        if (h && h == y) return fail("%s: h and y are the same rows", who);
+        if (!in_place(h, ld_h) || !in_place(y, ld_y)) return fail("%s: in place with another stride", who);
         if ((y || mx) && (!w || (uintptr_t)w % 4)) return fail("%s: no weights, or misaligned ones", who);
     }
     if (!lm_ready(who)) return false;

@@ -88,6 +88,17 @@ def test_norm_refusals():
         _refused(*norm(**bad))
 
 
+@pytest.mark.parametrize("bad, about", [
+    (dict(h=P, y=P), "same rows"), (dict(h=P, y=P, n=1), "same rows"), (dict(h=P, x=P, ldh=128), "stride"),
+    (dict(h=3 * P, y=P, x=P, ldx=128), "stride"), (dict(h=P, x=2 * P, res=P, ldr=65), "stride"),
+    (dict(h=2 * P, y=P, x=3 * P, res=P, ldy=100), "stride"), (dict(h=P, y=2 * P, x=P, res=P, ldr=65), "stride")], ids=str)
+def test_norm_in_place_refusals(bad, about):
+    """Outputs over inputs only row on row, and never one over the other."""
+    a = dict(h=None, y=None, x=5 * P, res=None, n=3, ldh=64, ldy=64, ldx=64, ldr=64) | bad
+    _refused(tcg.lib().tcg_add_rms_norm, a["h"], a["y"], None, a["x"], a["res"], P, 1e-6, a["n"], 64, a["ldh"], a["ldy"], a["ldx"],
+             a["ldr"], 0, about=about)
+
+
 def test_without_a_device():
     L, got, r = tcg.lib(), {}, C.byref
 
@@ -96,7 +107,7 @@ def test_without_a_device():
         got["quantize"] = (L.tcg_mx_quantize(r(m), P, 64, 0), tcg.err())
         got["dequantize"] = (L.tcg_mx_dequantize(P, r(m), 64, 0), tcg.err())
         got["linear"] = (L.tcg_mx_linear(P, r(m), r(w), None, 64, 0), tcg.err())
-        got["norm"] = (L.tcg_add_rms_norm(P, P, r(m), P, P, P, 1e-6, 3, 64, 64, 64, 64, 64, 0), tcg.err())
+        got["norm"] = (L.tcg_add_rms_norm(P, 2 * P, r(m), P, P, P, 1e-6, 3, 64, 64, 64, 64, 64, 0), tcg.err())
         # nothing to do is still nothing without a device
         got["none"] = (L.tcg_mx_quantize(r(_mx(rows=0, codes=None, scales=None)), None, 64, 0), tcg.err())
 
