@@ -11,9 +11,9 @@
 // where they have not (one value in 2^16 or so), the warp takes its values again as y + rest, good to 2^-46, and makes y's
 // last bit odd where a rest is left: rounding that once more cannot meet a tie that is none.
 //
-// All three are bound by memory: 14336 x 4096 fp32 values quantised to 4 bits in 39.4 us (6.8 TB/s), read back to bf16 in
-// 25.8 us (5.8 TB/s, what a fill of the same bytes reaches); 4096 rows of 4096 fp32 values with their residual to 8 bits in
-// 39.2 us (5.6 TB/s: its second pass over the row waits for the sum). One token's norm takes 3.0 us, 1.8 of them the launch.
+// All three are bound by memory: 14336 x 4096 fp32 values quantised to 4 bits in 39 us (6.8 TB/s), read back to bf16 in
+// 25.2 us (5.9 TB/s, what a fill of the same bytes reaches); 4096 rows of 4096 fp32 values with their residual to 8 bits in
+// 38.6 us (5.7 TB/s: its second pass over the row waits for the sum). One token's norm takes 3.0 us, 1.8 of them the launch.
 #include "mx.cuh"
 
 #include <cuda_fp4.h>
@@ -21,11 +21,13 @@
 
 #include <string.h>
 
+#include <type_traits>
+
 namespace tcg {
 namespace {
 
 constexpr int LANE = 8;             // consecutive columns of a lane: 4 lanes make a block, 16 a word of scales
-constexpr int MX_WARPS = 8;
+constexpr int MX_WARPS = 4;         // of a CTA (1501 rows of 4100 16-bit values, 4103 apart, to 4 bits 5.7 us, with 8 5.9)
 
 // 8 elements as they are held.
 template <typename T>
@@ -66,8 +68,7 @@ __device__ __forceinline__ void shift_bytes(uint32_t (&k)[N + 4], uint32_t off)
 }
 
 // A lane's 8 elements of a row, of which `left` exist (the others are 0). A row that starts on no 8-byte boundary is read
-// by the aligned 16-byte words around it and shifted, where those lie in [lo, hi), the array (1501 rows of 4100 16-bit values,
-// 4103 apart, quantised: 6.4 us, element by element 8.1).
+// by the aligned 16-byte words around it and shifted, where those lie in [lo, hi), the array (1501 rows of 4100 quantised: 6.4 us, element by element 8.1).
 // VEC: rows start on 16-byte boundaries.
 template <bool VEC, typename T>
 __device__ __forceinline__ Raw<T> load_row(const T *p, long long left, const void *lo, const void *hi)
@@ -362,9 +363,10 @@ __global__ void __launch_bounds__(32 * MX_WARPS) mx_quantize_kernel(const __grid
             if (first + 32 * i < p.rows) at[i] = word[i];
 }
 
-// C times 256 columns a warp, so that more than one row's 128 bytes of codes and its scales are under way.
+// C times 256 columns a warp, so that more than one row's 128 bytes of codes and its scales are under way. Ten CTAs' registers
+// of an SM for aligned rows: 14336 x 4096 from 4 bits to bf16 25.2 us, nine 25.7, twelve (with spills) 30.2.
 template <typename T, int C, bool VEC>
-__global__ void __launch_bounds__(32 * MX_WARPS) mx_dequantize_kernel(const __grid_constant__ QuantArgs p)
+__global__ void __launch_bounds__(32 * MX_WARPS, VEC ? 10 : 1) mx_dequantize_kernel(const __grid_constant__ QuantArgs p)
 {
     lm_begin();
     QuantTask t = quant_task(p);
@@ -456,7 +458,7 @@ struct NormArgs {
     MxOut o;                        // codes NULL: none
     int rows, cols;
     double eps, mean;               // 1 / cols
-    bool vec;
+    bool vec_in, vec_out;
 };
 
 // v * rstd * w to 2^-46, the last of its 24 bits odd where something is left.
@@ -476,11 +478,13 @@ __device__ __forceinline__ float normed_odd(float v, float r_hi, float r_lo, flo
 
 // A row's columns are dealt out to G threads (a warp's 32, or the CTA's, at most MOST), N pieces of 8 consecutive columns each.
 // CTAs an SM that registers are kept for. 4096 rows of 4096 fp32 values with their residual, to 8 bits: two pieces a thread of 256
-// and five CTAs 39.9 us (5.5 TB/s); two of 512 and two CTAs 40.9; one of 512 and three 43.2; four of 128 and five 50.0.
-constexpr int norm_ctas(int n, int most) { return n == 2 && most == 256 ? 5 : 1; }
+// and four CTAs 38.6 us (5.7 TB/s), five (with spills) 40.3; two of 512 and two CTAs 40.9; one of 512 and three 43.2; four of 128
+// and five 50.0. Without codes five fit.
+constexpr int norm_ctas(int n, int most, bool mx) { return n == 2 && most == 256 ? mx ? 4 : 5 : 1; }
 
-template <typename T, int N, int MOST, bool VEC>
-__global__ void __launch_bounds__(MOST == 32 ? 256 : MOST, norm_ctas(N, MOST)) add_rms_norm_kernel(const __grid_constant__ NormArgs p)
+// VIN, VOUT: rows of x, r and w, and of h and y, start on 16-byte boundaries. MX: there are codes to write.
+template <typename T, int N, int MOST, bool VIN, bool VOUT, bool MX>
+__global__ void __launch_bounds__(MOST == 32 ? 256 : MOST, norm_ctas(N, MOST, MX)) add_rms_norm_kernel(const __grid_constant__ NormArgs p)
 {
     constexpr bool WARP = MOST == 32;
     const int G = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
@@ -492,12 +496,12 @@ __global__ void __launch_bounds__(MOST == 32 ? 256 : MOST, norm_ctas(N, MOST)) a
 #pragma unroll
     for (int k = 0; k < N; k++) {
         const long long col = (long long)(k * G + t) * LANE;
-        h[k] = load_row<VEC>((const T *)p.x + row * p.ldx + col, p.cols - col, p.x, p.x_end);
-        if (p.r) r[k] = load_row<VEC>((const T *)p.r + row * p.ldr + col, p.cols - col, p.r, p.r_end);
+        h[k] = load_row<VIN>((const T *)p.x + row * p.ldx + col, p.cols - col, p.x, p.x_end);
+        if (p.r) r[k] = load_row<VIN>((const T *)p.r + row * p.ldr + col, p.cols - col, p.r, p.r_end);
     }
     // a thread of one piece has the registers to ask for its weights now
     Raw<float> w0;
-    if (N == 1 && p.w) w0 = load_row<VEC>(p.w + (long long)t * LANE, p.cols - (long long)t * LANE, p.w, p.w + p.cols);
+    if (N == 1 && p.w) w0 = load_row<VIN>(p.w + (long long)t * LANE, p.cols - (long long)t * LANE, p.w, p.w + p.cols);
     double ss = 0.0;
 #pragma unroll
     for (int k = 0; k < N; k++) {
@@ -518,9 +522,9 @@ __global__ void __launch_bounds__(MOST == 32 ? 256 : MOST, norm_ctas(N, MOST)) a
 #pragma unroll
         for (int k = 0; k < N; k++) {
             const long long col = (long long)(k * G + t) * LANE;
-            store_row<VEC>((T *)p.h + row * p.ldh + col, p.cols - col, h[k]);
+            store_row<VOUT>((T *)p.h + row * p.ldh + col, p.cols - col, h[k]);
         }
-    if (!p.y && !p.o.codes) return;
+    if (!MX && !p.y) return;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
     if (!WARP) {
@@ -538,17 +542,22 @@ __global__ void __launch_bounds__(MOST == 32 ? 256 : MOST, norm_ctas(N, MOST)) a
 #pragma unroll
     for (int k = 0; k < N; k++) {
         const long long col = (long long)(k * G + t) * LANE;
-        const Raw<float> w = N == 1 ? w0 : load_row<VEC>(p.w + col, p.cols - col, p.w, p.w + p.cols);
+        const Raw<float> w = N == 1 ? w0 : load_row<VIN>(p.w + col, p.cols - col, p.w, p.w + p.cols);
         float v[LANE], y[LANE];
         unpack(h[k], v);
+        if (plain) {
 #pragma unroll
-        for (int i = 0; i < LANE; i++) y[i] = plain ? v[i] * r_hi * w.at(i) : (float)(v[i] * rstd * w.at(i));
+            for (int i = 0; i < LANE; i++) y[i] = v[i] * r_hi * w.at(i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < LANE; i++) y[i] = (float)(v[i] * rstd * w.at(i));
+        }
         if (col + LANE > p.cols)
 #pragma unroll
             for (int i = 0; i < LANE; i++)
                 if (col + i >= p.cols) y[i] = 0.0f;                 // 0 * rstd may be NaN there
-        if (p.y) store_row<VEC>((T *)p.y + row * p.ldy + col, p.cols - col, packed<T>(y));
-        if (!p.o.codes) continue;
+        if (p.y) store_row<VOUT>((T *)p.y + row * p.ldy + col, p.cols - col, packed<T>(y));
+        if (!MX) continue;
         uint32_t word;
         if (!plain || !mx_store8_near(p.o, row, col, y, word)) {
 #pragma unroll
@@ -572,8 +581,16 @@ template <typename T, int N, int MOST>
 bool norm_launch(const NormArgs &p, int threads)
 {
     const unsigned grid = MOST == 32 ? ceil_div(p.rows, threads / 32) : (unsigned)p.rows;
-    void (*fn)(const NormArgs) = p.vec ? add_rms_norm_kernel<T, N, MOST, true> : add_rms_norm_kernel<T, N, MOST, false>;
-    TCG_CUDA(launch_pdl(fn, dim3(grid), dim3(threads), 0, ctx().cur, p));
+    const auto launch = [&](auto vin, auto vout, auto codes) {
+        constexpr auto fn = add_rms_norm_kernel<T, N, MOST, decltype(vin)::value, decltype(vout)::value, decltype(codes)::value>;
+        return launch_pdl(fn, dim3(grid), dim3(threads), 0, ctx().cur, p);
+    };
+    const auto by_codes = [&](auto vin, auto vout) {
+        return p.o.codes ? launch(vin, vout, std::true_type()) : launch(vin, vout, std::false_type());
+    };
+    const std::true_type yes;
+    const std::false_type no;
+    TCG_CUDA(!p.vec_in ? by_codes(no, no) : p.vec_out ? by_codes(yes, yes) : by_codes(yes, no));
     return true;
 }
 
@@ -683,7 +700,8 @@ extern "C" bool tcg_add_rms_norm(void *h, void *y, const tcg_mx_t *mx, const voi
     p.rows = n_tok, p.cols = cols;
     p.eps = eps;
     p.mean = 1.0 / cols;
-    p.vec = on_16(x, ld_x, t) && (!r || on_16(r, ld_r, t)) && (!h || on_16(h, ld_h, t)) && (!y || on_16(y, ld_y, t)) && (uintptr_t)w % 16 == 0;
+    p.vec_in = on_16(x, ld_x, t) && (!r || on_16(r, ld_r, t)) && (uintptr_t)w % 16 == 0;
+    p.vec_out = (!h || on_16(h, ld_h, t)) && (!y || on_16(y, ld_y, t));
     const int64_t size = (int64_t)lm_type_size(t);
     p.x_end = (const char *)x + ((n_tok - 1) * ld_x + cols) * size;
     p.r_end = (const char *)r + ((n_tok - 1) * ld_r + cols) * size;
