@@ -171,11 +171,54 @@ struct LinArgs {
     int tiles_n, tiles_m, split, per;   // CTAs of a tile, stages of each
     unsigned split_inv;                 // 2^16 / split, rounded up
     int tiles, whole;                   // of the pairs: how many, from which on halves
-    int acc_stages, accs;               // stages of an accumulator; accumulators of an issuing warp
+    int acc_stages, accs;               // stages of an accumulator; accumulators of an issuing warp, at most
+    int used[2][2];                     // accumulators of the first and the second issuing warp: of a tile's other CTAs, of its last
     int depth;                          // stages in shared memory
     int type;
     bool pairs;                         // two 16-bit results of a row as one word
 };
+
+// N columns of two accumulators, with one wait.
+__device__ __forceinline__ void tmem_ld_two(uint32_t at, uint32_t bt, uint32_t (&a)[8], uint32_t (&b)[8])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%16];\n\t"
+                 "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8,%9,%10,%11,%12,%13,%14,%15}, [%17];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]), "=r"(a[4]), "=r"(a[5]), "=r"(a[6]), "=r"(a[7]), "=r"(b[0]),
+                   "=r"(b[1]), "=r"(b[2]), "=r"(b[3]), "=r"(b[4]), "=r"(b[5]), "=r"(b[6]), "=r"(b[7])
+                 : "r"(at), "r"(bt)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld_two(uint32_t at, uint32_t bt, uint32_t (&a)[16], uint32_t (&b)[16])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n\t"
+                 "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%33];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]), "=r"(a[4]), "=r"(a[5]), "=r"(a[6]), "=r"(a[7]), "=r"(a[8]),
+                   "=r"(a[9]), "=r"(a[10]), "=r"(a[11]), "=r"(a[12]), "=r"(a[13]), "=r"(a[14]), "=r"(a[15]), "=r"(b[0]),
+                   "=r"(b[1]), "=r"(b[2]), "=r"(b[3]), "=r"(b[4]), "=r"(b[5]), "=r"(b[6]), "=r"(b[7]), "=r"(b[8]), "=r"(b[9]),
+                   "=r"(b[10]), "=r"(b[11]), "=r"(b[12]), "=r"(b[13]), "=r"(b[14]), "=r"(b[15])
+                 : "r"(at), "r"(bt)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld_two(uint32_t at, uint32_t bt, uint32_t (&a)[32], uint32_t (&b)[32])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%64];\n\t"
+                 "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+                 "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%65];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]), "=r"(a[4]), "=r"(a[5]), "=r"(a[6]), "=r"(a[7]), "=r"(a[8]),
+                   "=r"(a[9]), "=r"(a[10]), "=r"(a[11]), "=r"(a[12]), "=r"(a[13]), "=r"(a[14]), "=r"(a[15]), "=r"(a[16]),
+                   "=r"(a[17]), "=r"(a[18]), "=r"(a[19]), "=r"(a[20]), "=r"(a[21]), "=r"(a[22]), "=r"(a[23]), "=r"(a[24]),
+                   "=r"(a[25]), "=r"(a[26]), "=r"(a[27]), "=r"(a[28]), "=r"(a[29]), "=r"(a[30]), "=r"(a[31]), "=r"(b[0]),
+                   "=r"(b[1]), "=r"(b[2]), "=r"(b[3]), "=r"(b[4]), "=r"(b[5]), "=r"(b[6]), "=r"(b[7]), "=r"(b[8]), "=r"(b[9]),
+                   "=r"(b[10]), "=r"(b[11]), "=r"(b[12]), "=r"(b[13]), "=r"(b[14]), "=r"(b[15]), "=r"(b[16]), "=r"(b[17]),
+                   "=r"(b[18]), "=r"(b[19]), "=r"(b[20]), "=r"(b[21]), "=r"(b[22]), "=r"(b[23]), "=r"(b[24]), "=r"(b[25]),
+                   "=r"(b[26]), "=r"(b[27]), "=r"(b[28]), "=r"(b[29]), "=r"(b[30]), "=r"(b[31])
+                 : "r"(at), "r"(bt)
+                 : "memory");
+}
 
 // Results of rows row, row + 1 .. of x (as far as there are such rows) for weight row n.
 template <int STEP, typename T>
@@ -204,7 +247,7 @@ struct Stream {
 };
 
 // Of a CTA's stages those that the second issuing warp takes: slots are 0 .. depth - 1 in turn, the odd ones are its.
-__host__ __device__ __forceinline__ int second_issuer(int stages, int depth)
+int second_issuer(int stages, int depth)
 {
     const int cycles = stages / depth;
     return cycles * (depth / 2) + (stages - cycles * depth) / 2;
@@ -328,8 +371,7 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
     ok = wait_for(done, 0, abort, p.err, false) && ok && !*abort;
     fence_after();
     // accumulators that hold something: the first warp's, then the second's
-    const int own1 = second_issuer(count, p.depth), accs0 = (count - own1 - 1) / p.acc_stages + 1;
-    const int accs = accs0 + (own1 + p.acc_stages - 1) / p.acc_stages;
+    const int last = rank == p.split - 1, accs0 = p.used[last][0], accs = accs0 + p.used[last][1];
     const uint32_t lane_base = tmem + ((uint32_t)(warp & 3) << 21);
     // Two warps share 32 TMEM lanes (weight rows) and take every second step of columns (x's rows).
     const int t = tid & 127, half = tid >> 7;
@@ -351,17 +393,20 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
         const int per_rank = over_split(BN / 4 + p.split - 1);
         float4 *const sent = (float4 *)smem;
         const float4 *const part = (const float4 *)(smem + p.depth * S::STAGE);
-        constexpr int STEP = BN < 32 ? 8 : 16;
+        constexpr int STEP = BN < 32 ? 8 : BN / 2 < 32 ? BN / 2 : 32;
 #pragma unroll 1
         for (int c = half * STEP; c < BN && m0 + c < p.rows; c += 2 * STEP) {
             float v[STEP] = {};
-            for (int i = 0; i < accs; i++) {
-                uint32_t r[STEP];
-                const int acc = i < accs0 ? i : p.accs + i - accs0;
-                if constexpr (STEP == 8) tmem_ld8(lane_base + acc * BN + c, r);
-                else tmem_ld16(lane_base + acc * BN + c, r);
+            const auto acc = [&](int i) { return lane_base + (i < accs0 ? i : p.accs + i - accs0) * BN + c; };
+            for (int i = 0; i < accs; i += 2) {
+                uint32_t r[STEP], q[STEP];
+                const bool two = i + 1 < accs;
+                tmem_ld_two(acc(i), acc(two ? i + 1 : i), r, q);
 #pragma unroll
                 for (int j = 0; j < STEP; j++) v[j] += __uint_as_float(r[j]);
+                if (two)
+#pragma unroll
+                    for (int j = 0; j < STEP; j++) v[j] += __uint_as_float(q[j]);
             }
             if (p.split > 1) {
 #pragma unroll
@@ -373,7 +418,7 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
                 put_columns<STEP, T>(p, m0 + c, n, bias, v);
             }
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        if (p.split > 1) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         free_tmem();
         if (p.split == 1) return;
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");     // the peers' barriers are there
@@ -873,6 +918,11 @@ bool stream_launch(LinArgs &p, const tcg_mx_t &x, const tcg_mx_t &w)
     const int own = p.per - second_issuer(p.per, p.depth);  // stages of the first issuing warp, which has more
     p.acc_stages = p.type == GGML_TYPE_F32 ? max((own + S::MAX_ACC - 1) / S::MAX_ACC, SUM_K / S::K) : own;
     p.accs = (own + p.acc_stages - 1) / p.acc_stages;
+    for (int last = 0; last < 2; last++) {
+        const int count = last ? p.stages_k - (p.split - 1) * p.per : p.per, second = second_issuer(count, p.depth);
+        p.used[last][0] = (count - second + p.acc_stages - 1) / p.acc_stages;
+        p.used[last][1] = (second + p.acc_stages - 1) / p.acc_stages;
+    }
     if (tiles * p.split > 0x7fffffffll) return fail("tcg_mx_linear: %d rows and %d outputs are too many for one call", p.rows, p.outs);
     constexpr auto fn = mx_stream_kernel<BITS, BN>;
     if (!allow_smem<fn>(MOST_SMEM)) return false;
