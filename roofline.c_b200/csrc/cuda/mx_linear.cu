@@ -306,9 +306,10 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
     auto atoms_of = [&](int k) { return min(S::ATOMS, p.atoms - (k_begin + k) * S::ATOMS); };
     // warp indices as the compiler can see them to be uniform
     const int role = __shfl_sync(0xFFFFFFFFu, warp, 0);
+    int loads = 0;
     if (role == 0) {
-        int k = 0, slot = 0, phase = 1;
-        for (; k < count; k++) {
+        int slot = 0, phase = 1;
+        for (int &k = loads; k < count; k++) {
             const int kk = k_begin + k, na = atoms_of(k);
             ok = wait_lane(empty + 8 * slot, phase, abort, p.err);
             const uint32_t bar = full + 8 * slot, a = at(slot), b = a + S::A, sa = b + S::B, sb = sa + S::SF;
@@ -326,10 +327,6 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
             if (!ok) break;
             if (++slot == p.depth) slot = 0, phase ^= 1;
         }
-        // copies in flight land before the CTA ends (the one that it gave up on may have been issued, too)
-        if (!ok)
-            for (int j = max(0, k - p.depth); j <= k; j++)
-                wait_for(full + 8 * (j % p.depth), (j / p.depth) & 1, abort, p.err, false);
     } else if (role <= ISSUERS) {
         const int turn = role - 1;
         const uint32_t id = mx_idesc<BITS>(BN, TILE_N), sfa = tmem + S::SF_COL + turn * S::SF_COLS, sfb = sfa + 4 * S::ATOMS;
@@ -369,6 +366,11 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
     }
     __syncwarp();
     ok = wait_for(done, 0, abort, p.err, false) && ok && !*abort;
+    // After a wait that was given up, copies in flight land before the CTA ends (the one that the loading warp gave up on may
+    // have been issued, too).
+    if (!ok && role == 0)
+        for (int j = max(0, loads - p.depth); j <= min(loads, count - 1); j++)
+            wait_for(full + 8 * (j % p.depth), (j / p.depth) & 1, abort, p.err, false);
     fence_after();
     // accumulators that hold something: the first warp's, then the second's
     const int last = rank == p.split - 1, accs0 = p.used[last][0], accs = accs0 + p.used[last][1];
