@@ -424,9 +424,10 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
         free_tmem();
         if (p.split == 1) return;
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");     // the peers' barriers are there
-        if (tid < p.split && tid < groups && tid != rank)
-            push(peer_addr(su32(part + (rank - (rank > tid)) * per_rank * TILE_N), tid), su32(sent + tid * per_rank * TILE_N),
-                 over_split(groups - tid + p.split - 1) * TILE_N * 16, peer_addr(join, tid));
+        const int to = tid - 128;                       // not by warp 0, which gives the TMEM back meanwhile
+        if (to >= 0 && to < p.split && to < groups && to != rank)
+            push(peer_addr(su32(part + (rank - (rank > to)) * per_rank * TILE_N), to), su32(sent + to * per_rank * TILE_N),
+                 over_split(groups - to + p.split - 1) * TILE_N * 16, peer_addr(join, to));
         __syncwarp();
         const bool came = !mine || wait_for(join, 0, abort, p.err, false);
         ok = ok && came;
@@ -436,6 +437,7 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
             float sum[4] = {};
 #pragma unroll
             for (int s = 0; s < MAX_SPLIT; s++) {
+                if (s == 4 && p.split <= 4) break;          // one branch; the parts before it are loaded together
                 const float4 *const from = s == rank ? sent + rank * per_rank * TILE_N : part + (s - (s > rank)) * per_rank * TILE_N;
                 const float4 v = s < p.split ? from[i * TILE_N + t] : make_float4(0, 0, 0, 0);
                 sum[0] += v.x, sum[1] += v.y, sum[2] += v.z, sum[3] += v.w;
