@@ -13,7 +13,7 @@
 //   Few rows (mx_stream_kernel): bound by reading the weights. One wave of CTAs, K split over the CTAs of a cluster where the
 //     tiles are fewer than the SMs; parts meet in shared memory. One token 4096 -> 14336, x in 8 bits 7.5 us (31.2 MB: 4.2
 //     TB/s, of which ~3.5 us are start, first bytes and end), in 4 bits 6.6; 60000 outputs in 4 bits 25 us (5.2 TB/s); 64 rows
-//     of 14336 -> 4096 in 8 bits 11.1 us.
+//     of 14336 -> 4096 in 8 bits 10.9 us.
 //   Many (mx_pair_kernel): bound by the tensor core and the power that it takes. CTA pairs on tiles of 256 x 256, two
 //     accumulators. 4096 rows of 4096 -> 14336 in 4 bits 98 us (4.9 PFLOP/s at ~1.6 GHz: 60% of the cycles; the last round
 //     is 8 of 74 pairs' worth), 8192^3 189 us (5.8); 2048 rows of 14336 -> 4096 in 8 bits, fp32 results, 93 us (2.6: two
