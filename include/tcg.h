@@ -368,7 +368,7 @@ bool tcg_mx_linear(void *y, const tcg_mx_t *x, const tcg_mx_t *w, const float *b
 /* The residual's addition and the root-mean-square norm of the sum, in one
  * pass over n_tok rows of cols columns (at most TCG_NORM_MAX_COLS):
  *   h = x + r, rounded to t (r NULL: h = x),
- *   v = h / sqrt(mean(h^2) + eps) * w (w fp32 [cols]),
+ *   v = h / sqrt(mean(h^2) + eps) * w (w fp32 [cols], not read for h alone),
  * out as y (v to 4 roundings of fp32, rounded to t) and/or as mx (the codes of
  * v itself, where v is of fp32's normal numbers). Each of h,
  * y and mx may be NULL, not all of them. h and y may be x or r in place (the

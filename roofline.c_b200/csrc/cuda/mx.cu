@@ -694,13 +694,13 @@ extern "C" bool tcg_add_rms_norm(void *h, void *y, const tcg_mx_t *mx, const voi
     if (!lm_ready(who)) return false;
     if (!n_tok) return true;
     NormArgs p = {};
-    p.x = x, p.r = r, p.h = h, p.y = y, p.w = w;
+    p.x = x, p.r = r, p.h = h, p.y = y, p.w = y || mx ? w : nullptr;        // the sum alone reads no weights, whatever w is
     p.ldx = ld_x, p.ldr = ld_r, p.ldh = ld_h, p.ldy = ld_y;
     if (mx) p.o = mx_out(*mx);
     p.rows = n_tok, p.cols = cols;
     p.eps = eps;
     p.mean = 1.0 / cols;
-    p.vec_in = on_16(x, ld_x, t) && (!r || on_16(r, ld_r, t)) && (uintptr_t)w % 16 == 0;
+    p.vec_in = on_16(x, ld_x, t) && (!r || on_16(r, ld_r, t)) && (uintptr_t)p.w % 16 == 0;
     p.vec_out = (!h || on_16(h, ld_h, t)) && (!y || on_16(y, ld_y, t));
     const int64_t size = (int64_t)lm_type_size(t);
     p.x_end = (const char *)x + ((n_tok - 1) * ld_x + cols) * size;

@@ -305,6 +305,17 @@ def test_add_and_norm(lib, rows, cols, t, pad, offset):
     assert torch.equal(iv, h)
 
 
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 256), (2, 4096), (5, 20000), (400, 300), (300, 4096)])
+def test_the_sum_alone_reads_no_weights(lib, rows, cols):
+    """With h alone asked for, w may be any address: one that is not there, one that no float stands at."""
+    g = gen(cols)
+    x, r, h = randn(g, rows, cols), randn(g, rows, cols), torch.zeros((rows, cols), device="cuda")
+    for w in (None, 1, 4096, h.data_ptr() + 2):
+        h.zero_()
+        call(lib.tcg_add_rms_norm, h.data_ptr(), None, None, x.data_ptr(), r.data_ptr(), w, 1e-6, rows, cols, cols, 0, cols, cols, tcg.F32)
+        assert torch.equal(h, x + r)
+
+
 @pytest.mark.parametrize("bits", [4, 8])
 def test_norm_codes_next_to_borders(lib, bits):
     """Weights that put every value within an fp32 step of a border between codes, or of a power of two for the scale: the
