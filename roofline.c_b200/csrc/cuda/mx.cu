@@ -8,8 +8,8 @@
 // The norm's codes have to be those of y = h / sqrt(mean(h^2) + eps) * w, not of an fp32 approximation that may lie on
 // the other side of the border between two codes. The sum of squares and the root are taken in 64 bits; the products in
 // fp32, within 2^-21 of y. Where y (1 - 2^-21) and y (1 + 2^-21) have the same code, that is y's (rounding keeps order);
-// where they have not (one value in 2^16 or so), the warp takes its values again as y + rest, good to 2^-46, and makes y's
-// last bit odd where a rest is left: rounding that once more cannot meet a tie that is none.
+// where they have not (one value in 2^16 or so), the warp takes its values again in 64 bits, cut to fp32 with the last bit odd
+// where a rest is left: rounding that once more cannot meet a tie that is none.
 //
 // All three are bound by memory: 14336 x 4096 fp32 values quantised to 4 bits in 39 us (6.8 TB/s), read back to bf16 in
 // 25.2 us (5.9 TB/s, what a fill of the same bytes reaches); 4096 rows of 4096 fp32 values with their residual to 8 bits in
@@ -287,13 +287,13 @@ __device__ __forceinline__ uint32_t mx_store8(const MxOut &o, long long r, long 
     return mx_put(o, r, col, mx_codes(q, o.bits), s);
 }
 
-// The same for values known to within 2^-22 of themselves: false (and nothing stored) where some lane's codes or scales
-// depend on more than that.
+// The same for values known to within 2^-22 of themselves (an infinity may be a number that was rounded up): false (and
+// nothing stored) where some lane's codes or scales depend on more than that.
 __device__ __forceinline__ bool mx_store8_near(const MxOut &o, long long r, long long col, const float (&x)[LANE], uint32_t &word)
 {
     constexpr float LOW = 1.0f - 0x1p-21f, HIGH = 1.0f + 0x1p-21f;
     const uint32_t top = mx_top(x);
-    const uint32_t s = mx_scale(__float_as_uint(__uint_as_float(top) * LOW), o.bits);
+    const uint32_t s = mx_scale(__float_as_uint(__uint_as_float(min(top, 0x7F7FFFFFu)) * LOW), o.bits);
     const float low = mx_inverse(s) * LOW, high = mx_inverse(s) * HIGH;     // inverse is a power of two: both are exact
     float q[LANE];
 #pragma unroll
@@ -461,19 +461,13 @@ struct NormArgs {
     bool vec_in, vec_out;
 };
 
-// v * rstd * w to 2^-46, the last of its 24 bits odd where something is left.
-__device__ __forceinline__ float normed_odd(float v, float r_hi, float r_lo, float w)
+// v * rstd * w from 64 bits, cut to fp32 with its last bit odd where something is left. (Infinities and NaN as they are.)
+__device__ __forceinline__ float normed_odd(float v, double rstd, float w)
 {
-    const float q = v * r_hi, ql = fmaf(v, r_lo, fmaf(v, r_hi, -q));
-    const float y = q * w, rest = fmaf(ql, w, fmaf(q, w, -y));
-    const float near = y + rest, left = rest - (near - y);
-    uint32_t b = __float_as_uint(near);
-    if (left != 0.0f && (b & 0x7FFFFFFFu) < 0x7F800000u) {
-        // a magnitude rounded up goes back by one, then the last bit says that something is left
-        if (near != 0.0f && (__float_as_uint(left) ^ b) >> 31) b -= 1;
-        b |= 1;
-    }
-    return __uint_as_float(b);
+    const double d = v * rstd * w;
+    if (!(fabs(d) <= 0x1.fffffep+127)) return (float)d;
+    const float y = __double2float_rz(d);
+    return (double)y == d ? y : __uint_as_float(__float_as_uint(y) | 1);
 }
 
 // A row's columns are dealt out to G threads (a warp's 32, or the CTA's, at most MOST), N pieces of 8 consecutive columns each.
@@ -503,6 +497,7 @@ __global__ void __launch_bounds__(MOST == 32 ? 256 : MOST, norm_ctas(N, MOST, MX
     Raw<float> w0;
     if (N == 1 && p.w) w0 = load_row<VIN>(p.w + (long long)t * LANE, p.cols - (long long)t * LANE, p.w, p.w + p.cols);
     double ss = 0.0;
+    float low = INFINITY;               // the smallest magnitude
 #pragma unroll
     for (int k = 0; k < N; k++) {
         float v[LANE];
@@ -517,6 +512,8 @@ __global__ void __launch_bounds__(MOST == 32 ? 256 : MOST, norm_ctas(N, MOST, MX
         }
 #pragma unroll
         for (int i = 0; i < LANE; i++) ss = fma((double)v[i], (double)v[i], ss);
+#pragma unroll
+        for (int i = 0; i < LANE; i++) low = fminf(low, fabsf(v[i]));
     }
     if (p.h)
 #pragma unroll
@@ -536,16 +533,22 @@ __global__ void __launch_bounds__(MOST == 32 ? 256 : MOST, norm_ctas(N, MOST, MX
         for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
     }
     const double rstd = rsqrt(fma(ss, p.mean, p.eps));
-    const float r_hi = (float)rstd, r_lo = (float)(rstd - r_hi);
-    // rows whose root leaves fp32's normal numbers take the product in 64 bits
-    const bool plain = rstd > 1e-30 && rstd < 1e30;
+    const float r_hi = (float)rstd;
+    // Rows whose root leaves fp32's normal numbers take the products in 64 bits. So do a lane's 8 values where one of them,
+    // but for zeros, is so small beside its row that v * r_hi, below 2^-100, may lose bits before a large weight brings it
+    // back. (f16's smallest value is 2^-40 of its largest.)
+    const bool plain = rstd > 1e-30 && rstd < 1e30, look = low * r_hi < 0x1p-100f;
 #pragma unroll
     for (int k = 0; k < N; k++) {
         const long long col = (long long)(k * G + t) * LANE;
         const Raw<float> w = N == 1 ? w0 : load_row<VIN>(p.w + col, p.cols - col, p.w, p.w + p.cols);
         float v[LANE], y[LANE];
         unpack(h[k], v);
-        if (plain) {
+        bool fast = plain;
+        if (!std::is_same<T, __half>::value && look)                // zeros come here, too
+#pragma unroll
+            for (int i = 0; i < LANE; i++) fast = fast && (v[i] == 0.0f || fabsf(v[i]) * r_hi >= 0x1p-100f);
+        if (fast) {
 #pragma unroll
             for (int i = 0; i < LANE; i++) y[i] = v[i] * r_hi * w.at(i);
         } else {
@@ -562,12 +565,7 @@ __global__ void __launch_bounds__(MOST == 32 ? 256 : MOST, norm_ctas(N, MOST, MX
         if (!plain || !mx_store8_near(p.o, row, col, y, word)) {
 #pragma unroll
             for (int i = 0; i < LANE; i++) {
-                if (plain) y[i] = normed_odd(v[i], r_hi, r_lo, w.at(i));
-                else if (fabsf(y[i]) < INFINITY) {
-                    const double d = v[i] * rstd * w.at(i);
-                    y[i] = __double2float_rz(d);
-                    if ((double)y[i] != d) y[i] = __uint_as_float(__float_as_uint(y[i]) | 1);
-                }
+                y[i] = normed_odd(v[i], rstd, w.at(i));
                 if (col + i >= p.cols) y[i] = 0.0f;
             }
             word = mx_store8(p.o, row, col, y);

@@ -362,6 +362,64 @@ def test_norm_of_odd_rows(lib):
     assert (sc[5, :10] == 255).all() and sc[4, 0] == 255 and (sc[4, 1:] == 0).all()
 
 
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,cols", [(3, 256), (2, 4096), (310, 700), (300, 6000), (2, 20000)])
+def test_norm_of_rows_of_unlike_values(lib, rows, cols, t):
+    """Values 40 orders below their own row's size, which large weights bring back to ordinary numbers: the factor between is
+    below fp32's normal numbers, and the results and their codes are those of the formula all the same."""
+    dt, code = TYPES[t]
+    g, eps = gen(rows + cols), float(torch.tensor(1e-6))
+    col = torch.arange(cols, device="cuda")
+    small = col // 32 % 3 == 1
+    x = randn(g, rows, cols, dtype=torch.float64)
+    x = torch.where(x.abs() < 0.05, 0.05, x) * torch.where(small, 1e-22, 1e20)
+    x[:, 64:96] = torch.where(col[64:96] % 5 == 0, 1e-25, 1e18) * x[:, 64:96].sign()     # one block holds both
+    x[:, 70] = 0
+    x = x.to(dt)
+    w = ((randn(g, cols) * 0.1 + 1) * torch.where(small | (col // 32 == 2), 1e10, 1.0)).float()
+    want = normed(x.double(), w, eps)
+    y = torch.zeros_like(x)
+    for bits in (4, 8):
+        m = Held(rows, cols, bits)
+        call(lib.tcg_add_rms_norm, None, y.data_ptr(), C.byref(m.mx()), x.data_ptr(), None, w.data_ptr(), eps, rows, cols, 0, cols, cols, 0, code)
+        assert want.abs()[want != 0].min() > 2.0 ** -126
+        assert ((y.double() - want).abs() <= want.abs() * (4 * U + (half_step(dt) if t == "bf16" else 0))).all()
+        m.check(*quantised(want, bits))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("shift", [-121, 0, 118])
+def test_norm_codes_at_the_ends_of_the_range(lib, bits, shift):
+    """Borders between codes as in test_norm_codes_next_to_borders, down to fp32's smallest normal numbers, where what is left
+    of a product falls below fp32 altogether, and up to the largest, where its fp32 form is an infinity."""
+    g, cols, eps = gen(bits + shift), 4096, float(torch.tensor(1e-6))
+    grid = code_values(bits)
+    mid = (grid[1:] + grid[:-1]) / 2
+    mid = mid[mid > 2.0 ** -5]
+    x = randn(g, 3, cols)
+    x = torch.where(x.abs() < 0.05, 0.05, x)
+    inv = 1 / torch.sqrt((x.double() ** 2).mean(-1, keepdim=True) + eps)
+    pick = mid[torch.randint(0, mid.numel(), (cols,), generator=g).cuda()]
+    pick[::32] = 2.0 ** TOP[bits] * torch.where(torch.rand(cols // 32, generator=g).cuda() < 0.5, 1.0, 2.0)
+    if shift > 0:                                                        # next to the largest number, from below
+        x = torch.where(x.abs() < 1, x.sign() * 1.25, x)
+        inv = 1 / torch.sqrt((x.double() ** 2).mean(-1, keepdim=True) + eps)
+        pick = torch.where(torch.rand(cols, generator=g).cuda() < 0.5, torch.finfo(torch.float32).max, pick.clamp(max=64) * 2.0 ** shift)
+        w = (pick / (x[0].double().abs() * inv[0])).clamp(max=3e38).float()
+        w = torch.nextafter(w, torch.zeros_like(w))
+        x = x[:1]
+    else:
+        w = (pick * 2.0 ** shift / (x[0].double() * inv[0])).float()
+        w = torch.where(torch.rand(cols, generator=g).cuda() < 0.3, torch.nextafter(w, torch.zeros_like(w)), w)
+    want = normed(x.double(), w, eps)
+    assert want[0].abs().min() >= 2.0 ** -126 and want.abs().max() <= torch.finfo(torch.float32).max
+    m = Held(len(x), cols, bits)
+    call(lib.tcg_add_rms_norm, None, None, C.byref(m.mx()), x.data_ptr(), None, w.data_ptr(), eps, len(x), cols, 0, cols, cols, 0, tcg.F32)
+    code, scale = quantised(want, bits)
+    sure = (want.abs() >= 2.0 ** -126).all(-1)                            # rows whose values are all normal numbers
+    assert sure[0] and torch.equal(m.code()[:len(x)][sure], code[sure]) and torch.equal(m.scale()[:len(x)][sure], scale[sure])
+
+
 # ------------------------------------------------------------------ the product
 
 def product(x, w, t, bits, bias=None):
