@@ -844,13 +844,15 @@ double stream_ns(int rows, long long tiles, int stages, int split)
     return waves * (3000 + 11 * r + (stages + split - 1) / split * stage) + (split > 1 ? 600 + 20 * r : 0);
 }
 
-// Clusters of `split` CTAs that run at once. Those of eight with an SM's shared memory each are 15 on a B200, not 148 / 8: 16
-// of them take two rounds (200 rows of 4096 -> 1024 in 8 bits in eight parts 13.1 us, in five 9.1). 0 after an error.
+// Clusters of `split` CTAs that run at once on this thread's device. Those of eight with an SM's shared memory each are 15 on a
+// B200, not 148 / 8: 16 of them take two rounds (200 rows of 4096 -> 1024 in 8 bits in eight parts 13.1 us, in five 9.1). 0
+// after an error.
 template <int BITS, int BN>
 int clusters_at_once(int split)
 {
-    static std::atomic<int> known[MAX_SPLIT + 1];
-    int n = known[split].load(std::memory_order_relaxed);
+    static std::atomic<int> of_device[64][MAX_SPLIT + 1];
+    std::atomic<int> &known = of_device[ctx().device & 63][split];
+    int n = known.load(std::memory_order_relaxed);
     if (n) return n;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -867,7 +869,7 @@ int clusters_at_once(int split)
         cudaGetLastError();
         return 0;
     }
-    known[split].store(n, std::memory_order_relaxed);
+    known.store(n, std::memory_order_relaxed);
     return n;
 }
 
