@@ -21,6 +21,7 @@
 #include "mx.cuh"
 #include "tc05.cuh"
 
+#include <limits.h>
 #include <string.h>
 
 #include <atomic>
@@ -30,6 +31,7 @@ namespace tcg {
 namespace {
 
 constexpr int ERR_WAIT = TCG_ERR_MX_WAIT;
+constexpr unsigned long long MX_WAIT_NS = 1000000000ull;    // limit of a wait; the longest, over 2^24 columns, take 0.1 s
 constexpr int STREAM_THREADS = 256, MAX_DEPTH = 16, ISSUERS = 2;
 constexpr int HALF_SM = 112 * 1024, MOST_SMEM = 226 * 1024;     // of dynamic shared memory; the static part is below 1 KB
 constexpr int SUM_K = 4096;             // columns that the tensor core sums before fp32 results are added up outside
@@ -132,34 +134,6 @@ __device__ __forceinline__ void arrive_cluster(uint32_t bar)
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-// Wait for the phase of parity `parity`. Gives up when another role has (abort), or WAIT_NS after its first thousand tests
-// (bar_wait, tc05.cuh, reads the timer at its start). wait_lane: a warp's lanes may come to differ; they agree again after
-// the elected lane has issued what it waited for. wait_for: they agree at once.
-__device__ __forceinline__ bool wait_lane(uint32_t bar, uint32_t parity, volatile int *abort, int *err, bool heed_abort = true)
-{
-    bool here = bar_test(bar, parity);
-    unsigned long long since = 0;
-    for (uint32_t i = 1; !here; i++) {
-        here = bar_test(bar, parity);
-        if (!here && (i & 1023) == 0) {
-            const unsigned long long now = now_ns();
-            if (since == 0) since = now;
-            if (now - since > WAIT_NS) {
-                *abort = 1;
-                atomicExch(err, ERR_WAIT);
-                break;
-            }
-            if (heed_abort && *abort) break;
-        }
-    }
-    return here;
-}
-__device__ __forceinline__ bool agree(bool ok) { return __all_sync(0xFFFFFFFFu, ok); }
-__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int *abort, int *err, bool heed_abort = true)
-{
-    return agree(wait_lane(bar, parity, abort, err, heed_abort));
-}
-
 struct LinArgs {
     const uint8_t *xs, *ws;             // scales
     const float *bias;
@@ -176,7 +150,36 @@ struct LinArgs {
     int depth;                          // stages in shared memory
     int type;
     bool pairs;                         // two 16-bit results of a row as one word
+    int most_loads;                     // stages that a loading warp asks for, at most (tcg_test_mx_withhold_loads)
 };
+
+// Wait for the phase of parity `parity`. Gives up when another role has (abort), or MX_WAIT_NS after its first thousand tests
+// (bar_wait, tc05.cuh, reads the timer at its start). wait_lane: a warp's lanes may come to differ; they agree again after
+// the elected lane has issued what it waited for. wait_for: they agree at once.
+__device__ __forceinline__ bool wait_lane(uint32_t bar, uint32_t parity, volatile int *abort, int *err, bool heed_abort = true)
+{
+    bool here = bar_test(bar, parity);
+    unsigned long long since = 0;
+    for (uint32_t i = 1; !here; i++) {
+        here = bar_test(bar, parity);
+        if (!here && (i & 1023) == 0) {
+            const unsigned long long now = now_ns();
+            if (since == 0) since = now;
+            if (now - since > MX_WAIT_NS) {
+                *abort = 1;
+                atomicExch(err, ERR_WAIT);
+                break;
+            }
+            if (heed_abort && *abort) break;
+        }
+    }
+    return here;
+}
+__device__ __forceinline__ bool agree(bool ok) { return __all_sync(0xFFFFFFFFu, ok); }
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int *abort, int *err, bool heed_abort = true)
+{
+    return agree(wait_lane(bar, parity, abort, err, heed_abort));
+}
 
 // N columns of two accumulators, with one wait.
 __device__ __forceinline__ void tmem_ld_two(uint32_t at, uint32_t bt, uint32_t (&a)[8], uint32_t (&b)[8])
@@ -308,8 +311,9 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
     const int role = __shfl_sync(0xFFFFFFFFu, warp, 0);
     int loads = 0;
     if (role == 0) {
+        const int all = min(count, p.most_loads);
         int slot = 0, phase = 1;
-        for (int &k = loads; k < count; k++) {
+        for (int &k = loads; k < all; k++) {
             const int kk = k_begin + k, na = atoms_of(k);
             ok = wait_lane(empty + 8 * slot, phase, abort, p.err);
             const uint32_t bar = full + 8 * slot, a = at(slot), b = a + S::A, sa = b + S::B, sb = sa + S::SF;
@@ -578,7 +582,7 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ C
         for (int tile = first; tile < p.tiles && ok; tile += step) {
             const PairTile at = tile_at(p, tile);
             const int n0 = at.n0 + rank * 128, m0 = at.m0, mine = m0 + rank * (at.rows / 2);    // a half's box brings 64 rows too many
-            for (int k = 0; k < p.stages_k; k++) {
+            for (int k = 0; k < p.stages_k && issued < p.most_loads; k++) {
                 ok = wait_lane(empty + 8 * slot, phase, abort, p.err);
                 const uint32_t a = base + slot * S::STAGE, b = a + S::A, sa = b + S::B, sb = sa + S::SF;
                 const uint32_t bar = peer_addr(full + 8 * slot, 0);
@@ -643,6 +647,8 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ C
                 __syncwarp();
             }
         }
+        // the other CTA's roles leave, too
+        if (!ok && elect()) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_addr(su32(&s_abort), 1)), "r"(1) : "memory");
         // every product issued above has ended once this flips
         if (elect())
             asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(end) : "memory");
@@ -962,10 +968,21 @@ bool linear_go(LinArgs &p, const tcg_mx_t &x, const tcg_mx_t &w)
     return stream_launch<BITS, 128>(p, x, w);
 }
 
+std::atomic<int> g_most_loads{INT_MAX};
+
 }  // namespace
 }  // namespace tcg
 
 using namespace tcg;
+
+// Test hook for the paths of a wait that gives up: with stages >= 0, the loading warps of the calls after it (of every
+// thread) ask for that many stages and no more, so that the waits for the next one run out; a negative number restores
+// normal operation. Returns the number before.
+extern "C" int tcg_test_mx_withhold_loads(int stages)
+{
+    const int before = g_most_loads.exchange(stages < 0 ? INT_MAX : stages);
+    return before == INT_MAX ? -1 : before;
+}
 
 extern "C" bool tcg_mx_linear(void *y, const tcg_mx_t *x, const tcg_mx_t *w, const float *bias, int64_t ld_y, ggml_type_t t)
 {
@@ -980,6 +997,7 @@ extern "C" bool tcg_mx_linear(void *y, const tcg_mx_t *x, const tcg_mx_t *w, con
     if (!x->rows || !w->rows) return true;
     LinArgs p = {};
     p.xs = x->scales, p.ws = w->scales, p.bias = bias, p.y = y, p.ldy = ld_y, p.err = lm_error_word();
+    p.most_loads = g_most_loads;
     p.rows = x->rows, p.outs = w->rows, p.atoms = (int)(mx_wide(x->cols) / MX_ATOM), p.type = t;
     return x->bits == 4 ? linear_go<4>(p, *x, *w) : linear_go<8>(p, *x, *w);
 }

@@ -230,6 +230,7 @@ _SIGS = [
     ("tcg_mx_quantize", boolean, [C.POINTER(Mx), vp, i64, C.c_int]),
     ("tcg_mx_dequantize", boolean, [vp, C.POINTER(Mx), i64, C.c_int]),
     ("tcg_mx_linear", boolean, [vp, C.POINTER(Mx), C.POINTER(Mx), vp, i64, C.c_int]),
+    ("tcg_test_mx_withhold_loads", i32, [i32]),
     ("tcg_add_rms_norm", boolean, [vp, vp, C.POINTER(Mx), vp, vp, vp, f32, i32, i32, i64, i64, i64, i64, C.c_int]),
     ("tcg_nccl_unique_id", boolean, [C.c_char_p]),
     ("tcg_vit_upload_bcast", vp, [C.POINTER(Vit), i32, i32, i32, C.c_char_p]),

@@ -515,6 +515,35 @@ def test_linear_with_far_scales(lib, rows, bits):
         assert ((y.double() - want).abs() <= tol).all()
 
 
+WITHHELD = [  # rows, cols, outs, bits, type, stages that are loaded
+    (1, 4096, 14336, 8, "f32", 0), (40, 4096, 14336, 4, "bf16", 7),      # K undivided
+    (1, 14336, 4096, 8, "f32", 1), (64, 14336, 4096, 4, "f16", 0), (100, 14336, 4096, 8, "f32", 7),      # split over clusters
+    (1024, 4096, 4096, 4, "bf16", 0), (1024, 4096, 4096, 8, "f32", 7), (3000, 2304, 5000, 8, "bf16", 1), (3000, 2304, 5000, 4, "f32", 0),
+]
+
+
+@pytest.mark.parametrize("rows,cols,outs,bits,t,stages", WITHHELD)
+def test_waits_that_give_up(lib, rows, cols, outs, bits, t, stages):
+    """Loading warps that stop asking after some stages: the waits for the next one run out after their second, the kernel
+    returns without a store and reports it, and the next call is right."""
+    dt, code = TYPES[t]
+    g = gen(rows + stages)
+    x, w = random_held(g, rows, cols, bits, -8 if bits == 8 else -2), random_held(g, outs, cols, 4, -4)
+    flat, view, ptr, ld = rows_of(torch.full((rows, outs), 7.0, dtype=dt, device="cuda"), 2, 4)
+    args = (ptr, C.byref(x.mx()), C.byref(w.mx()), None, ld, code)
+    assert lib.tcg_test_mx_withhold_loads(stages) == -1
+    try:
+        call(lib.tcg_mx_linear, *args)
+    finally:
+        assert lib.tcg_test_mx_withhold_loads(-1) == stages
+    assert lib.tcg_device_error() == tcg.ERR_MX_WAIT
+    assert (flat == 7).all()
+    tcg.check(lib.tcg_clear_device_error())
+    call(lib.tcg_mx_linear, *args)
+    want, tol = product(x.values(), w.values(), t, bits)
+    assert ((view.double() - want).abs() <= tol).all() and lib.tcg_device_error() == 0
+
+
 # ------------------------------------------------------------------ together
 
 class Layer:

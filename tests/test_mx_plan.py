@@ -58,7 +58,6 @@ void **__cudaRegisterFatBinary(void *) { static void *handle; return &handle; }
 void __cudaRegisterFatBinaryEnd(void **) {}
 void __cudaUnregisterFatBinary(void **) {}
 void __cudaRegisterFunction(void **, const char *, char *, const char *, int, void *, void *, void *, void *, int *) {}
-void __cudaRegisterVar(void **, char *, char *, const char *, int, size_t, int, int) {}
 cudaError_t __cudaPopCallConfiguration(dim3 *, dim3 *, size_t *, void *) { return cudaSuccess; }
 cudaError_t cudaFuncSetAttribute(const void *, cudaFuncAttribute, int) { return cudaSuccess; }
 cudaError_t cudaGetDevice(int *d) { *d = device; return cudaSuccess; }
@@ -68,8 +67,6 @@ cudaError_t cudaGetDriverEntryPoint(const char *, void **fn, unsigned long long,
     return cudaSuccess;
 }
 cudaError_t cudaGetLastError() { return cudaSuccess; }
-cudaError_t cudaStreamSynchronize(cudaStream_t) { return cudaSuccess; }
-cudaError_t cudaMemcpyToSymbol(const void *, const void *, size_t, size_t, cudaMemcpyKind) { return cudaSuccess; }
 cudaError_t cudaLaunchKernel(const void *, dim3, dim3, void **, size_t, cudaStream_t) { return cudaErrorUnknown; }
 cudaError_t cudaOccupancyMaxActiveClusters(int *n, const void *, const cudaLaunchConfig_t *)
 {
