@@ -305,6 +305,51 @@ def test_add_and_norm(lib, rows, cols, t, pad, offset):
     assert torch.equal(iv, h)
 
 
+LAYOUTS = [  # of x and r, of h and y: (elements a row is longer, the first one's offset), 16-byte boundaries unless odd; of w
+    ((8, 0), (3, 0), 0), ((0, 8), (0, 1), 0), ((3, 1), (8, 0), 0), ((8, 8), (1, 3), 4), ((8, 0), (8, 0), 1), ((5, 2), (2, 5), 3),
+]
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("rows,cols", [(3, 200), (300, 256), (1, 2571), (310, 512), (777, 2571), (300, 4104), (297, 8000), (2, 9001), (2, 20000)])
+def test_norm_with_unlike_layouts(lib, rows, cols, t):
+    """Rows that are read and rows that are written on unlike boundaries, weights off their own; one token's and many rows'
+    kernels of each width."""
+    dt, code = TYPES[t]
+    g, eps = gen(rows * 7 + cols), float(torch.tensor(1e-5))
+    x, r = randn(g, rows, cols, dtype=dt, spread=2.0), randn(g, rows, cols, dtype=dt)
+    h = (x.float() + r.float()).to(dt)
+    cols_up = -(-cols // 8) * 8
+    for i, ((in_pad, in_off), (out_pad, out_off), w_off) in enumerate(LAYOUTS):
+        in_pad, out_pad = in_pad + cols_up - cols, out_pad + cols_up - cols
+        x_rows, _, xp, ldx = rows_of(x, in_pad, in_off)
+        r_rows, _, rp, ldr = rows_of(r, in_pad, in_off)
+        w_all = randn(g, cols + w_off) * 0.2 + 1
+        w, wp = w_all[w_off:], w_all.data_ptr() + 4 * w_off
+        for residual in (True, False):
+            want_h = h if residual else x
+            want = normed(want_h.double(), w, eps)
+            for bits in ((0, 4, 8) if i % 2 else (0, 8)):
+                m = Held(rows, cols, bits) if bits else None
+                h_rows, hv, hp, ldh = rows_of(torch.zeros_like(x), out_pad, out_off)
+                y_rows, yv, yp, ldy = rows_of(torch.zeros_like(x), out_pad + 8, out_off)
+                call(lib.tcg_add_rms_norm, hp, yp, C.byref(m.mx()) if m else None, xp, rp if residual else None, wp, eps, rows, cols,
+                     ldh, ldy, ldx, ldr, code)
+                assert torch.equal(hv, want_h)
+                # three fp32 factors and the root, each rounded, then the type's rounding
+                tol = want.abs() * (4 * U + (half_step(dt) if t != "f32" else 0)) + (2.0 ** -24 if t == "f16" else 0)
+                assert ((yv.double() - want).abs() <= tol).all()
+                for flat in (h_rows, y_rows):
+                    wide = (flat.numel() - out_off) // rows
+                    assert (flat[:out_off] == 7).all() and (flat[out_off:].view(rows, wide)[:, cols:] == 7).all()
+                if m:
+                    m.check(*quantised(want, bits))
+            # the sum alone, or a copy of x where there is none to add
+            h_rows, hv, hp, ldh = rows_of(torch.zeros_like(x), out_pad, out_off)
+            call(lib.tcg_add_rms_norm, hp, None, None, xp, rp if residual else None, None, eps, rows, cols, ldh, 0, ldx, ldr, code)
+            assert torch.equal(hv, want_h)
+
+
 @pytest.mark.parametrize("rows,cols", [(1, 1), (3, 256), (2, 4096), (5, 20000), (400, 300), (300, 4096)])
 def test_the_sum_alone_reads_no_weights(lib, rows, cols):
     """With h alone asked for, w may be any address: one that is not there, one that no float stands at."""
@@ -462,6 +507,27 @@ def test_linear(lib, rows, cols, outs, bits):
         assert (flat[:(rows + i) % 2] == 7).all() and (flat[(rows + i) % 2:].view(rows, -1)[:, outs:] == 7).all()
         call(lib.tcg_mx_linear, ptr, C.byref(x.mx()), C.byref(w.mx()), b.data_ptr() if b is not None else None, ld, code)
         assert torch.equal(view, first)                                  # the same bits again
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("outs", [20011, 40000])
+@pytest.mark.parametrize("rows,cols", [(1, 128), (1, 1100), (12, 128), (12, 1100), (30, 300), (30, 1100), (64, 128), (64, 1100), (100, 700)])
+def test_linear_of_few_rows_in_several_waves(lib, rows, cols, outs, bits):
+    """More tiles than SMs: CTAs that share an SM's memory and TMEM (up to 32 rows of x), or take turns at TMEM (up to 64)."""
+    g = gen(rows + cols + outs + bits)
+    x, w = random_held(g, rows, cols, bits, -8 if bits == 8 else -2), random_held(g, outs, cols, 4, -4)
+    xv, wv = x.values(), w.values()
+    for t in ("f32", "bf16"):
+        dt, code = TYPES[t]
+        want, tol = product(xv, wv, t, bits)
+        out = []
+        for _ in range(3):
+            flat, view, ptr, ld = rows_of(torch.zeros((rows, outs), dtype=dt, device="cuda"), 1, 1)
+            call(lib.tcg_mx_linear, ptr, C.byref(x.mx()), C.byref(w.mx()), None, ld, code)
+            assert ((view.double() - want).abs() <= tol).all()
+            assert flat[0] == 7 and (flat[1:].view(rows, -1)[:, outs:] == 7).all()
+            out.append(view.clone())
+        assert torch.equal(out[0], out[1]) and torch.equal(out[0], out[2])
 
 
 def test_linear_of_nothing(lib):
