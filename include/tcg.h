@@ -360,8 +360,12 @@ bool tcg_mx_dequantize(void *y, const tcg_mx_t *m, int64_t ld, ggml_type_t t);
 /* y = x w^T + bias: x [rows, cols] in 8 or 4 bits, w [outs, cols] in 4 bits,
  * bias fp32 [outs] or NULL, y [rows, outs]. Products are exact; the tensor core
  * adds 32 columns (x in 8 bits) or 64 (4 bits) at a time to a sum of 24 bits,
- * cutting what lies below (F32 results: such sums of 4096 columns each, or of
- * more where they have no room, are added up); the sum is rounded once to t.
+ * cutting what lies below, 2^-22 of the sum of magnitudes a step at most (F32
+ * results: such sums of 4096 columns each, or of more where they have no room,
+ * are added up); the sum is rounded once to t. Sums of one sign come out low,
+ * by 2^-25 a step in 8 bits as measured (3e-6 over 4096 columns). Up to 65536
+ * columns (131072 in 4 bits) the cuts are less than one rounding to F16, up to
+ * 524288 (1048576) to BF16.
  * What stands behind cols in the codes must be 0, with any scale but 255.
  * y must not overlap x or w. */
 bool tcg_mx_linear(void *y, const tcg_mx_t *x, const tcg_mx_t *w, const float *bias, int64_t ld_y, ggml_type_t t);

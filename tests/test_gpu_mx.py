@@ -510,6 +510,26 @@ def test_linear(lib, rows, cols, outs, bits):
 
 
 @pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("rows,cols,outs", [(1, 70000, 300), (64, 262144, 130), (128, 100000, 200), (600, 70000, 1024), (2000, 66000, 4100)])
+def test_linear_of_long_sums_of_one_sign(lib, rows, cols, outs, bits):
+    """Where the tensor core's cuts add up: results stay within what the header gives for a step (2^-22 of the sum), whatever
+    the type, and 16-bit ones within two of their own roundings up to the columns that it names."""
+    g = gen(rows + cols)
+    x, w = random_held(g, rows, cols, bits, -12 if bits == 8 else -6), random_held(g, outs, cols, 4, -8)
+    for m in (x, w):
+        m.put(m.code() % (1 << (m.bits - 1)), m.scale()[:m.rows])
+    xv, wv = x.values(), w.values()
+    for t, (dt, code) in TYPES.items():
+        y = torch.zeros((rows, outs), dtype=dt, device="cuda")
+        call(lib.tcg_mx_linear, y.data_ptr(), C.byref(x.mx()), C.byref(w.mx()), None, outs, code)
+        want, tol = product(xv, wv, t, bits)
+        assert want.min() > 1 and want.max() < 60000
+        assert ((y.double() - want).abs() <= tol).all()
+        if t == "bf16" or (t == "f16" and cols <= (65536 if bits == 8 else 131072)):
+            assert ((y.double() - want).abs() <= 2 * half_step(dt) * want).all()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("outs", [20011, 40000])
 @pytest.mark.parametrize("rows,cols", [(1, 128), (1, 1100), (12, 128), (12, 1100), (30, 300), (30, 1100), (64, 128), (64, 1100), (100, 700)])
 def test_linear_of_few_rows_in_several_waves(lib, rows, cols, outs, bits):
