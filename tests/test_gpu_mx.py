@@ -755,3 +755,87 @@ def test_streams_at_once(lib):
         tcg.check(lib.tcg_set_stream(None))
     for x, w, want, got in jobs:
         assert all(torch.equal(o, want) for o in got)
+
+
+THREADS_FIRST = """
+import sys, threading, torch
+sys.path[:0] = sys.argv[1:3]
+import tcg, test_gpu_mx as T
+L, g, N = tcg.lib(), T.gen(31), 8
+tcg.init(0)
+C, jobs = T.C, []
+for rows, cols, outs, bits in ((1, 14336, 4096, 8), (40, 4096, 2000, 4), (100, 2080, 500, 8), (700, 640, 4100, 4)):
+    v = T.randn(g, rows, cols)
+    x, w = T.Held(rows, cols, bits), T.random_held(g, outs, cols, 4, -6)
+    jobs.append((v, torch.ones(cols, device="cuda"), x, w, T.normed(v.double(), torch.ones(cols, device="cuda"), 0.0)))
+mine = [[(T.Held(x.rows, x.cols, x.bits), torch.zeros((x.rows, w.rows), device="cuda"), torch.zeros_like(v)) for v, _, x, w, _ in jobs]
+        for _ in range(N)]
+wall, bad = threading.Barrier(N), []
+torch.cuda.synchronize()
+
+def work(i):
+    try:
+        tcg.init(0)
+        for (v, one, x, w, _), (m, y, back) in zip(jobs, mine[i]):
+            wall.wait(60)
+            tcg.check(L.tcg_add_rms_norm(None, None, C.byref(m.mx()), v.data_ptr(), None, one.data_ptr(), 0.0, x.rows, x.cols, 0, 0, x.cols, 0, 0))
+            tcg.check(L.tcg_mx_linear(y.data_ptr(), C.byref(m.mx()), C.byref(w.mx()), None, w.rows, 0))
+            tcg.check(L.tcg_mx_dequantize(back.data_ptr(), C.byref(m.mx()), x.cols, 0))
+        tcg.check(L.tcg_sync())
+        assert L.tcg_device_error() == 0
+    except Exception as e:
+        bad.append(e)
+        wall.abort()
+
+threads = [threading.Thread(target=work, args=(i,)) for i in range(N)]
+[t.start() for t in threads]
+[t.join() for t in threads]
+torch.cuda.synchronize()
+assert not bad, bad
+for k, (v, one, x, w, norm) in enumerate(jobs):
+    for i in range(N):
+        m, y, back = mine[i][k]
+        m.check(*T.quantised(norm, x.bits))
+        want, tol = T.product(m.values(), w.values(), "f32", x.bits)
+        assert ((y.double() - want).abs() <= tol).all() and torch.equal(y, mine[0][k][1]) and torch.equal(back.double(), m.values())
+print("together")
+"""
+
+
+def test_first_calls_of_several_threads_at_once():
+    """Threads whose first calls of each operator come together: each has a context of its own, none runs unprepared."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    pkg = os.path.join(os.path.dirname(here), "roofline.c_b200")
+    out = subprocess.run([sys.executable, "-c", THREADS_FIRST, here, pkg], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "together" in out.stdout, out.stderr[-2000:]
+
+
+@pytest.mark.parametrize("kind", ["Q4_K", "Q6_K"])
+def test_weights_of_a_gguf_tensor(lib, kind):
+    """From a tensor's K-quant blocks over its values to 4 bits and into a product: the codes are those of the values, each
+    within a quarter of itself or of its block's unit, and the product is that of what is held."""
+    import numpy as np
+    import oracle
+    import tcg_gguf as G
+    outs, cols, qt = 512, 2048, getattr(G, kind)
+    raw = G.make_kquant_like(qt, outs, cols, 17, 1e-3)
+    v = torch.from_numpy(np.ascontiguousarray(oracle.dequant(raw, outs * cols, qt))).view(outs, cols).cuda().double()
+    blocks, f32 = torch.from_numpy(raw).cuda(), torch.zeros((outs, cols), device="cuda")
+    call(lib.tcg_dequant, f32.data_ptr(), blocks.data_ptr(), outs * cols, qt)
+    assert torch.equal(f32.double(), v)
+    w = Held(outs, cols, 4)
+    call(lib.tcg_mx_quantize, C.byref(w.mx()), f32.data_ptr(), cols, tcg.F32)
+    w.check(*quantised(v, 4))
+    unit = power(w.scale()[:outs] - 127).repeat_interleave(32, 1)
+    assert ((w.values() - v).abs() <= torch.maximum(v.abs(), unit) / 4).all()
+    for rows, bits in ((1, 8), (70, 4)):
+        x = Held(rows, cols, bits)
+        a = randn(gen(rows), rows, cols)
+        call(lib.tcg_mx_quantize, C.byref(x.mx()), a.data_ptr(), cols, tcg.F32)
+        y = torch.zeros((rows, outs), device="cuda")
+        call(lib.tcg_mx_linear, y.data_ptr(), C.byref(x.mx()), C.byref(w.mx()), None, outs, tcg.F32)
+        want, tol = product(x.values(), w.values(), "f32", bits)
+        assert ((y.double() - want).abs() <= tol).all()
