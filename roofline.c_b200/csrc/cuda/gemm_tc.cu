@@ -119,35 +119,6 @@ __device__ __forceinline__ void epi_store4(const GemmEpi &e, int src_row, size_t
 // CTAs. Each CTA drains its own 128 TMEM lanes and releases chunk buffers on
 // the leader's barriers.
 
-__device__ __forceinline__ uint32_t cta_rank_in_cluster()
-{
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-// address of the same shared-memory offset in CTA `rank` of the cluster
-__device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank)
-{
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ void bar_arrive_cluster(uint32_t cluster_addr)
-{
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-__device__ __forceinline__ void cluster_sync()
-{
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// TMA load into this CTA's shared memory whose bytes complete on the
-// leader's barrier (cluster address).
-__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap *map, uint32_t bar_cluster, int x, int y)
-{
-    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
-                 " [%0], [%1, {%2, %3}], [%4];"
-                 ::"r"(dst), "l"((unsigned long long)map), "r"(x), "r"(y), "r"(bar_cluster) : "memory");
-}
 __device__ __forceinline__ void mma_tf32_pair(uint32_t d, unsigned long long a, unsigned long long b, uint32_t id, uint32_t acc)
 {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -1137,30 +1108,10 @@ gemm_tf32x3_kernel(const __grid_constant__ CUtensorMap a_hi, const __grid_consta
 
 // ------------------------------------------------------------------ host
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
-                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
-                                  CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn()
-{
-    static EncodeTiledFn fn = nullptr;
-    if (!fn) {
-        void *p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = (EncodeTiledFn)p;
-        else
-            cudaGetLastError();
-    }
-    return fn;
-}
-
 // [rows, K] fp32, row stride K, box = BK x box_rows, swizzle = BK*4 bytes.
 bool encode_kmajor(CUtensorMap *m, const float *ptr, int rows, int K, int box_rows, int BK)
 {
-    EncodeTiledFn fn = encode_fn();
+    EncodeTiledFn fn = encode_tiled_fn();
     if (!fn) return fail("cuTensorMapEncodeTiled is not available from the driver");
     if (((uintptr_t)ptr & 15) || (K & 3)) return fail("GEMM operand not 16-byte aligned / K=%d not a multiple of 4", K);
     cuuint64_t dims[2] = { (cuuint64_t)K, (cuuint64_t)rows };
@@ -1180,7 +1131,7 @@ bool encode_kmajor(CUtensorMap *m, const float *ptr, int rows, int K, int box_ro
 // one 128-byte swizzled row; 32: one 64-byte swizzled row) x box_rows.
 bool encode_kmajor_f16(CUtensorMap *m, const void *ptr, int rows, int K, int box_rows, int box_k)
 {
-    EncodeTiledFn fn = encode_fn();
+    EncodeTiledFn fn = encode_tiled_fn();
     if (!fn) return fail("cuTensorMapEncodeTiled is not available from the driver");
     if (((uintptr_t)ptr & 15) || (K & 7)) return fail("fp16 GEMM operand not 16-byte aligned / K=%d not a multiple of 8", K);
     cuuint64_t dims[2] = { (cuuint64_t)K, (cuuint64_t)rows };
@@ -1199,7 +1150,7 @@ bool encode_kmajor_f16(CUtensorMap *m, const void *ptr, int rows, int K, int box
 // 32 rows x 16 columns (32 bytes) in the 32-byte swizzle.
 bool encode_out_f16(CUtensorMap *m, const void *ptr, int rows, int cols, int ld)
 {
-    EncodeTiledFn fn = encode_fn();
+    EncodeTiledFn fn = encode_tiled_fn();
     if (!fn) return fail("cuTensorMapEncodeTiled is not available from the driver");
     cuuint64_t dims[2] = { (cuuint64_t)cols, (cuuint64_t)rows };
     cuuint64_t strides[1] = { (cuuint64_t)ld * 2u };
@@ -1215,7 +1166,7 @@ bool encode_out_f16(CUtensorMap *m, const void *ptr, int rows, int cols, int ld)
 // ld, boxes of 32 rows x 8 columns in the 32-byte swizzle.
 bool encode_out(CUtensorMap *m, const float *ptr, int rows, int cols, int ld)
 {
-    EncodeTiledFn fn = encode_fn();
+    EncodeTiledFn fn = encode_tiled_fn();
     if (!fn) return fail("cuTensorMapEncodeTiled is not available from the driver");
     cuuint64_t dims[2] = { (cuuint64_t)cols, (cuuint64_t)rows };
     cuuint64_t strides[1] = { (cuuint64_t)ld * 4u };

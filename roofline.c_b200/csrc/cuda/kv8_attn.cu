@@ -60,7 +60,6 @@
 
 #include <math.h>
 
-#include <atomic>
 #include <type_traits>
 
 namespace tcg {
@@ -83,11 +82,6 @@ __device__ __forceinline__ uint4 lds128(uint32_t a)
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
     return v;
-}
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
-{
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 // 4 consecutive values of a query row.
 __device__ __forceinline__ void load_q4(const AttnArgs &p, long long off, float (&x)[4])
@@ -714,27 +708,6 @@ kv8_attn_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUte
     cluster_sync();                                          // no CTA leaves while another reads its shared memory
 }
 
-
-typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                             const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                             CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeFn attn_encode_fn()
-{
-    static std::atomic<EncodeFn> known{nullptr};             // threads that come first together find the same
-    EncodeFn fn = known.load(std::memory_order_acquire);
-    if (!fn) {
-        void *p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            known.store(fn = (EncodeFn)p, std::memory_order_release);
-        else
-            cudaGetLastError();
-    }
-    return fn;
-}
-
 template <int KS, int NP, int RW, int WM, int WN, int NSLOT, int MINB>
 bool attn_launch(AttnArgs &p, const CUtensorMap &map, long long tiles)
 {
@@ -797,7 +770,7 @@ extern "C" bool tcg_kv8_attention(void *out, const void *q, const tcg_kv8_t *c, 
     }
 
     // K as [pages x heads x 64, D] bytes; a box is 64 keys of 64 dims, zeros past D
-    EncodeFn fn = attn_encode_fn();
+    EncodeTiledFn fn = encode_tiled_fn();
     if (!fn) return fail("cuTensorMapEncodeTiled is not available from the driver");
     CUtensorMap map;
     const cuuint64_t dims[2] = { (cuuint64_t)p.D, (cuuint64_t)c->n_pages * c->n_kv_head * PAGE };

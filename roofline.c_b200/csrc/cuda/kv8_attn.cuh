@@ -3,6 +3,7 @@
 #pragma once
 
 #include "lm.cuh"
+#include "tc05.cuh"
 
 #include <math.h>
 
@@ -131,10 +132,6 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t a)
     float4 v;
     asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
     return v;
-}
-__device__ __forceinline__ void cluster_sync()
-{
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 constexpr int MAX_SPLIT = 10;            // CTAs of a cluster; of 11 or more a B200 holds 7 clusters at a time

@@ -763,25 +763,6 @@ static int mm_unit_superblocks(int nsb)
     return best;
 }
 
-typedef CUresult (*EncodeFn3)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                              const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeFn3 mm_encode_fn()
-{
-    static EncodeFn3 fn = nullptr;
-    if (!fn) {
-        void *p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = (EncodeFn3)p;
-        else
-            cudaGetLastError();
-    }
-    return fn;
-}
-
 // The order in which MMA rows g = 0..7 read the slot's rows (and rows + 8),
 // three bits each: a half-warp's lanes (rows g = 0..3, then 4..7, quad lanes
 // t = 0..3) load 8 bytes at word (rs/4) * sigma(g) + 2t (+ a common offset),
@@ -961,7 +942,7 @@ static bool launch_matvec_mma(float *y, const void *W, const float *x, int N, in
     const int dev = ctx().device & 63;
     MmMap &mp = g_mm_map[dev];
     if (mp.w != W || mp.n != N || mp.k != K || mp.spb != spb || mp.qt != QT) {
-        EncodeFn3 fn = mm_encode_fn();
+        EncodeTiledFn fn = encode_tiled_fn();
         if (!fn) return fail("cuTensorMapEncodeTiled is not available from the driver");
         CUresult r;
         if constexpr (QT == 4) {

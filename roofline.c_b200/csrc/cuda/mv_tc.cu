@@ -62,12 +62,6 @@ constexpr size_t MQ_SMEM = MQ_SMEM_USED + 1024;  // + alignment slack
 
 static_assert(MQ_SMEM <= 232448, "shared memory");
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
-{
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
-}
-
 // 16 columns of this thread's TMEM lane from registers; waits for the store.
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16])
 {
@@ -411,25 +405,6 @@ mvq_tc_kernel(const __grid_constant__ CUtensorMap wmap, const uint8_t *__restric
     }
 }
 
-typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                             const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                             CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeFn mq_encode_fn()
-{
-    static EncodeFn fn = nullptr;
-    if (!fn) {
-        void *p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = (EncodeFn)p;
-        else
-            cudaGetLastError();
-    }
-    return fn;
-}
-
 // Working memory of this host thread's calls on a device (the library
 // context is per thread too): tile counters (zero between calls), partial
 // sums, B tiles and x factors. Grown (and zeroed) on demand. Calls of one
@@ -484,7 +459,7 @@ bool launch_matvec_tc_q4k(float *y, const void *W, const float *x, int N, int K,
     float *F = (float *)(Bt + (size_t)nb * MQ_BT);
 
     if (b.map_w != W || b.map_n != N || b.map_k != K) {
-        EncodeFn fn = mq_encode_fn();
+        EncodeTiledFn fn = encode_tiled_fn();
         if (!fn) return fail("cuTensorMapEncodeTiled is not available from the driver");
         // 32-bit elements: a row is nb * 36 of them, a box MQ_SPS superblocks of 128 rows
         cuuint64_t dims[2] = { (cuuint64_t)nb * (MQ_BB / 4), (cuuint64_t)N };

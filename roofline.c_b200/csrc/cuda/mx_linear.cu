@@ -80,17 +80,6 @@ __device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint32_t smem)
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
 }
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
-{
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
-}
-
-__device__ __forceinline__ void prefetch_map(const CUtensorMap *map)
-{
-    asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)map) : "memory");
-}
-
 // One lane of a converged warp. The role loops below run in whole warps and issue under this, so that what they issue is
 // known to be the same in all lanes: descriptors then live in uniform registers, where a branch to lane 0 moves each of them
 // there (105 cycles a product, which takes 64).
@@ -101,26 +90,10 @@ __device__ __forceinline__ bool elect()
     return one != 0;
 }
 
-__device__ __forceinline__ int special_rank()
-{
-    int r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
 __device__ __forceinline__ int special_cluster()
 {
     int r;
     asm volatile("mov.u32 %0, %%clusterid.x;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync()
-{
-    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank)
-{
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
 // Bytes from this CTA's shared memory to a peer's, counted by its barrier.
@@ -128,10 +101,6 @@ __device__ __forceinline__ void push(uint32_t to, uint32_t from, uint32_t bytes,
 {
     asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(to), "r"(from), "r"(bytes), "r"(bar) : "memory");
-}
-__device__ __forceinline__ void arrive_cluster(uint32_t bar)
-{
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 struct LinArgs {
@@ -274,7 +243,7 @@ __global__ void __launch_bounds__(STREAM_THREADS) mx_stream_kernel(const __grid_
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t base = su32(smem), full = su32(bars), empty = full + 8 * MAX_DEPTH, done = empty + 8 * MAX_DEPTH, join = done + 8;
     // a cluster a tile; a division costs as much as a few dozen instructions, so none where there is one tile of rows
-    const int rank = special_rank(), tile = special_cluster(), tm = BN < MX_ATOM ? 0 : tile / p.tiles_n;
+    const int rank = (int)cta_rank_in_cluster(), tile = special_cluster(), tm = BN < MX_ATOM ? 0 : tile / p.tiles_n;
     const int n0 = (tile - tm * p.tiles_n) * TILE_N, m0 = tm * BN;
     const int k_begin = rank * p.per, k_end = min(p.stages_k, k_begin + p.per), count = k_end - k_begin;
     // Where a tile's K is split, its results meet by fours of x's rows: the CTA of rank g % split adds up group g.
@@ -478,13 +447,6 @@ struct Pair {
 
 constexpr int PAIR_EPI = 16, PAIR_THREADS = 32 * (2 + PAIR_EPI);
 
-// A copy into this CTA's shared memory whose bytes complete on the leader's barrier.
-__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y)
-{
-    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
-                 " [%0], [%1, {%2, %3}], [%4];"
-                 ::"r"(dst), "l"((unsigned long long)map), "r"(x), "r"(y), "r"(bar) : "memory");
-}
 template <int BITS>
 __device__ __forceinline__ void mma_mx_pair(uint32_t d, unsigned long long a, unsigned long long b, uint32_t id, uint32_t sa,
                                             uint32_t sb, uint32_t acc)
@@ -688,12 +650,12 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ C
                     if (i == 1) {                           // the shared columns are drained
                         fence_before();
                         __syncwarp();
-                        if (h == (buf ? 0 : 3) && lane == 0) arrive_cluster(lap_bar + 8 * buf);
+                        if (h == (buf ? 0 : 3) && lane == 0) bar_arrive_cluster(lap_bar + 8 * buf);
                     }
                 }
                 fence_before();
                 __syncwarp();
-                if (lane == 0) arrive_cluster(free_bar + 8 * buf);
+                if (lane == 0) bar_arrive_cluster(free_bar + 8 * buf);
             }
             if (!ok) break;
             int again = tile;                               // taken anew: the registers are the accumulators' until here
@@ -737,28 +699,10 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ C
 
 // ------------------------------------------------------------------ launch
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
-                                  const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn()
-{
-    static const EncodeTiledFn fn = [] {
-        void *p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            return (EncodeTiledFn)p;
-        cudaGetLastError();
-        return (EncodeTiledFn) nullptr;
-    }();
-    return fn;
-}
-
 // Boxes of 128 bytes of shared memory x box_rows in the 128-byte swizzle. spread: 4-bit codes, 16 of them to 16 bytes.
 bool encode_mx(CUtensorMap *map, const tcg_mx_t &m, int box_rows, bool spread)
 {
-    const EncodeTiledFn fn = encode_fn();
+    const EncodeTiledFn fn = encode_tiled_fn();
     if (!fn) return fail("cuTensorMapEncodeTiled is not available from the driver");
     const cuuint64_t pitch = (cuuint64_t)mx_pitch(m.cols, m.bits);
     cuuint64_t dims[2] = { spread ? (cuuint64_t)mx_wide(m.cols) : pitch, (cuuint64_t)m.rows };
@@ -775,7 +719,7 @@ bool encode_mx(CUtensorMap *map, const tcg_mx_t &m, int box_rows, bool spread)
 // The scales as rows of 64-bit words, a row for each 128 rows of the matrix; boxes of a stage's scales of `blocks` rows.
 bool encode_scales(CUtensorMap *map, const tcg_mx_t &m, int atoms, int blocks)
 {
-    const EncodeTiledFn fn = encode_fn();
+    const EncodeTiledFn fn = encode_tiled_fn();
     if (!fn) return fail("cuTensorMapEncodeTiled is not available from the driver");
     const cuuint64_t wide = (cuuint64_t)mx_wide(m.cols) / MX_ATOM * 64;
     cuuint64_t dims[2] = { wide, ((cuuint64_t)m.rows + MX_ATOM - 1) / MX_ATOM };
