@@ -473,12 +473,15 @@ __device__ __forceinline__ float normed_odd(float v, double rstd, float w)
 // A row's columns are dealt out to G threads (a warp's 32, or the CTA's, at most MOST), N pieces of 8 consecutive columns each.
 // CTAs an SM that registers are kept for. 4096 rows of 4096 fp32 values with their residual, to 8 bits: two pieces a thread of 256
 // and four CTAs 38.6 us (5.7 TB/s), five (with spills) 40.3; two of 512 and two CTAs 40.9; one of 512 and three 43.2; four of 128
-// and five 50.0. Without codes five fit.
-constexpr int norm_ctas(int n, int most, bool mx) { return n == 2 && most == 256 ? mx ? 4 : 5 : 1; }
+// and five 50.0. Without codes five fit. 512 bf16 rows of 16384 without codes: two CTAs 16.5 us, one (76 registers) 19.9.
+constexpr int norm_ctas(int size, int n, int most, bool mx)
+{
+    return n == 2 && most == 256 ? mx ? 4 : 5 : n == 4 && most == 512 && size == 2 && !mx ? 2 : 1;
+}
 
 // VIN, VOUT: rows of x, r and w, and of h and y, start on 16-byte boundaries. MX: there are codes to write.
 template <typename T, int N, int MOST, bool VIN, bool VOUT, bool MX>
-__global__ void __launch_bounds__(MOST == 32 ? 256 : MOST, norm_ctas(N, MOST, MX)) add_rms_norm_kernel(const __grid_constant__ NormArgs p)
+__global__ void __launch_bounds__(MOST == 32 ? 256 : MOST, norm_ctas(sizeof(T), N, MOST, MX)) add_rms_norm_kernel(const __grid_constant__ NormArgs p)
 {
     constexpr bool WARP = MOST == 32;
     const int G = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
@@ -497,7 +500,7 @@ __global__ void __launch_bounds__(MOST == 32 ? 256 : MOST, norm_ctas(N, MOST, MX
     Raw<float> w0;
     if (N == 1 && p.w) w0 = load_row<VIN>(p.w + (long long)t * LANE, p.cols - (long long)t * LANE, p.w, p.w + p.cols);
     double ss = 0.0;
-    float low = INFINITY;               // the smallest magnitude
+    uint32_t low = 0xFFFFFFFFu;         // the smallest magnitude but for zeros, as twice its bits less one
 #pragma unroll
     for (int k = 0; k < N; k++) {
         float v[LANE];
@@ -512,8 +515,9 @@ __global__ void __launch_bounds__(MOST == 32 ? 256 : MOST, norm_ctas(N, MOST, MX
         }
 #pragma unroll
         for (int i = 0; i < LANE; i++) ss = fma((double)v[i], (double)v[i], ss);
+        if (!std::is_same<T, __half>::value)
 #pragma unroll
-        for (int i = 0; i < LANE; i++) low = fminf(low, fabsf(v[i]));
+            for (int i = 0; i < LANE; i++) low = min(low, 2 * __float_as_uint(v[i]) - 1);
     }
     if (p.h)
 #pragma unroll
@@ -534,20 +538,17 @@ __global__ void __launch_bounds__(MOST == 32 ? 256 : MOST, norm_ctas(N, MOST, MX
     }
     const double rstd = rsqrt(fma(ss, p.mean, p.eps));
     const float r_hi = (float)rstd;
-    // Rows whose root leaves fp32's normal numbers take the products in 64 bits. So do a lane's 8 values where one of them,
-    // but for zeros, is so small beside its row that v * r_hi, below 2^-100, may lose bits before a large weight brings it
-    // back. (f16's smallest value is 2^-40 of its largest.)
-    const bool plain = rstd > 1e-30 && rstd < 1e30, look = low * r_hi < 0x1p-100f;
+    // Rows whose root leaves fp32's normal numbers take the products in 64 bits. So does a warp that holds a value, but for
+    // zeros, which is so small beside its row that v * r_hi, below 2^-100, may lose bits before a large weight brings it back.
+    // (f16's smallest value is 2^-40 of its largest. Lanes that choose for themselves: 4096 x 4096 bf16 24.8 us, warps 24.2.)
+    const bool plain = rstd > 1e-30 && rstd < 1e30, tiny = __uint_as_float(low >> 1) * r_hi < 0x1p-100f;
+    const bool fast = plain && (std::is_same<T, __half>::value || !__any_sync(0xFFFFFFFFu, tiny));
 #pragma unroll
     for (int k = 0; k < N; k++) {
         const long long col = (long long)(k * G + t) * LANE;
         const Raw<float> w = N == 1 ? w0 : load_row<VIN>(p.w + col, p.cols - col, p.w, p.w + p.cols);
         float v[LANE], y[LANE];
         unpack(h[k], v);
-        bool fast = plain;
-        if (!std::is_same<T, __half>::value && look)                // zeros come here, too
-#pragma unroll
-            for (int i = 0; i < LANE; i++) fast = fast && (v[i] == 0.0f || fabsf(v[i]) * r_hi >= 0x1p-100f);
         if (fast) {
 #pragma unroll
             for (int i = 0; i < LANE; i++) y[i] = v[i] * r_hi * w.at(i);
