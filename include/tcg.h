@@ -374,9 +374,10 @@ bool tcg_mx_linear(void *y, const tcg_mx_t *x, const tcg_mx_t *w, const float *b
  *   h = x + r, rounded to t (r NULL: h = x),
  *   v = h / sqrt(mean(h^2) + eps) * w (w fp32 [cols], not read for h alone),
  * out as y (v to 4 roundings of fp32, rounded to t) and/or as mx (the codes of
- * v itself, where v is of fp32's normal numbers). Each of h,
- * y and mx may be NULL, not all of them. h and y may be x or r in place (the
- * same pointer and stride), not each other; otherwise nothing overlaps. */
+ * v itself), where v is of fp32's normal numbers, whatever the sizes of h and w
+ * beside it. Each of h, y and mx may be NULL, not all of them. h and y may be x
+ * or r in place (the same pointer and stride), not each other; otherwise
+ * nothing overlaps. */
 bool tcg_add_rms_norm(void *h, void *y, const tcg_mx_t *mx, const void *x, const void *r, const float *w, float eps,
                       int n_tok, int cols, int64_t ld_h, int64_t ld_y, int64_t ld_x, int64_t ld_r, ggml_type_t t);
 

@@ -13,7 +13,7 @@
 //
 // All three are bound by memory: 14336 x 4096 fp32 values quantised to 4 bits in 39 us (6.8 TB/s), read back to bf16 in
 // 25.2 us (5.9 TB/s, what a fill of the same bytes reaches); 4096 rows of 4096 fp32 values with their residual to 8 bits in
-// 38.6 us (5.7 TB/s: its second pass over the row waits for the sum). One token's norm takes 3.0 us, 1.8 of them the launch.
+// 38.6 us (5.7 TB/s: its second pass over the row waits for the sum). One token's norm takes 2.7 us, 1.8 of them the launch.
 #include "mx.cuh"
 
 #include <cuda_fp4.h>
@@ -364,7 +364,8 @@ __global__ void __launch_bounds__(32 * MX_WARPS) mx_quantize_kernel(const __grid
 }
 
 // C times 256 columns a warp, so that more than one row's 128 bytes of codes and its scales are under way. Ten CTAs' registers
-// of an SM for aligned rows: 14336 x 4096 from 4 bits to bf16 25.2 us, nine 25.7, twelve (with spills) 30.2.
+// of an SM for aligned rows, with two chunks at the price of 24 bytes spilled: 14336 x 4096 from 4 bits to bf16 25.1 us, nine
+// 25.7, twelve (with more spills) 30.2.
 template <typename T, int C, bool VEC>
 __global__ void __launch_bounds__(32 * MX_WARPS, VEC ? 10 : 1) mx_dequantize_kernel(const __grid_constant__ QuantArgs p)
 {
@@ -473,7 +474,9 @@ __device__ __forceinline__ float normed_odd(float v, double rstd, float w)
 // A row's columns are dealt out to G threads (a warp's 32, or the CTA's, at most MOST), N pieces of 8 consecutive columns each.
 // CTAs an SM that registers are kept for. 4096 rows of 4096 fp32 values with their residual, to 8 bits: two pieces a thread of 256
 // and four CTAs 38.6 us (5.7 TB/s), five (with spills) 40.3; two of 512 and two CTAs 40.9; one of 512 and three 43.2; four of 128
-// and five 50.0. Without codes five fit. 512 bf16 rows of 16384 without codes: two CTAs 16.5 us, one (76 registers) 19.9.
+// and five 50.0. Without codes five fit. 512 bf16 rows of 16384 without codes: two CTAs 16.5 us, one (76 registers) 19.9. Four
+// pieces of 1024 (more than 16384 columns) have 64 registers by the block's size, and fp32 rows spill 80 bytes, up to 376 with
+// codes off 16-byte boundaries: 256 rows of 32768 with their residual 31.9 us (4.2 TB/s), in bf16 18.2.
 constexpr int norm_ctas(int size, int n, int most, bool mx)
 {
     return n == 2 && most == 256 ? mx ? 4 : 5 : n == 4 && most == 512 && size == 2 && !mx ? 2 : 1;

@@ -11,13 +11,14 @@
 // The weights are the MMA's first operand: 128 weight rows are TMEM lanes, x's rows columns, so that a warp's 32 lanes hold
 // neighbouring results of one row of y and store them as they come, and one token costs 8 columns and not 128 rows.
 //   Few rows (mx_stream_kernel): bound by reading the weights. One wave of CTAs, K split over the CTAs of a cluster where the
-//     tiles are fewer than the SMs; parts meet in shared memory. One token 4096 -> 14336, x in 8 bits 7.5 us (31.2 MB: 4.2
-//     TB/s, of which ~3.5 us are start, first bytes and end), in 4 bits 6.6; 60000 outputs in 4 bits 25 us (5.2 TB/s); 64 rows
-//     of 14336 -> 4096 in 8 bits 10.9 us.
+//     tiles are fewer than the SMs; parts meet in shared memory. One token 4096 -> 14336, x in 8 bits, with weights that
+//     are in L2 7.4 us, with weights from DRAM 8.5 (31.2 MB: 3.7 TB/s; ~3.5 us are start, first bytes and end), in 4 bits 6.8
+//     and 8.4; 60000 outputs in 4 bits 25 us (5.3 TB/s); 64 rows of 14336 -> 4096 in 8 bits 10.9 and 11.3.
 //   Many (mx_pair_kernel): bound by the tensor core and the power that it takes. CTA pairs on tiles of 256 x 256, two
-//     accumulators. 4096 rows of 4096 -> 14336 in 4 bits 98 us (4.9 PFLOP/s at ~1.6 GHz: 60% of the cycles; the last round
-//     is 8 of 74 pairs' worth), 8192^3 189 us (5.8); 2048 rows of 14336 -> 4096 in 8 bits, fp32 results, 93 us (2.6: two
-//     rounds of which the second is three quarters full), 8192^3 363 us (3.0).
+//     accumulators. 4096 rows of 4096 -> 14336 in 4 bits 99 us (4.9 PFLOP/s at ~1.65 GHz: 60% of the cycles; the last round
+//     is 8 of 74 pairs' worth), 8192^3 188 us (5.9); 2048 rows of 14336 -> 4096 in 8 bits, fp32 results, 92 us (2.6: two
+//     rounds of which the second is three quarters full), 8192^3 358 us (3.1). These are bursts: in a loop of seconds the two
+//     prompts take 116 and 108 us under the power cap. (fp32 results: 64 sums a thread in registers, of which 72 bytes spill.)
 #include "mx.cuh"
 #include "tc05.cuh"
 
